@@ -12,6 +12,8 @@ LIB_PATH = Path(__file__).resolve().parents[1] / 'libqwen_b200.so'
 OK, EINVAL, ETIMEOUT, EDEVICE, ETOKEN, EOUTPUT, ENOMEM, EIO, ESTATE, ESCRATCH = 0, -1, -2, -3, -4, -5, -6, -7, -8, -9
 NOALLOC_SCRATCH_BYTES = 16 << 20
 FLAG_RTL_KV = 1
+KV8, KV_BF16, NO_SEQ = 0, 1, 0xffffffff
+PAGES_OK, PAGES_FULL, PAGES_BAD = 0, 1, 2
 VOCAB, HIDDEN, FFN, LAYERS = 151936, 896, 4864, 24
 
 
@@ -20,10 +22,19 @@ class Config(ctypes.Structure):
                 ('rms_eps', c_float), ('flags', c_uint32)]
 
 
+class PagedKV(ctypes.Structure):
+    """qwen_b200_paged_kv: device addresses and sizes of a paged cache."""
+    _fields_ = [('k', c_void_p), ('v', c_void_p), ('kscales', c_void_p), ('vscales', c_void_p), ('table', c_void_p),
+                ('lengths', c_void_p), ('refs', c_void_p), ('layer_stride', c_uint64), ('page_stride', c_uint64),
+                ('format', c_uint32), ('layers', c_uint32), ('pages', c_uint32), ('kv_heads', c_uint32),
+                ('page_tokens', c_uint32), ('head_dim', c_uint32), ('seqs', c_uint32), ('max_pages', c_uint32)]
+
+
 _P8 = POINTER(ctypes.c_int8)
 _P16 = POINTER(c_uint16)
 _P32 = POINTER(c_uint32)
 _PF = POINTER(c_float)
+_PKV = POINTER(PagedKV)
 
 _SIGNATURES = {
     'qwen_b200_default_config': (None, [POINTER(Config)]),
@@ -96,6 +107,22 @@ _SIGNATURES = {
     'qwen_b200_lm_head_workspace': (c_size_t, [c_uint32, c_uint32]),
     'qwen_b200_op_lm_head_argmax': (c_int, [c_void_p, c_uint32, c_void_p, c_float, c_void_p, c_void_p, c_uint32,
                                             c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'qwen_b200_op_paged_append': (c_int, [_PKV, c_uint32, c_void_p, c_void_p, c_uint64, c_uint32, c_void_p, c_void_p,
+                                          c_void_p]),
+    'qwen_b200_paged_decode_workspace': (c_size_t, [_PKV, c_uint32, c_uint32]),
+    'qwen_b200_op_paged_decode': (c_int, [_PKV, c_uint32, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_uint32,
+                                          c_uint32, c_float, c_void_p, c_uint64, c_void_p, c_size_t, c_void_p]),
+    'qwen_b200_paged_prefill_workspace': (c_size_t, [_PKV, c_uint32, c_uint32, c_uint32]),
+    'qwen_b200_op_paged_prefill': (c_int, [_PKV, c_uint32, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_void_p,
+                                           c_uint32, c_uint32, c_uint32, c_float, c_void_p, c_uint64, c_void_p,
+                                           c_size_t, c_void_p]),
+    'qwen_b200_pages_workspace': (c_size_t, [_PKV]),
+    'qwen_b200_op_pages_reserve': (c_int, [_PKV, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'qwen_b200_op_pages_fork': (c_int, [_PKV, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_size_t,
+                                        c_void_p]),
+    'qwen_b200_op_pages_free': (c_int, [_PKV, c_void_p, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'qwen_b200_op_pages_compact': (c_int, [_PKV, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'qwen_b200_op_pages_copy': (c_int, [_PKV, c_void_p, c_void_p, c_uint32, c_void_p]),
 }
 
 _lib = None

@@ -407,6 +407,135 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
                                 const int8_t *w, const float *scale, uint32_t vocab, uint16_t *logits,
                                 uint32_t *tokens, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- paged KV cache: operator level ---------------------------------------- */
+/* A cache whose sequences hold pages of page_tokens tokens out of one pool,
+ * instead of a contiguous slot each. The reference has one contiguous cache
+ * of one request (src/software/main.c:162-170); pages let sequences share a
+ * prompt's pages and grow one page at a time. The descriptor is plain host
+ * data: device addresses and sizes, read during a call and not kept.
+ *
+ * Pool: a row is one token's key (or value) of one KV head in one layer,
+ * head_dim int8 codes with one fp32 scale (QWEN_B200_KV8, the rule of
+ * qwen_b200_op_kv8_append) or head_dim bf16 values (QWEN_B200_KV_BF16). Row
+ * of (layer, page, head, token in page) =
+ *     layer * layer_stride + page * page_stride + head * page_tokens + token,
+ * so a pool may be [layers][pages][..] or [pages][layers][..]; 64-bit offsets.
+ * Tables: table[s][j] is the page of tokens j * page_tokens .. of sequence s,
+ * for j < ceil(lengths[s] / page_tokens); entries beyond are not read.
+ * refs[p] counts the sequences that hold page p (0: free); only the
+ * qwen_b200_op_pages_* calls read it, and it may be NULL for the others.
+ *
+ * Requirements (QWEN_B200_EINVAL otherwise): head_dim 64 or 128; page_tokens
+ * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables
+ * 4-byte aligned; strides multiples of 16 rows that keep pages and layers
+ * apart; pages < 2^31, seqs <= 65536, max_pages * page_tokens < 2^31; the
+ * pool on the current device. The page ids, lengths and indexes in device
+ * memory are not seen by the host: a sequence index >= seqs (for example
+ * QWEN_B200_NO_SEQ in a padded batch) is no sequence, a length beyond the
+ * table is cut to it, and tokens on a page id >= pages are not there. */
+#define QWEN_B200_KV8 0u
+#define QWEN_B200_KV_BF16 1u
+#define QWEN_B200_NO_SEQ 0xffffffffu
+typedef struct qwen_b200_paged_kv {
+    void *k, *v;               /* pools: int8_t (KV8) or bf16 bit patterns */
+    float *kscales, *vscales;  /* one per row; KV8 only */
+    uint32_t *table;           /* [seqs][max_pages] */
+    uint32_t *lengths;         /* [seqs] tokens */
+    uint32_t *refs;            /* [pages] */
+    uint64_t layer_stride, page_stride; /* in rows */
+    uint32_t format, layers, pages, kv_heads, page_tokens, head_dim, seqs, max_pages;
+} qwen_b200_paged_kv;
+
+/* Writes new tokens' keys and values into one layer of the cache: row r of k
+ * and v (bf16 [kv_heads][head_dim], rows row_stride elements apart, for
+ * example inside a fused q|k|v row; 16-byte aligned, row_stride a multiple of
+ * 8) becomes token positions[r] of sequence seqs[r]. KV8 pools quantise each
+ * (row, head): scale = amax / 127, code = clamp(rne(x / scale), +-127). The
+ * tokens have to be within lengths (qwen_b200_op_pages_reserve first); rows at
+ * or beyond it, and rows of no sequence, write nothing. No token may be named
+ * twice in a call, and its page must not be shared (never so after
+ * qwen_b200_op_pages_fork, which copies the page that a fork ends in). */
+int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *k, const uint16_t *v,
+                              uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
+                              void *stream);
+/* Attention of one token per sequence (the last one, whose key is in the
+ * cache): row r of q ([q_heads][head_dim] bf16, rows q_stride elements apart)
+ * attends to sequence seqs[r] (seqs NULL: sequence r) of `layer`, len =
+ * lengths[seqs[r]]:
+ *     ctx[r][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j - max),
+ * over the keys j < len with window == 0, or len - 1 - j < window (a sliding
+ * window that counts the token itself), or j < sinks (first tokens that stay
+ * visible). Query head h reads KV head h / (q_heads / kv_heads); q_heads is a
+ * multiple of kv_heads. A row with no key (length 0, no sequence) is zero.
+ * Unlike qwen_b200_op_attention this is not the oracle's bit-exact order: the
+ * weights are not rounded to bf16, sums are fp32, ctx is rounded once, and the
+ * result does not depend on anything but the inputs, the batch and the GPU's
+ * number of SMs. Only visible keys are read: what a page holds beyond the
+ * length or outside the window does not matter, NaN included. ctx rows are
+ * ctx_stride elements apart; q, ctx 16-byte aligned, strides multiples of 8
+ * and at least q_heads * head_dim. The context is split over the GPU and
+ * joined in the workspace (contents do not matter before or after; calls that
+ * overlap on the GPU need one each). */
+size_t qwen_b200_paged_decode_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t rows);
+int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
+                              uint32_t q_heads, uint32_t rows, const uint32_t *seqs, uint32_t window, uint32_t sinks,
+                              float scale, uint16_t *ctx, uint64_t ctx_stride, void *workspace,
+                              size_t workspace_bytes, void *stream);
+/* The same attention for the newest rows of n sequences (prompts and prompt
+ * chunks): rows starts[i] .. starts[i + 1] - 1 of q are the last tokens of
+ * sequence seqs[i] (seqs NULL: sequence i), the last of them at position
+ * lengths - 1, their keys already in the cache; each row sees the keys up to its own position
+ * under the window and first tokens. starts is [n + 1] on the device, not
+ * decreasing; q and ctx hold `rows` rows, and those at or behind starts[n] are
+ * left as they were. Rows before the sequence's first token (more rows than
+ * its length) and rows of no sequence are zero. Keys that no row of the
+ * sequence in this call sees may hold anything; a NaN or infinity in a value
+ * that some row sees may reach the rows around it. Softmax weights are rounded to bf16 for the second
+ * product, with the rounded weights in the sum; the other sums are fp32. */
+size_t qwen_b200_paged_prefill_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
+int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
+                               uint32_t q_heads, uint32_t n, const uint32_t *seqs, const uint32_t *starts,
+                               uint32_t rows, uint32_t window, uint32_t sinks, float scale, uint16_t *ctx,
+                               uint64_t ctx_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Page management, all on the device (index lists and counts included), so
+ * that it can be captured with the steps around it. Each call writes
+ * status[0] = QWEN_B200_PAGES_OK, _FULL (not enough free pages) or _BAD (an
+ * index out of range or named twice, a child that is not empty, a prefix
+ * longer than its parent, a length beyond the table, a held page id >= pages),
+ * and status[1] = the free pages after the call. When status[0] is not OK the
+ * call changed nothing else. Free pages are taken lowest id first, in the
+ * order of the list, so tables do not depend on timing. Calls on one cache
+ * run one after the other; each needs qwen_b200_pages_workspace bytes
+ * (16-byte aligned, contents do not matter). */
+#define QWEN_B200_PAGES_OK 0u
+#define QWEN_B200_PAGES_FULL 1u
+#define QWEN_B200_PAGES_BAD 2u
+size_t qwen_b200_pages_workspace(const qwen_b200_paged_kv *kv);
+/* lengths[seqs[i]] += tokens[i], with fresh pages where the held ones end. */
+int qwen_b200_op_pages_reserve(const qwen_b200_paged_kv *kv, const uint32_t *seqs, const uint32_t *tokens, uint32_t n,
+                               uint32_t *status, void *workspace, size_t workspace_bytes, void *stream);
+/* The empty sequence children[i] becomes the first prefix[i] tokens of
+ * parents[i] in every layer: full pages are shared (refs + 1), a partial last
+ * page is copied to a fresh one, so no token that is appended later falls on
+ * a shared page. A parent may be named many times. */
+int qwen_b200_op_pages_fork(const qwen_b200_paged_kv *kv, const uint32_t *parents, const uint32_t *children,
+                            const uint32_t *prefix, uint32_t n, uint32_t *status, void *workspace,
+                            size_t workspace_bytes, void *stream);
+/* Empties the sequences: refs - 1 on each page, lengths 0. */
+int qwen_b200_op_pages_free(const qwen_b200_paged_kv *kv, const uint32_t *seqs, uint32_t n, uint32_t *status,
+                            void *workspace, size_t workspace_bytes, void *stream);
+/* Moves pages in use to the front of the pool: with L pages in use, the i-th
+ * free page below L takes the i-th used page at or above L, in every layer,
+ * and tables and refs follow. After it pages 0 .. L-1 are in use. */
+int qwen_b200_op_pages_compact(const qwen_b200_paged_kv *kv, uint32_t *status, void *workspace,
+                               size_t workspace_bytes, void *stream);
+/* Copies whole pages in every layer: dst[i] = src[i]. No tables change. A
+ * page may be copied to several places; no dst may be named twice or be a src.
+ * Pairs with an id >= pages are left out. */
+int qwen_b200_op_pages_copy(const qwen_b200_paged_kv *kv, const uint32_t *src, const uint32_t *dst, uint32_t n,
+                            void *stream);
+
 #ifdef __cplusplus
 }
 #endif
