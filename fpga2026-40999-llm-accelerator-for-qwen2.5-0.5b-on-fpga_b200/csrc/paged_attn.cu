@@ -74,9 +74,7 @@ static int launch_attn(const PagedAttnArgs &a, cudaStream_t st) {
     return QB_LAUNCH_CHECK();
 }
 
-size_t paged_decode_ws(uint32_t, uint32_t, uint32_t, uint32_t) { return 256; }
 size_t paged_prefill_ws(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 256; }
-int launch_paged_decode(const PagedAttnArgs &a, void *, cudaStream_t st) { return launch_attn(a, st); }
 int launch_paged_prefill(const PagedAttnArgs &a, const qwen_b200_paged_kv &, uint32_t, void *, cudaStream_t st) {
     return launch_attn(a, st);
 }

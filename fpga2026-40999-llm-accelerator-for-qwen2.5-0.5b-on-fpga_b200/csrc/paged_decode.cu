@@ -1,0 +1,636 @@
+// Decode attention over the paged KV cache: one query token per sequence, the
+// context split evenly over the GPU and joined.
+//
+// Mathematics, per (row, query head), over the visible keys j:
+//   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
+// with a running maximum m that is only raised when some x_j passes m + 8 (p
+// stays below 2^8, so nothing overflows and the rescaling is rare), sums in
+// fp32. KV8: the key's scale multiplies its score and the value's scale its
+// weight, so both products run on the codes.
+//
+// Work: the unit is 16 keys of one (row, block of up to 8 query heads that
+// share a KV head). All units of the batch are numbered in a row and CTA c of G takes
+// the c-th equal run of them, whatever the lengths, windows and empty rows
+// (every CTA derives the numbering from the lengths, so the launch does not
+// depend on them and can be captured). A run that covers an item alone writes ctx; pieces
+// go to the workspace (at most two per CTA) and the join kernel, launched
+// behind with programmatic serialisation, adds them in CTA order.
+//
+// Bound by HBM (the cache is read once: 8 heads share each key): keys are
+// copied to shared memory by 16-byte cp.async, every warp with a ring of its
+// own, so no barrier stands between the loads and the products. Both products
+// are mma.sync m16n8k16 with the keys (then the dims) as the 16-row side and the
+// heads as the 8-column side: a row has up to 8 useful columns, where a
+// 128-row tcgen05 tile would be 6 % full, and per byte of cache these
+// instructions need less than half of the issue slots. S^T = K Q^T: int8 codes
+// become fp16 exactly (1024 + 128 + c minus 1152), q is scaled by a power of
+// two into fp16 range (bf16 values fit its 11 bits); bf16 keys are used as they are. O^T = V^T P^T:
+// weights as two bf16 halves (hi + lo, 16 bits together, and bf16's range
+// for any value scale), V^T fragments by byte permutes from the row-major rows.
+#include "paged.cuh"
+
+namespace qb {
+
+constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_STEP = 16, PD_HEADS = 8;
+constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
+constexpr uint32_t PD_MIN_UNITS = 16;  // a CTA takes at least 16 steps (2 per warp), or joining costs more than it saves
+
+template <bool KV8, int DIM>
+struct PdCfg {
+    static constexpr int RB = KV8 ? DIM : 2 * DIM;  // bytes of a row
+    static constexpr int CPR = RB / 16;             // 16-byte chunks of a row
+    static constexpr int STEP_BYTES = 2 * PD_STEP * RB + (KV8 ? 2 * PD_STEP * 4 : 0);
+    static constexpr int STAGES = RB == 64 ? 5 : 3;
+    static constexpr int MINB = RB == 256 ? 1 : 2;  // CTAs per SM
+    static constexpr int RING = PD_WARPS * STAGES * STEP_BYTES;
+    static constexpr int OUT = PD_WARPS * PD_HEADS * (DIM + 1) * 4;  // the warps' contexts, over the drained ring
+    static constexpr int SMEM = RING > OUT ? RING : OUT;
+    static constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;  // floats of a partial result: m, l, o
+};
+
+struct PdWork {
+    uint32_t group, hb;   // query heads per KV head, blocks of 8 of them
+    uint32_t items;       // (KV head, block) pairs of a row
+    uint32_t max_ctas;
+    unsigned long long *prefix;  // [rows + 1] units of one item in the rows before
+    float *pieces;        // [CTA][2][PIECE]
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float lds32f(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four codes (bytes of w) as two fp16 pairs, exactly.
+__device__ __forceinline__ void codes4_to_f16(uint32_t w, uint32_t &k01, uint32_t &k23) {
+    const uint32_t u = w ^ 0x80808080u;  // c + 128
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(k01) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(k23) : "r"(b), "r"(0x64806480u));
+}
+// Byte i of wa and of wb as a bf16 pair, exactly (see codes4_to_bf16).
+template <int I>
+__device__ __forceinline__ uint32_t codes_pair_bf16(uint32_t wa, uint32_t wb) {
+    const uint32_t t = __byte_perm(wa, wb, ((4 + I) << 8) | I);
+    return bf16x2_sub(lop_or(t, 0x007F007Fu, 0x43004300u), lop_or(t, 0x00800080u, 0x43004300u));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// Visible keys of a row as steps of 16: those of the first tokens [0, s16),
+// then those from low16 on.
+struct PdRow {
+    int len, first, low, s16, low16, steps;
+};
+__device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
+    PdRow r;
+    r.len = paged_length(a.c, a.seqs ? a.seqs[row] : row);
+    const KeySpan k = key_span(r.len - 1, a.window, a.sinks);
+    r.first = k.first;
+    r.low = k.low;
+    r.low16 = k.low >> 4;
+    r.s16 = min((k.first + 15) >> 4, r.low16);
+    r.steps = r.len > 0 ? r.s16 + ((r.len + 15) >> 4) - r.low16 : 0;
+    return r;
+}
+
+// CTA c of g takes units [start(c), start(c + 1)) of `total`.
+struct PdSplit {
+    unsigned long long q, r;
+    uint32_t g;
+    __device__ __forceinline__ PdSplit(unsigned long long total, uint32_t max_ctas) {
+        const unsigned long long want = (total + PD_MIN_UNITS - 1) / PD_MIN_UNITS;
+        g = (uint32_t)min((unsigned long long)max_ctas, max(want, 1ull));
+        q = total / g;
+        r = total % g;
+    }
+    __device__ __forceinline__ unsigned long long start(uint32_t c) const {
+        return c * q + min((unsigned long long)c, r);
+    }
+    __device__ __forceinline__ uint32_t cta_of(unsigned long long u) const {
+        const unsigned long long edge = r * (q + 1);
+        return (uint32_t)(u < edge ? u / (q + 1) : r + (u - edge) / q);
+    }
+};
+
+template <bool KV8, int DIM>
+__global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decode_kernel(PagedAttnArgs a, PdWork w) {
+    using C = PdCfg<KV8, DIM>;
+    constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ unsigned long long wsum[PD_WARPS];
+    __shared__ unsigned long long at_prefix;
+    __shared__ uint32_t at_row;
+    __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS];
+    pdl_trigger();  // the join kernel waits for this one to end
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+
+    // ---- the numbering of the units: prefix sums of the rows' steps
+    const uint32_t per = (a.rows + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * per, a.rows),
+                   r1 = min(r0 + per, a.rows);
+    unsigned long long mine = 0;
+    for (uint32_t r = r0; r < r1; ++r) mine += pd_row(a, r).steps;
+    unsigned long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    unsigned long long all = 0;
+#pragma unroll
+    for (int i = 0; i < PD_WARPS; ++i) {
+        if (i < warp) incl += wsum[i];
+        all += wsum[i];
+    }
+    const unsigned long long before = incl - mine;
+    if (blockIdx.x == 0) {
+        unsigned long long p = before;
+        for (uint32_t r = r0; r < r1; ++r) {
+            w.prefix[r] = p;
+            p += pd_row(a, r).steps;
+        }
+        if (tid == 0) w.prefix[a.rows] = all;
+    }
+    const PdSplit split(all * w.items, w.max_ctas);
+    if (blockIdx.x >= split.g || all == 0) return;
+    unsigned long long u = split.start(blockIdx.x);
+    const unsigned long long u_end = split.start(blockIdx.x + 1);
+    if (before * w.items <= u && u < incl * w.items) {
+        unsigned long long p = before;
+        uint32_t r = r0;
+        for (;; ++r) {
+            const int n = pd_row(a, r).steps;
+            if (u < (p + n) * w.items) break;
+            p += n;
+        }
+        at_row = r;
+        at_prefix = p;
+    }
+    __syncthreads();
+    uint32_t row = at_row;
+    unsigned long long base = at_prefix * w.items;
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::STAGES * C::STEP_BYTES);
+    const float fac0 = a.scale * 1.44269504f;
+    bool first_segment = true;
+    while (u < u_end) {
+        const PdRow R = pd_row(a, row);
+        if (R.steps == 0) {
+            ++row;
+            continue;
+        }
+        const uint32_t rem = (uint32_t)((u - base) % R.steps), item = (uint32_t)((u - base) / R.steps);
+        const int cnt = (int)min((unsigned long long)(R.steps - rem), u_end - u);
+        const uint32_t kvh = item / w.hb, hblk = item % w.hb;
+        const uint32_t seq = a.seqs ? a.seqs[row] : row;
+        const uint32_t *table = a.c.table + (uint64_t)seq * a.c.max_pages;
+        const int pmask = (1 << a.c.tshift) - 1;
+
+        // ---- this warp's steps: warp, warp + 8, .. of the segment
+        const int nst = cnt > warp ? (cnt - warp + PD_WARPS - 1) / PD_WARPS : 0;
+        auto key_of = [&](int i) {
+            const int s = (int)rem + warp + i * PD_WARPS;
+            return (s < R.s16 ? s : s - R.s16 + R.low16) << 4;
+        };
+        auto page_at = [&](int i) { return i < nst ? __ldg(&table[key_of(i) >> a.c.tshift]) : PG_NO_PAGE; };
+        uint32_t there = 0;  // bit i % 32: step i's page exists
+        auto load = [&](int i, uint32_t page) {
+            if (i < nst) {
+                const int key = key_of(i);
+                const bool ok = page < a.c.pages;
+                there = (there & ~(1u << (i & 31))) | ((uint32_t)ok << (i & 31));
+                const uint64_t r = ok ? paged_row(a.c, page, kvh) + (key & pmask) : 0;
+                const uint8_t *kp = a.c.k + r * C::RB, *vp = a.c.v + r * C::RB;
+                const uint32_t dst = ring + (i % C::STAGES) * C::STEP_BYTES;
+#pragma unroll
+                for (int j = 0; j < C::CPR / 2; ++j) {
+                    const int n = j * 32 + lane, kr = n / C::CPR, c = n % C::CPR;
+                    const int key_r = key + kr;
+                    // only visible keys are read; the others are zero
+                    const uint32_t bytes = ok && key_r < R.len && (key_r >= R.low || key_r < R.first) ? 16 : 0;
+                    const int kc = C::CPR == 4 ? c : c ^ ((kr & 1) << 2);
+                    const int vpos = C::CPR == 4 ? ((kr >> 1) << 3) + ((((kr & 1) << 2) | c) ^ (((kr >> 1) & 3) << 1))
+                                                 : kr * C::CPR + (c ^ (((kr >> 1) & 3) << 1));
+                    cp16(dst + (kr * C::CPR + kc) * 16, kp + n * 16, bytes);
+                    cp16(dst + PD_STEP * C::RB + vpos * 16, vp + n * 16, bytes);
+                }
+                if constexpr (KV8) {
+                    const int kr = lane & 15, key_r = key + kr;
+                    const uint32_t bytes = ok && key_r < R.len && (key_r >= R.low || key_r < R.first) ? 4 : 0;
+                    cp4(dst + 2 * PD_STEP * C::RB + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + r + kr, bytes);
+                }
+            }
+            cp_commit();
+        };
+        uint32_t next = page_at(0);
+#pragma unroll
+        for (int i = 0; i < C::STAGES - 1; ++i) {
+            const uint32_t page = next;
+            next = page_at(i + 1);
+            load(i, page);
+        }
+
+        // ---- the query heads as B fragments: head 8 hblk + g, dims by the
+        // permutation that the key rows' 16-byte chunks give the first product
+        uint32_t qf[KS][2];
+        float fac[2];
+        {
+            const uint32_t hl = hblk * PD_HEADS + g;
+            const bool live = hl < w.group;
+            const uint16_t *qp = a.q + row * a.q_stride + (uint64_t)(kvh * w.group + (live ? hl : 0)) * DIM;
+            if constexpr (KV8) {
+                float x[KS][4], amax = 0.f;
+#pragma unroll
+                for (int j = 0; j < KS / 4; ++j) {  // chunk t + 4 j: dims 16 (t + 4 j) .. + 15
+                    uint4 v[2];
+                    v[0] = reinterpret_cast<const uint4 *>(qp + 16 * (t + 4 * j))[0];
+                    v[1] = reinterpret_cast<const uint4 *>(qp + 16 * (t + 4 * j))[1];
+                    const uint32_t word[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        x[4 * j + k][0] = bflo(word[2 * k]);
+                        x[4 * j + k][1] = bfhi(word[2 * k]);
+                        x[4 * j + k][2] = bflo(word[2 * k + 1]);
+                        x[4 * j + k][3] = bfhi(word[2 * k + 1]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // 2^(14 - e): the largest |q| lands in [2^14, 2^15); values 2^-28 of it and smaller lose bits
+                const int e = amax > 0.f ? min(max(ilogbf(amax), -100), 127) : 0;
+                const float up = live ? pow2i(min(14 - e, 126)) : 0.f;
+                const float down = fac0 * pow2i(-min(14 - e, 126));
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    qf[k][0] = pack_f16(x[k][0] * up, x[k][1] * up);
+                    qf[k][1] = pack_f16(x[k][2] * up, x[k][3] * up);
+                }
+                fac[0] = __shfl_sync(0xffffffffu, down, 8 * t);  // of head 2t: lane 4 (2t)
+                fac[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < KS / 2; ++j) {  // chunk t + 4 j: dims 8 (t + 4 j) .. + 7
+                    uint4 v = *reinterpret_cast<const uint4 *>(qp + 8 * (t + 4 * j));
+                    if (!live) v = make_uint4(0, 0, 0, 0);
+                    qf[2 * j][0] = v.x;
+                    qf[2 * j][1] = v.y;
+                    qf[2 * j + 1][0] = v.z;
+                    qf[2 * j + 1][1] = v.w;
+                }
+                fac[0] = fac[1] = fac0;
+            }
+        }
+
+        float o[KS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+        for (int i = 0; i < nst; ++i) {
+            {
+                const uint32_t page = next;
+                next = page_at(i + C::STAGES);
+                load(i + C::STAGES - 1, page);
+            }
+            cp_wait<C::STAGES - 1>();
+            __syncwarp();
+            const uint32_t buf = ring + (i % C::STAGES) * C::STEP_BYTES;
+            // ---- scores of 16 keys (rows g, g + 8) x 8 heads (columns 2t, 2t + 1)
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (KV8) {
+#pragma unroll
+                for (int j = 0; j < C::CPR / 4; ++j) {
+                    const int c = t + 4 * j, x = C::CPR == 4 ? 0 : (g & 1) << 2;
+                    const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
+                    const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
+                    const uint32_t wl4[4] = {lo.x, lo.y, lo.z, lo.w}, wh4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t a0, a1, a2, a3;
+                        codes4_to_f16(wl4[k], a0, a2);
+                        codes4_to_f16(wh4[k], a1, a3);
+                        mma16816<true>(s, a0, a1, a2, a3, qf[4 * j + k][0], qf[4 * j + k][1]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < C::CPR / 4; ++j) {
+                    const int c = t + 4 * j, x = (g & 1) << 2;
+                    const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
+                    const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
+                    mma16816<false>(s, lo.x, hi.x, lo.y, hi.y, qf[2 * j][0], qf[2 * j][1]);
+                    mma16816<false>(s, lo.z, hi.z, lo.w, hi.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+                }
+            }
+            float vs[2] = {1.f, 1.f};
+            if constexpr (KV8) {
+                const uint32_t sc = buf + 2 * PD_STEP * C::RB;
+                const float k0 = lds32f(sc + g * 4), k1 = lds32f(sc + g * 4 + 32);
+                vs[0] = lds32f(sc + 64 + g * 4);
+                vs[1] = lds32f(sc + 96 + g * 4);
+                s[0] *= k0 * fac[0];
+                s[1] *= k0 * fac[1];
+                s[2] *= k1 * fac[0];
+                s[3] *= k1 * fac[1];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[k] *= fac0;
+            }
+            const int key = key_of(i);
+            if (!(there >> (i & 31) & 1) || key + 16 > R.len || (key < R.low && key + 16 > R.first)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int kr = key + g + 8 * h;
+                    if (!(there >> (i & 31) & 1) || kr >= R.len || (kr < R.low && kr >= R.first))
+                        s[2 * h] = s[2 * h + 1] = -INFINITY;
+                }
+            }
+            // ---- the maximum, raised only where a score passes it by 2^8
+            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m[0] + 8.f || fmaxf(s[1], s[3]) > m[1] + 8.f)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = fmaxf(s[h], s[h + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    x = fmaxf(x, m[h]);
+                    const float f = m[h] == x ? 1.f : ex2(m[h] - x);
+                    m[h] = x;
+                    l[h] *= f;
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        o[j][h] *= f;
+                        o[j][h + 2] *= f;
+                    }
+                }
+            }
+            const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+            float p[4] = {ex2(s[0] - m0), ex2(s[1] - m1), ex2(s[2] - m0), ex2(s[3] - m1)};
+            l[0] += p[0] + p[2];
+            l[1] += p[1] + p[3];
+            if constexpr (KV8) {
+                p[0] *= vs[0];
+                p[1] *= vs[0];
+                p[2] *= vs[1];
+                p[3] *= vs[1];
+            }
+            // ---- weights as hi + lo, transposed to (keys x heads) B fragments
+            const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
+            const uint32_t b0 = movmatrix(h0), b1 = movmatrix(h1);
+            const uint32_t c0 = movmatrix(pack_bf16(p[0] - bflo(h0), p[1] - bfhi(h0)));
+            const uint32_t c1 = movmatrix(pack_bf16(p[2] - bflo(h1), p[3] - bfhi(h1)));
+            // ---- O^T += V^T P^T: tile j holds dims D0(g) + 2 j (row g) and + 1 (row g + 8)
+            const uint32_t vb = buf + PD_STEP * C::RB;
+            const int ra = 2 * t, rb = 2 * t + 8;  // keys 2t, 2t + 1 and 2t + 8, 2t + 9
+            if constexpr (KV8 && DIM == 64) {
+                uint2 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int kr = (k < 2 ? ra : rb) + (k & 1);
+                    const int pos = ((kr >> 1) << 3) + ((((kr & 1) << 2) | (g >> 1)) ^ (((kr >> 1) & 3) << 1));
+                    v[k] = lds64(vb + pos * 16 + (g & 1) * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t x0 = j < 2 ? v[0].x : v[0].y, x1 = j < 2 ? v[1].x : v[1].y,
+                                   x2 = j < 2 ? v[2].x : v[2].y, x3 = j < 2 ? v[3].x : v[3].y;
+                    uint32_t a0, a1, a2, a3;
+                    if (j & 1) {
+                        a0 = codes_pair_bf16<2>(x0, x1), a1 = codes_pair_bf16<3>(x0, x1);
+                        a2 = codes_pair_bf16<2>(x2, x3), a3 = codes_pair_bf16<3>(x2, x3);
+                    } else {
+                        a0 = codes_pair_bf16<0>(x0, x1), a1 = codes_pair_bf16<1>(x0, x1);
+                        a2 = codes_pair_bf16<0>(x2, x3), a3 = codes_pair_bf16<1>(x2, x3);
+                    }
+                    mma16816<false>(o[j], a0, a1, a2, a3, b0, b1);
+                    mma16816<false>(o[j], a0, a1, a2, a3, c0, c1);
+                }
+            } else {
+                constexpr int NC = KV8 ? 1 : DIM / 64;  // 16-byte chunks of a key that this lane's dims take
+#pragma unroll
+                for (int q = 0; q < NC; ++q) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int kr = (k < 2 ? ra : rb) + (k & 1);
+                        v[k] = lds128(vb + (kr * C::CPR + ((g + 8 * q) ^ (((kr >> 1) & 3) << 1))) * 16);
+                    }
+                    const uint32_t x[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
+                                              {v[1].x, v[1].y, v[1].z, v[1].w},
+                                              {v[2].x, v[2].y, v[2].z, v[2].w},
+                                              {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {  // word k of the chunks
+                        if constexpr (KV8) {
+                            uint32_t a0 = codes_pair_bf16<0>(x[0][k], x[1][k]), a1 = codes_pair_bf16<1>(x[0][k], x[1][k]);
+                            uint32_t a2 = codes_pair_bf16<0>(x[2][k], x[3][k]), a3 = codes_pair_bf16<1>(x[2][k], x[3][k]);
+                            mma16816<false>(o[2 * k], a0, a1, a2, a3, b0, b1);
+                            mma16816<false>(o[2 * k], a0, a1, a2, a3, c0, c1);
+                            a0 = codes_pair_bf16<2>(x[0][k], x[1][k]), a1 = codes_pair_bf16<3>(x[0][k], x[1][k]);
+                            a2 = codes_pair_bf16<2>(x[2][k], x[3][k]), a3 = codes_pair_bf16<3>(x[2][k], x[3][k]);
+                            mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, b0, b1);
+                            mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, c0, c1);
+                        } else {
+                            const uint32_t a0 = __byte_perm(x[0][k], x[1][k], 0x5410),
+                                           a1 = __byte_perm(x[0][k], x[1][k], 0x7632);
+                            const uint32_t a2 = __byte_perm(x[2][k], x[3][k], 0x5410),
+                                           a3 = __byte_perm(x[2][k], x[3][k], 0x7632);
+                            mma16816<false>(o[4 * q + k], a0, a1, a2, a3, b0, b1);
+                            mma16816<false>(o[4 * q + k], a0, a1, a2, a3, c0, c1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();  // the stage may be refilled
+        }
+        cp_wait<0>();
+
+        // ---- the warps' results joined through shared memory (over the drained rings)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+        __syncthreads();
+        float *os = reinterpret_cast<float *>(smem);
+        if (g == 0) {
+            wm[warp][2 * t] = m[0];
+            wm[warp][2 * t + 1] = m[1];
+            wl[warp][2 * t] = l[0];
+            wl[warp][2 * t + 1] = l[1];
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            int d = 2 * j + (KV8 || DIM == 64 ? (DIM / 8) * g : 0);
+            if (!KV8 && DIM == 128) d = (j < 4 ? 8 * g + 2 * j : 64 + 8 * g + 2 * (j - 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                os[(warp * PD_HEADS + 2 * t + (k & 1)) * (DIM + 1) + d + (k >> 1)] = o[j][k];
+        }
+        __syncthreads();
+        const bool whole = cnt == R.steps;
+        float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
+        for (int x = tid; x < PD_HEADS * DIM; x += PD_THREADS) {
+            const int h = x / DIM, d = x % DIM;
+            float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+            for (int i = 0; i < PD_WARPS; ++i) M = fmaxf(M, wm[i][h]);
+            const float M0 = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int i = 0; i < PD_WARPS; ++i) {
+                const float f = ex2(wm[i][h] - M0);
+                L += wl[i][h] * f;
+                O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f;
+            }
+            const uint32_t hl = hblk * PD_HEADS + h;
+            if (whole) {
+                if (hl < w.group)
+                    a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
+            } else {
+                piece[2 * PD_HEADS + x] = O;
+                if (d == 0) {
+                    piece[h] = M;
+                    piece[PD_HEADS + h] = L;
+                }
+            }
+        }
+        __syncthreads();  // os is read before the next segment's loads
+        first_segment = false;
+        u += cnt;
+        if (u == base + (unsigned long long)R.steps * w.items) {
+            base = u;
+            ++row;
+        }
+    }
+}
+
+// One CTA per (item, query head): the pieces of the item's context added in
+// CTA order; items without keys are zero, items of one CTA are already written.
+template <int DIM>
+__global__ void __launch_bounds__(DIM) paged_join_kernel(PagedAttnArgs a, PdWork w) {
+    constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;
+    __shared__ float wt[2 * PD_MAX_SMS];
+    pdl_wait();
+    const uint64_t index = blockIdx.x;
+    const uint32_t qh = w.items * PD_HEADS;  // heads, the last block of each KV head filled up
+    const uint32_t row = (uint32_t)(index / qh), item = (uint32_t)(index % qh) / PD_HEADS, h = (uint32_t)(index % PD_HEADS);
+    const uint32_t kvh = item / w.hb, hl = (item % w.hb) * PD_HEADS + h;
+    if (hl >= w.group) return;
+    const int d = threadIdx.x;
+    uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d;
+    const unsigned long long p0 = w.prefix[row], steps = w.prefix[row + 1] - p0;
+    if (steps == 0) {
+        *out = 0;
+        return;
+    }
+    const PdSplit split(w.prefix[a.rows] * w.items, w.max_ctas);
+    const unsigned long long u0 = p0 * w.items + item * steps;
+    const uint32_t c0 = split.cta_of(u0), c1 = split.cta_of(u0 + steps - 1), n = c1 - c0 + 1;
+    if (n == 1) return;
+    auto piece = [&](uint32_t i) {  // the item's segment of CTA c0 + i: the CTA's first one unless c0 began before the item
+        return w.pieces + ((uint64_t)(c0 + i) * 2 + (i == 0 && split.start(c0) < u0)) * PIECE;
+    };
+    for (uint32_t i = d; i < n; i += DIM) wt[i] = piece(i)[h];
+    __syncthreads();
+    float M = -INFINITY;
+    for (uint32_t i = 0; i < n; ++i) M = fmaxf(M, wt[i]);
+    const float M0 = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+#pragma unroll 8
+    for (uint32_t i = 0; i < n; ++i) {
+        const float *p = piece(i);
+        const float f = ex2(wt[i] - M0);
+        L += p[PD_HEADS + h] * f;
+        O += p[2 * PD_HEADS + h * DIM + d] * f;
+    }
+    *out = f2bf(L == 0.f ? 0.f : O / L);
+}
+
+static size_t pd_prefix_bytes(uint32_t rows) { return (((size_t)rows + 1) * 8 + 255) & ~(size_t)255; }
+
+size_t paged_decode_ws(uint32_t, uint32_t, uint32_t dim, uint32_t rows) {
+    return pd_prefix_bytes(rows) + (size_t)2 * PD_MAX_SMS * 2 * (2 * PD_HEADS + PD_HEADS * dim) * 4;
+}
+
+template <bool KV8, int DIM>
+static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t st) {
+    using C = PdCfg<KV8, DIM>;
+    auto *kernel = paged_decode_kernel<KV8, DIM>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
+    w.max_ctas = (uint32_t)(sms * C::MINB);
+    PdlChain chain;
+    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PD_THREADS), C::SMEM, st, 1, a, w)) return rc;
+    return launch_pdl(paged_join_kernel<DIM>, dim3(a.rows * w.items * PD_HEADS), dim3(DIM), 0, st, 1, a, w);
+}
+
+int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
+    const int sms = paged_sms();
+    if (sms <= 0) return -3;
+    PdWork w;
+    w.group = a.qh / a.c.hkv;
+    w.hb = (w.group + PD_HEADS - 1) / PD_HEADS;
+    w.items = a.c.hkv * w.hb;
+    if ((uint64_t)a.rows * w.items * PD_HEADS >= 1ull << 31) return -1;
+    w.prefix = (unsigned long long *)ws;
+    w.pieces = reinterpret_cast<float *>((char *)ws + pd_prefix_bytes(a.rows));
+    const int n = sms < PD_MAX_SMS ? sms : PD_MAX_SMS;
+    if (a.format == QWEN_B200_KV8)
+        return a.dim == 64 ? launch_decode<true, 64>(a, w, n, st) : launch_decode<true, 128>(a, w, n, st);
+    return a.dim == 64 ? launch_decode<false, 64>(a, w, n, st) : launch_decode<false, 128>(a, w, n, st);
+}
+
+}  // namespace qb
