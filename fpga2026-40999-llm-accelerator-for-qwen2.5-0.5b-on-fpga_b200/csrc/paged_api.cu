@@ -172,7 +172,7 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
     a.rows = rows;
     a.n = n;
     a.starts = starts;
-    return launch_paged_prefill(a, *kv, layer, workspace, (cudaStream_t)stream);
+    return launch_paged_prefill(a, workspace, (cudaStream_t)stream);
 }
 
 size_t qwen_b200_pages_workspace(const qwen_b200_paged_kv *kv) {

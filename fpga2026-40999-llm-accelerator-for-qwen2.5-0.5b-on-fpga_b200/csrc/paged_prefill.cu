@@ -1,0 +1,937 @@
+// Causal attention of the newest rows of several sequences over their pages,
+// with a sliding window and first tokens that stay visible; both products on
+// the tensor cores (tcgen05.mma kind::f16, bf16 operands, fp32 accumulators in
+// TMEM).
+//
+// Mathematics, per (row, query head), over its visible keys j in blocks of 128:
+//   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
+// m is the running maximum, raised only where a block passes it by more than
+// 8 (p stays below 2^8), so that the accumulator is rarely rescaled. The weights
+// are rounded to bf16 for the second product (half a step is 2^-8 of a weight, unbiased);
+// everything else is fp32. KV8: codes become bf16 exactly on the way to
+// shared memory, the key's scale multiplies its column of scores and the
+// value's scale its column of weights.
+//
+// Tiles: the rows of a sequence and the query heads that share a KV head are one
+// axis (row-major: token, head), cut into tiles of 256 = two MMA tiles of 128 rows,
+// so any group size fills them and a block of keys is read once for
+// 256 (row, head) pairs. Per tile only the blocks that some row sees are
+// visited. All (tile, KV head, block) units are numbered in a row and CTA c of
+// G takes the c-th equal run: long and short prompts, windows and single rows
+// balance by themselves, and few rows over many keys split along the keys. A
+// tile that two or more CTAs share is joined by a second kernel (at most two
+// pieces per CTA, fp32, added in CTA order).
+//
+// Warps (512 threads, one CTA per SM, registers moved to the softmax warps):
+//   0-3, 4-7  softmax of the first / second MMA tile, one thread per row:
+//             scores from TMEM, weights back over the scores' columns
+//   8-11      loaders: queries and bf16 rows by cp.async (zero-filled where a
+//             key is not visible, so garbage never reaches the products), KV8 rows
+//             through registers; 128-byte swizzled K-major tiles, the value
+//             tile read as an MN-major operand
+//   12        one thread issues the MMAs; while one tile's softmax runs, the
+//             other's products do
+//   13        walks the units and publishes segments (tile, KV head, block range)
+//   14        zeroes the rows in front of a sequence's first token
+// Bound by the exponentials at 64 dims (16 per clock and SM) and by the tensor
+// cores at 128. Every wait is bounded (error codes 60-69).
+#include "kernels.h"
+#include "paged.cuh"
+#include "tc05.cuh"
+
+namespace qb {
+
+constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 512, PP_WARPS = PF_THREADS / 32;
+constexpr int PP_MAX_SMS = 192;
+constexpr uint32_t PP_MIN_UNITS = 4;  // blocks a CTA takes at least: less and the join costs more than the split saves
+constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
+constexpr int PP_SEG = 2;             // segments published ahead
+
+template <bool KV8, int DIM>
+struct PpCfg {
+    static constexpr int HALVES = DIM / 64;
+    static constexpr int TILE_BYTES = 128 * 128 * HALVES;  // 128 rows of DIM bf16, 64 dims per swizzled half
+    static constexpr int SLOTS = DIM == 64 ? 8 : 4;        // K and V tiles in flight (K0 V0 K1 V1 ..)
+    static constexpr int Q = 0, RING = 2 * TILE_BYTES;
+    static constexpr int SC = RING + SLOTS * TILE_BYTES;   // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
+    static constexpr int MASK = SC + PP_SC * 256 * 4;
+    static constexpr int SEG = MASK + PP_SC * 16;
+    static constexpr int BARS = SEG + PP_SEG * 64;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9;
+    static constexpr int SLOT = BARS + NBARS * 8;
+    static constexpr int TOTAL = SLOT + 16;
+    static constexpr int ALLOC = TOTAL + 1024;
+    static constexpr int PIECE = 2 * PP_TILE + PP_TILE * DIM;  // floats: m, l, o
+    static_assert(ALLOC <= 232448, "shared memory per CTA");
+};
+
+// One tile's run of blocks for one KV head.
+struct PpSeg {
+    uint32_t seq, row0, m0, mrows;  // rows of q from row0; flattened rows m0 .. of mrows
+    int pos0;                       // position of the sequence's first row (negative: more rows than tokens)
+    uint32_t kvh;
+    int b0, nblk;                   // virtual blocks; nblk 0 ends the list
+    int s128, low128;               // virtual block b: b < s128 ? b : b - s128 + low128
+    int first, low, last;           // keys that some row sees: [0, first) and [low, last]
+    int piece;                      // -1: the tile's whole list; else the piece's index
+    int pad[2];
+};
+static_assert(sizeof(PpSeg) == 64, "segment record");
+
+struct PpRec {  // the tile that a CTA starts in the middle of
+    uint32_t valid, row0, m0, mrows, kvh, c0, c1, slot0;
+    int pos0;
+    uint32_t pad[7];
+};
+static_assert(sizeof(PpRec) == 64, "join record");
+
+struct PpWork {
+    uint32_t group, max_ctas;
+    float fac;       // log2(e) |scale|
+    uint32_t negate; // scale < 0: the first product negates the queries
+    unsigned *err;
+    PpRec *recs;     // [max_ctas]
+    float *pieces;   // [max_ctas][2][PIECE]
+};
+
+struct PpSeqInfo {
+    uint32_t row0, seq, mrows;
+    int pos0, nt;
+};
+__device__ __forceinline__ PpSeqInfo pp_seq(const PagedAttnArgs &a, const PpWork &w, uint32_t i) {
+    PpSeqInfo s;
+    const uint32_t s0 = min(a.starts[i], a.rows), s1 = min(max(a.starts[i + 1], s0), a.rows);
+    s.row0 = s0;
+    s.seq = a.seqs ? a.seqs[i] : i;
+    s.mrows = (s1 - s0) * w.group;
+    const int len = paged_length(a.c, s.seq);
+    s.pos0 = len - (int)(s1 - s0);
+    s.nt = len > 0 ? (int)((s.mrows + PP_TILE - 1) / PP_TILE) : 0;
+    return s;
+}
+struct PpBlocks {
+    int s128, low128, first, low, last, n;
+};
+__device__ __forceinline__ PpBlocks pp_blocks(const PagedAttnArgs &a, const PpWork &w, int pos0, uint32_t mrows, int k) {
+    PpBlocks b;
+    const uint32_t m0 = (uint32_t)k * PP_TILE, m1 = min(m0 + PP_TILE, mrows) - 1;
+    const int pmin = max(pos0 + (int)(m0 / w.group), 0);
+    b.last = pos0 + (int)(m1 / w.group);
+    b.low = key_span(pmin, a.window, a.sinks).low;
+    b.first = key_span(max(b.last, 0), a.window, a.sinks).first;
+    b.low128 = b.low >> 7;
+    b.s128 = min((b.first + 127) >> 7, b.low128);
+    b.n = b.last < 0 ? 0 : b.s128 + (b.last >> 7) + 1 - b.low128;
+    return b;
+}
+// Blocks of a sequence's tiles, summed by a whole warp.
+__device__ __forceinline__ uint32_t pp_units_warp(const PagedAttnArgs &a, const PpWork &w, int pos0, uint32_t mrows,
+                                                  int nt) {
+    uint32_t u = 0;
+    for (int k = threadIdx.x & 31; k < nt; k += 32) u += pp_blocks(a, w, pos0, mrows, k).n;
+    return __reduce_add_sync(0xffffffffu, u);
+}
+// Blocks of the sequences base + lane < end, one per lane.
+__device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const PpWork &w, uint32_t base, uint32_t end) {
+    const uint32_t i = base + (threadIdx.x & 31);
+    PpSeqInfo s = {};
+    uint32_t u = 0;
+    if (i < end) {
+        s = pp_seq(a, w, i);
+        if (s.nt <= 4)
+            for (int k = 0; k < s.nt; ++k) u += pp_blocks(a, w, s.pos0, s.mrows, k).n;
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, s.nt > 4); todo; todo &= todo - 1) {
+        const int l = __ffs(todo) - 1;
+        const uint32_t x = pp_units_warp(a, w, __shfl_sync(0xffffffffu, s.pos0, l), __shfl_sync(0xffffffffu, s.mrows, l),
+                                         __shfl_sync(0xffffffffu, s.nt, l));
+        if ((int)(threadIdx.x & 31) == l) u = x;
+    }
+    return u;
+}
+
+struct PpSplit {
+    unsigned long long q, r;
+    uint32_t g;
+    __device__ __forceinline__ PpSplit(unsigned long long total, uint32_t max_ctas) {
+        const unsigned long long want = (total + PP_MIN_UNITS - 1) / PP_MIN_UNITS;
+        g = (uint32_t)min((unsigned long long)max_ctas, max(want, 1ull));
+        q = total / g;
+        r = total % g;
+    }
+    __device__ __forceinline__ unsigned long long start(uint32_t c) const {
+        return c * q + min((unsigned long long)c, r);
+    }
+    __device__ __forceinline__ uint32_t cta_of(unsigned long long u) const {
+        const unsigned long long edge = r * (q + 1);
+        return (uint32_t)(u < edge ? u / (q + 1) : r + (u - edge) / q);
+    }
+};
+
+// ---------------------------------------------------------------- tcgen05
+// kind::f16: D f32, A and B bf16, M 128.
+__host__ __device__ constexpr uint32_t pp_idesc(int n, bool b_mn_major) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void pp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void pp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+// Descriptor of the value tile as an MN-major operand (dims contiguous): rows
+// (keys) of 128 bytes = 64 dims, 8-row groups 1024 bytes apart, the next 64
+// dims one half further.
+__device__ __forceinline__ uint64_t pp_desc_mn(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((128u * 128u) >> 4) << 16;  // leading byte offset: next 64 dims
+    d |= (uint64_t)(1024u >> 4) << 32;          // stride byte offset: next 8 keys
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;  // SWIZZLE_128B
+    return d;
+}
+#define PP_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define PP_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void pp_ld32(uint32_t addr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : PP_R8(r, 0), PP_R8(r, 8), PP_R8(r, 16), PP_R8(r, 24)
+        : "r"(addr));
+}
+__device__ __forceinline__ void pp_st32(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::PP_W8(r, 0),
+        PP_W8(r, 8), PP_W8(r, 16), PP_W8(r, 24), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void pp_ld16(uint32_t addr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : PP_R8(r, 0), PP_R8(r, 8)
+                 : "r"(addr));
+}
+__device__ __forceinline__ void pp_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PP_W8(
+                     r, 0),
+                 PP_W8(r, 8), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void pp_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pp_pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ void pp_cp16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void pp_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pp_cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void pp_sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// Byte offset of 16-byte chunk c (of DIM / 8) of row r in a swizzled tile.
+__device__ __forceinline__ uint32_t pp_off(int r, int c) {
+    return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// The reading side of the segment ring.
+struct PpReader {
+    const PpSeg *ring;
+    uint64_t *full, *empty;
+    uint32_t n = 0;
+    // Copies the next segment; every lane of the warp calls it. false: a wait ran out.
+    __device__ __forceinline__ bool next(PpSeg &s, unsigned *err) {
+        const uint32_t d = n % PP_SEG;
+        const bool ok = tc::mbar_wait(&full[d], (n / PP_SEG) & 1, err, 60);
+        s = ring[d];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&empty[d]);
+        ++n;
+        return __all_sync(0xffffffffu, ok);
+    }
+};
+
+template <bool KV8, int DIM>
+__global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnArgs a, PpWork w) {
+    using C = PpCfg<KV8, DIM>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ unsigned long long wsum[PP_WARPS], at_prefix;
+    __shared__ uint32_t at_seq;
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sbase = tc::smem_u32(sm);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BARS);
+    uint64_t *kv_full = bars, *kv_empty = kv_full + C::SLOTS, *sc_full = kv_empty + C::SLOTS, *sc_empty = sc_full + PP_SC;
+    uint64_t *seg_full = sc_empty + PP_SC, *seg_empty = seg_full + PP_SEG;
+    uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 4,
+             *o_full = q_full + 6, *mdone = q_full + 8;
+    uint32_t *slot_p = reinterpret_cast<uint32_t *>(sm + C::SLOT);
+    float *scales = reinterpret_cast<float *>(sm + C::SC);
+    uint32_t *masks = reinterpret_cast<uint32_t *>(sm + C::MASK);
+    PpSeg *ring = reinterpret_cast<PpSeg *>(sm + C::SEG);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_trigger();  // the join kernel waits for this one to end
+
+    if (tid == 0) {
+        for (int i = 0; i < C::SLOTS; ++i) {
+            tc::mbar_init(&kv_full[i], 4);
+            tc::mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < PP_SC; ++i) {
+            tc::mbar_init(&sc_full[i], 4);
+            tc::mbar_init(&sc_empty[i], 8);
+        }
+        for (int i = 0; i < PP_SEG; ++i) {
+            tc::mbar_init(&seg_full[i], 1);
+            tc::mbar_init(&seg_empty[i], 13);  // 4 loader warps, the MMA warp, 8 softmax warps
+        }
+        tc::mbar_init(q_full, 4);
+        tc::mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&s_full[i], 1);
+            tc::mbar_init(&p_ready[i], 128);
+            tc::mbar_init(&o_full[i], 1);
+        }
+        tc::mbar_init(mdone, 1);
+        tc::mbar_fence_init();
+    }
+    if (warp == 12) tc::tmem_alloc(slot_p, 512);
+
+    // ---- numbering of the units: a warp takes a run of sequences
+    const uint32_t per = (a.n + PP_WARPS - 1) / PP_WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
+    unsigned long long mine = 0;
+    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane(a, w, b, i1));
+    if (lane == 0) wsum[warp] = mine;
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *slot_p;
+    unsigned long long before = 0, all = 0;
+    for (int i = 0; i < PP_WARPS; ++i) {
+        if (i < warp) before += wsum[i];
+        all += wsum[i];
+    }
+    const PpSplit split(all * a.c.hkv, w.max_ctas);
+    const bool active = blockIdx.x < split.g && all > 0;
+    const unsigned long long u0 = split.start(blockIdx.x), u1 = split.start(blockIdx.x + 1);
+    if (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv) {
+        unsigned long long p = before;
+        for (uint32_t b = i0; b < i1; b += 32) {
+            uint32_t u = pp_units_lane(a, w, b, i1), x = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const bool here = (p + x - u) * a.c.hkv <= u0 && u0 < (p + x) * a.c.hkv;
+            if (here) {
+                at_seq = b + lane;
+                at_prefix = p + x - u;
+            }
+            if (__any_sync(0xffffffffu, here)) break;
+            p += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+    bool ok = true;
+
+    if (!active) {
+        // ---------------- nothing to compute
+        if (tid == 0) w.recs[blockIdx.x].valid = 0;
+    } else if (warp < 8) {
+        // ---------------- softmax: thread = row of tile `x`
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int x = warp >> 2, r = tid & 127;
+        const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 (warp % 4) ..
+        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM;
+        PpReader rd{ring, seg_full, seg_empty};
+        uint32_t bc = 0, ns = 0, no = 0;  // blocks of the CTA; scores and contexts of this tile
+        PpSeg g;
+        while (ok) {
+            ok = rd.next(g, w.err);
+            if (!ok || g.nblk == 0) break;
+            const uint32_t mt = g.m0 + 128 * x;  // this MMA tile's first flattened row
+            if (mt >= g.mrows) {                 // no rows: only let the scales go
+                for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
+                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sc_full[bc % PP_SC], (bc / PP_SC) & 1, w.err, 61));
+                    if (lane == 0) tc::mbar_arrive(&sc_empty[bc % PP_SC]);
+                }
+                continue;
+            }
+            const uint32_t m_row = mt + r, row_i = m_row / w.group;
+            const int pos = m_row < g.mrows ? g.pos0 + (int)row_i : -1;
+            const KeySpan ks = key_span(max(pos, 0), a.window, a.sinks);
+            const int first = pos < 0 ? 0 : ks.first, low = ks.low;
+            // keys seen by every row of the MMA tile: [0, all_first) and [all_low, all_last]
+            const uint32_t m_end = min(mt + 128, g.mrows) - 1;
+            const int all_last = m_end == mt + 127 ? g.pos0 + (int)(mt / w.group) : -1;
+            const int all_first = key_span(max(all_last, 0), a.window, a.sinks).first;
+            const int all_low = key_span(max(g.pos0 + (int)(m_end / w.group), 0), a.window, a.sinks).low;
+            float m = -INFINITY, l = 0.f;
+            for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
+                const int vb = g.b0 + i, kb = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
+                const uint32_t st = bc % PP_SC;
+                ok = tc::mbar_wait(&sc_full[st], (bc / PP_SC) & 1, w.err, 61) &&
+                     tc::mbar_wait(&s_full[x], ns & 1, w.err, 62);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++ns;
+                tc::tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) pp_ld32(s_addr + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
+                pp_ld_wait();
+                if constexpr (KV8) {
+                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float4 f = kf[j];
+                        unpk2(mul2(pk2(s[4 * j], s[4 * j + 1]), pk2(f.x, f.y)), s[4 * j], s[4 * j + 1]);
+                        unpk2(mul2(pk2(s[4 * j + 2], s[4 * j + 3]), pk2(f.z, f.w)), s[4 * j + 2], s[4 * j + 3]);
+                    }
+                }
+                const uint4 there = *reinterpret_cast<const uint4 *>(masks + 4 * st);
+                const bool full = kb + 127 <= all_last && (kb >= all_low || kb + 128 <= all_first) &&
+                                  (there.x & there.y & there.z & there.w) == 0xffffffffu;
+                if (!full) {
+                    const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        // bits of keys kb + 32 k ..: up to the row's position, from `low` on or before `first`
+                        auto below = [&](int e) {  // bits j with kb + 32 k + j < e
+                            const int n = e - (kb + 32 * k);
+                            return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+                        };
+                        const uint32_t bits = tw[k] & below(pos + 1) & (~below(low) | below(first));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(bits >> j & 1)) s[32 * k + j] = -INFINITY;
+                    }
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if constexpr (!KV8) top *= w.fac;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                    const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
+                    m = up;
+                    l *= f;
+                    if (i > 0) {  // this tile's earlier products are complete (s_full follows them)
+#pragma unroll
+                        for (int j = 0; j < DIM; j += 16) {
+                            uint32_t o[16];
+                            pp_ld16(o_addr + j, o);
+                            pp_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            pp_st16(o_addr + j, o);
+                        }
+                    }
+                }
+                const float mu = m == -INFINITY ? 0.f : m;
+                const unsigned long long nm = dup2(-mu), fc = dup2(w.fac);
+                unsigned long long sum[2] = {0ull, 0ull};
+                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int k = 64 * h + 2 * j;
+                        float e0, e1;
+                        if constexpr (KV8)
+                            unpk2(add2(pk2(s[k], s[k + 1]), nm), e0, e1);
+                        else
+                            unpk2(fma2(pk2(s[k], s[k + 1]), fc, nm), e0, e1);
+                        e0 = pp_ex2(e0);
+                        e1 = pp_ex2(e1);
+                        const unsigned long long e = pk2(e0, e1);
+                        sum[j & 1] = add2(sum[j & 1], e);
+                        if constexpr (KV8) {
+                            const float4 f = vf[k >> 2];
+                            unpk2(mul2(e, (k & 2) ? pk2(f.z, f.w) : pk2(f.x, f.y)), e0, e1);
+                        }
+                        p[j] = pp_pack(e0, e1);
+                    }
+                    pp_st32(s_addr + 32 * h, p);
+                }
+                float a0, a1;
+                unpk2(add2(sum[0], sum[1]), a0, a1);
+                l += a0 + a1;
+                pp_st_wait();
+                tc::tc_fence_before();
+                tc::mbar_arrive(&p_ready[x]);
+                if (lane == 0) tc::mbar_arrive(&sc_empty[st]);
+            }
+            if (!ok) break;
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], no & 1, w.err, 63));
+            if (!ok) break;
+            ++no;
+            tc::tc_fence_after();
+            const bool live = m_row < g.mrows && pos >= 0;
+            if (g.piece < 0) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                uint16_t *out = a.ctx + (g.row0 + (uint64_t)row_i) * a.ctx_stride +
+                                (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM;
+#pragma unroll
+                for (int j = 0; j < DIM; j += 32) {
+                    uint32_t o[32];
+                    pp_ld32(o_addr + j, o);
+                    pp_ld_wait();
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            uint4 v;
+                            v.x = pp_pack(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+                            v.y = pp_pack(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+                            v.z = pp_pack(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
+                            v.w = pp_pack(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
+                            if (l == 0.f) v = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4 *>(out + j + k) = v;
+                        }
+                    }
+                }
+            } else {
+                float *piece = w.pieces + (uint64_t)g.piece * C::PIECE;
+                const int t = 128 * x + r;
+                piece[t] = m;
+                piece[PP_TILE + t] = l;
+                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM;
+#pragma unroll
+                for (int j = 0; j < DIM; j += 32) {
+                    uint32_t o[32];
+                    pp_ld32(o_addr + j, o);
+                    pp_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4 *>(po + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+            }
+            tc::tc_fence_before();
+        }
+    } else if (warp < 12) {
+        // ---------------- loaders: warp lw takes rows 32 lw .. of each tile
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int lw = warp - 8;
+        constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
+        PpReader rd{ring, seg_full, seg_empty};
+        uint32_t bc = 0, nseg = 0, issued = 0, landed = 0;  // blocks; segments; K / V tiles begun and announced (bf16)
+        auto announce = [&](uint32_t n) {  // tiles up to n are in shared memory
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            for (; landed < n; ++landed)
+                if (lane == 0) tc::mbar_arrive(&kv_full[landed % C::SLOTS]);
+        };
+        PpSeg g;
+        while (ok) {
+            ok = rd.next(g, w.err);
+            if (!ok || g.nblk == 0) break;
+            const uint32_t *table = a.c.table + (uint64_t)g.seq * a.c.max_pages;
+            auto kb_of = [&](int i) {
+                const int vb = g.b0 + i;
+                return (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
+            };
+            auto seen = [&](int key) { return key <= g.last && (key >= g.low || key < g.first); };
+            auto page_of = [&](int i) {
+                const int key = kb_of(i) + 32 * lw + lane;
+                return i < g.nblk && seen(key) ? __ldg(&table[key >> a.c.tshift]) : PG_NO_PAGE;
+            };
+            uint32_t next = page_of(0);
+            // queries: flattened row m of the tile is row0 + m / group, head m % group of this KV head
+            if (nseg > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty, (nseg - 1) & 1, w.err, 64));
+            if (!ok) break;
+            ++nseg;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll 4
+                for (int j = 0; j < CPR; ++j) {
+                    const int n = j * 32 + lane, r = 32 * lw + n / CPR, c = n % CPR;
+                    const uint32_t mr = g.m0 + 128 * x + r;
+                    const bool live = mr < g.mrows;
+                    const uint64_t src = live ? (g.row0 + (uint64_t)(mr / w.group)) * a.q_stride +
+                                                    (uint64_t)(g.kvh * w.group + mr % w.group) * DIM + 8 * c
+                                              : 0;
+                    pp_cp16(sbase + C::Q + x * C::TILE_BYTES + pp_off(r, c), a.q + src, live ? 16 : 0);
+                }
+            }
+            pp_cp_commit();
+            pp_cp_wait<0>();
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(q_full);
+            for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
+                const uint32_t page = next;
+                next = page_of(i + 1);
+                const int key = kb_of(i) + 32 * lw + lane;
+                const bool vis = page < a.c.pages;
+                const uint64_t row = vis ? paged_row(a.c, page, g.kvh) + (key & ((1 << a.c.tshift) - 1)) : 0;
+                // scales and the mask of keys that are there
+                const uint32_t st = bc % PP_SC;
+                float ksc = 0.f, vsc = 0.f;
+                if constexpr (KV8) {
+                    if (vis) {
+                        ksc = __ldg(a.c.ks + row);
+                        vsc = __ldg(a.c.vs + row);
+                    }
+                }
+                const uint32_t bits = __ballot_sync(0xffffffffu, vis);
+                if (bc >= PP_SC)
+                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sc_empty[st], ((bc / PP_SC) & 1) ^ 1, w.err, 65));
+                if (!ok) break;
+                if constexpr (KV8) {
+                    scales[st * 256 + 32 * lw + lane] = w.negate ? -ksc * w.fac : ksc * w.fac;
+                    scales[st * 256 + 128 + 32 * lw + lane] = vsc;
+                }
+                if (lane == 0) masks[4 * st + lw] = bits;
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sc_full[st]);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint32_t slot = issued % C::SLOTS;
+                    const uint8_t *pool = kv ? a.c.v : a.c.k;
+                    const uint32_t dst = sbase + C::RING + slot * C::TILE_BYTES;
+                    if constexpr (KV8) {
+                        constexpr int NL = DIM / 16;  // 16-code chunks per row = loads per lane
+                        uint4 v[NL];
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            const int n = j * 32 + lane, rl = n / NL, c = n % NL;
+                            const uint64_t rr = __shfl_sync(0xffffffffu, row, rl);
+                            v[j] = bits >> rl & 1 ? ldg_stream(pool + rr * DIM + 16 * c) : make_uint4(0, 0, 0, 0);
+                        }
+                        if (issued >= C::SLOTS)
+                            ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_empty[slot], ((issued / C::SLOTS) & 1) ^ 1, w.err, 66));
+                        if (!ok) break;
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            const int n = j * 32 + lane, r = 32 * lw + n / NL, c = n % NL;
+                            // bytes (0, 1) and (2, 3) of each word as bf16 pairs
+                            uint32_t o[8];
+                            const uint32_t wd[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t lo = __byte_perm(wd[k], 0, 0x4140), hi = __byte_perm(wd[k], 0, 0x4342);
+                                o[2 * k] = bf16x2_sub(lop_or(lo, 0x007F007Fu, 0x43004300u), lop_or(lo, 0x00800080u, 0x43004300u));
+                                o[2 * k + 1] = bf16x2_sub(lop_or(hi, 0x007F007Fu, 0x43004300u), lop_or(hi, 0x00800080u, 0x43004300u));
+                            }
+                            pp_sts128(dst + pp_off(r, 2 * c), o[0], o[1], o[2], o[3]);
+                            pp_sts128(dst + pp_off(r, 2 * c + 1), o[4], o[5], o[6], o[7]);
+                        }
+                        ++issued;
+                        announce(issued);
+                    } else {
+                        if (issued >= C::SLOTS)
+                            ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_empty[slot], ((issued / C::SLOTS) & 1) ^ 1, w.err, 66));
+                        if (!ok) break;
+#pragma unroll
+                        for (int j = 0; j < CPR; ++j) {
+                            const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
+                            const uint64_t rr = __shfl_sync(0xffffffffu, row, rl);
+                            pp_cp16(dst + pp_off(32 * lw + rl, c), pool + rr * (2 * DIM) + 16 * c, bits >> rl & 1 ? 16 : 0);
+                        }
+                        pp_cp_commit();
+                        ++issued;
+                        // announced two tiles behind; a wait for a free slot only needs tiles SLOTS back
+                        if (issued - landed > 2) {
+                            pp_cp_wait<2>();
+                            announce(issued - 2);
+                        }
+                    }
+                }
+            }
+            if constexpr (!KV8) {  // before waiting for anything of the next segment
+                pp_cp_wait<0>();
+                if (ok) announce(issued);
+            }
+        }
+        pp_cp_wait<0>();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12) {
+            // ---------------- MMA issuer
+            PpReader rd{ring, seg_full, seg_empty};
+            uint32_t bc = 0, nseg = 0, np[2] = {0, 0};
+            const uint32_t id_qk = pp_idesc(128, false) | (!KV8 && w.negate ? 1u << 13 : 0u);
+            constexpr uint32_t id_pv = pp_idesc(DIM, true);
+            PpSeg g;
+            while (ok) {
+                ok = rd.next(g, w.err);
+                if (!ok || g.nblk == 0) break;
+                if (lane == 0) {
+                    const int tiles = g.m0 + 128 < g.mrows ? 2 : 1;
+                    auto tile_at = [&](uint32_t n) { return sbase + C::RING + (n % C::SLOTS) * C::TILE_BYTES; };
+                    auto wait_tile = [&](uint32_t n) {
+                        return tc::mbar_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
+                    };
+                    auto qk = [&](int x, uint32_t n) {
+                        const uint32_t qa = sbase + C::Q + x * C::TILE_BYTES, ka = tile_at(n);
+#pragma unroll
+                        for (int j = 0; j < DIM / 16; ++j) {
+                            const uint32_t off = (j >> 2) * (128 * 128) + (j & 3) * 32;
+                            pp_mma_ss(tmem + 128 * x, tc::smem_desc_sw128(qa + off), tc::smem_desc_sw128(ka + off), id_qk, j > 0);
+                        }
+                        tc::mma_commit(&s_full[x]);
+                    };
+                    ok = tc::mbar_wait(q_full, nseg & 1, w.err, 68) && wait_tile(2 * bc);
+                    if (ok) {
+                        tc::tc_fence_after();
+                        for (int x = 0; x < tiles; ++x) qk(x, 2 * bc);
+                        tc::mma_commit(&kv_empty[2 * bc % C::SLOTS]);
+                        if (g.nblk == 1) tc::mma_commit(q_empty);
+                    }
+                    for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
+                        const bool more = i + 1 < g.nblk;
+                        for (int x = 0; x < tiles && ok; ++x) {
+                            ok = tc::mbar_wait(&p_ready[x], np[x]++ & 1, w.err, 69) && (x > 0 || wait_tile(2 * bc + 1));
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            const uint32_t va = tile_at(2 * bc + 1);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, pp_desc_mn(va + j * 2048), id_pv,
+                                          i > 0 || j > 0);
+                            if (x == tiles - 1) tc::mma_commit(&kv_empty[(2 * bc + 1) % C::SLOTS]);
+                            if (more) {
+                                if (x == 0) ok = wait_tile(2 * bc + 2);
+                                if (!ok) break;
+                                tc::tc_fence_after();
+                                qk(x, 2 * bc + 2);
+                                if (x == tiles - 1) {
+                                    tc::mma_commit(&kv_empty[(2 * bc + 2) % C::SLOTS]);
+                                    if (i + 2 == g.nblk) tc::mma_commit(q_empty);
+                                }
+                            } else {
+                                tc::mma_commit(&o_full[x]);
+                            }
+                        }
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                bc = __shfl_sync(0xffffffffu, bc, 0);
+                ++nseg;
+            }
+            // every MMA is complete before TMEM is freed
+            if (lane == 0) {
+                tc::mma_commit(mdone);
+                tc::mbar_wait(mdone, 0, w.err, 69);
+            }
+            __syncwarp();
+        } else if (warp == 13) {
+            // ---------------- segments
+            uint32_t n = 0;
+            uint32_t i = at_seq;
+            unsigned long long u = u0, base = at_prefix * a.c.hkv;  // units before sequence i
+            bool first_segment = true;
+            if (lane == 0) w.recs[blockIdx.x].valid = 0;
+            while (ok) {
+                const uint32_t d = n % PP_SEG;
+                PpSeg g = {};
+                if (u < u1) {
+                    const PpSeqInfo s = pp_seq(a, w, i);
+                    const uint32_t units = pp_units_warp(a, w, s.pos0, s.mrows, s.nt);
+                    if (units == 0 || u >= base + (unsigned long long)units * a.c.hkv) {
+                        base += (unsigned long long)units * a.c.hkv;
+                        ++i;
+                        continue;
+                    }
+                    const uint32_t kvh = (uint32_t)((u - base) / units), off = (uint32_t)((u - base) % units);
+                    // the tile that holds unit `off` of this KV head
+                    uint32_t seen = 0;
+                    int k = 0, b0 = 0;
+                    PpBlocks bl = {};
+                    for (int kb = 0;; kb += 32) {
+                        const PpBlocks mine_b = pp_blocks(a, w, s.pos0, s.mrows, min(kb + lane, s.nt - 1));
+                        const uint32_t cnt = kb + lane < s.nt ? mine_b.n : 0;
+                        uint32_t xs = cnt;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const uint32_t y = __shfl_up_sync(0xffffffffu, xs, o);
+                            if (lane >= o) xs += y;
+                        }
+                        const uint32_t hit = __ballot_sync(0xffffffffu, seen + xs > off);
+                        if (hit || kb + 32 >= s.nt) {
+                            const int l = hit ? __ffs(hit) - 1 : 31;
+                            k = kb + l;
+                            b0 = (int)(off - (seen + __shfl_sync(0xffffffffu, xs - cnt, l)));
+                            break;
+                        }
+                        seen += __shfl_sync(0xffffffffu, xs, 31);
+                    }
+                    // this tile and those behind it in the KV head: one segment each
+                    bool more = true;
+                    while (more && ok) {
+                        bl = pp_blocks(a, w, s.pos0, s.mrows, k);
+                        const int cnt = (int)min((unsigned long long)(bl.n - b0), u1 - u);
+                        if (cnt > 0) {
+                            g.seq = s.seq;
+                            g.row0 = s.row0;
+                            g.m0 = (uint32_t)k * PP_TILE;
+                            g.mrows = s.mrows;
+                            g.pos0 = s.pos0;
+                            g.kvh = kvh;
+                            g.b0 = b0;
+                            g.nblk = cnt;
+                            g.s128 = bl.s128;
+                            g.low128 = bl.low128;
+                            g.first = bl.first;
+                            g.low = bl.low;
+                            g.last = bl.last;
+                            g.piece = cnt == bl.n ? -1 : (int)(2 * blockIdx.x + (first_segment ? 0 : 1));
+                            const uint32_t dd = n % PP_SEG;
+                            if (n >= PP_SEG)
+                                ok = __all_sync(0xffffffffu, tc::mbar_wait(&seg_empty[dd], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
+                            if (!ok) break;
+                            if (lane == 0) {
+                                ring[dd] = g;
+                                tc::mbar_arrive(&seg_full[dd]);
+                            }
+                            __syncwarp();
+                            ++n;
+                            if (first_segment && b0 > 0 && lane == 0) {
+                                PpRec rec = {};
+                                const unsigned long long t0 = u - b0;
+                                rec.valid = 1;
+                                rec.row0 = s.row0;
+                                rec.m0 = g.m0;
+                                rec.mrows = s.mrows;
+                                rec.kvh = kvh;
+                                rec.pos0 = s.pos0;
+                                rec.c0 = split.cta_of(t0);
+                                rec.c1 = split.cta_of(t0 + bl.n - 1);
+                                rec.slot0 = split.start(rec.c0) < t0;
+                                w.recs[blockIdx.x] = rec;
+                            }
+                            first_segment = false;
+                            u += cnt;
+                        }
+                        ++k;
+                        b0 = 0;
+                        more = u < u1 && k < s.nt;
+                    }
+                    continue;
+                }
+                if (n >= PP_SEG) ok = __all_sync(0xffffffffu, tc::mbar_wait(&seg_empty[d], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
+                if (ok && lane == 0) {
+                    ring[d] = g;  // nblk 0: the end
+                    tc::mbar_arrive(&seg_full[d]);
+                }
+                break;
+            }
+        }
+    }
+    if (warp == 14) {
+        // ---------------- rows in front of the first token, and of no sequence
+        for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+            const PpSeqInfo s = pp_seq(a, w, i);
+            const uint32_t nrows = s.mrows / w.group, zero = s.pos0 >= 0 ? 0 : min((uint32_t)-s.pos0, nrows);
+            const uint32_t chunks = a.qh * (DIM / 8);
+            for (uint32_t r = 0; r < zero; ++r)
+                for (uint32_t c = lane; c < chunks; c += 32)
+                    *reinterpret_cast<uint4 *>(a.ctx + (s.row0 + (uint64_t)r) * a.ctx_stride + 8 * c) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+// Tiles that several CTAs share. Block (c, y): 32 rows of the tile in whose
+// middle CTA c starts, if c is the tile's second CTA; 8 threads per row.
+template <int DIM>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(PagedAttnArgs a, PpWork w) {
+    constexpr int PIECE = 2 * PP_TILE + PP_TILE * DIM, PER = DIM / 8;
+    pdl_wait();
+    const PpRec rec = w.recs[blockIdx.x];
+    if (!rec.valid || rec.c0 + 1 != blockIdx.x) return;
+    const uint32_t t = blockIdx.y * 32 + threadIdx.x / 8, d0 = (threadIdx.x % 8) * PER, m = rec.m0 + t;
+    if (m >= rec.mrows || rec.pos0 + (int)(m / w.group) < 0) return;
+    const uint32_t n = rec.c1 - rec.c0 + 1;
+    auto piece = [&](uint32_t i) { return w.pieces + ((uint64_t)(rec.c0 + i) * 2 + (i == 0 ? rec.slot0 : 0)) * PIECE; };
+    float M = -INFINITY, L = 0.f, O[PER];
+    for (uint32_t i = 0; i < n; ++i) M = fmaxf(M, piece(i)[t]);
+    const float M0 = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) O[j] = 0.f;
+#pragma unroll 2
+    for (uint32_t i = 0; i < n; ++i) {
+        const float *p = piece(i);
+        const float f = pp_ex2(p[t] - M0);
+        L += p[PP_TILE + t] * f;
+        const float4 *o = reinterpret_cast<const float4 *>(p + 2 * PP_TILE + (uint64_t)t * DIM + d0);
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) {
+            const float4 v = o[j];
+            O[4 * j] += v.x * f;
+            O[4 * j + 1] += v.y * f;
+            O[4 * j + 2] += v.z * f;
+            O[4 * j + 3] += v.w * f;
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint16_t *out = a.ctx + (rec.row0 + (uint64_t)(m / w.group)) * a.ctx_stride +
+                    (uint64_t)(rec.kvh * w.group + m % w.group) * DIM + d0;
+#pragma unroll
+    for (int j = 0; j < PER; j += 8) {
+        uint4 v = make_uint4(pp_pack(O[j] * inv, O[j + 1] * inv), pp_pack(O[j + 2] * inv, O[j + 3] * inv),
+                             pp_pack(O[j + 4] * inv, O[j + 5] * inv), pp_pack(O[j + 6] * inv, O[j + 7] * inv));
+        if (L == 0.f) v = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4 *>(out + j) = v;
+    }
+}
+
+size_t paged_prefill_ws(uint32_t, uint32_t, uint32_t dim, uint32_t, uint32_t) {
+    return 256 + (size_t)PP_MAX_SMS * (sizeof(PpRec) + 2 * (2 * PP_TILE + PP_TILE * (size_t)dim) * 4);
+}
+
+template <bool KV8, int DIM>
+static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t st) {
+    using C = PpCfg<KV8, DIM>;
+    auto *kernel = paged_prefill_kernel<KV8, DIM>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::ALLOC) != cudaSuccess) return -3;
+    PdlChain chain;
+    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PF_THREADS), C::ALLOC, st, 1, a, w)) return rc;
+    return launch_pdl(paged_prefill_join_kernel<DIM>, dim3(w.max_ctas, PP_TILE / 32), dim3(256), 0, st, 1, a, w);
+}
+
+int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
+    const int sms = paged_sms();
+    if (sms <= 0) return -3;
+    PpWork w;
+    w.group = a.qh / a.c.hkv;
+    w.max_ctas = (uint32_t)(sms < PP_MAX_SMS ? sms : PP_MAX_SMS);
+    w.negate = a.scale < 0.f;
+    const float f = fabsf(a.scale) * 1.44269504f;
+    w.fac = f > 1e-30f ? f : 1e-30f;  // a scale of 0 leaves masked scores at -inf
+    w.err = (unsigned *)ws;
+    w.recs = reinterpret_cast<PpRec *>((char *)ws + 256);
+    w.pieces = reinterpret_cast<float *>((char *)ws + 256 + PP_MAX_SMS * sizeof(PpRec));
+    if (a.format == QWEN_B200_KV8)
+        return a.dim == 64 ? launch_prefill<true, 64>(a, w, st) : launch_prefill<true, 128>(a, w, st);
+    return a.dim == 64 ? launch_prefill<false, 64>(a, w, st) : launch_prefill<false, 128>(a, w, st);
+}
+
+}  // namespace qb
