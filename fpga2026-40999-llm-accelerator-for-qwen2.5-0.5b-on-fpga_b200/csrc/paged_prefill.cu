@@ -22,26 +22,28 @@
 // tile that two or more CTAs share is joined by a second kernel (at most two
 // pieces per CTA, fp32, added in CTA order).
 //
-// Warps (512 threads, one CTA per SM, registers moved to the softmax warps):
-//   0-3, 4-7  softmax of the first / second MMA tile, one thread per row:
+// Warps (768 threads, one CTA per SM, registers moved to the softmax warps):
+//   0-7, 8-15 softmax of the first / second MMA tile, two threads per row (64
+//             keys each, which fit their registers; one thread with all 128
+//             ran at a third of the rate, waiting for instructions and latencies):
 //             scores from TMEM, weights back over the scores' columns
-//   8-11      loaders: queries and bf16 rows by cp.async (zero-filled where a
+//   16-19     loaders: queries and bf16 rows by cp.async (zero-filled where a
 //             key is not visible, so garbage never reaches the products), KV8 rows
 //             through registers; 128-byte swizzled K-major tiles, the value
 //             tile read as an MN-major operand
-//   12        one thread issues the MMAs; while one tile's softmax runs, the
+//   20        one thread issues the MMAs; while one tile's softmax runs, the
 //             other's products do
-//   13        walks the units and publishes segments (tile, KV head, block range)
-//   14        zeroes the rows in front of a sequence's first token
+//   21        walks the units and publishes segments (tile, KV head, block range)
+//   22        zeroes the rows in front of a sequence's first token
 // Bound by the exponentials at 64 dims (16 per clock and SM) and by the tensor
-// cores at 128. Every wait is bounded (error codes 60-69).
+// cores at 128. Every wait is bounded (error codes 59-69).
 #include "kernels.h"
 #include "paged.cuh"
 #include "tc05.cuh"
 
 namespace qb {
 
-constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 512, PP_WARPS = PF_THREADS / 32;
+constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 768, PP_WARPS = PF_THREADS / 32;
 constexpr int PP_MAX_SMS = 192;
 constexpr uint32_t PP_MIN_UNITS = 4;  // blocks a CTA takes at least: less and the join costs more than the split saves
 constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
@@ -55,9 +57,10 @@ struct PpCfg {
     static constexpr int Q = 0, RING = 2 * TILE_BYTES;
     static constexpr int SC = RING + SLOTS * TILE_BYTES;   // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
     static constexpr int MASK = SC + PP_SC * 256 * 4;
-    static constexpr int SEG = MASK + PP_SC * 16;
+    static constexpr int XCH = MASK + PP_SC * 16;          // [2 tiles][2 halves][128 rows] floats
+    static constexpr int SEG = XCH + 2 * 2 * 128 * 4;
     static constexpr int BARS = SEG + PP_SEG * 64;
-    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 8;
     static constexpr int SLOT = BARS + NBARS * 8;
     static constexpr int TOTAL = SLOT + 16;
     static constexpr int ALLOC = TOTAL + 1024;
@@ -255,6 +258,16 @@ __device__ __forceinline__ uint32_t pp_off(int r, int c) {
     return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// One lane of a converged warp. A branch on its result is known to the compiler to
+// be taken by one thread, so that tcgen05 instructions inside it take their
+// operands from uniform registers directly; under `lane == 0` each of
+// them cost 110-150 cycles of issue (half of the kernel's time).
+__device__ __forceinline__ bool pp_elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // The reading side of the segment ring.
 struct PpReader {
     const PpSeg *ring;
@@ -299,23 +312,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
         }
         for (int i = 0; i < PP_SC; ++i) {
             tc::mbar_init(&sc_full[i], 4);
-            tc::mbar_init(&sc_empty[i], 8);
+            tc::mbar_init(&sc_empty[i], 16);
         }
         for (int i = 0; i < PP_SEG; ++i) {
             tc::mbar_init(&seg_full[i], 1);
-            tc::mbar_init(&seg_empty[i], 13);  // 4 loader warps, the MMA warp, 8 softmax warps
+            tc::mbar_init(&seg_empty[i], 21);  // 4 loader warps, the MMA warp, 16 softmax warps
         }
         tc::mbar_init(q_full, 4);
         tc::mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
-            tc::mbar_init(&p_ready[i], 128);
+            tc::mbar_init(&p_ready[i], 256);
             tc::mbar_init(&o_full[i], 1);
         }
         tc::mbar_init(mdone, 1);
+        for (int i = 0; i < 8; ++i) tc::mbar_init(mdone + 1 + i, 2);  // pairs of softmax warps
         tc::mbar_fence_init();
     }
-    if (warp == 12) tc::tmem_alloc(slot_p, 512);
+    if (warp == 20) tc::tmem_alloc(slot_p, 512);
 
     // ---- numbering of the units: a warp takes a run of sequences
     const uint32_t per = (a.n + PP_WARPS - 1) / PP_WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
@@ -358,12 +372,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
     if (!active) {
         // ---------------- nothing to compute
         if (tid == 0) w.recs[blockIdx.x].valid = 0;
-    } else if (warp < 8) {
-        // ---------------- softmax: thread = row of tile `x`
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        const int x = warp >> 2, r = tid & 127;
+    } else if (warp < 16) {
+        // ---------------- softmax: thread = row r of tile `x`, keys 64 hf .. of each block
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+        const int x = warp >> 3, hf = (warp >> 2) & 1, r = tid & 127;
+        float *xch = reinterpret_cast<float *>(sm + C::XCH) + x * 256;
+        uint64_t *pair = mdone + 1 + x * 4 + (warp & 3);  // this warp and the one with the rows' other keys
+        uint32_t np = 0;
+        auto pair_sync = [&] {
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(pair);
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(pair, np++ & 1, w.err, 59));
+        };
         const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 (warp % 4) ..
-        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM;
+        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM + hf * (DIM / 2);
         PpReader rd{ring, seg_full, seg_empty};
         uint32_t bc = 0, ns = 0, no = 0;  // blocks of the CTA; scores and contexts of this tile
         PpSeg g;
@@ -397,14 +419,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 if (!ok) break;
                 ++ns;
                 tc::tc_fence_after();
-                float s[128];
+                float s[64];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) pp_ld32(s_addr + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
+                for (int j = 0; j < 2; ++j) pp_ld32(s_addr + 64 * hf + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
                 pp_ld_wait();
                 if constexpr (KV8) {
-                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256);
+                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256 + 64 * hf);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
+                    for (int j = 0; j < 16; ++j) {
                         const float4 f = kf[j];
                         unpk2(mul2(pk2(s[4 * j], s[4 * j + 1]), pk2(f.x, f.y)), s[4 * j], s[4 * j + 1]);
                         unpk2(mul2(pk2(s[4 * j + 2], s[4 * j + 3]), pk2(f.z, f.w)), s[4 * j + 2], s[4 * j + 3]);
@@ -414,12 +436,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 const bool full = kb + 127 <= all_last && (kb >= all_low || kb + 128 <= all_first) &&
                                   (there.x & there.y & there.z & there.w) == 0xffffffffu;
                 if (!full) {
-                    const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
+                    const uint32_t tw[2] = {hf ? there.z : there.x, hf ? there.w : there.y};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // bits of keys kb + 32 k ..: up to the row's position, from `low` on or before `first`
-                        auto below = [&](int e) {  // bits j with kb + 32 k + j < e
-                            const int n = e - (kb + 32 * k);
+                    for (int k = 0; k < 2; ++k) {
+                        // bits of 32 keys from k0: up to the row's position, from `low` on or before `first`
+                        const int k0 = kb + 64 * hf + 32 * k;
+                        auto below = [&](int e) {  // bits j with k0 + j < e
+                            const int n = e - k0;
                             return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
                         };
                         const uint32_t bits = tw[k] & below(pos + 1) & (~below(low) | below(first));
@@ -430,16 +453,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+                for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if constexpr (!KV8) top *= w.fac;
+                // the row's other half; both halves have read their scores by then, so weights may overwrite them
+                xch[128 * hf + r] = top;
+                pair_sync();
+                if (!ok) break;
+                top = fmaxf(top, xch[128 * (hf ^ 1) + r]);
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
                     m = up;
                     l *= f;
                     if (i > 0) {  // this tile's earlier products are complete (s_full follows them)
-#pragma unroll
-                        for (int j = 0; j < DIM; j += 16) {
+#pragma unroll 1
+                        for (int j = 0; j < DIM / 2; j += 16) {
                             uint32_t o[16];
                             pp_ld16(o_addr + j, o);
                             pp_ld_wait();
@@ -452,30 +480,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 const float mu = m == -INFINITY ? 0.f : m;
                 const unsigned long long nm = dup2(-mu), fc = dup2(w.fac);
                 unsigned long long sum[2] = {0ull, 0ull};
-                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128);
+                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128 + 64 * hf);
+                uint32_t p[32];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int k = 64 * h + 2 * j;
-                        float e0, e1;
-                        if constexpr (KV8)
-                            unpk2(add2(pk2(s[k], s[k + 1]), nm), e0, e1);
-                        else
-                            unpk2(fma2(pk2(s[k], s[k + 1]), fc, nm), e0, e1);
-                        e0 = pp_ex2(e0);
-                        e1 = pp_ex2(e1);
-                        const unsigned long long e = pk2(e0, e1);
-                        sum[j & 1] = add2(sum[j & 1], e);
-                        if constexpr (KV8) {
-                            const float4 f = vf[k >> 2];
-                            unpk2(mul2(e, (k & 2) ? pk2(f.z, f.w) : pk2(f.x, f.y)), e0, e1);
-                        }
-                        p[j] = pp_pack(e0, e1);
+                for (int j = 0; j < 32; ++j) {
+                    const int k = 2 * j;
+                    float e0, e1;
+                    if constexpr (KV8)
+                        unpk2(add2(pk2(s[k], s[k + 1]), nm), e0, e1);
+                    else
+                        unpk2(fma2(pk2(s[k], s[k + 1]), fc, nm), e0, e1);
+                    e0 = pp_ex2(e0);
+                    e1 = pp_ex2(e1);
+                    const unsigned long long e = pk2(e0, e1);
+                    sum[j & 1] = add2(sum[j & 1], e);
+                    if constexpr (KV8) {
+                        const float4 f = vf[k >> 2];
+                        unpk2(mul2(e, (k & 2) ? pk2(f.z, f.w) : pk2(f.x, f.y)), e0, e1);
                     }
-                    pp_st32(s_addr + 32 * h, p);
+                    p[j] = pp_pack(e0, e1);
                 }
+                pp_st32(s_addr + 32 * hf, p);
                 float a0, a1;
                 unpk2(add2(sum[0], sum[1]), a0, a1);
                 l += a0 + a1;
@@ -490,18 +515,23 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
             ++no;
             tc::tc_fence_after();
             const bool live = m_row < g.mrows && pos >= 0;
+            xch[128 * hf + r] = l;
+            pair_sync();
+            l += xch[128 * (hf ^ 1) + r];
+            pair_sync();  // read before the next segment's maxima are written
+            if (!ok) break;
             if (g.piece < 0) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 uint16_t *out = a.ctx + (g.row0 + (uint64_t)row_i) * a.ctx_stride +
-                                (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM;
-#pragma unroll
-                for (int j = 0; j < DIM; j += 32) {
-                    uint32_t o[32];
-                    pp_ld32(o_addr + j, o);
+                                (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM + hf * (DIM / 2);
+#pragma unroll 1
+                for (int j = 0; j < DIM / 2; j += 16) {
+                    uint32_t o[16];
+                    pp_ld16(o_addr + j, o);
                     pp_ld_wait();
                     if (live) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
+                        for (int k = 0; k < 16; k += 8) {
                             uint4 v;
                             v.x = pp_pack(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
                             v.y = pp_pack(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
@@ -515,25 +545,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
             } else {
                 float *piece = w.pieces + (uint64_t)g.piece * C::PIECE;
                 const int t = 128 * x + r;
-                piece[t] = m;
-                piece[PP_TILE + t] = l;
-                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM;
-#pragma unroll
-                for (int j = 0; j < DIM; j += 32) {
-                    uint32_t o[32];
-                    pp_ld32(o_addr + j, o);
+                if (hf == 0) {
+                    piece[t] = m;
+                    piece[PP_TILE + t] = l;
+                }
+                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM + hf * (DIM / 2);
+#pragma unroll 1
+                for (int j = 0; j < DIM / 2; j += 16) {
+                    uint32_t o[16];
+                    pp_ld16(o_addr + j, o);
                     pp_ld_wait();
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
+                    for (int k = 0; k < 16; k += 4)
                         *reinterpret_cast<uint4 *>(po + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                 }
             }
             tc::tc_fence_before();
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ---------------- loaders: warp lw takes rows 32 lw .. of each tile
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int lw = warp - 8;
+        const int lw = warp - 16;
         constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
         PpReader rd{ring, seg_full, seg_empty};
         uint32_t bc = 0, nseg = 0, issued = 0, landed = 0;  // blocks; segments; K / V tiles begun and announced (bf16)
@@ -668,58 +700,57 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
         pp_cp_wait<0>();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12) {
+        if (warp == 20) {
             // ---------------- MMA issuer
             PpReader rd{ring, seg_full, seg_empty};
             uint32_t bc = 0, nseg = 0, np[2] = {0, 0};
             const uint32_t id_qk = pp_idesc(128, false) | (!KV8 && w.negate ? 1u << 13 : 0u);
             constexpr uint32_t id_pv = pp_idesc(DIM, true);
+            const uint64_t q_desc = tc::smem_desc_sw128(sbase + C::Q), k_desc = tc::smem_desc_sw128(sbase + C::RING),
+                           v_desc = pp_desc_mn(sbase + C::RING);
             PpSeg g;
             while (ok) {
                 ok = rd.next(g, w.err);
                 if (!ok || g.nblk == 0) break;
-                if (lane == 0) {
-                    const int tiles = g.m0 + 128 < g.mrows ? 2 : 1;
-                    auto tile_at = [&](uint32_t n) { return sbase + C::RING + (n % C::SLOTS) * C::TILE_BYTES; };
+                const int tiles = g.m0 + 128 < g.mrows ? 2 : 1;
+                if (pp_elect()) {
                     auto wait_tile = [&](uint32_t n) {
                         return tc::mbar_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
                     };
+                    // descriptors differ in their address field only: bases once, steps by adding
                     auto qk = [&](int x, uint32_t n) {
-                        const uint32_t qa = sbase + C::Q + x * C::TILE_BYTES, ka = tile_at(n);
-#pragma unroll
+                        const uint64_t qd = q_desc + x * (C::TILE_BYTES >> 4), kd = k_desc + (n % C::SLOTS) * (C::TILE_BYTES >> 4);
+#pragma unroll 1
                         for (int j = 0; j < DIM / 16; ++j) {
-                            const uint32_t off = (j >> 2) * (128 * 128) + (j & 3) * 32;
-                            pp_mma_ss(tmem + 128 * x, tc::smem_desc_sw128(qa + off), tc::smem_desc_sw128(ka + off), id_qk, j > 0);
+                            const uint32_t off = ((j >> 2) * (128 * 128) + (j & 3) * 32) >> 4;
+                            pp_mma_ss(tmem + 128 * x, qd + off, kd + off, id_qk, j > 0);
                         }
                         tc::mma_commit(&s_full[x]);
                     };
-                    ok = tc::mbar_wait(q_full, nseg & 1, w.err, 68) && wait_tile(2 * bc);
-                    if (ok) {
-                        tc::tc_fence_after();
-                        for (int x = 0; x < tiles; ++x) qk(x, 2 * bc);
-                        tc::mma_commit(&kv_empty[2 * bc % C::SLOTS]);
-                        if (g.nblk == 1) tc::mma_commit(q_empty);
-                    }
-                    for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
-                        const bool more = i + 1 < g.nblk;
+                    ok = tc::mbar_wait(q_full, nseg & 1, w.err, 68);
+                    // block i: the weights' product of block i - 1, then the scores of block i
+                    for (int i = 0; i <= g.nblk && ok; ++i) {
+                        const uint32_t kt = 2 * (bc + i);
                         for (int x = 0; x < tiles && ok; ++x) {
-                            ok = tc::mbar_wait(&p_ready[x], np[x]++ & 1, w.err, 69) && (x > 0 || wait_tile(2 * bc + 1));
-                            if (!ok) break;
-                            tc::tc_fence_after();
-                            const uint32_t va = tile_at(2 * bc + 1);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, pp_desc_mn(va + j * 2048), id_pv,
-                                          i > 0 || j > 0);
-                            if (x == tiles - 1) tc::mma_commit(&kv_empty[(2 * bc + 1) % C::SLOTS]);
-                            if (more) {
-                                if (x == 0) ok = wait_tile(2 * bc + 2);
+                            const bool final = x == tiles - 1;
+                            if (i > 0) {
+                                ok = tc::mbar_wait(&p_ready[x], (np[x] + i - 1) & 1, w.err, 69) && (x > 0 || wait_tile(kt - 1));
                                 if (!ok) break;
                                 tc::tc_fence_after();
-                                qk(x, 2 * bc + 2);
-                                if (x == tiles - 1) {
-                                    tc::mma_commit(&kv_empty[(2 * bc + 2) % C::SLOTS]);
-                                    if (i + 2 == g.nblk) tc::mma_commit(q_empty);
+                                uint64_t vd = v_desc + ((kt - 1) % C::SLOTS) * (C::TILE_BYTES >> 4);
+#pragma unroll 1
+                                for (int j = 0; j < 8; ++j, vd += 2048 >> 4)
+                                    pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, vd, id_pv, i > 1 || j > 0);
+                                if (final) tc::mma_commit(&kv_empty[(kt - 1) % C::SLOTS]);
+                            }
+                            if (i < g.nblk) {
+                                if (x == 0) ok = wait_tile(kt);
+                                if (!ok) break;
+                                tc::tc_fence_after();
+                                qk(x, kt);
+                                if (final) {
+                                    tc::mma_commit(&kv_empty[kt % C::SLOTS]);
+                                    if (i + 1 == g.nblk) tc::mma_commit(q_empty);
                                 }
                             } else {
                                 tc::mma_commit(&o_full[x]);
@@ -728,7 +759,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
-                bc = __shfl_sync(0xffffffffu, bc, 0);
+                bc += g.nblk;
+                np[0] += g.nblk;
+                if (tiles == 2) np[1] += g.nblk;
                 ++nseg;
             }
             // every MMA is complete before TMEM is freed
@@ -737,7 +770,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 tc::mbar_wait(mdone, 0, w.err, 69);
             }
             __syncwarp();
-        } else if (warp == 13) {
+        } else if (warp == 21) {
             // ---------------- segments
             uint32_t n = 0;
             uint32_t i = at_seq;
@@ -840,7 +873,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
             }
         }
     }
-    if (warp == 14) {
+    if (warp == 22) {
         // ---------------- rows in front of the first token, and of no sequence
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
             const PpSeqInfo s = pp_seq(a, w, i);
@@ -853,7 +886,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
