@@ -983,6 +983,22 @@ int make_kcache_map(CUtensorMap *map, const int8_t *kc, long long rows) {
     return r == CUDA_SUCCESS ? 0 : -3;
 }
 
+// Page map of a bf16 paged cache (paged_prefill.cu): [page][head, token][dim],
+// box of 64 dims x `box_rows` tokens of one page, 128-byte swizzle.
+int make_page_map(CUtensorMap *map, const void *pool, int dim, uint64_t rows_per_page, uint64_t pages,
+                  uint64_t page_stride_bytes, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return -3;
+    cuuint64_t dims[3] = {(cuuint64_t)dim, rows_per_page, pages};
+    cuuint64_t strides[2] = {(cuuint64_t)dim * 2, page_stride_bytes};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    cuuint32_t es[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(pool), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -3;
+}
+
 // Limb map: limbs[l][row][k] int8 (plane bytes apart, rows ld bytes apart,
 // rows_alloc rows), box [4][64 rows][128 k], 128-byte swizzle; rows past
 // rows_alloc read as zero.

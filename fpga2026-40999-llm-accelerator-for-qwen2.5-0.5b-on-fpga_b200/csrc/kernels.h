@@ -160,6 +160,8 @@ int attention_tile_plan(int rows, const uint32_t *slots, const uint32_t *positio
 int launch_attention_tiles(const CUtensorMap &kmap, long long krow0, const AtTile *d_tiles, const AtGroup &grp,
                            const uint16_t *q, const int8_t *vc, const float *ks, const float *vs, int cap,
                            uint16_t *ctx, unsigned *err, cudaStream_t st);
+int make_page_map(CUtensorMap *map, const void *pool, int dim, uint64_t rows_per_page, uint64_t pages,
+                  uint64_t page_stride_bytes, int box_rows);
 int make_kcache_map(CUtensorMap *map, const int8_t *kc, long long rows);
 // The engine's RTL KV mode (kv8_rtl.cu): kv [rows][256] post-RoPE k | v (bf16)
 // appended in the accelerator's K16 and V formats into one layer's caches:

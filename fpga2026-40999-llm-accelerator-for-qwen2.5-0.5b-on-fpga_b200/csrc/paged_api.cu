@@ -24,7 +24,7 @@ int paged_check(const qwen_b200_paged_kv *kv) {
         return QWEN_B200_EINVAL;
     // pages of one layer and layers of one page apart: one of the two strides
     // spans the other's whole range
-    const uint64_t block = (uint64_t)kv->kv_heads * t, most = 1ull << 40;
+    const uint64_t block = (uint64_t)kv->kv_heads * t, most = 1ull << 32;  // strides below 2^40 bytes (tensor maps)
     if ((kv->layer_stride | kv->page_stride) & 15) return QWEN_B200_EINVAL;
     if (kv->layer_stride > most || kv->page_stride > most) return QWEN_B200_EINVAL;
     if (kv->pages > 1 && kv->page_stride < block) return QWEN_B200_EINVAL;

@@ -27,16 +27,17 @@
 //             keys each, which fit their registers; one thread with all 128
 //             ran at a third of the rate, waiting for instructions and latencies):
 //             scores from TMEM, weights back over the scores' columns
-//   16-19     loaders: queries and bf16 rows by cp.async (zero-filled where a
-//             key is not visible, so garbage never reaches the products), KV8 rows
-//             through registers; 128-byte swizzled K-major tiles, the value
-//             tile read as an MN-major operand
+//   16-19     tile warps: queries (cp.async), key masks and scales, KV8 codes to
+//             bf16, bf16 values that are not visible to 0 (what a page
+//             holds there never reaches the products); 128-byte swizzled
+//             K-major tiles, the value tile read as an MN-major operand
 //   20        one thread issues the MMAs; while one tile's softmax runs, the
 //             other's products do
 //   21        walks the units and publishes segments (tile, KV head, block range)
 //   22        zeroes the rows in front of a sequence's first token
+//   23        copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
 // Bound by the exponentials at 64 dims (16 per clock and SM) and by the tensor
-// cores at 128. Every wait is bounded (error codes 59-69).
+// cores at 128. Every wait is bounded (error codes 57-69).
 #include "kernels.h"
 #include "paged.cuh"
 #include "tc05.cuh"
@@ -53,19 +54,23 @@ template <bool KV8, int DIM>
 struct PpCfg {
     static constexpr int HALVES = DIM / 64;
     static constexpr int TILE_BYTES = 128 * 128 * HALVES;  // 128 rows of DIM bf16, 64 dims per swizzled half
-    static constexpr int SLOTS = DIM == 64 ? 8 : 4;        // K and V tiles in flight (K0 V0 K1 V1 ..)
+    // K and V tiles in flight (K0 V0 K1 V1 ..), and KV8 tiles as codes in front of them
+    static constexpr int SLOTS = DIM == 64 ? 6 : KV8 ? 3 : 4;
+    static constexpr int RAW = KV8 ? (DIM == 64 ? 4 : 2) : SLOTS / 2, RAW_BYTES = KV8 ? 128 * DIM : 0;
     static constexpr int Q = 0, RING = 2 * TILE_BYTES;
-    static constexpr int SC = RING + SLOTS * TILE_BYTES;   // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
+    static constexpr int CODES = RING + SLOTS * TILE_BYTES;  // [RAW][128][DIM] codes
+    static constexpr int SC = CODES + RAW * RAW_BYTES;       // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
     static constexpr int MASK = SC + PP_SC * 256 * 4;
     static constexpr int XCH = MASK + PP_SC * 16;          // [2 tiles][2 halves][128 rows] floats
     static constexpr int SEG = XCH + 2 * 2 * 128 * 4;
     static constexpr int BARS = SEG + PP_SEG * 64;
-    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 8;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 8 + 2 * RAW;
     static constexpr int SLOT = BARS + NBARS * 8;
     static constexpr int TOTAL = SLOT + 16;
     static constexpr int ALLOC = TOTAL + 1024;
     static constexpr int PIECE = 2 * PP_TILE + PP_TILE * DIM;  // floats: m, l, o
     static_assert(ALLOC <= 232448, "shared memory per CTA");
+    static_assert(KV8 || SLOTS % 2 == 0, "bf16: even slots hold keys, odd ones values");
 };
 
 // One tile's run of blocks for one KV head.
@@ -95,6 +100,10 @@ struct PpWork {
     unsigned *err;
     PpRec *recs;     // [max_ctas]
     float *pieces;   // [max_ctas][2][PIECE]
+};
+
+struct PpMaps {  // bf16 pools
+    CUtensorMap k, v;
 };
 
 struct PpSeqInfo {
@@ -258,6 +267,13 @@ __device__ __forceinline__ uint32_t pp_off(int r, int c) {
     return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+__device__ __forceinline__ void pp_tma_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
 // One lane of a converged warp. A branch on its result is known to the compiler to
 // be taken by one thread, so that tcgen05 instructions inside it take their
 // operands from uniform registers directly; under `lane == 0` each of
@@ -286,7 +302,7 @@ struct PpReader {
 };
 
 template <bool KV8, int DIM>
-__global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnArgs a, PpWork w) {
+__global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __grid_constant__ PpMaps maps, PagedAttnArgs a, PpWork w) {
     using C = PpCfg<KV8, DIM>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ unsigned long long wsum[PP_WARPS], at_prefix;
@@ -297,7 +313,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
     uint64_t *kv_full = bars, *kv_empty = kv_full + C::SLOTS, *sc_full = kv_empty + C::SLOTS, *sc_empty = sc_full + PP_SC;
     uint64_t *seg_full = sc_empty + PP_SC, *seg_empty = seg_full + PP_SEG;
     uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 4,
-             *o_full = q_full + 6, *mdone = q_full + 8;
+             *o_full = q_full + 6, *mdone = q_full + 8, *raw_full = mdone + 9, *raw_empty = raw_full + C::RAW;
     uint32_t *slot_p = reinterpret_cast<uint32_t *>(sm + C::SLOT);
     float *scales = reinterpret_cast<float *>(sm + C::SC);
     uint32_t *masks = reinterpret_cast<uint32_t *>(sm + C::MASK);
@@ -307,7 +323,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
 
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; ++i) {
-            tc::mbar_init(&kv_full[i], 4);
+            tc::mbar_init(&kv_full[i], KV8 || (i & 1) ? 4 : 1);  // the converting warps; bf16 keys: the copy itself
             tc::mbar_init(&kv_empty[i], 1);
         }
         for (int i = 0; i < PP_SC; ++i) {
@@ -316,7 +332,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
         }
         for (int i = 0; i < PP_SEG; ++i) {
             tc::mbar_init(&seg_full[i], 1);
-            tc::mbar_init(&seg_empty[i], 21);  // 4 loader warps, the MMA warp, 16 softmax warps
+            tc::mbar_init(&seg_empty[i], 22);  // 4 tile warps, the copy and MMA warps, 16 softmax warps
         }
         tc::mbar_init(q_full, 4);
         tc::mbar_init(q_empty, 1);
@@ -327,6 +343,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
         }
         tc::mbar_init(mdone, 1);
         for (int i = 0; i < 8; ++i) tc::mbar_init(mdone + 1 + i, 2);  // pairs of softmax warps
+        for (int i = 0; i < C::RAW; ++i) {
+            tc::mbar_init(&raw_full[i], 1);
+            tc::mbar_init(&raw_empty[i], 4);
+        }
         tc::mbar_fence_init();
     }
     if (warp == 20) tc::tmem_alloc(slot_p, 512);
@@ -563,71 +583,44 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
             tc::tc_fence_before();
         }
     } else if (warp < 20) {
-        // ---------------- loaders: warp lw takes rows 32 lw .. of each tile
+        // ---------------- tile warps: warp lw has keys 32 lw .. of each block
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int lw = warp - 16;
         constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
         PpReader rd{ring, seg_full, seg_empty};
-        uint32_t bc = 0, nseg = 0, issued = 0, landed = 0;  // blocks; segments; K / V tiles begun and announced (bf16)
-        auto announce = [&](uint32_t n) {  // tiles up to n are in shared memory
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            for (; landed < n; ++landed)
-                if (lane == 0) tc::mbar_arrive(&kv_full[landed % C::SLOTS]);
-        };
+        uint32_t bc = 0, nseg = 0, tiles = 0;  // blocks; segments; K and V tiles
         PpSeg g;
         while (ok) {
             ok = rd.next(g, w.err);
             if (!ok || g.nblk == 0) break;
             const uint32_t *table = a.c.table + (uint64_t)g.seq * a.c.max_pages;
-            auto kb_of = [&](int i) {
+            // lane = key: its page two blocks ahead, its pool row and scales one ahead
+            auto key_of = [&](int i) {
                 const int vb = g.b0 + i;
-                return (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
+                return (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK + 32 * lw + lane;
             };
-            auto seen = [&](int key) { return key <= g.last && (key >= g.low || key < g.first); };
             auto page_of = [&](int i) {
-                const int key = kb_of(i) + 32 * lw + lane;
-                return i < g.nblk && seen(key) ? __ldg(&table[key >> a.c.tshift]) : PG_NO_PAGE;
+                const int key = key_of(i);
+                return i < g.nblk && key <= g.last && (key >= g.low || key < g.first) ? __ldg(&table[key >> a.c.tshift])
+                                                                                       : PG_NO_PAGE;
             };
-            uint32_t next = page_of(0);
-            // queries: flattened row m of the tile is row0 + m / group, head m % group of this KV head
-            if (nseg > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty, (nseg - 1) & 1, w.err, 64));
-            if (!ok) break;
-            ++nseg;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll 4
-                for (int j = 0; j < CPR; ++j) {
-                    const int n = j * 32 + lane, r = 32 * lw + n / CPR, c = n % CPR;
-                    const uint32_t mr = g.m0 + 128 * x + r;
-                    const bool live = mr < g.mrows;
-                    const uint64_t src = live ? (g.row0 + (uint64_t)(mr / w.group)) * a.q_stride +
-                                                    (uint64_t)(g.kvh * w.group + mr % w.group) * DIM + 8 * c
-                                              : 0;
-                    pp_cp16(sbase + C::Q + x * C::TILE_BYTES + pp_off(r, c), a.q + src, live ? 16 : 0);
-                }
-            }
-            pp_cp_commit();
-            pp_cp_wait<0>();
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(q_full);
-            for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
-                const uint32_t page = next;
-                next = page_of(i + 1);
-                const int key = kb_of(i) + 32 * lw + lane;
+            uint32_t bits = 0;
+            float ksc = 0.f, vsc = 0.f;
+            auto scales_of = [&](int i, uint32_t page) {
                 const bool vis = page < a.c.pages;
-                const uint64_t row = vis ? paged_row(a.c, page, g.kvh) + (key & ((1 << a.c.tshift) - 1)) : 0;
+                bits = __ballot_sync(0xffffffffu, vis);
+                ksc = vsc = 0.f;
+                if (KV8 && vis) {
+                    const uint64_t row = paged_row(a.c, page, g.kvh) + (key_of(i) & ((1 << a.c.tshift) - 1));
+                    ksc = __ldg(a.c.ks + row);
+                    vsc = __ldg(a.c.vs + row);
+                }
+            };
+            scales_of(0, page_of(0));
+            uint32_t page = page_of(1);
+            for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
                 // scales and the mask of keys that are there
                 const uint32_t st = bc % PP_SC;
-                float ksc = 0.f, vsc = 0.f;
-                if constexpr (KV8) {
-                    if (vis) {
-                        ksc = __ldg(a.c.ks + row);
-                        vsc = __ldg(a.c.vs + row);
-                    }
-                }
-                const uint32_t bits = __ballot_sync(0xffffffffu, vis);
                 if (bc >= PP_SC)
                     ok = __all_sync(0xffffffffu, tc::mbar_wait(&sc_empty[st], ((bc / PP_SC) & 1) ^ 1, w.err, 65));
                 if (!ok) break;
@@ -635,34 +628,62 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                     scales[st * 256 + 32 * lw + lane] = w.negate ? -ksc * w.fac : ksc * w.fac;
                     scales[st * 256 + 128 + 32 * lw + lane] = vsc;
                 }
-                if (lane == 0) masks[4 * st + lw] = bits;
+                const uint32_t now = bits;
+                if (lane == 0) masks[4 * st + lw] = now;
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&sc_full[st]);
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const uint32_t slot = issued % C::SLOTS;
-                    const uint8_t *pool = kv ? a.c.v : a.c.k;
-                    const uint32_t dst = sbase + C::RING + slot * C::TILE_BYTES;
-                    if constexpr (KV8) {
-                        constexpr int NL = DIM / 16;  // 16-code chunks per row = loads per lane
-                        uint4 v[NL];
-#pragma unroll
-                        for (int j = 0; j < NL; ++j) {
-                            const int n = j * 32 + lane, rl = n / NL, c = n % NL;
-                            const uint64_t rr = __shfl_sync(0xffffffffu, row, rl);
-                            v[j] = bits >> rl & 1 ? ldg_stream(pool + rr * DIM + 16 * c) : make_uint4(0, 0, 0, 0);
+                scales_of(i + 1, page);
+                page = page_of(i + 2);
+                if (i == 0) {
+                    // queries: flattened row m of the tile is token m / group, head m % group of this KV
+                    // head; lane = row, its address handed to the lanes that copy it
+                    if (nseg > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty, (nseg - 1) & 1, w.err, 64));
+                    if (!ok) break;
+                    ++nseg;
+#pragma unroll 1
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t mr = g.m0 + 128 * x + 32 * lw + lane;
+                        const bool live = mr < g.mrows;
+                        const uint64_t mine = live ? (g.row0 + (uint64_t)(mr / w.group)) * a.q_stride +
+                                                         (uint64_t)(g.kvh * w.group + mr % w.group) * DIM
+                                                   : 0;
+                        const uint32_t lives = __ballot_sync(0xffffffffu, live);
+#pragma unroll 4
+                        for (int j = 0; j < CPR; ++j) {
+                            const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
+                            const uint64_t src = __shfl_sync(0xffffffffu, mine, rl);
+                            pp_cp16(sbase + C::Q + x * C::TILE_BYTES + pp_off(32 * lw + rl, c), a.q + src + 8 * c,
+                                    lives >> rl & 1 ? 16 : 0);
                         }
-                        if (issued >= C::SLOTS)
-                            ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_empty[slot], ((issued / C::SLOTS) & 1) ^ 1, w.err, 66));
+                    }
+                    pp_cp_commit();
+                    pp_cp_wait<0>();
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(q_full);
+                }
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv, ++tiles) {
+                    const uint32_t slot = tiles % C::SLOTS, dst = sbase + C::RING + slot * C::TILE_BYTES;
+                    if constexpr (KV8) {
+                        // codes -> bf16, exactly; a code that is not visible is some code, and its
+                        // scale and weight are 0
+                        const uint32_t rs = tiles % C::RAW;
+                        ok = tc::mbar_wait(&raw_full[rs], (tiles / C::RAW) & 1, w.err, 58) &&
+                             (tiles < C::SLOTS || tc::mbar_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 66));
+                        ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
+                        constexpr int NL = DIM / 16;
+                        const uint32_t src = sbase + C::CODES + rs * C::RAW_BYTES + 32 * lw * DIM;
 #pragma unroll
                         for (int j = 0; j < NL; ++j) {
                             const int n = j * 32 + lane, r = 32 * lw + n / NL, c = n % NL;
-                            // bytes (0, 1) and (2, 3) of each word as bf16 pairs
-                            uint32_t o[8];
-                            const uint32_t wd[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                            uint32_t wd[4], o[8];
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3])
+                                         : "r"(src + n * 16));
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
+                            for (int k = 0; k < 4; ++k) {  // bytes (0, 1) and (2, 3) of each word as bf16 pairs
                                 const uint32_t lo = __byte_perm(wd[k], 0, 0x4140), hi = __byte_perm(wd[k], 0, 0x4342);
                                 o[2 * k] = bf16x2_sub(lop_or(lo, 0x007F007Fu, 0x43004300u), lop_or(lo, 0x00800080u, 0x43004300u));
                                 o[2 * k + 1] = bf16x2_sub(lop_or(hi, 0x007F007Fu, 0x43004300u), lop_or(hi, 0x00800080u, 0x43004300u));
@@ -670,34 +691,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                             pp_sts128(dst + pp_off(r, 2 * c), o[0], o[1], o[2], o[3]);
                             pp_sts128(dst + pp_off(r, 2 * c + 1), o[4], o[5], o[6], o[7]);
                         }
-                        ++issued;
-                        announce(issued);
-                    } else {
-                        if (issued >= C::SLOTS)
-                            ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_empty[slot], ((issued / C::SLOTS) & 1) ^ 1, w.err, 66));
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tc::mbar_arrive(&kv_full[slot]);
+                            tc::mbar_arrive(&raw_empty[rs]);
+                        }
+                    } else if (kv == 1) {
+                        // values that are not visible become 0 (a weight of 0 times NaN would not be)
+                        const uint32_t vt = tiles / 2, rs = vt % C::RAW;
+                        ok = __all_sync(0xffffffffu, tc::mbar_wait(&raw_full[rs], (vt / C::RAW) & 1, w.err, 58));
                         if (!ok) break;
-#pragma unroll
-                        for (int j = 0; j < CPR; ++j) {
-                            const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
-                            const uint64_t rr = __shfl_sync(0xffffffffu, row, rl);
-                            pp_cp16(dst + pp_off(32 * lw + rl, c), pool + rr * (2 * DIM) + 16 * c, bits >> rl & 1 ? 16 : 0);
+                        if (now != 0xffffffffu) {
+                            if (!(now >> lane & 1))
+                                for (int c = 0; c < CPR; ++c) pp_sts128(dst + pp_off(32 * lw + lane, c), 0, 0, 0, 0);
+                            tc::fence_proxy_async_smem();
                         }
-                        pp_cp_commit();
-                        ++issued;
-                        // announced two tiles behind; a wait for a free slot only needs tiles SLOTS back
-                        if (issued - landed > 2) {
-                            pp_cp_wait<2>();
-                            announce(issued - 2);
-                        }
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&kv_full[slot]);
                     }
                 }
             }
-            if constexpr (!KV8) {  // before waiting for anything of the next segment
-                pp_cp_wait<0>();
-                if (ok) announce(issued);
-            }
         }
-        pp_cp_wait<0>();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 20) {
@@ -770,6 +785,62 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(PagedAttnA
                 tc::mbar_wait(mdone, 0, w.err, 69);
             }
             __syncwarp();
+        } else if (warp == 23) {
+            // ---------------- copies: lane p has page p of a block (its first 128 tokens' worth
+            // of it); KV8 pages as runs of codes, bf16 pages as swizzled boxes
+            PpReader rd{ring, seg_full, seg_empty};
+            const int per = min(1 << a.c.tshift, PP_BLK), npages = PP_BLK / per;  // tokens of a copy, copies of a block
+            constexpr uint32_t RB = KV8 ? DIM : 2 * DIM;
+            uint32_t tiles = 0;
+            PpSeg g;
+            while (ok) {
+                ok = rd.next(g, w.err);
+                if (!ok || g.nblk == 0) break;
+                const uint32_t *table = a.c.table + (uint64_t)g.seq * a.c.max_pages;
+                auto page_of = [&](int i) {
+                    const int vb = g.b0 + i, key = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK + lane * per;
+                    const bool some = i < g.nblk && lane < npages && key <= g.last && (key + per > g.low || key < g.first);
+                    return some ? __ldg(&table[key >> a.c.tshift]) : PG_NO_PAGE;
+                };
+                uint32_t next = page_of(0);
+                for (int i = 0; i < g.nblk && ok; ++i) {
+                    const uint32_t page = next;
+                    next = page_of(i + 1);
+                    const int vb = g.b0 + i, key = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK + lane * per;
+                    const bool have = page < a.c.pages;
+                    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * per * RB;
+                    const int row = ((int)g.kvh << a.c.tshift) + (key & ((1 << a.c.tshift) - 1));  // within the page
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv, ++tiles) {
+                        uint64_t *bar;
+                        uint32_t slot;
+                        if constexpr (KV8) {
+                            slot = tiles % C::RAW;
+                            bar = &raw_full[slot];
+                            if (tiles >= C::RAW) ok = tc::mbar_wait(&raw_empty[slot], ((tiles / C::RAW) & 1) ^ 1, w.err, 57);
+                        } else {
+                            slot = tiles % C::SLOTS;
+                            bar = kv ? &raw_full[tiles / 2 % C::RAW] : &kv_full[slot];
+                            if (tiles >= C::SLOTS) ok = tc::mbar_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 57);
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) tc::mbar_arrive_expect_tx(bar, bytes);
+                        __syncwarp();
+                        if (have) {
+                            if constexpr (KV8) {
+                                const uint8_t *src = (kv ? a.c.v : a.c.k) + ((uint64_t)page * a.c.page_rows + row) * RB;
+                                tc::bulk_load(sm + C::CODES + slot * C::RAW_BYTES + lane * per * RB, src, per * RB, bar);
+                            } else {
+#pragma unroll
+                                for (int h = 0; h < C::HALVES; ++h)
+                                    pp_tma_3d(sm + C::RING + slot * C::TILE_BYTES + h * (128 * 128) + lane * per * 128,
+                                              kv ? &maps.v : &maps.k, bar, 64 * h, row, (int)page);
+                            }
+                        }
+                    }
+                }
+            }
         } else if (warp == 21) {
             // ---------------- segments
             uint32_t n = 0;
@@ -945,8 +1016,15 @@ static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t 
     using C = PpCfg<KV8, DIM>;
     auto *kernel = paged_prefill_kernel<KV8, DIM>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::ALLOC) != cudaSuccess) return -3;
+    PpMaps maps = {};
+    if (!KV8) {
+        const uint64_t rows = (uint64_t)a.c.hkv << a.c.tshift, stride = (a.c.page_rows > rows ? a.c.page_rows : rows) * DIM * 2;
+        const int box = a.c.tshift < 7 ? 1 << a.c.tshift : PP_BLK;
+        if (int rc = make_page_map(&maps.k, a.c.k, DIM, rows, a.c.pages, stride, box)) return rc;
+        if (int rc = make_page_map(&maps.v, a.c.v, DIM, rows, a.c.pages, stride, box)) return rc;
+    }
     PdlChain chain;
-    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PF_THREADS), C::ALLOC, st, 1, a, w)) return rc;
+    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PF_THREADS), C::ALLOC, st, 1, maps, a, w)) return rc;
     return launch_pdl(paged_prefill_join_kernel<DIM>, dim3(w.max_ctas, PP_TILE / 32), dim3(256), 0, st, 1, a, w);
 }
 
