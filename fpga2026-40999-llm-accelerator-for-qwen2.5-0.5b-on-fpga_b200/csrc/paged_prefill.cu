@@ -22,20 +22,20 @@
 // tile that two or more CTAs share is joined by a second kernel (at most two
 // pieces per CTA, fp32, added in CTA order).
 //
-// Warps (768 threads, one CTA per SM, registers moved to the softmax warps):
-//   0-7, 8-15 softmax of the first / second MMA tile, two threads per row (64
-//             keys each, which fit their registers; one thread with all 128
-//             ran at a third of the rate, waiting for instructions and latencies):
+// Warps (512 threads, one CTA per SM, registers moved to the softmax warps):
+//   0-3, 4-7  softmax of the first / second MMA tile, one thread per row (no
+//             exchange between threads; two per row spent 700 to 1200 of 7000
+//             clocks a block waiting for each other's maximum):
 //             scores from TMEM, weights back over the scores' columns
-//   16-19     tile warps: queries (cp.async), key masks and scales, KV8 codes to
+//   8-11      tile warps: queries (cp.async), key masks and scales, KV8 codes to
 //             bf16, bf16 values that are not visible to 0 (what a page
 //             holds there never reaches the products); 128-byte swizzled
 //             K-major tiles, the value tile read as an MN-major operand
-//   20        one thread issues the MMAs; while one tile's softmax runs, the
+//   12        one thread issues the MMAs; while one tile's softmax runs, the
 //             other's products do
-//   21        walks the units and publishes segments (tile, KV head, block range)
-//   22        zeroes the rows in front of a sequence's first token
-//   23        copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
+//   13        walks the units and publishes segments (tile, KV head, block range)
+//   14        zeroes the rows in front of a sequence's first token
+//   15        copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
 // Bound by the exponentials at 64 dims (16 per clock and SM) and by the tensor
 // cores at 128. Every wait is bounded (error codes 57-69).
 #include "kernels.h"
@@ -44,7 +44,7 @@
 
 namespace qb {
 
-constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 768, PP_WARPS = PF_THREADS / 32;
+constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 512, PP_WARPS = PF_THREADS / 32;
 constexpr int PP_MAX_SMS = 192;
 constexpr uint32_t PP_MIN_UNITS = 4;  // blocks a CTA takes at least: less and the join costs more than the split saves
 constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
@@ -61,10 +61,9 @@ struct PpCfg {
     static constexpr int CODES = RING + SLOTS * TILE_BYTES;  // [RAW][128][DIM] codes
     static constexpr int SC = CODES + RAW * RAW_BYTES;       // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
     static constexpr int MASK = SC + PP_SC * 256 * 4;
-    static constexpr int XCH = MASK + PP_SC * 16;          // [2 tiles][2 halves][128 rows] floats
-    static constexpr int SEG = XCH + 2 * 2 * 128 * 4;
+    static constexpr int SEG = MASK + PP_SC * 16;
     static constexpr int BARS = SEG + PP_SEG * 64;
-    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 8 + 2 * RAW;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 2 * RAW;
     static constexpr int SLOT = BARS + NBARS * 8;
     static constexpr int TOTAL = SLOT + 16;
     static constexpr int ALLOC = TOTAL + 1024;
@@ -313,7 +312,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     uint64_t *kv_full = bars, *kv_empty = kv_full + C::SLOTS, *sc_full = kv_empty + C::SLOTS, *sc_empty = sc_full + PP_SC;
     uint64_t *seg_full = sc_empty + PP_SC, *seg_empty = seg_full + PP_SEG;
     uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 4,
-             *o_full = q_full + 6, *mdone = q_full + 8, *raw_full = mdone + 9, *raw_empty = raw_full + C::RAW;
+             *o_full = q_full + 6, *mdone = q_full + 8, *raw_full = mdone + 1, *raw_empty = raw_full + C::RAW;
     uint32_t *slot_p = reinterpret_cast<uint32_t *>(sm + C::SLOT);
     float *scales = reinterpret_cast<float *>(sm + C::SC);
     uint32_t *masks = reinterpret_cast<uint32_t *>(sm + C::MASK);
@@ -328,28 +327,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
         }
         for (int i = 0; i < PP_SC; ++i) {
             tc::mbar_init(&sc_full[i], 4);
-            tc::mbar_init(&sc_empty[i], 16);
+            tc::mbar_init(&sc_empty[i], 8);
         }
         for (int i = 0; i < PP_SEG; ++i) {
             tc::mbar_init(&seg_full[i], 1);
-            tc::mbar_init(&seg_empty[i], 22);  // 4 tile warps, the copy and MMA warps, 16 softmax warps
+            tc::mbar_init(&seg_empty[i], 14);  // 4 tile warps, the copy and MMA warps, 8 softmax warps
         }
         tc::mbar_init(q_full, 4);
         tc::mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
-            tc::mbar_init(&p_ready[i], 256);
+            tc::mbar_init(&p_ready[i], 4);
             tc::mbar_init(&o_full[i], 1);
         }
         tc::mbar_init(mdone, 1);
-        for (int i = 0; i < 8; ++i) tc::mbar_init(mdone + 1 + i, 2);  // pairs of softmax warps
         for (int i = 0; i < C::RAW; ++i) {
             tc::mbar_init(&raw_full[i], 1);
             tc::mbar_init(&raw_empty[i], 4);
         }
         tc::mbar_fence_init();
     }
-    if (warp == 20) tc::tmem_alloc(slot_p, 512);
+    if (warp == 12) tc::tmem_alloc(slot_p, 512);
 
     // ---- numbering of the units: a warp takes a run of sequences
     const uint32_t per = (a.n + PP_WARPS - 1) / PP_WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
@@ -392,20 +390,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     if (!active) {
         // ---------------- nothing to compute
         if (tid == 0) w.recs[blockIdx.x].valid = 0;
-    } else if (warp < 16) {
-        // ---------------- softmax: thread = row r of tile `x`, keys 64 hf .. of each block
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
-        const int x = warp >> 3, hf = (warp >> 2) & 1, r = tid & 127;
-        float *xch = reinterpret_cast<float *>(sm + C::XCH) + x * 256;
-        uint64_t *pair = mdone + 1 + x * 4 + (warp & 3);  // this warp and the one with the rows' other keys
-        uint32_t np = 0;
-        auto pair_sync = [&] {
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(pair);
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(pair, np++ & 1, w.err, 59));
-        };
+    } else if (warp < 8) {
+        // ---------------- softmax: thread = row r of tile `x`
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int x = warp >> 2, r = tid & 127;
         const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 (warp % 4) ..
-        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM + hf * (DIM / 2);
+        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM;
         PpReader rd{ring, seg_full, seg_empty};
         uint32_t bc = 0, ns = 0, no = 0;  // blocks of the CTA; scores and contexts of this tile
         PpSeg g;
@@ -439,30 +429,31 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                 if (!ok) break;
                 ++ns;
                 tc::tc_fence_after();
-                float s[64];
+                float s[128];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) pp_ld32(s_addr + 64 * hf + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
+                for (int j = 0; j < 4; ++j) pp_ld32(s_addr + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
                 pp_ld_wait();
                 if constexpr (KV8) {
-                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256 + 64 * hf);
+                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
+                    for (int j = 0; j < 32; ++j) {
                         const float4 f = kf[j];
-                        unpk2(mul2(pk2(s[4 * j], s[4 * j + 1]), pk2(f.x, f.y)), s[4 * j], s[4 * j + 1]);
-                        unpk2(mul2(pk2(s[4 * j + 2], s[4 * j + 3]), pk2(f.z, f.w)), s[4 * j + 2], s[4 * j + 3]);
+                        s[4 * j] *= f.x;
+                        s[4 * j + 1] *= f.y;
+                        s[4 * j + 2] *= f.z;
+                        s[4 * j + 3] *= f.w;
                     }
                 }
                 const uint4 there = *reinterpret_cast<const uint4 *>(masks + 4 * st);
                 const bool full = kb + 127 <= all_last && (kb >= all_low || kb + 128 <= all_first) &&
                                   (there.x & there.y & there.z & there.w) == 0xffffffffu;
                 if (!full) {
-                    const uint32_t tw[2] = {hf ? there.z : there.x, hf ? there.w : there.y};
+                    const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        // bits of 32 keys from k0: up to the row's position, from `low` on or before `first`
-                        const int k0 = kb + 64 * hf + 32 * k;
-                        auto below = [&](int e) {  // bits j with k0 + j < e
-                            const int n = e - k0;
+                    for (int k = 0; k < 4; ++k) {
+                        // bits of keys kb + 32 k ..: up to the row's position, from `low` on or before `first`
+                        auto below = [&](int e) {  // bits j with kb + 32 k + j < e
+                            const int n = e - (kb + 32 * k);
                             return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
                         };
                         const uint32_t bits = tw[k] & below(pos + 1) & (~below(low) | below(first));
@@ -473,21 +464,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if constexpr (!KV8) top *= w.fac;
-                // the row's other half; both halves have read their scores by then, so weights may overwrite them
-                xch[128 * hf + r] = top;
-                pair_sync();
-                if (!ok) break;
-                top = fmaxf(top, xch[128 * (hf ^ 1) + r]);
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
                     m = up;
                     l *= f;
                     if (i > 0) {  // this tile's earlier products are complete (s_full follows them)
 #pragma unroll 1
-                        for (int j = 0; j < DIM / 2; j += 16) {
+                        for (int j = 0; j < DIM; j += 16) {
                             uint32_t o[16];
                             pp_ld16(o_addr + j, o);
                             pp_ld_wait();
@@ -498,35 +484,37 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                     }
                 }
                 const float mu = m == -INFINITY ? 0.f : m;
-                const unsigned long long nm = dup2(-mu), fc = dup2(w.fac);
-                unsigned long long sum[2] = {0ull, 0ull};
-                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128 + 64 * hf);
-                uint32_t p[32];
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const int k = 2 * j;
-                    float e0, e1;
-                    if constexpr (KV8)
-                        unpk2(add2(pk2(s[k], s[k + 1]), nm), e0, e1);
-                    else
-                        unpk2(fma2(pk2(s[k], s[k + 1]), fc, nm), e0, e1);
-                    e0 = pp_ex2(e0);
-                    e1 = pp_ex2(e1);
-                    const unsigned long long e = pk2(e0, e1);
-                    sum[j & 1] = add2(sum[j & 1], e);
-                    if constexpr (KV8) {
-                        const float4 f = vf[k >> 2];
-                        unpk2(mul2(e, (k & 2) ? pk2(f.z, f.w) : pk2(f.x, f.y)), e0, e1);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const int k = 64 * h + 2 * j;
+                        float e[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            e[c] = pp_ex2(KV8 ? s[k + c] - mu : fmaf(s[k + c], w.fac, -mu));
+                            sum[c] += e[c];
+                        }
+                        if constexpr (KV8) {
+                            const float4 f = vf[k >> 2];
+                            e[0] *= f.x;
+                            e[1] *= f.y;
+                            e[2] *= f.z;
+                            e[3] *= f.w;
+                        }
+                        p[j] = pp_pack(e[0], e[1]);
+                        p[j + 1] = pp_pack(e[2], e[3]);
                     }
-                    p[j] = pp_pack(e0, e1);
+                    pp_st32(s_addr + 32 * h, p);
                 }
-                pp_st32(s_addr + 32 * hf, p);
-                float a0, a1;
-                unpk2(add2(sum[0], sum[1]), a0, a1);
-                l += a0 + a1;
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 pp_st_wait();
                 tc::tc_fence_before();
-                tc::mbar_arrive(&p_ready[x]);
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&p_ready[x]);
                 if (lane == 0) tc::mbar_arrive(&sc_empty[st]);
             }
             if (!ok) break;
@@ -535,17 +523,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             ++no;
             tc::tc_fence_after();
             const bool live = m_row < g.mrows && pos >= 0;
-            xch[128 * hf + r] = l;
-            pair_sync();
-            l += xch[128 * (hf ^ 1) + r];
-            pair_sync();  // read before the next segment's maxima are written
-            if (!ok) break;
             if (g.piece < 0) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 uint16_t *out = a.ctx + (g.row0 + (uint64_t)row_i) * a.ctx_stride +
-                                (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM + hf * (DIM / 2);
+                                (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM;
 #pragma unroll 1
-                for (int j = 0; j < DIM / 2; j += 16) {
+                for (int j = 0; j < DIM; j += 16) {
                     uint32_t o[16];
                     pp_ld16(o_addr + j, o);
                     pp_ld_wait();
@@ -565,13 +548,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             } else {
                 float *piece = w.pieces + (uint64_t)g.piece * C::PIECE;
                 const int t = 128 * x + r;
-                if (hf == 0) {
-                    piece[t] = m;
-                    piece[PP_TILE + t] = l;
-                }
-                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM + hf * (DIM / 2);
+                piece[t] = m;
+                piece[PP_TILE + t] = l;
+                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM;
 #pragma unroll 1
-                for (int j = 0; j < DIM / 2; j += 16) {
+                for (int j = 0; j < DIM; j += 16) {
                     uint32_t o[16];
                     pp_ld16(o_addr + j, o);
                     pp_ld_wait();
@@ -582,10 +563,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             }
             tc::tc_fence_before();
         }
-    } else if (warp < 20) {
+    } else if (warp < 12) {
         // ---------------- tile warps: warp lw has keys 32 lw .. of each block
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int lw = warp - 16;
+        const int lw = warp - 8;
         constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
         PpReader rd{ring, seg_full, seg_empty};
         uint32_t bc = 0, nseg = 0, tiles = 0;  // blocks; segments; K and V tiles
@@ -715,7 +696,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 20) {
+        if (warp == 12) {
             // ---------------- MMA issuer
             PpReader rd{ring, seg_full, seg_empty};
             uint32_t bc = 0, nseg = 0, np[2] = {0, 0};
@@ -735,7 +716,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                     // descriptors differ in their address field only: bases once, steps by adding
                     auto qk = [&](int x, uint32_t n) {
                         const uint64_t qd = q_desc + x * (C::TILE_BYTES >> 4), kd = k_desc + (n % C::SLOTS) * (C::TILE_BYTES >> 4);
-#pragma unroll 1
+#pragma unroll
                         for (int j = 0; j < DIM / 16; ++j) {
                             const uint32_t off = ((j >> 2) * (128 * 128) + (j & 3) * 32) >> 4;
                             pp_mma_ss(tmem + 128 * x, qd + off, kd + off, id_qk, j > 0);
@@ -752,10 +733,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                                 ok = tc::mbar_wait(&p_ready[x], (np[x] + i - 1) & 1, w.err, 69) && (x > 0 || wait_tile(kt - 1));
                                 if (!ok) break;
                                 tc::tc_fence_after();
-                                uint64_t vd = v_desc + ((kt - 1) % C::SLOTS) * (C::TILE_BYTES >> 4);
-#pragma unroll 1
-                                for (int j = 0; j < 8; ++j, vd += 2048 >> 4)
-                                    pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, vd, id_pv, i > 1 || j > 0);
+                                const uint64_t vd = v_desc + ((kt - 1) % C::SLOTS) * (C::TILE_BYTES >> 4);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, vd + j * (2048 >> 4), id_pv,
+                                              i > 1 || j > 0);
                                 if (final) tc::mma_commit(&kv_empty[(kt - 1) % C::SLOTS]);
                             }
                             if (i < g.nblk) {
@@ -785,7 +767,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                 tc::mbar_wait(mdone, 0, w.err, 69);
             }
             __syncwarp();
-        } else if (warp == 23) {
+        } else if (warp == 15) {
             // ---------------- copies: lane p has page p of a block (its first 128 tokens' worth
             // of it); KV8 pages as runs of codes, bf16 pages as swizzled boxes
             PpReader rd{ring, seg_full, seg_empty};
@@ -841,7 +823,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                     }
                 }
             }
-        } else if (warp == 21) {
+        } else if (warp == 13) {
             // ---------------- segments
             uint32_t n = 0;
             uint32_t i = at_seq;
@@ -944,7 +926,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             }
         }
     }
-    if (warp == 22) {
+    if (warp == 14) {
         // ---------------- rows in front of the first token, and of no sequence
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
             const PpSeqInfo s = pp_seq(a, w, i);
@@ -957,7 +939,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 20) {
+    if (warp == 12) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
