@@ -5,46 +5,50 @@
 //
 // Mathematics, per (row, query head), over its visible keys j in blocks of 128:
 //   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
-// m is the running maximum, raised only where a block passes it by more than
-// 8 (p stays below 2^8), so that the accumulator is rarely rescaled. The weights
+// m is a reference near the running maximum: the maximum of the row's first
+// 64 keys, and a new one only where 64 keys' weights sum to more than 2^15 (so
+// most keys need no comparison at all and the accumulator is rarely rescaled;
+// fp32 and bf16 keep their relative precision far above and below 1). The weights
 // are rounded to bf16 for the second product (half a step is 2^-8 of a weight, unbiased);
 // everything else is fp32. KV8: codes become bf16 exactly on the way to
 // shared memory, the key's scale multiplies its column of scores and the
 // value's scale its column of weights.
 //
 // Tiles: the rows of a sequence and the query heads that share a KV head are one
-// axis (row-major: token, head), cut into tiles of 256 = two MMA tiles of 128 rows,
-// so any group size fills them and a block of keys is read once for
-// 256 (row, head) pairs. Per tile only the blocks that some row sees are
-// visited. All (tile, KV head, block) units are numbered in a row and CTA c of
-// G takes the c-th equal run: long and short prompts, windows and single rows
-// balance by themselves, and few rows over many keys split along the keys. A
-// tile that two or more CTAs share is joined by a second kernel (at most two
-// pieces per CTA, fp32, added in CTA order).
+// axis (row-major: token, head), cut into tiles of 512 (64 dims) or 256 (128
+// dims) = four or two MMA tiles of 128 rows, so any group size fills them and a
+// block of keys is read once for all of them. Per tile only the blocks that
+// some row sees are visited. All (tile, KV head, block) units are numbered in a
+// row and CTA c of G takes the c-th equal run: long and short prompts, windows
+// and single rows balance by themselves, and few rows over many keys split
+// along the keys. A tile that two or more CTAs share is joined by a second
+// kernel (at most two pieces per CTA, fp32, added in CTA order).
 //
-// Warps (512 threads, one CTA per SM, registers moved to the softmax warps):
-//   0-3, 4-7  softmax of the first / second MMA tile, one thread per row (no
-//             exchange between threads; two per row spent 700 to 1200 of 7000
-//             clocks a block waiting for each other's maximum):
-//             scores from TMEM, weights back over the scores' columns
-//   8-11      tile warps: queries (cp.async), key masks and scales, KV8 codes to
+// A step is 64 keys (half a block) of one MMA tile: scores into 64 TMEM columns,
+// weights (bf16) back over them, second product into the tile's context
+// columns. At 64 dims TMEM holds four tiles with one score buffer each, at 128
+// dims two tiles with two each: either way four steps are in flight and the
+// tensor cores work on three while the softmax has one.
+//
+// Warps (one CTA per SM, registers moved to the softmax warps):
+//   0 ..      four softmax warps per MMA tile, one thread per row
+//   then 4    tile warps: queries (cp.async), key masks and scales, KV8 codes to
 //             bf16, bf16 values that are not visible to 0 (what a page
 //             holds there never reaches the products); 128-byte swizzled
 //             K-major tiles, the value tile read as an MN-major operand
-//   12        one thread issues the MMAs; while one tile's softmax runs, the
-//             other's products do
-//   13        walks the units and publishes segments (tile, KV head, block range)
-//   14        zeroes the rows in front of a sequence's first token
-//   15        copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
-// Bound by the exponentials at 64 dims (16 per clock and SM) and by the tensor
-// cores at 128. Every wait is bounded (error codes 57-69).
+//   then 1    one thread issues the MMAs
+//   1         walks the units and publishes segments (tile, KV head, block range)
+//   1         zeroes the rows in front of a sequence's first token
+//   1         copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
+// Bound by the exponentials at 64 dims (16 per clock and SM), by them and the
+// tensor cores alike at 128. Every wait is bounded (error codes 57-69).
 #include "kernels.h"
 #include "paged.cuh"
 #include "tc05.cuh"
 
 namespace qb {
 
-constexpr int PP_TILE = 256, PP_BLK = 128, PF_THREADS = 512, PP_WARPS = PF_THREADS / 32;
+constexpr int PP_BLK = 128;
 constexpr int PP_MAX_SMS = 192;
 constexpr uint32_t PP_MIN_UNITS = 4;  // blocks a CTA takes at least: less and the join costs more than the split saves
 constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
@@ -52,22 +56,25 @@ constexpr int PP_SEG = 2;             // segments published ahead
 
 template <bool KV8, int DIM>
 struct PpCfg {
+    static constexpr int TILES = DIM == 64 ? 4 : 2, NB = 4 / TILES;  // MMA tiles, score buffers of each
+    static constexpr int TILE = 128 * TILES;                         // flattened rows of a tile
+    static constexpr int SW = 4 * TILES, WARPS = SW + 8, THREADS = 32 * WARPS;
     static constexpr int HALVES = DIM / 64;
     static constexpr int TILE_BYTES = 128 * 128 * HALVES;  // 128 rows of DIM bf16, 64 dims per swizzled half
     // K and V tiles in flight (K0 V0 K1 V1 ..), and KV8 tiles as codes in front of them
     static constexpr int SLOTS = DIM == 64 ? 6 : KV8 ? 3 : 4;
     static constexpr int RAW = KV8 ? (DIM == 64 ? 4 : 2) : SLOTS / 2, RAW_BYTES = KV8 ? 128 * DIM : 0;
-    static constexpr int Q = 0, RING = 2 * TILE_BYTES;
+    static constexpr int Q = 0, RING = TILES * TILE_BYTES;
     static constexpr int CODES = RING + SLOTS * TILE_BYTES;  // [RAW][128][DIM] codes
     static constexpr int SC = CODES + RAW * RAW_BYTES;       // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
     static constexpr int MASK = SC + PP_SC * 256 * 4;
     static constexpr int SEG = MASK + PP_SC * 16;
     static constexpr int BARS = SEG + PP_SEG * 64;
-    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 9 + 2 * RAW;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 11 + 2 * RAW;
     static constexpr int SLOT = BARS + NBARS * 8;
     static constexpr int TOTAL = SLOT + 16;
     static constexpr int ALLOC = TOTAL + 1024;
-    static constexpr int PIECE = 2 * PP_TILE + PP_TILE * DIM;  // floats: m, l, o
+    static constexpr int PIECE = 2 * TILE + TILE * DIM;  // floats: m, l, o
     static_assert(ALLOC <= 232448, "shared memory per CTA");
     static_assert(KV8 || SLOTS % 2 == 0, "bf16: even slots hold keys, odd ones values");
 };
@@ -94,6 +101,7 @@ static_assert(sizeof(PpRec) == 64, "join record");
 
 struct PpWork {
     uint32_t group, max_ctas;
+    uint32_t tile;   // flattened rows of a tile
     float fac;       // log2(e) |scale|
     uint32_t negate; // scale < 0: the first product negates the queries
     unsigned *err;
@@ -117,7 +125,7 @@ __device__ __forceinline__ PpSeqInfo pp_seq(const PagedAttnArgs &a, const PpWork
     s.mrows = (s1 - s0) * w.group;
     const int len = paged_length(a.c, s.seq);
     s.pos0 = len - (int)(s1 - s0);
-    s.nt = len > 0 ? (int)((s.mrows + PP_TILE - 1) / PP_TILE) : 0;
+    s.nt = len > 0 ? (int)((s.mrows + w.tile - 1) / w.tile) : 0;
     return s;
 }
 struct PpBlocks {
@@ -125,7 +133,7 @@ struct PpBlocks {
 };
 __device__ __forceinline__ PpBlocks pp_blocks(const PagedAttnArgs &a, const PpWork &w, int pos0, uint32_t mrows, int k) {
     PpBlocks b;
-    const uint32_t m0 = (uint32_t)k * PP_TILE, m1 = min(m0 + PP_TILE, mrows) - 1;
+    const uint32_t m0 = (uint32_t)k * w.tile, m1 = min(m0 + w.tile, mrows) - 1;
     const int pmin = max(pos0 + (int)(m0 / w.group), 0);
     b.last = pos0 + (int)(m1 / w.group);
     b.low = key_span(pmin, a.window, a.sinks).low;
@@ -238,6 +246,13 @@ __device__ __forceinline__ void pp_st16(uint32_t addr, const uint32_t *r) {
                  PP_W8(r, 8), "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ void pp_ld8(uint32_t addr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : PP_R8(r, 0) : "r"(addr));
+}
+__device__ __forceinline__ void pp_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
 __device__ __forceinline__ void pp_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float pp_ex2(float x) {
@@ -301,18 +316,18 @@ struct PpReader {
 };
 
 template <bool KV8, int DIM>
-__global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __grid_constant__ PpMaps maps, PagedAttnArgs a, PpWork w) {
+__global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ PpMaps maps, PagedAttnArgs a, PpWork w) {
     using C = PpCfg<KV8, DIM>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ unsigned long long wsum[PP_WARPS], at_prefix;
+    __shared__ unsigned long long wsum[C::WARPS], at_prefix;
     __shared__ uint32_t at_seq;
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = tc::smem_u32(sm);
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BARS);
     uint64_t *kv_full = bars, *kv_empty = kv_full + C::SLOTS, *sc_full = kv_empty + C::SLOTS, *sc_empty = sc_full + PP_SC;
     uint64_t *seg_full = sc_empty + PP_SC, *seg_empty = seg_full + PP_SEG;
-    uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 4,
-             *o_full = q_full + 6, *mdone = q_full + 8, *raw_full = mdone + 1, *raw_empty = raw_full + C::RAW;
+    uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 6,
+             *mdone = q_full + 10, *raw_full = mdone + 1, *raw_empty = raw_full + C::RAW;
     uint32_t *slot_p = reinterpret_cast<uint32_t *>(sm + C::SLOT);
     float *scales = reinterpret_cast<float *>(sm + C::SC);
     uint32_t *masks = reinterpret_cast<uint32_t *>(sm + C::MASK);
@@ -327,18 +342,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
         }
         for (int i = 0; i < PP_SC; ++i) {
             tc::mbar_init(&sc_full[i], 4);
-            tc::mbar_init(&sc_empty[i], 8);
+            tc::mbar_init(&sc_empty[i], C::SW);
         }
         for (int i = 0; i < PP_SEG; ++i) {
             tc::mbar_init(&seg_full[i], 1);
-            tc::mbar_init(&seg_empty[i], 14);  // 4 tile warps, the copy and MMA warps, 8 softmax warps
+            tc::mbar_init(&seg_empty[i], 6 + C::SW);  // 4 tile warps, the copy and MMA warps, the softmax warps
         }
         tc::mbar_init(q_full, 4);
         tc::mbar_init(q_empty, 1);
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {  // [tile][score buffer]
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_ready[i], 4);
-            tc::mbar_init(&o_full[i], 1);
         }
         tc::mbar_init(mdone, 1);
         for (int i = 0; i < C::RAW; ++i) {
@@ -347,10 +361,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
         }
         tc::mbar_fence_init();
     }
-    if (warp == 12) tc::tmem_alloc(slot_p, 512);
+    if (warp == C::SW + 4) tc::tmem_alloc(slot_p, 512);
 
     // ---- numbering of the units: a warp takes a run of sequences
-    const uint32_t per = (a.n + PP_WARPS - 1) / PP_WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
+    const uint32_t per = (a.n + C::WARPS - 1) / C::WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
     unsigned long long mine = 0;
     for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane(a, w, b, i1));
     if (lane == 0) wsum[warp] = mine;
@@ -359,7 +373,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     tc::tc_fence_after();
     const uint32_t tmem = *slot_p;
     unsigned long long before = 0, all = 0;
-    for (int i = 0; i < PP_WARPS; ++i) {
+    for (int i = 0; i < C::WARPS; ++i) {
         if (i < warp) before += wsum[i];
         all += wsum[i];
     }
@@ -390,14 +404,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     if (!active) {
         // ---------------- nothing to compute
         if (tid == 0) w.recs[blockIdx.x].valid = 0;
-    } else if (warp < 8) {
-        // ---------------- softmax: thread = row r of tile `x`
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    } else if (warp < C::SW) {
+        // ---------------- softmax: thread = row r of MMA tile `x`
+        if constexpr (DIM == 64)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int x = warp >> 2, r = tid & 127;
         const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 (warp % 4) ..
-        const uint32_t s_addr = lane_addr + x * 128, o_addr = lane_addr + 256 + x * DIM;
+        const uint32_t s_base = lane_addr + x * (64 * C::NB), o_addr = lane_addr + 256 + x * DIM;
+        uint64_t *const s_bar = s_full + x * C::NB, *const p_bar = p_ready + x * C::NB;
         PpReader rd{ring, seg_full, seg_empty};
-        uint32_t bc = 0, ns = 0, no = 0;  // blocks of the CTA; scores and contexts of this tile
+        uint32_t bc = 0, round = 0;  // blocks of the CTA; rounds of this tile's score barriers before the segment
         PpSeg g;
         while (ok) {
             ok = rd.next(g, w.err);
@@ -419,108 +437,167 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             const int all_last = m_end == mt + 127 ? g.pos0 + (int)(mt / w.group) : -1;
             const int all_first = key_span(max(all_last, 0), a.window, a.sinks).first;
             const int all_low = key_span(max(g.pos0 + (int)(m_end / w.group), 0), a.window, a.sinks).low;
-            float m = -INFINITY, l = 0.f;
-            for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
-                const int vb = g.b0 + i, kb = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
-                const uint32_t st = bc % PP_SC;
-                ok = tc::mbar_wait(&sc_full[st], (bc / PP_SC) & 1, w.err, 61) &&
-                     tc::mbar_wait(&s_full[x], ns & 1, w.err, 62);
-                ok = __all_sync(0xffffffffu, ok);
+            // a row that sees nothing needs no maximum
+            float m = pos < 0 ? 0.f : -INFINITY, l = 0.f;
+            const uint32_t steps = 2 * g.nblk;
+            uint32_t st = 0;
+            int kb = 0;
+            for (uint32_t n = 0; n < steps && ok; ++n) {
+                const int h = n & 1;
+                if (h == 0) {
+                    const int vb = g.b0 + (int)(n >> 1);
+                    kb = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
+                    st = bc % PP_SC;
+                    ok = tc::mbar_wait(&sc_full[st], (bc / PP_SC) & 1, w.err, 61);
+                }
+                const uint32_t buf = n % C::NB, sh = s_base + 64 * buf;
+                ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&s_bar[buf], (round + n / C::NB) & 1, w.err, 62));
                 if (!ok) break;
-                ++ns;
                 tc::tc_fence_after();
-                float s[128];
+                const int k0 = kb + 64 * h;
+                const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256 + 64 * h), *vf = kf + 32;
+                const uint2 there = *reinterpret_cast<const uint2 *>(masks + 4 * st + 2 * h);
+                // every key visible to every row, and every row has a reference
+                const bool full = k0 + 63 <= all_last && (k0 >= all_low || k0 + 64 <= all_first) &&
+                                  (there.x & there.y) == 0xffffffffu;
+                bool done = false;
+                if (full && !__any_sync(0xffffffffu, m == -INFINITY)) {
+                    // A row takes a maximum only until it has a reference: 2^(x - m) may pass 1 by far (the step is
+                    // done again, with a maximum, where its weights sum to more than 2^15), and below it keeps its
+                    // relative precision in bf16 and fp32 alike.
+                    uint32_t p[32];
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    auto weights = [&](const float *s, int c) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) pp_ld32(s_addr + 32 * j, reinterpret_cast<uint32_t *>(s) + 32 * j);
-                pp_ld_wait();
-                if constexpr (KV8) {
-                    const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256);
+                        for (int j = 0; j < 32; j += 4) {
+                            float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
+                            if constexpr (KV8) {
+                                const float4 k4 = kf[8 * c + (j >> 2)];
+                                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
+                            }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float4 f = kf[j];
-                        s[4 * j] *= f.x;
-                        s[4 * j + 1] *= f.y;
-                        s[4 * j + 2] *= f.z;
-                        s[4 * j + 3] *= f.w;
+                            for (int k = 0; k < 4; ++k) {
+                                e[k] = pp_ex2(fmaf(s[j + k], f[k], -m));
+                                part[k] += e[k];
+                            }
+                            if constexpr (KV8) {
+                                const float4 v4 = vf[8 * c + (j >> 2)];
+                                e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
+                            }
+                            p[16 * c + j / 2] = pp_pack(e[0], e[1]);
+                            p[16 * c + j / 2 + 1] = pp_pack(e[2], e[3]);
+                        }
+                    };
+                    if constexpr (DIM == 64) {
+                        float s[32];
+                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
+                        pp_ld_wait();
+                        weights(s, 0);
+                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s));
+                        pp_ld_wait();
+                        weights(s, 1);
+                    } else {
+                        float s[64];
+                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
+                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s) + 32);
+                        pp_ld_wait();
+                        weights(s, 0);
+                        weights(s + 32, 1);
+                    }
+                    const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+                    done = !__any_sync(0xffffffffu, sum > 32768.f);
+                    if (done) {
+                        l += sum;
+                        pp_st32(sh, p);
                     }
                 }
-                const uint4 there = *reinterpret_cast<const uint4 *>(masks + 4 * st);
-                const bool full = kb + 127 <= all_last && (kb >= all_low || kb + 128 <= all_first) &&
-                                  (there.x & there.y & there.z & there.w) == 0xffffffffu;
-                if (!full) {
-                    const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
+                if (!done) {
+                    // ---- hidden keys, rows without a reference, sums too large: the maximum first, then
+                    // weights, 8 columns at a time (short code: it runs at the edges only)
+                    uint32_t bits[2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // bits of keys kb + 32 k ..: up to the row's position, from `low` on or before `first`
-                        auto below = [&](int e) {  // bits j with kb + 32 k + j < e
-                            const int n = e - (kb + 32 * k);
-                            return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+                    for (int k = 0; k < 2; ++k) {
+                        auto below = [&](int e) {  // bits j with k0 + 32 k + j < e
+                            const int d = e - (k0 + 32 * k);
+                            return d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
                         };
-                        const uint32_t bits = tw[k] & below(pos + 1) & (~below(low) | below(first));
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!(bits >> j & 1)) s[32 * k + j] = -INFINITY;
+                        bits[k] = (k ? there.y : there.x) & below(pos + 1) & (~below(low) | below(first));
                     }
-                }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
+                    auto scores = [&](int c, float (&y)[8]) {  // keys k0 + 8 c ..: x, or -inf where hidden
+                        pp_ld8(sh + 8 * c, reinterpret_cast<uint32_t *>(y));
+                        pp_ld_wait();
+                        const uint32_t bt = (c < 4 ? bits[0] : bits[1]) >> (8 * (c & 3));
+                        float4 f = make_float4(w.fac, w.fac, w.fac, w.fac), f2 = f;
+                        if constexpr (KV8) f = kf[2 * c], f2 = kf[2 * c + 1];
+                        const float ff[8] = {f.x, f.y, f.z, f.w, f2.x, f2.y, f2.z, f2.w};
 #pragma unroll
-                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if constexpr (!KV8) top *= w.fac;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                    const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
-                    m = up;
-                    l *= f;
-                    if (i > 0) {  // this tile's earlier products are complete (s_full follows them)
+                        for (int j = 0; j < 8; ++j) y[j] = bt >> j & 1 ? y[j] * ff[j] : -INFINITY;
+                    };
+                    float top = -INFINITY;
 #pragma unroll 1
-                        for (int j = 0; j < DIM; j += 16) {
-                            uint32_t o[16];
-                            pp_ld16(o_addr + j, o);
-                            pp_ld_wait();
+                    for (int c = 0; c < 8; ++c) {
+                        float y[8];
+                        scores(c, y);
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            pp_st16(o_addr + j, o);
+                        for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
+                    }
+                    if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                        const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
+                        m = up;
+                        l *= f;
+                        if (n > 0) {
+                            // every product into the context so far is complete: those over this buffer precede
+                            // its scores, that over the other buffer precedes that buffer's next scores
+                            if (C::NB == 2)
+                                ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
+                            if (!ok) break;
+                            tc::tc_fence_after();
+#pragma unroll 1
+                            for (int j = 0; j < DIM; j += 16) {
+                                uint32_t o[16];
+                                pp_ld16(o_addr + j, o);
+                                pp_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                pp_st16(o_addr + j, o);
+                            }
                         }
                     }
-                }
-                const float mu = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                const float4 *vf = reinterpret_cast<const float4 *>(scales + st * 256 + 128);
+                    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        float y[8];
+                        scores(c, y);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const int k = 64 * h + 2 * j;
-                        float e[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            e[c] = pp_ex2(KV8 ? s[k + c] - mu : fmaf(s[k + c], w.fac, -mu));
-                            sum[c] += e[c];
+                        for (int j = 0; j < 8; ++j) {
+                            y[j] = pp_ex2(y[j] - mu);
+                            l += y[j];
                         }
                         if constexpr (KV8) {
-                            const float4 f = vf[k >> 2];
-                            e[0] *= f.x;
-                            e[1] *= f.y;
-                            e[2] *= f.z;
-                            e[3] *= f.w;
+                            const float4 f = vf[2 * c], f2 = vf[2 * c + 1];
+                            y[0] *= f.x, y[1] *= f.y, y[2] *= f.z, y[3] *= f.w;
+                            y[4] *= f2.x, y[5] *= f2.y, y[6] *= f2.z, y[7] *= f2.w;
                         }
-                        p[j] = pp_pack(e[0], e[1]);
-                        p[j + 1] = pp_pack(e[2], e[3]);
+                        // over columns whose scores have been read
+                        pp_st4(sh + 4 * c, pp_pack(y[0], y[1]), pp_pack(y[2], y[3]), pp_pack(y[4], y[5]), pp_pack(y[6], y[7]));
                     }
-                    pp_st32(s_addr + 32 * h, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 pp_st_wait();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&p_ready[x]);
-                if (lane == 0) tc::mbar_arrive(&sc_empty[st]);
+                if (lane == 0) tc::mbar_arrive(&p_bar[buf]);
+                if (h == 1) {
+                    if (lane == 0) tc::mbar_arrive(&sc_empty[st]);
+                    ++bc;
+                }
             }
             if (!ok) break;
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], no & 1, w.err, 63));
+            // the last products: one more round of each barrier
+            round += steps / C::NB;
+            for (int b = 0; b < C::NB; ++b) ok = ok && tc::mbar_wait(&s_bar[b], round & 1, w.err, 63);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            ++no;
+            ++round;
             tc::tc_fence_after();
             const bool live = m_row < g.mrows && pos >= 0;
             if (g.piece < 0) {
@@ -549,8 +626,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                 float *piece = w.pieces + (uint64_t)g.piece * C::PIECE;
                 const int t = 128 * x + r;
                 piece[t] = m;
-                piece[PP_TILE + t] = l;
-                float *po = piece + 2 * PP_TILE + (uint64_t)t * DIM;
+                piece[C::TILE + t] = l;
+                float *po = piece + 2 * C::TILE + (uint64_t)t * DIM;
 #pragma unroll 1
                 for (int j = 0; j < DIM; j += 16) {
                     uint32_t o[16];
@@ -563,10 +640,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             }
             tc::tc_fence_before();
         }
-    } else if (warp < 12) {
+    } else if (warp < C::SW + 4) {
         // ---------------- tile warps: warp lw has keys 32 lw .. of each block
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int lw = warp - 8;
+        if constexpr (DIM == 64)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int lw = warp - C::SW;
         constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
         PpReader rd{ring, seg_full, seg_empty};
         uint32_t bc = 0, nseg = 0, tiles = 0;  // blocks; segments; K and V tiles
@@ -622,7 +702,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                     if (!ok) break;
                     ++nseg;
 #pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
+                    for (int x = 0; x < C::TILES; ++x) {
+                        if (g.m0 + 128 * x >= g.mrows) break;
                         const uint32_t mr = g.m0 + 128 * x + 32 * lw + lane;
                         const bool live = mr < g.mrows;
                         const uint64_t mine = live ? (g.row0 + (uint64_t)(mr / w.group)) * a.q_stride +
@@ -695,12 +776,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12) {
+        if constexpr (DIM == 64)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == C::SW + 4) {
             // ---------------- MMA issuer
             PpReader rd{ring, seg_full, seg_empty};
-            uint32_t bc = 0, nseg = 0, np[2] = {0, 0};
-            const uint32_t id_qk = pp_idesc(128, false) | (!KV8 && w.negate ? 1u << 13 : 0u);
+            uint32_t bc = 0, nseg = 0, round[C::TILES] = {};  // rounds of each tile's barriers before the segment
+            const uint32_t id_qk = pp_idesc(64, false) | (!KV8 && w.negate ? 1u << 13 : 0u);
             constexpr uint32_t id_pv = pp_idesc(DIM, true);
             const uint64_t q_desc = tc::smem_desc_sw128(sbase + C::Q), k_desc = tc::smem_desc_sw128(sbase + C::RING),
                            v_desc = pp_desc_mn(sbase + C::RING);
@@ -708,57 +792,55 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             while (ok) {
                 ok = rd.next(g, w.err);
                 if (!ok || g.nblk == 0) break;
-                const int tiles = g.m0 + 128 < g.mrows ? 2 : 1;
+                const int tiles = (int)min((g.mrows - g.m0 + 127) / 128, (uint32_t)C::TILES), steps = 2 * g.nblk;
                 if (pp_elect()) {
                     auto wait_tile = [&](uint32_t n) {
                         return tc::mbar_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
                     };
-                    // descriptors differ in their address field only: bases once, steps by adding
-                    auto qk = [&](int x, uint32_t n) {
-                        const uint64_t qd = q_desc + x * (C::TILE_BYTES >> 4), kd = k_desc + (n % C::SLOTS) * (C::TILE_BYTES >> 4);
-#pragma unroll
-                        for (int j = 0; j < DIM / 16; ++j) {
-                            const uint32_t off = ((j >> 2) * (128 * 128) + (j & 3) * 32) >> 4;
-                            pp_mma_ss(tmem + 128 * x, qd + off, kd + off, id_qk, j > 0);
-                        }
-                        tc::mma_commit(&s_full[x]);
-                    };
+                    // step n: the weights' product of step n - NB, then the scores of step n over its
+                    // columns; descriptors differ in their address field only
                     ok = tc::mbar_wait(q_full, nseg & 1, w.err, 68);
-                    // block i: the weights' product of block i - 1, then the scores of block i
-                    for (int i = 0; i <= g.nblk && ok; ++i) {
-                        const uint32_t kt = 2 * (bc + i);
+                    for (int n = 0; n < steps + C::NB && ok; ++n) {
+                        const int pn = n - C::NB, h = n & 1, ph = pn & 1;
+                        const bool scores = n < steps, product = pn >= 0;
+                        const uint32_t kt = 2 * (bc + n / 2), vt = 2 * (bc + pn / 2) + 1;
+                        if (scores && h == 0) ok = wait_tile(kt);
+                        if (ok && product && ph == 0) ok = wait_tile(vt);
+                        const uint32_t buf = n % C::NB;
                         for (int x = 0; x < tiles && ok; ++x) {
-                            const bool final = x == tiles - 1;
-                            if (i > 0) {
-                                ok = tc::mbar_wait(&p_ready[x], (np[x] + i - 1) & 1, w.err, 69) && (x > 0 || wait_tile(kt - 1));
-                                if (!ok) break;
-                                tc::tc_fence_after();
-                                const uint64_t vd = v_desc + ((kt - 1) % C::SLOTS) * (C::TILE_BYTES >> 4);
+                            const uint32_t sc = tmem + 64 * (x * C::NB + buf);
+                            if (product) ok = tc::mbar_wait(&p_ready[x * C::NB + buf], (round[x] + pn / C::NB) & 1, w.err, 69);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            if (product) {
+                                const uint64_t vd = v_desc + (((vt % C::SLOTS) * C::TILE_BYTES + ph * 8192) >> 4);
 #pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    pp_mma_ts(tmem + 256 + x * DIM, tmem + 128 * x + 8 * j, vd + j * (2048 >> 4), id_pv,
-                                              i > 1 || j > 0);
-                                if (final) tc::mma_commit(&kv_empty[(kt - 1) % C::SLOTS]);
+                                for (int j = 0; j < 4; ++j)
+                                    pp_mma_ts(tmem + 256 + x * DIM, sc + 8 * j, vd + j * (2048 >> 4), id_pv, pn > 0 || j > 0);
                             }
-                            if (i < g.nblk) {
-                                if (x == 0) ok = wait_tile(kt);
-                                if (!ok) break;
-                                tc::tc_fence_after();
-                                qk(x, kt);
-                                if (final) {
-                                    tc::mma_commit(&kv_empty[kt % C::SLOTS]);
-                                    if (i + 1 == g.nblk) tc::mma_commit(q_empty);
+                            if (scores) {
+                                const uint64_t qd = q_desc + ((x * C::TILE_BYTES) >> 4),
+                                               kd = k_desc + (((kt % C::SLOTS) * C::TILE_BYTES + h * 8192) >> 4);
+#pragma unroll
+                                for (int j = 0; j < DIM / 16; ++j) {
+                                    const uint32_t off = ((j >> 2) * (128 * 128) + (j & 3) * 32) >> 4;
+                                    pp_mma_ss(sc, qd + off, kd + off, id_qk, j > 0);
                                 }
-                            } else {
-                                tc::mma_commit(&o_full[x]);
                             }
+                            tc::mma_commit(&s_full[x * C::NB + buf]);
+                        }
+                        if (ok && product && ph == 1) tc::mma_commit(&kv_empty[vt % C::SLOTS]);
+                        if (ok && scores && h == 1) {
+                            tc::mma_commit(&kv_empty[kt % C::SLOTS]);
+                            if (n + 1 == steps) tc::mma_commit(q_empty);
                         }
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 bc += g.nblk;
-                np[0] += g.nblk;
-                if (tiles == 2) np[1] += g.nblk;
+#pragma unroll
+                for (int x = 0; x < C::TILES; ++x)
+                    if (x < tiles) round[x] += steps / C::NB;
                 ++nseg;
             }
             // every MMA is complete before TMEM is freed
@@ -767,7 +849,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                 tc::mbar_wait(mdone, 0, w.err, 69);
             }
             __syncwarp();
-        } else if (warp == 15) {
+        } else if (warp == C::SW + 7) {
             // ---------------- copies: lane p has page p of a block (its first 128 tokens' worth
             // of it); KV8 pages as runs of codes, bf16 pages as swizzled boxes
             PpReader rd{ring, seg_full, seg_empty};
@@ -823,7 +905,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                     }
                 }
             }
-        } else if (warp == 13) {
+        } else if (warp == C::SW + 5) {
             // ---------------- segments
             uint32_t n = 0;
             uint32_t i = at_seq;
@@ -872,7 +954,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
                         if (cnt > 0) {
                             g.seq = s.seq;
                             g.row0 = s.row0;
-                            g.m0 = (uint32_t)k * PP_TILE;
+                            g.m0 = (uint32_t)k * C::TILE;
                             g.mrows = s.mrows;
                             g.pos0 = s.pos0;
                             g.kvh = kvh;
@@ -926,7 +1008,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
             }
         }
     }
-    if (warp == 14) {
+    if (warp == C::SW + 6) {
         // ---------------- rows in front of the first token, and of no sequence
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
             const PpSeqInfo s = pp_seq(a, w, i);
@@ -939,7 +1021,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == C::SW + 4) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
@@ -949,7 +1031,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const __gr
 // middle CTA c starts, if c is the tile's second CTA; 8 threads per row.
 template <int DIM>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(PagedAttnArgs a, PpWork w) {
-    constexpr int PIECE = 2 * PP_TILE + PP_TILE * DIM, PER = DIM / 8;
+    constexpr int TILE = PpCfg<false, DIM>::TILE, PIECE = 2 * TILE + TILE * DIM, PER = DIM / 8;
     pdl_wait();
     const PpRec rec = w.recs[blockIdx.x];
     if (!rec.valid || rec.c0 + 1 != blockIdx.x) return;
@@ -966,8 +1048,8 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(PagedAttnArgs a
     for (uint32_t i = 0; i < n; ++i) {
         const float *p = piece(i);
         const float f = pp_ex2(p[t] - M0);
-        L += p[PP_TILE + t] * f;
-        const float4 *o = reinterpret_cast<const float4 *>(p + 2 * PP_TILE + (uint64_t)t * DIM + d0);
+        L += p[TILE + t] * f;
+        const float4 *o = reinterpret_cast<const float4 *>(p + 2 * TILE + (uint64_t)t * DIM + d0);
 #pragma unroll
         for (int j = 0; j < PER / 4; ++j) {
             const float4 v = o[j];
@@ -990,7 +1072,8 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(PagedAttnArgs a
 }
 
 size_t paged_prefill_ws(uint32_t, uint32_t, uint32_t dim, uint32_t, uint32_t) {
-    return 256 + (size_t)PP_MAX_SMS * (sizeof(PpRec) + 2 * (2 * PP_TILE + PP_TILE * (size_t)dim) * 4);
+    const size_t tile = dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
+    return 256 + (size_t)PP_MAX_SMS * (sizeof(PpRec) + 2 * (2 * tile + tile * dim) * 4);
 }
 
 template <bool KV8, int DIM>
@@ -1006,8 +1089,8 @@ static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t 
         if (int rc = make_page_map(&maps.v, a.c.v, DIM, rows, a.c.pages, stride, box)) return rc;
     }
     PdlChain chain;
-    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PF_THREADS), C::ALLOC, st, 1, maps, a, w)) return rc;
-    return launch_pdl(paged_prefill_join_kernel<DIM>, dim3(w.max_ctas, PP_TILE / 32), dim3(256), 0, st, 1, a, w);
+    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(C::THREADS), C::ALLOC, st, 1, maps, a, w)) return rc;
+    return launch_pdl(paged_prefill_join_kernel<DIM>, dim3(w.max_ctas, C::TILE / 32), dim3(256), 0, st, 1, a, w);
 }
 
 int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
@@ -1016,6 +1099,7 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     PpWork w;
     w.group = a.qh / a.c.hkv;
     w.max_ctas = (uint32_t)(sms < PP_MAX_SMS ? sms : PP_MAX_SMS);
+    w.tile = a.dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
     w.negate = a.scale < 0.f;
     const float f = fabsf(a.scale) * 1.44269504f;
     w.fac = f > 1e-30f ? f : 1e-30f;  // a scale of 0 leaves masked scores at -inf
