@@ -36,9 +36,10 @@
 //             bf16, bf16 values that are not visible to 0 (what a page
 //             holds there never reaches the products); 128-byte swizzled
 //             K-major tiles, the value tile read as an MN-major operand
-//   then 1    one thread issues the MMAs
-//   1         walks the units and publishes segments (tile, KV head, block range)
-//   1         zeroes the rows in front of a sequence's first token
+//   then 2    a thread of each issues the MMAs of every second tile (with one
+//             issuer the tensor cores idled while it waited for the next weights)
+//   1         walks the units and publishes segments (tile, KV head, block
+//             range), then zeroes the rows in front of a sequence's first token
 //   1         copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
 // Bound by the exponentials at 64 dims (16 per clock and SM), by them and the
 // tensor cores alike at 128. Every wait is bounded (error codes 57-69).
@@ -246,13 +247,6 @@ __device__ __forceinline__ void pp_st16(uint32_t addr, const uint32_t *r) {
                  PP_W8(r, 8), "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ void pp_ld8(uint32_t addr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : PP_R8(r, 0) : "r"(addr));
-}
-__device__ __forceinline__ void pp_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-                 : "memory");
-}
 __device__ __forceinline__ void pp_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float pp_ex2(float x) {
@@ -338,7 +332,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; ++i) {
             tc::mbar_init(&kv_full[i], KV8 || (i & 1) ? 4 : 1);  // the converting warps; bf16 keys: the copy itself
-            tc::mbar_init(&kv_empty[i], 1);
+            tc::mbar_init(&kv_empty[i], 2);  // both issuers
         }
         for (int i = 0; i < PP_SC; ++i) {
             tc::mbar_init(&sc_full[i], 4);
@@ -346,15 +340,15 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
         }
         for (int i = 0; i < PP_SEG; ++i) {
             tc::mbar_init(&seg_full[i], 1);
-            tc::mbar_init(&seg_empty[i], 6 + C::SW);  // 4 tile warps, the copy and MMA warps, the softmax warps
+            tc::mbar_init(&seg_empty[i], 7 + C::SW);  // 4 tile warps, the copy warp, 2 issuers, the softmax warps
         }
         tc::mbar_init(q_full, 4);
-        tc::mbar_init(q_empty, 1);
+        tc::mbar_init(q_empty, 2);
         for (int i = 0; i < 4; ++i) {  // [tile][score buffer]
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_ready[i], 4);
         }
-        tc::mbar_init(mdone, 1);
+        tc::mbar_init(mdone, 2);
         for (int i = 0; i < C::RAW; ++i) {
             tc::mbar_init(&raw_full[i], 1);
             tc::mbar_init(&raw_empty[i], 4);
@@ -512,8 +506,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     }
                 }
                 if (!done) {
-                    // ---- hidden keys, rows without a reference, sums too large: the maximum first, then
-                    // weights, 8 columns at a time (short code: it runs at the edges only)
+                    // ---- hidden keys, rows without a reference, sums too large: the maximum first, then the
+                    // weights, in loops of 32 columns (short code: it runs at the edges only)
                     uint32_t bits[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
@@ -523,63 +517,76 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         };
                         bits[k] = (k ? there.y : there.x) & below(pos + 1) & (~below(low) | below(first));
                     }
-                    auto scores = [&](int c, float (&y)[8]) {  // keys k0 + 8 c ..: x, or -inf where hidden
-                        pp_ld8(sh + 8 * c, reinterpret_cast<uint32_t *>(y));
+                    auto scores = [&](int c, float (&y)[32]) {  // keys k0 + 32 c ..: x, or -inf where hidden
+                        pp_ld32(sh + 32 * c, reinterpret_cast<uint32_t *>(y));
                         pp_ld_wait();
-                        const uint32_t bt = (c < 4 ? bits[0] : bits[1]) >> (8 * (c & 3));
-                        float4 f = make_float4(w.fac, w.fac, w.fac, w.fac), f2 = f;
-                        if constexpr (KV8) f = kf[2 * c], f2 = kf[2 * c + 1];
-                        const float ff[8] = {f.x, f.y, f.z, f.w, f2.x, f2.y, f2.z, f2.w};
+                        const uint32_t bt = c ? bits[1] : bits[0];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) y[j] = bt >> j & 1 ? y[j] * ff[j] : -INFINITY;
+                        for (int j = 0; j < 32; j += 4) {
+                            float4 f = make_float4(w.fac, w.fac, w.fac, w.fac);
+                            if constexpr (KV8) f = kf[8 * c + (j >> 2)];
+                            y[j] = bt & (1u << j) ? y[j] * f.x : -INFINITY;
+                            y[j + 1] = bt & (2u << j) ? y[j + 1] * f.y : -INFINITY;
+                            y[j + 2] = bt & (4u << j) ? y[j + 2] * f.z : -INFINITY;
+                            y[j + 3] = bt & (8u << j) ? y[j + 3] * f.w : -INFINITY;
+                        }
                     };
-                    float top = -INFINITY;
+                    if (!__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
+                        // no key for any of the warp's rows
+                        const uint32_t zero[32] = {};
+                        pp_st32(sh, zero);
+                    } else {
+                        float top = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        float y[8];
-                        scores(c, y);
+                        for (int c = 0; c < 2; ++c) {
+                            float y[32];
+                            scores(c, y);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
-                    }
-                    if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                        const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
-                        m = up;
-                        l *= f;
-                        if (n > 0) {
-                            // every product into the context so far is complete: those over this buffer precede
-                            // its scores, that over the other buffer precedes that buffer's next scores
-                            if (C::NB == 2)
-                                ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
-                            if (!ok) break;
-                            tc::tc_fence_after();
+                            for (int j = 0; j < 32; ++j) top = fmaxf(top, y[j]);
+                        }
+                        if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                            const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
+                            m = up;
+                            l *= f;
+                            if (n > 0) {
+                                // every product into the context so far is complete: those over this buffer precede
+                                // its scores, that over the other buffer precedes that buffer's next scores
+                                if (C::NB == 2)
+                                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
+                                if (!ok) break;
+                                tc::tc_fence_after();
 #pragma unroll 1
-                            for (int j = 0; j < DIM; j += 16) {
-                                uint32_t o[16];
-                                pp_ld16(o_addr + j, o);
-                                pp_ld_wait();
+                                for (int j = 0; j < DIM; j += 16) {
+                                    uint32_t o[16];
+                                    pp_ld16(o_addr + j, o);
+                                    pp_ld_wait();
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                pp_st16(o_addr + j, o);
+                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                    pp_st16(o_addr + j, o);
+                                }
                             }
                         }
-                    }
-                    const float mu = m == -INFINITY ? 0.f : m;
+                        const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        float y[8];
-                        scores(c, y);
+                        for (int c = 0; c < 2; ++c) {
+                            float y[32];
+                            uint32_t p[16];
+                            scores(c, y);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            y[j] = pp_ex2(y[j] - mu);
-                            l += y[j];
+                            for (int j = 0; j < 32; j += 4) {
+                                float part[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) part[k] = y[j + k] = pp_ex2(y[j + k] - mu);
+                                l += (part[0] + part[1]) + (part[2] + part[3]);
+                                if constexpr (KV8) {
+                                    const float4 f = vf[8 * c + (j >> 2)];
+                                    y[j] *= f.x, y[j + 1] *= f.y, y[j + 2] *= f.z, y[j + 3] *= f.w;
+                                }
+                                p[j / 2] = pp_pack(y[j], y[j + 1]);
+                                p[j / 2 + 1] = pp_pack(y[j + 2], y[j + 3]);
+                            }
+                            pp_st16(sh + 16 * c, p);  // over columns whose scores have been read
                         }
-                        if constexpr (KV8) {
-                            const float4 f = vf[2 * c], f2 = vf[2 * c + 1];
-                            y[0] *= f.x, y[1] *= f.y, y[2] *= f.z, y[3] *= f.w;
-                            y[4] *= f2.x, y[5] *= f2.y, y[6] *= f2.z, y[7] *= f2.w;
-                        }
-                        // over columns whose scores have been read
-                        pp_st4(sh + 4 * c, pp_pack(y[0], y[1]), pp_pack(y[2], y[3]), pp_pack(y[4], y[5]), pp_pack(y[6], y[7]));
                     }
                 }
                 pp_st_wait();
@@ -780,10 +787,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         else
             asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == C::SW + 4) {
-            // ---------------- MMA issuer
+        if (warp < C::SW + 6) {
+            // ---------------- MMA issuers: tiles `who`, who + 2
+            const int who = warp - (C::SW + 4);
             PpReader rd{ring, seg_full, seg_empty};
-            uint32_t bc = 0, nseg = 0, round[C::TILES] = {};  // rounds of each tile's barriers before the segment
+            uint32_t bc = 0, nseg = 0, round[C::TILES / 2] = {};  // rounds of the tiles' barriers before the segment
             const uint32_t id_qk = pp_idesc(64, false) | (!KV8 && w.negate ? 1u << 13 : 0u);
             constexpr uint32_t id_pv = pp_idesc(DIM, true);
             const uint64_t q_desc = tc::smem_desc_sw128(sbase + C::Q), k_desc = tc::smem_desc_sw128(sbase + C::RING),
@@ -792,7 +800,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             while (ok) {
                 ok = rd.next(g, w.err);
                 if (!ok || g.nblk == 0) break;
-                const int tiles = (int)min((g.mrows - g.m0 + 127) / 128, (uint32_t)C::TILES), steps = 2 * g.nblk;
+                const int all_tiles = (int)min((g.mrows - g.m0 + 127) / 128, (uint32_t)C::TILES);
+                const int tiles = (all_tiles + 1 - who) / 2, steps = 2 * g.nblk;  // this issuer's
                 if (pp_elect()) {
                     auto wait_tile = [&](uint32_t n) {
                         return tc::mbar_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
@@ -807,9 +816,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         if (scores && h == 0) ok = wait_tile(kt);
                         if (ok && product && ph == 0) ok = wait_tile(vt);
                         const uint32_t buf = n % C::NB;
-                        for (int x = 0; x < tiles && ok; ++x) {
+#pragma unroll
+                        for (int t = 0; t < C::TILES / 2; ++t) {
+                            if (t >= tiles || !ok) break;
+                            const int x = 2 * t + who;
                             const uint32_t sc = tmem + 64 * (x * C::NB + buf);
-                            if (product) ok = tc::mbar_wait(&p_ready[x * C::NB + buf], (round[x] + pn / C::NB) & 1, w.err, 69);
+                            if (product) ok = tc::mbar_wait(&p_ready[x * C::NB + buf], (round[t] + pn / C::NB) & 1, w.err, 69);
                             if (!ok) break;
                             tc::tc_fence_after();
                             if (product) {
@@ -829,6 +841,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             }
                             tc::mma_commit(&s_full[x * C::NB + buf]);
                         }
+                        // an issuer without a tile here only lets the slots go (its commit follows nothing)
                         if (ok && product && ph == 1) tc::mma_commit(&kv_empty[vt % C::SLOTS]);
                         if (ok && scores && h == 1) {
                             tc::mma_commit(&kv_empty[kt % C::SLOTS]);
@@ -839,8 +852,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 ok = __all_sync(0xffffffffu, ok);
                 bc += g.nblk;
 #pragma unroll
-                for (int x = 0; x < C::TILES; ++x)
-                    if (x < tiles) round[x] += steps / C::NB;
+                for (int t = 0; t < C::TILES / 2; ++t)
+                    if (t < tiles) round[t] += steps / C::NB;
                 ++nseg;
             }
             // every MMA is complete before TMEM is freed
@@ -905,7 +918,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     }
                 }
             }
-        } else if (warp == C::SW + 5) {
+        } else if (warp == C::SW + 6) {
             // ---------------- segments
             uint32_t n = 0;
             uint32_t i = at_seq;
@@ -1008,7 +1021,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             }
         }
     }
-    if (warp == C::SW + 6) {
+    if (warp == C::SW + 6) {  // (behind its segments)
         // ---------------- rows in front of the first token, and of no sequence
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
             const PpSeqInfo s = pp_seq(a, w, i);
