@@ -43,6 +43,8 @@
 //   1         copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
 // Bound by the exponentials at 64 dims (16 per clock and SM), by them and the
 // tensor cores alike at 128. Every wait is bounded (error codes 57-69).
+#include <type_traits>
+
 #include "kernels.h"
 #include "paged.cuh"
 #include "tc05.cuh"
@@ -246,6 +248,12 @@ __device__ __forceinline__ void pp_st16(uint32_t addr, const uint32_t *r) {
                      r, 0),
                  PP_W8(r, 8), "r"(addr)
                  : "memory");
+}
+__device__ __forceinline__ void pp_ld8(uint32_t addr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : PP_R8(r, 0) : "r"(addr));
+}
+__device__ __forceinline__ void pp_st8(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::PP_W8(r, 0), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void pp_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -451,109 +459,94 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 const int k0 = kb + 64 * h;
                 const float4 *kf = reinterpret_cast<const float4 *>(scales + st * 256 + 64 * h), *vf = kf + 32;
                 const uint2 there = *reinterpret_cast<const uint2 *>(masks + 4 * st + 2 * h);
-                // every key visible to every row, and every row has a reference
+                // the 64 keys' visibility to this row
+                uint32_t bits[2] = {there.x, there.y};
                 const bool full = k0 + 63 <= all_last && (k0 >= all_low || k0 + 64 <= all_first) &&
                                   (there.x & there.y) == 0xffffffffu;
-                bool done = false;
-                if (full && !__any_sync(0xffffffffu, m == -INFINITY)) {
-                    // A row takes a maximum only until it has a reference: 2^(x - m) may pass 1 by far (the step is
-                    // done again, with a maximum, where its weights sum to more than 2^15), and below it keeps its
-                    // relative precision in bf16 and fp32 alike.
-                    uint32_t p[32];
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-                    auto weights = [&](const float *s, int c) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
-                            if constexpr (KV8) {
-                                const float4 k4 = kf[8 * c + (j >> 2)];
-                                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                e[k] = pp_ex2(fmaf(s[j + k], f[k], -m));
-                                part[k] += e[k];
-                            }
-                            if constexpr (KV8) {
-                                const float4 v4 = vf[8 * c + (j >> 2)];
-                                e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
-                            }
-                            p[16 * c + j / 2] = pp_pack(e[0], e[1]);
-                            p[16 * c + j / 2 + 1] = pp_pack(e[2], e[3]);
-                        }
-                    };
-                    if constexpr (DIM == 64) {
-                        float s[32];
-                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
-                        pp_ld_wait();
-                        weights(s, 0);
-                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s));
-                        pp_ld_wait();
-                        weights(s, 1);
-                    } else {
-                        float s[64];
-                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
-                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s) + 32);
-                        pp_ld_wait();
-                        weights(s, 0);
-                        weights(s + 32, 1);
-                    }
-                    const float sum = (part[0] + part[1]) + (part[2] + part[3]);
-                    done = !__any_sync(0xffffffffu, sum > 32768.f);
-                    if (done) {
-                        l += sum;
-                        pp_st32(sh, p);
-                    }
-                }
-                if (!done) {
-                    // ---- hidden keys, rows without a reference, sums too large: the maximum first, then the
-                    // weights, in loops of 32 columns (short code: it runs at the edges only)
-                    uint32_t bits[2];
+                if (!full) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         auto below = [&](int e) {  // bits j with k0 + 32 k + j < e
                             const int d = e - (k0 + 32 * k);
                             return d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1;
                         };
-                        bits[k] = (k ? there.y : there.x) & below(pos + 1) & (~below(low) | below(first));
+                        bits[k] &= below(pos + 1) & (~below(low) | below(first));
                     }
-                    auto scores = [&](int c, float (&y)[32]) {  // keys k0 + 32 c ..: x, or -inf where hidden
-                        pp_ld32(sh + 32 * c, reinterpret_cast<uint32_t *>(y));
-                        pp_ld_wait();
-                        const uint32_t bt = c ? bits[1] : bits[0];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float4 f = make_float4(w.fac, w.fac, w.fac, w.fac);
-                            if constexpr (KV8) f = kf[8 * c + (j >> 2)];
-                            y[j] = bt & (1u << j) ? y[j] * f.x : -INFINITY;
-                            y[j + 1] = bt & (2u << j) ? y[j + 1] * f.y : -INFINITY;
-                            y[j + 2] = bt & (4u << j) ? y[j + 2] * f.z : -INFINITY;
-                            y[j + 3] = bt & (8u << j) ? y[j + 3] * f.w : -INFINITY;
-                        }
-                    };
-                    if (!__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
-                        // no key for any of the warp's rows
-                        const uint32_t zero[32] = {};
-                        pp_st32(sh, zero);
-                    } else {
-                        float top = -INFINITY;
+                }
+                // The weights, CW columns at a time in a loop whose code stays in the instruction cache. A row takes
+                // the maximum of CW keys only until it has a reference: 2^(x - m) may pass 1 by far, and below it keeps
+                // its relative precision in bf16 and fp32 alike; only where CW weights sum to more than 2^15 the
+                // reference goes up, by a whole number, so that what is done is rescaled exactly.
+                constexpr int CW = DIM == 64 ? 16 : 32;
+                auto step = [&](auto masked) {
 #pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            float y[32];
-                            scores(c, y);
+                    for (int c = 0; c < 64 / CW; ++c) {
+                        float s[CW];
+                        if constexpr (CW == 16)
+                            pp_ld16(sh + CW * c, reinterpret_cast<uint32_t *>(s));
+                        else
+                            pp_ld32(sh + CW * c, reinterpret_cast<uint32_t *>(s));
+                        const float4 *kc = kf + CW / 4 * c;
+                        uint32_t bt = 0xffffffffu;
+                        if constexpr (masked.value) bt = CW == 32 ? bits[c] : bits[c >> 1] >> (16 * (c & 1)) & 0xffffu;
+                        uint32_t p[CW / 2];
+                        float sum;
+                        pp_ld_wait();
+                        auto weights = [&](float mu) {
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) top = fmaxf(top, y[j]);
-                        }
-                        if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                            const float up = fmaxf(top, m), f = up == m ? 1.f : pp_ex2(m - up);
-                            m = up;
-                            l *= f;
+                            for (int j = 0; j < CW; j += 4) {
+                                float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
+                                if constexpr (KV8) {
+                                    const float4 k4 = kc[j >> 2];
+                                    f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
+                                }
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    float y = fmaf(s[j + k], f[k], -mu);
+                                    if constexpr (masked.value) y = bt & (1u << (j + k)) ? y : -INFINITY;
+                                    e[k] = pp_ex2(y);
+                                    part[k] += e[k];
+                                }
+                                if constexpr (KV8) {
+                                    const float4 v4 = vf[CW / 4 * c + (j >> 2)];
+                                    e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
+                                }
+                                p[j / 2] = pp_pack(e[0], e[1]);
+                                p[j / 2 + 1] = pp_pack(e[2], e[3]);
+                            }
+                            sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        };
+                        bool lift = m == -INFINITY && bt != 0;
+                        weights(m == -INFINITY ? 0.f : m);
+                        lift |= sum > 32768.f;
+                        if (__builtin_expect(__any_sync(0xffffffffu, lift), 0)) {
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < CW; ++j) {
+                                const float f = KV8 ? reinterpret_cast<const float *>(kc)[j] : w.fac;
+                                top = fmaxf(top, bt & (1u << j) ? s[j] * f : -INFINITY);
+                            }
+                            // 2^-by in two factors (nothing that counts is that far below: 0 beyond 2^-252)
+                            float f = 1.f, f2 = 1.f;
+                            if (lift) {
+                                const float by = ceilf(top - m);
+                                if (m == -INFINITY || by > 252.f) {
+                                    f = 0.f;
+                                    m = top;
+                                } else if (by > 0.f) {
+                                    const int d = (int)by;
+                                    f = pow2i(-(d >> 1));
+                                    f2 = pow2i(-(d - (d >> 1)));
+                                    m += by;
+                                }
+                            }
+                            l = l * f * f2;
                             if (n > 0) {
                                 // every product into the context so far is complete: those over this buffer precede
                                 // its scores, that over the other buffer precedes that buffer's next scores
                                 if (C::NB == 2)
                                     ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
-                                if (!ok) break;
                                 tc::tc_fence_after();
 #pragma unroll 1
                                 for (int j = 0; j < DIM; j += 16) {
@@ -561,34 +554,38 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     pp_ld16(o_addr + j, o);
                                     pp_ld_wait();
 #pragma unroll
-                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f * f2);
                                     pp_st16(o_addr + j, o);
                                 }
                             }
-                        }
-                        const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            float y[32];
-                            uint32_t p[16];
-                            scores(c, y);
+                            for (int j = 0; j < CW / 2 * c; j += 8) {  // this step's weights so far
+                                uint32_t o[8];
+                                pp_st_wait();
+                                pp_ld8(sh + j, o);
+                                pp_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                float part[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) part[k] = y[j + k] = pp_ex2(y[j + k] - mu);
-                                l += (part[0] + part[1]) + (part[2] + part[3]);
-                                if constexpr (KV8) {
-                                    const float4 f = vf[8 * c + (j >> 2)];
-                                    y[j] *= f.x, y[j + 1] *= f.y, y[j + 2] *= f.z, y[j + 3] *= f.w;
-                                }
-                                p[j / 2] = pp_pack(y[j], y[j + 1]);
-                                p[j / 2 + 1] = pp_pack(y[j + 2], y[j + 3]);
+                                for (int k = 0; k < 8; ++k) o[k] = pp_pack(bflo(o[k]) * f * f2, bfhi(o[k]) * f * f2);
+                                pp_st8(sh + j, o);
                             }
-                            pp_st16(sh + 16 * c, p);  // over columns whose scores have been read
+                            weights(m == -INFINITY ? 0.f : m);
                         }
+                        l += sum;
+                        if constexpr (CW == 16)
+                            pp_st8(sh + CW / 2 * c, p);  // over columns whose scores have been read
+                        else
+                            pp_st16(sh + CW / 2 * c, p);
                     }
+                };
+                if (full) {
+                    step(std::false_type{});
+                } else if (__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
+                    step(std::true_type{});
+                } else {
+                    const uint32_t zero[32] = {};
+                    pp_st32(sh, zero);
                 }
+                if (!ok) break;
                 pp_st_wait();
                 tc::tc_fence_before();
                 __syncwarp();
