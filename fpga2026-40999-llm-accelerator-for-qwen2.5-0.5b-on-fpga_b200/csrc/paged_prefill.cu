@@ -477,18 +477,15 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 // the maximum of CW keys only until it has a reference: 2^(x - m) may pass 1 by far, and below it keeps
                 // its relative precision in bf16 and fp32 alike; only where CW weights sum to more than 2^15 the
                 // reference goes up, by a whole number, so that what is done is rescaled exactly.
-                constexpr int CW = DIM == 64 ? 16 : 32;
+                constexpr int CW = 16;
                 auto step = [&](auto masked) {
 #pragma unroll 1
                     for (int c = 0; c < 64 / CW; ++c) {
                         float s[CW];
-                        if constexpr (CW == 16)
-                            pp_ld16(sh + CW * c, reinterpret_cast<uint32_t *>(s));
-                        else
-                            pp_ld32(sh + CW * c, reinterpret_cast<uint32_t *>(s));
+                        pp_ld16(sh + CW * c, reinterpret_cast<uint32_t *>(s));
                         const float4 *kc = kf + CW / 4 * c;
                         uint32_t bt = 0xffffffffu;
-                        if constexpr (masked.value) bt = CW == 32 ? bits[c] : bits[c >> 1] >> (16 * (c & 1)) & 0xffffu;
+                        if constexpr (masked.value) bt = (c < 2 ? bits[0] : bits[1]) >> (16 * (c & 1)) & 0xffffu;
                         uint32_t p[CW / 2];
                         float sum;
                         pp_ld_wait();
@@ -571,13 +568,49 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             weights(m == -INFINITY ? 0.f : m);
                         }
                         l += sum;
-                        if constexpr (CW == 16)
-                            pp_st8(sh + CW / 2 * c, p);  // over columns whose scores have been read
-                        else
-                            pp_st16(sh + CW / 2 * c, p);
+                        pp_st8(sh + CW / 2 * c, p);  // over columns whose scores have been read
                     }
                 };
-                if (full) {
+                bool done = false;
+                if constexpr (DIM == 128) {
+                    // two warps of a scheduler are not enough to hide that loop's latencies: 64 columns at once
+                    // (630 us against 554 for the benchmark's longest prompts; at 64 dims, with four warps, the
+                    // unrolled code is the slower one, 594 against 391 us)
+                    if (full && !__any_sync(0xffffffffu, m == -INFINITY)) {
+                        float s[64], part[4] = {0.f, 0.f, 0.f, 0.f};
+                        uint32_t p[32];
+                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
+                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s) + 32);
+                        pp_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 64; j += 4) {
+                            float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
+                            if constexpr (KV8) {
+                                const float4 k4 = kf[j >> 2];
+                                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                e[k] = pp_ex2(fmaf(s[j + k], f[k], -m));
+                                part[k] += e[k];
+                            }
+                            if constexpr (KV8) {
+                                const float4 v4 = vf[j >> 2];
+                                e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
+                            }
+                            p[j / 2] = pp_pack(e[0], e[1]);
+                            p[j / 2 + 1] = pp_pack(e[2], e[3]);
+                        }
+                        const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        done = !__any_sync(0xffffffffu, sum > 32768.f);
+                        if (done) {
+                            l += sum;
+                            pp_st32(sh, p);
+                        }
+                    }
+                }
+                if (done) {
+                } else if (DIM == 64 && full) {
                     step(std::false_type{});
                 } else if (__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
                     step(std::true_type{});
