@@ -409,13 +409,13 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     x = fmaxf(x, m[h]);
-                    const float f = m[h] == x ? 1.f : ex2(m[h] - x);
+                    const float f = m[h] == x ? 1.f : ex2(0.5f * (m[h] - x));
                     m[h] = x;
-                    l[h] *= f;
+                    l[h] = l[h] * f * f;
 #pragma unroll
                     for (int j = 0; j < KS; ++j) {
-                        o[j][h] *= f;
-                        o[j][h + 2] *= f;
+                        o[j][h] = o[j][h] * f * f;
+                        o[j][h + 2] = o[j][h + 2] * f * f;
                     }
                 }
             }
@@ -532,9 +532,9 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             const float M0 = M == -INFINITY ? 0.f : M;
 #pragma unroll
             for (int i = 0; i < PD_WARPS; ++i) {
-                const float f = ex2(wm[i][h] - M0);
-                L += wl[i][h] * f;
-                O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f;
+                const float f = ex2(0.5f * (wm[i][h] - M0));  // applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+                L += wl[i][h] * f * f;
+                O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f * f;
             }
             const uint32_t hl = hblk * PD_HEADS + h;
             if (whole) {
@@ -593,9 +593,9 @@ __global__ void __launch_bounds__(DIM) paged_join_kernel(PagedAttnArgs a, PdWork
 #pragma unroll 8
     for (uint32_t i = 0; i < n; ++i) {
         const float *p = piece(i);
-        const float f = ex2(wt[i] - M0);
-        L += p[PD_HEADS + h] * f;
-        O += p[2 * PD_HEADS + h * DIM + d] * f;
+        const float f = ex2(0.5f * (wt[i] - M0));
+        L += p[PD_HEADS + h] * f * f;
+        O += p[2 * PD_HEADS + h * DIM + d] * f * f;
     }
     *out = f2bf(L == 0.f ? 0.f : O / L);
 }

@@ -53,7 +53,7 @@ namespace qb {
 
 constexpr int PP_BLK = 128;
 constexpr int PP_MAX_SMS = 192;
-constexpr uint32_t PP_MIN_UNITS = 4;  // blocks a CTA takes at least: less and the join costs more than the split saves
+constexpr uint32_t PP_MIN_UNITS = 1;  // blocks a CTA takes at least (16 rows on 276 keys: 21.0 us, 23.2 with 2, 27.0 with 4)
 constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
 constexpr int PP_SEG = 2;             // segments published ahead
 
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 pp_st_wait();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&p_bar[buf]);
+                if (pp_elect()) tc::mbar_arrive(&p_bar[buf]);
                 if (h == 1) {
                     if (lane == 0) tc::mbar_arrive(&sc_empty[st]);
                     ++bc;
@@ -1090,16 +1090,16 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(PagedAttnArgs a
 #pragma unroll 2
     for (uint32_t i = 0; i < n; ++i) {
         const float *p = piece(i);
-        const float f = pp_ex2(p[t] - M0);
-        L += p[TILE + t] * f;
+        const float f = pp_ex2(0.5f * (p[t] - M0));  // applied twice: 2^(m - M) itself may underflow where o f does not
+        L += p[TILE + t] * f * f;
         const float4 *o = reinterpret_cast<const float4 *>(p + 2 * TILE + (uint64_t)t * DIM + d0);
 #pragma unroll
         for (int j = 0; j < PER / 4; ++j) {
             const float4 v = o[j];
-            O[4 * j] += v.x * f;
-            O[4 * j + 1] += v.y * f;
-            O[4 * j + 2] += v.z * f;
-            O[4 * j + 3] += v.w * f;
+            O[4 * j] += v.x * f * f;
+            O[4 * j + 1] += v.y * f * f;
+            O[4 * j + 2] += v.z * f * f;
+            O[4 * j + 3] += v.w * f * f;
         }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
