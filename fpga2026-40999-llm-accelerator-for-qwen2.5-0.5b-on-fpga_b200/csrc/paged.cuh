@@ -40,6 +40,42 @@ __host__ __device__ __forceinline__ KeySpan key_span(int pos, uint32_t window, u
     return {(int)(sinks < (uint32_t)low ? sinks : (uint32_t)low), low};
 }
 
+// n / d and n % d, by 32-bit division where both fit (a 64-bit one is over 100
+// instructions).
+__device__ __forceinline__ void div64(unsigned long long n, unsigned long long d, unsigned long long &q,
+                                      unsigned long long &r) {
+    if (((n | d) >> 32) == 0) {
+        q = (uint32_t)n / (uint32_t)d;
+        r = (uint32_t)n - (uint32_t)q * (uint32_t)d;
+    } else {
+        q = n / d;
+        r = n - q * d;
+    }
+}
+
+// An equal split of `total` units over g CTAs, each with at least `least` of
+// them: CTA c takes units [start(c), start(c + 1)).
+struct UnitSplit {
+    unsigned long long q, r;
+    uint32_t g;
+    UnitSplit() = default;
+    __device__ __forceinline__ UnitSplit(unsigned long long total, uint32_t max_ctas, uint32_t least) {
+        unsigned long long want, rest;
+        div64(total + least - 1, least, want, rest);
+        g = (uint32_t)min((unsigned long long)max_ctas, max(want, 1ull));
+        div64(total, g, q, r);
+    }
+    __device__ __forceinline__ unsigned long long start(uint32_t c) const {
+        return c * q + min((unsigned long long)c, r);
+    }
+    __device__ __forceinline__ uint32_t cta_of(unsigned long long u) const {
+        const unsigned long long edge = r * (q + 1);
+        unsigned long long c, rest;
+        div64(u < edge ? u : u - edge, u < edge ? q + 1 : q, c, rest);
+        return (uint32_t)(u < edge ? c : r + c);
+    }
+};
+
 // Host side: 0, or the status of a descriptor that cannot be used.
 int paged_check(const qwen_b200_paged_kv *kv);
 // Whether p is memory of the current device (QWEN_B200_OK / EINVAL / EDEVICE).

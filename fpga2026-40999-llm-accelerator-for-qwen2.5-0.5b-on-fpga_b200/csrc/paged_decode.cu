@@ -28,11 +28,13 @@
 // weights as two bf16 halves (hi + lo, 16 bits together, and bf16's range
 // for any value scale), V^T fragments by byte permutes from the row-major rows.
 #include "paged.cuh"
+#include "tc05.cuh"
 
 namespace qb {
 
 constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_STEP = 16, PD_HEADS = 8;
 constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
+constexpr uint32_t PD_PART_KEYS = 512;  // keys that a CTA of a cluster has at least to be worth its join
 constexpr uint32_t PD_MIN_UNITS = 16;  // a CTA takes at least 16 steps (2 per warp), or joining costs more than it saves
 
 template <bool KV8, int DIM>
@@ -51,8 +53,9 @@ struct PdCfg {
 struct PdWork {
     uint32_t group, hb;   // query heads per KV head, blocks of 8 of them
     uint32_t items;       // (KV head, block) pairs of a row
+    uint32_t parts;       // CTAs of a cluster (one launch)
     uint32_t max_ctas;
-    unsigned long long *prefix;  // [rows + 1] units of one item in the rows before
+    uint32_t *prefix;     // [rows + 1] units of one item in the rows before
     float *pieces;        // [CTA][2][PIECE]
 };
 
@@ -128,10 +131,19 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return d;
 }
 
+__device__ __forceinline__ float pd_dsmem(uint32_t local_saddr, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_saddr), "r"(rank));
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    return v;
+}
+
 // Visible keys of a row as steps of 16: those of the first tokens [0, s16),
 // then those from low16 on.
 struct PdRow {
-    int len, first, low, s16, low16, steps;
+    int len, first, low, s16, low16;
+    uint32_t steps;
 };
 __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     PdRow r;
@@ -141,99 +153,101 @@ __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     r.low = k.low;
     r.low16 = k.low >> 4;
     r.s16 = min((k.first + 15) >> 4, r.low16);
-    r.steps = r.len > 0 ? r.s16 + ((r.len + 15) >> 4) - r.low16 : 0;
+    r.steps = r.len > 0 ? (uint32_t)(r.s16 + ((r.len + 15) >> 4) - r.low16) : 0u;
     return r;
 }
 
-// CTA c of g takes units [start(c), start(c + 1)) of `total`.
-struct PdSplit {
-    unsigned long long q, r;
-    uint32_t g;
-    __device__ __forceinline__ PdSplit(unsigned long long total, uint32_t max_ctas) {
-        const unsigned long long want = (total + PD_MIN_UNITS - 1) / PD_MIN_UNITS;
-        g = (uint32_t)min((unsigned long long)max_ctas, max(want, 1ull));
-        q = total / g;
-        r = total % g;
-    }
-    __device__ __forceinline__ unsigned long long start(uint32_t c) const {
-        return c * q + min((unsigned long long)c, r);
-    }
-    __device__ __forceinline__ uint32_t cta_of(unsigned long long u) const {
-        const unsigned long long edge = r * (q + 1);
-        return (uint32_t)(u < edge ? u / (q + 1) : r + (u - edge) / q);
-    }
-};
-
-template <bool KV8, int DIM>
+// DIRECT: CTA (or cluster of `parts` CTAs) b has row b / items, item b % items;
+// its CTAs take equal parts of the context and join them over distributed
+// shared memory. Otherwise CTA c takes the c-th run of all units.
+template <bool KV8, int DIM, bool DIRECT>
 __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decode_kernel(PagedAttnArgs a, PdWork w) {
     using C = PdCfg<KV8, DIM>;
     constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ unsigned long long wsum[PD_WARPS];
-    __shared__ unsigned long long at_prefix;
-    __shared__ uint32_t at_row;
-    __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS];
-    pdl_trigger();  // the join kernel waits for this one to end
+    __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS];
+    __shared__ __align__(16) float fin[DIRECT ? C::PIECE : 4];  // this CTA's m, l, o (clusters)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-
-    // ---- the numbering of the units: prefix sums of the rows' steps
-    const uint32_t per = (a.rows + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * per, a.rows),
-                   r1 = min(r0 + per, a.rows);
-    unsigned long long mine = 0;
-    for (uint32_t r = r0; r < r1; ++r) mine += pd_row(a, r).steps;
-    unsigned long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) wsum[warp] = incl;
-    __syncthreads();
-    unsigned long long all = 0;
-#pragma unroll
-    for (int i = 0; i < PD_WARPS; ++i) {
-        if (i < warp) incl += wsum[i];
-        all += wsum[i];
-    }
-    const unsigned long long before = incl - mine;
-    if (blockIdx.x == 0) {
-        unsigned long long p = before;
-        for (uint32_t r = r0; r < r1; ++r) {
-            w.prefix[r] = p;
-            p += pd_row(a, r).steps;
+    uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
+    UnitSplit split;
+    if constexpr (DIRECT) {
+        const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
+        row = unit / w.items;
+        const PdRow R = pd_row(a, row);
+        base = 0;
+        const uint32_t first = unit % w.items * R.steps;
+        u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
+        u_end = first + (uint32_t)((uint64_t)R.steps * (part + 1) / w.parts);
+        if (R.steps == 0) {  // no key (the whole cluster): zero
+            const uint32_t item = unit % w.items, kvh = item / w.hb, h0 = item % w.hb * PD_HEADS;
+            const uint32_t heads = min(w.group - h0, (uint32_t)PD_HEADS);
+            uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + h0) * DIM;
+            if (part == 0)
+                for (uint32_t x = tid; x < heads * DIM / 8; x += PD_THREADS)
+                    reinterpret_cast<uint4 *>(out)[x] = make_uint4(0, 0, 0, 0);
+            return;
         }
-        if (tid == 0) w.prefix[a.rows] = all;
-    }
-    const PdSplit split(all * w.items, w.max_ctas);
-    if (blockIdx.x >= split.g || all == 0) return;
-    unsigned long long u = split.start(blockIdx.x);
-    const unsigned long long u_end = split.start(blockIdx.x + 1);
-    if (before * w.items <= u && u < incl * w.items) {
-        unsigned long long p = before;
-        uint32_t r = r0;
-        for (;; ++r) {
-            const int n = pd_row(a, r).steps;
-            if (u < (p + n) * w.items) break;
-            p += n;
+    } else {
+        // ---- the numbering of the units: prefix sums of the rows' steps
+        __shared__ uint32_t wsum[PD_WARPS], at_prefix, at_row;
+        pdl_trigger();  // the join kernel waits for this one to end
+        const uint32_t per = (a.rows + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * per, a.rows),
+                       r1 = min(r0 + per, a.rows);
+        uint32_t mine = 0;
+        for (uint32_t r = r0; r < r1; ++r) mine += pd_row(a, r).steps;
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
         }
-        at_row = r;
-        at_prefix = p;
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < PD_WARPS; ++i) {
+            if (i < warp) incl += wsum[i];
+            all += wsum[i];
+        }
+        const uint32_t before = incl - mine;
+        if (blockIdx.x == 0) {
+            uint32_t p = before;
+            for (uint32_t r = r0; r < r1; ++r) {
+                w.prefix[r] = p;
+                p += pd_row(a, r).steps;
+            }
+            if (tid == 0) w.prefix[a.rows] = all;
+        }
+        split = UnitSplit(all * w.items, w.max_ctas, PD_MIN_UNITS);
+        if (blockIdx.x >= split.g || all == 0) return;
+        u = split.start(blockIdx.x);
+        u_end = split.start(blockIdx.x + 1);
+        if (before * w.items <= u && u < incl * w.items) {
+            uint32_t p = before, r = r0;
+            for (;; ++r) {
+                const uint32_t n = pd_row(a, r).steps;
+                if (u < (p + n) * w.items) break;
+                p += n;
+            }
+            at_row = r;
+            at_prefix = p;
+        }
+        __syncthreads();
+        row = at_row;
+        base = at_prefix * w.items;
     }
-    __syncthreads();
-    uint32_t row = at_row;
-    unsigned long long base = at_prefix * w.items;
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::STAGES * C::STEP_BYTES);
     const float fac0 = a.scale * 1.44269504f;
     bool first_segment = true;
-    while (u < u_end) {
+    while (DIRECT || u < u_end) {  // DIRECT: once, also for a CTA of a cluster that has no step
         const PdRow R = pd_row(a, row);
-        if (R.steps == 0) {
+        if (!DIRECT && R.steps == 0) {
             ++row;
             continue;
         }
-        const uint32_t rem = (uint32_t)((u - base) % R.steps), item = (uint32_t)((u - base) / R.steps);
-        const int cnt = (int)min((unsigned long long)(R.steps - rem), u_end - u);
+        const uint32_t item = (u - base) / R.steps, rem = u - base - item * R.steps;
+        const int cnt = (int)min(R.steps - rem, u_end - u);
         const uint32_t kvh = item / w.hb, hblk = item % w.hb;
         const uint32_t seq = a.seqs ? a.seqs[row] : row;
         const uint32_t *table = a.c.table + (uint64_t)seq * a.c.max_pages;
@@ -255,23 +269,29 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 const uint64_t r = ok ? paged_row(a.c, page, kvh) + (key & pmask) : 0;
                 const uint8_t *kp = a.c.k + r * C::RB, *vp = a.c.v + r * C::RB;
                 const uint32_t dst = ring + (i % C::STAGES) * C::STEP_BYTES;
+                // only visible keys are read; the others are zero
+                auto copy = [&](auto bytes_of) {
 #pragma unroll
-                for (int j = 0; j < C::CPR / 2; ++j) {
-                    const int n = j * 32 + lane, kr = n / C::CPR, c = n % C::CPR;
-                    const int key_r = key + kr;
-                    // only visible keys are read; the others are zero
-                    const uint32_t bytes = ok && key_r < R.len && (key_r >= R.low || key_r < R.first) ? 16 : 0;
-                    const int kc = C::CPR == 4 ? c : c ^ ((kr & 1) << 2);
-                    const int vpos = C::CPR == 4 ? ((kr >> 1) << 3) + ((((kr & 1) << 2) | c) ^ (((kr >> 1) & 3) << 1))
-                                                 : kr * C::CPR + (c ^ (((kr >> 1) & 3) << 1));
-                    cp16(dst + (kr * C::CPR + kc) * 16, kp + n * 16, bytes);
-                    cp16(dst + PD_STEP * C::RB + vpos * 16, vp + n * 16, bytes);
-                }
-                if constexpr (KV8) {
-                    const int kr = lane & 15, key_r = key + kr;
-                    const uint32_t bytes = ok && key_r < R.len && (key_r >= R.low || key_r < R.first) ? 4 : 0;
-                    cp4(dst + 2 * PD_STEP * C::RB + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + r + kr, bytes);
-                }
+                    for (int j = 0; j < C::CPR / 2; ++j) {
+                        const int n = j * 32 + lane, kr = n / C::CPR, c = n % C::CPR;
+                        const uint32_t bytes = bytes_of(kr, 16);
+                        const int kc = C::CPR == 4 ? c : c ^ ((kr & 1) << 2);
+                        const int vpos = C::CPR == 4 ? ((kr >> 1) << 3) + ((((kr & 1) << 2) | c) ^ (((kr >> 1) & 3) << 1))
+                                                     : kr * C::CPR + (c ^ (((kr >> 1) & 3) << 1));
+                        cp16(dst + (kr * C::CPR + kc) * 16, kp + n * 16, bytes);
+                        cp16(dst + PD_STEP * C::RB + vpos * 16, vp + n * 16, bytes);
+                    }
+                    if constexpr (KV8)
+                        cp4(dst + 2 * PD_STEP * C::RB + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + r + (lane & 15),
+                            bytes_of(lane & 15, 4));
+                };
+                if (ok && key + 16 <= R.len && (key >= R.low || key + 16 <= R.first))
+                    copy([](int, int n) { return n; });
+                else
+                    copy([&](int kr, int n) {
+                        const int key_r = key + kr;
+                        return ok && key_r < R.len && (key_r >= R.low || key_r < R.first) ? n : 0;
+                    });
             }
             cp_commit();
         };
@@ -522,17 +542,22 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 os[(warp * PD_HEADS + 2 * t + (k & 1)) * (DIM + 1) + d + (k >> 1)] = o[j][k];
         }
         __syncthreads();
-        const bool whole = cnt == R.steps;
-        float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
+        const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
+        float *piece = DIRECT ? fin : w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
+        if (tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+            const int h = tid % PD_HEADS, i = tid / PD_HEADS;
+            float M = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < PD_WARPS; ++k) M = fmaxf(M, wm[k][h]);
+            wf[i][h] = ex2(0.5f * (wm[i][h] - (M == -INFINITY ? 0.f : M)));
+        }
+        __syncthreads();
         for (int x = tid; x < PD_HEADS * DIM; x += PD_THREADS) {
             const int h = x / DIM, d = x % DIM;
-            float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll
-            for (int i = 0; i < PD_WARPS; ++i) M = fmaxf(M, wm[i][h]);
-            const float M0 = M == -INFINITY ? 0.f : M;
+            float L = 0.f, O = 0.f;
 #pragma unroll
             for (int i = 0; i < PD_WARPS; ++i) {
-                const float f = ex2(0.5f * (wm[i][h] - M0));  // applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+                const float f = wf[i][h];
                 L += wl[i][h] * f * f;
                 O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f * f;
             }
@@ -543,64 +568,114 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             } else {
                 piece[2 * PD_HEADS + x] = O;
                 if (d == 0) {
+                    float M = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < PD_WARPS; ++k) M = fmaxf(M, wm[k][h]);
                     piece[h] = M;
                     piece[PD_HEADS + h] = L;
                 }
             }
         }
+        if constexpr (DIRECT) {
+            if (w.parts > 1) {
+                // every CTA of the cluster joins its share of the (head, dim) values
+                tc::cluster_sync();
+                const uint32_t part = blockIdx.x % w.parts;
+                const uint32_t fs = (uint32_t)__cvta_generic_to_shared(fin);
+                for (uint32_t x = (part * PD_THREADS + tid) * 4; x < PD_HEADS * DIM; x += w.parts * PD_THREADS * 4) {
+                    const uint32_t h = x / DIM;
+                    float M = -INFINITY, L = 0.f;
+                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, pd_dsmem(fs + 4 * h, i));
+                    const float M0 = M == -INFINITY ? 0.f : M;
+                    for (uint32_t i = 0; i < w.parts; ++i) {
+                        const float f = ex2(0.5f * (pd_dsmem(fs + 4 * h, i) - M0));
+                        L += pd_dsmem(fs + 4 * (PD_HEADS + h), i) * f * f;
+                        const float4 o4 = tc::ld_dsmem_f4(fs + 4 * (2 * PD_HEADS + x), i);
+                        O.x += o4.x * f * f, O.y += o4.y * f * f, O.z += o4.z * f * f, O.w += o4.w * f * f;
+                    }
+                    const uint32_t hl = hblk * PD_HEADS + h;
+                    if (hl < w.group) {
+                        uint2 v = make_uint2(pack_bf16(O.x / L, O.y / L), pack_bf16(O.z / L, O.w / L));
+                        if (L == 0.f) v = make_uint2(0, 0);
+                        *reinterpret_cast<uint2 *>(a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + x % DIM) = v;
+                    }
+                }
+                tc::cluster_sync();  // no CTA leaves while its values are read
+            }
+            return;
+        }
         __syncthreads();  // os is read before the next segment's loads
         first_segment = false;
         u += cnt;
-        if (u == base + (unsigned long long)R.steps * w.items) {
+        if (u == base + R.steps * w.items) {
             base = u;
             ++row;
         }
     }
 }
 
-// One CTA per (item, query head): the pieces of the item's context added in
-// CTA order; items without keys are zero, items of one CTA are already written.
+// One CTA per (item, query head): the pieces of the item's context, PJ_GROUPS of
+// them at a time, added in a fixed order; items without keys are zero, items
+// of one CTA are already written.
+constexpr int PJ_GROUPS = 8;
 template <int DIM>
-__global__ void __launch_bounds__(DIM) paged_join_kernel(PagedAttnArgs a, PdWork w) {
+__global__ void __launch_bounds__(DIM *PJ_GROUPS) paged_join_kernel(PagedAttnArgs a, PdWork w) {
     constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;
-    __shared__ float wt[2 * PD_MAX_SMS];
+    __shared__ float wt[2 * PD_MAX_SMS], lt[2 * PD_MAX_SMS], top[PJ_GROUPS * DIM / 32], so[PJ_GROUPS][DIM];
     pdl_wait();
-    const uint64_t index = blockIdx.x;
     const uint32_t qh = w.items * PD_HEADS;  // heads, the last block of each KV head filled up
-    const uint32_t row = (uint32_t)(index / qh), item = (uint32_t)(index % qh) / PD_HEADS, h = (uint32_t)(index % PD_HEADS);
+    const uint32_t row = blockIdx.x / qh, item = blockIdx.x % qh / PD_HEADS, h = blockIdx.x % PD_HEADS;
     const uint32_t kvh = item / w.hb, hl = (item % w.hb) * PD_HEADS + h;
     if (hl >= w.group) return;
-    const int d = threadIdx.x;
+    const int d = threadIdx.x % DIM, grp = threadIdx.x / DIM;
     uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d;
-    const unsigned long long p0 = w.prefix[row], steps = w.prefix[row + 1] - p0;
+    const uint32_t p0 = w.prefix[row], steps = w.prefix[row + 1] - p0;
     if (steps == 0) {
-        *out = 0;
+        if (grp == 0) *out = 0;
         return;
     }
-    const PdSplit split(w.prefix[a.rows] * w.items, w.max_ctas);
-    const unsigned long long u0 = p0 * w.items + item * steps;
+    const UnitSplit split(w.prefix[a.rows] * w.items, w.max_ctas, PD_MIN_UNITS);
+    const uint32_t u0 = p0 * w.items + item * steps;
     const uint32_t c0 = split.cta_of(u0), c1 = split.cta_of(u0 + steps - 1), n = c1 - c0 + 1;
     if (n == 1) return;
     auto piece = [&](uint32_t i) {  // the item's segment of CTA c0 + i: the CTA's first one unless c0 began before the item
         return w.pieces + ((uint64_t)(c0 + i) * 2 + (i == 0 && split.start(c0) < u0)) * PIECE;
     };
-    for (uint32_t i = d; i < n; i += DIM) wt[i] = piece(i)[h];
-    __syncthreads();
     float M = -INFINITY;
-    for (uint32_t i = 0; i < n; ++i) M = fmaxf(M, wt[i]);
-    const float M0 = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O = 0.f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < n; ++i) {
+    for (uint32_t i = threadIdx.x; i < n; i += DIM * PJ_GROUPS) {
         const float *p = piece(i);
-        const float f = ex2(0.5f * (wt[i] - M0));
-        L += p[PD_HEADS + h] * f * f;
-        O += p[2 * PD_HEADS + h * DIM + d] * f * f;
+        wt[i] = p[h];
+        lt[i] = p[PD_HEADS + h];
+        M = fmaxf(M, wt[i]);
     }
+    M = warp_max(M);
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = M;
+    __syncthreads();
+    M = top[0];
+#pragma unroll
+    for (int i = 1; i < PJ_GROUPS * DIM / 32; ++i) M = fmaxf(M, top[i]);
+    const float M0 = M == -INFINITY ? 0.f : M;
+    float O = 0.f;
+#pragma unroll 4
+    for (uint32_t i = grp; i < n; i += PJ_GROUPS) {
+        const float f = ex2(0.5f * (wt[i] - M0));
+        O += piece(i)[2 * PD_HEADS + h * DIM + d] * f * f;
+    }
+    so[grp][d] = O;
+    __syncthreads();
+    if (grp) return;
+    float L = 0.f;
+    for (uint32_t i = 0; i < n; ++i) {
+        const float f = ex2(0.5f * (wt[i] - M0));
+        L += lt[i] * f * f;
+    }
+#pragma unroll
+    for (int i = 1; i < PJ_GROUPS; ++i) O += so[i][d];
     *out = f2bf(L == 0.f ? 0.f : O / L);
 }
 
-static size_t pd_prefix_bytes(uint32_t rows) { return (((size_t)rows + 1) * 8 + 255) & ~(size_t)255; }
+static size_t pd_prefix_bytes(uint32_t rows) { return (((size_t)rows + 1) * 4 + 255) & ~(size_t)255; }
 
 size_t paged_decode_ws(uint32_t, uint32_t, uint32_t dim, uint32_t rows) {
     return pd_prefix_bytes(rows) + (size_t)2 * PD_MAX_SMS * 2 * (2 * PD_HEADS + PD_HEADS * dim) * 4;
@@ -609,12 +684,29 @@ size_t paged_decode_ws(uint32_t, uint32_t, uint32_t dim, uint32_t rows) {
 template <bool KV8, int DIM>
 static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM>;
-    auto *kernel = paged_decode_kernel<KV8, DIM>;
+    // Which way: a CTA or cluster per (row, item) where those fill the GPU, or where no context can be long
+    // (the host knows the table's width and the window only); else equal runs of units and a join kernel.
+    const uint32_t slots = (uint32_t)(sms * C::MINB), units = a.rows * w.items;
+    uint64_t most = (uint64_t)a.c.max_pages << a.c.tshift;
+    if (a.window) {
+        const uint64_t seen = (uint64_t)a.window + a.sinks;
+        most = most < seen ? most : seen;
+    }
+    const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS;
+    const uint32_t room = units < slots ? slots / units : 1;
+    w.parts = 1;
+    while (w.parts < 8 && 2 * w.parts <= room && w.parts < want) w.parts *= 2;
+    if ((uint64_t)units * w.parts * 2 >= slots || want <= 8) {
+        auto *kernel = paged_decode_kernel<KV8, DIM, true>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
+        return launch_pdl(kernel, dim3(units * w.parts), dim3(PD_THREADS), C::SMEM, st, w.parts, a, w);
+    }
+    auto *kernel = paged_decode_kernel<KV8, DIM, false>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
-    w.max_ctas = (uint32_t)(sms * C::MINB);
+    w.max_ctas = slots;
     PdlChain chain;
     if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PD_THREADS), C::SMEM, st, 1, a, w)) return rc;
-    return launch_pdl(paged_join_kernel<DIM>, dim3(a.rows * w.items * PD_HEADS), dim3(DIM), 0, st, 1, a, w);
+    return launch_pdl(paged_join_kernel<DIM>, dim3(units * PD_HEADS), dim3(DIM * PJ_GROUPS), 0, st, 1, a, w);
 }
 
 int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
@@ -624,8 +716,10 @@ int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     w.group = a.qh / a.c.hkv;
     w.hb = (w.group + PD_HEADS - 1) / PD_HEADS;
     w.items = a.c.hkv * w.hb;
+    // units are counted in 32 bits
     if ((uint64_t)a.rows * w.items * PD_HEADS >= 1ull << 31) return -1;
-    w.prefix = (unsigned long long *)ws;
+    if ((uint64_t)a.rows * w.items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 2) >= 1ull << 32) return -1;
+    w.prefix = (uint32_t *)ws;
     w.pieces = reinterpret_cast<float *>((char *)ws + pd_prefix_bytes(a.rows));
     const int n = sms < PD_MAX_SMS ? sms : PD_MAX_SMS;
     if (a.format == QWEN_B200_KV8)

@@ -172,24 +172,6 @@ __device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const 
     return u;
 }
 
-struct PpSplit {
-    unsigned long long q, r;
-    uint32_t g;
-    __device__ __forceinline__ PpSplit(unsigned long long total, uint32_t max_ctas) {
-        const unsigned long long want = (total + PP_MIN_UNITS - 1) / PP_MIN_UNITS;
-        g = (uint32_t)min((unsigned long long)max_ctas, max(want, 1ull));
-        q = total / g;
-        r = total % g;
-    }
-    __device__ __forceinline__ unsigned long long start(uint32_t c) const {
-        return c * q + min((unsigned long long)c, r);
-    }
-    __device__ __forceinline__ uint32_t cta_of(unsigned long long u) const {
-        const unsigned long long edge = r * (q + 1);
-        return (uint32_t)(u < edge ? u / (q + 1) : r + (u - edge) / q);
-    }
-};
-
 // ---------------------------------------------------------------- tcgen05
 // kind::f16: D f32, A and B bf16, M 128.
 __host__ __device__ constexpr uint32_t pp_idesc(int n, bool b_mn_major) {
@@ -379,7 +361,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
         if (i < warp) before += wsum[i];
         all += wsum[i];
     }
-    const PpSplit split(all * a.c.hkv, w.max_ctas);
+    const UnitSplit split(all * a.c.hkv, w.max_ctas, PP_MIN_UNITS);
     const bool active = blockIdx.x < split.g && all > 0;
     const unsigned long long u0 = split.start(blockIdx.x), u1 = split.start(blockIdx.x + 1);
     if (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv) {
@@ -966,7 +948,9 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         ++i;
                         continue;
                     }
-                    const uint32_t kvh = (uint32_t)((u - base) / units), off = (uint32_t)((u - base) % units);
+                    unsigned long long kvh64, off64;
+                    div64(u - base, units, kvh64, off64);
+                    const uint32_t kvh = (uint32_t)kvh64, off = (uint32_t)off64;
                     // the tile that holds unit `off` of this KV head
                     uint32_t seen = 0;
                     int k = 0, b0 = 0;
