@@ -32,17 +32,19 @@
 
 namespace qb {
 
-constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_STEP = 16, PD_HEADS = 8;
+constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_SUB = 16, PD_HEADS = 8;
 constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
 constexpr uint32_t PD_PART_KEYS = 512;  // keys that a CTA of a cluster has at least to be worth its join
-constexpr uint32_t PD_MIN_UNITS = 16;  // a CTA takes at least 16 steps (2 per warp), or joining costs more than it saves
+constexpr uint32_t PD_MIN_UNITS = 8;  // a CTA takes at least 8 steps (1 per warp)
 
 template <bool KV8, int DIM>
 struct PdCfg {
     static constexpr int RB = KV8 ? DIM : 2 * DIM;  // bytes of a row
     static constexpr int CPR = RB / 16;             // 16-byte chunks of a row
-    static constexpr int STEP_BYTES = 2 * PD_STEP * RB + (KV8 ? 2 * PD_STEP * 4 : 0);
-    static constexpr int STAGES = RB == 64 ? 5 : 3;
+    static constexpr int SUBS = RB == 64 ? 2 : 1, STEP = SUBS * PD_SUB;  // 16-key pieces of a step; its keys
+    static constexpr int LOG = STEP == 32 ? 5 : 4;
+    static constexpr int SUB_BYTES = 2 * PD_SUB * RB + (KV8 ? 2 * PD_SUB * 4 : 0), STEP_BYTES = SUBS * SUB_BYTES;
+    static constexpr int STAGES = 3;
     static constexpr int MINB = RB == 256 ? 1 : 2;  // CTAs per SM
     static constexpr int RING = PD_WARPS * STAGES * STEP_BYTES;
     static constexpr int OUT = PD_WARPS * PD_HEADS * (DIM + 1) * 4;  // the warps' contexts, over the drained ring
@@ -131,29 +133,32 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return d;
 }
 
-__device__ __forceinline__ float pd_dsmem(uint32_t local_saddr, uint32_t rank) {
+// v to the word at this address of CTA `rank`'s shared memory.
+__device__ __forceinline__ void pd_dsmem_store(uint32_t local_saddr, uint32_t rank, float v) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_saddr), "r"(rank));
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-    return v;
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
+__device__ __forceinline__ void pd_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pd_cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
-// Visible keys of a row as steps of 16: those of the first tokens [0, s16),
-// then those from low16 on.
+// Visible keys of a row as steps of 2^LOG: those of the first tokens [0, nfirst),
+// then those from nlow on.
 struct PdRow {
-    int len, first, low, s16, low16;
+    int len, first, low, nfirst, nlow;
     uint32_t steps;
 };
+template <int LOG>
 __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     PdRow r;
     r.len = paged_length(a.c, a.seqs ? a.seqs[row] : row);
     const KeySpan k = key_span(r.len - 1, a.window, a.sinks);
     r.first = k.first;
     r.low = k.low;
-    r.low16 = k.low >> 4;
-    r.s16 = min((k.first + 15) >> 4, r.low16);
-    r.steps = r.len > 0 ? (uint32_t)(r.s16 + ((r.len + 15) >> 4) - r.low16) : 0u;
+    constexpr int up = (1 << LOG) - 1;
+    r.nlow = k.low >> LOG;
+    r.nfirst = min((k.first + up) >> LOG, r.nlow);
+    r.steps = r.len > 0 ? (uint32_t)(r.nfirst + ((r.len + up) >> LOG) - r.nlow) : 0u;
     return r;
 }
 
@@ -165,15 +170,28 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     using C = PdCfg<KV8, DIM>;
     constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS];
-    __shared__ __align__(16) float fin[DIRECT ? C::PIECE : 4];  // this CTA's m, l, o (clusters)
+    __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS], wM[PD_HEADS];
+    __shared__ float fin[DIRECT ? PD_HEADS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    // 16-byte chunks of a lane's query head: head 8 hblk + g, dims by the permutation that the key rows' chunks
+    // give the first product (chunk t + 4 j of a row of keys)
+    constexpr int NQ = DIM / 32;
+    uint4 qraw[NQ];
+    auto load_q = [&](uint32_t row_, uint32_t item_) {
+        const uint32_t kvh_ = item_ / w.hb, hl = item_ % w.hb * PD_HEADS + g;
+        const uint16_t *qp = a.q + row_ * a.q_stride + (uint64_t)(kvh_ * w.group + (hl < w.group ? hl : 0)) * DIM;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+            qraw[j] = *reinterpret_cast<const uint4 *>(qp + (KV8 ? 16 * (t + 4 * (j >> 1)) + 8 * (j & 1) : 8 * (t + 4 * j)));
+    };
     uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
     UnitSplit split;
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
+        if (w.parts > 1) pd_cluster_arrive();
         row = unit / w.items;
-        const PdRow R = pd_row(a, row);
+        load_q(row, unit % w.items);  // needs no length
+        const PdRow R = pd_row<C::LOG>(a, row);
         base = 0;
         const uint32_t first = unit % w.items * R.steps;
         u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
@@ -185,6 +203,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             if (part == 0)
                 for (uint32_t x = tid; x < heads * DIM / 8; x += PD_THREADS)
                     reinterpret_cast<uint4 *>(out)[x] = make_uint4(0, 0, 0, 0);
+            if (w.parts > 1) pd_cluster_wait();
             return;
         }
     } else {
@@ -194,7 +213,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         const uint32_t per = (a.rows + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * per, a.rows),
                        r1 = min(r0 + per, a.rows);
         uint32_t mine = 0;
-        for (uint32_t r = r0; r < r1; ++r) mine += pd_row(a, r).steps;
+        for (uint32_t r = r0; r < r1; ++r) mine += pd_row<C::LOG>(a, r).steps;
         uint32_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             uint32_t p = before;
             for (uint32_t r = r0; r < r1; ++r) {
                 w.prefix[r] = p;
-                p += pd_row(a, r).steps;
+                p += pd_row<C::LOG>(a, r).steps;
             }
             if (tid == 0) w.prefix[a.rows] = all;
         }
@@ -225,7 +244,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         if (before * w.items <= u && u < incl * w.items) {
             uint32_t p = before, r = r0;
             for (;; ++r) {
-                const uint32_t n = pd_row(a, r).steps;
+                const uint32_t n = pd_row<C::LOG>(a, r).steps;
                 if (u < (p + n) * w.items) break;
                 p += n;
             }
@@ -241,7 +260,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     const float fac0 = a.scale * 1.44269504f;
     bool first_segment = true;
     while (DIRECT || u < u_end) {  // DIRECT: once, also for a CTA of a cluster that has no step
-        const PdRow R = pd_row(a, row);
+        const PdRow R = pd_row<C::LOG>(a, row);
         if (!DIRECT && R.steps == 0) {
             ++row;
             continue;
@@ -249,6 +268,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         const uint32_t item = (u - base) / R.steps, rem = u - base - item * R.steps;
         const int cnt = (int)min(R.steps - rem, u_end - u);
         const uint32_t kvh = item / w.hb, hblk = item % w.hb;
+        if constexpr (!DIRECT) load_q(row, item);
         const uint32_t seq = a.seqs ? a.seqs[row] : row;
         const uint32_t *table = a.c.table + (uint64_t)seq * a.c.max_pages;
         const int pmask = (1 << a.c.tshift) - 1;
@@ -257,18 +277,32 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         const int nst = cnt > warp ? (cnt - warp + PD_WARPS - 1) / PD_WARPS : 0;
         auto key_of = [&](int i) {
             const int s = (int)rem + warp + i * PD_WARPS;
-            return (s < R.s16 ? s : s - R.s16 + R.low16) << 4;
+            return (s < R.nfirst ? s : s - R.nfirst + R.nlow) << C::LOG;
         };
-        auto page_at = [&](int i) { return i < nst ? __ldg(&table[key_of(i) >> a.c.tshift]) : PG_NO_PAGE; };
-        uint32_t there = 0;  // bit i % 32: step i's page exists
-        auto load = [&](int i, uint32_t page) {
-            if (i < nst) {
-                const int key = key_of(i);
-                const bool ok = page < a.c.pages;
-                there = (there & ~(1u << (i & 31))) | ((uint32_t)ok << (i & 31));
-                const uint64_t r = ok ? paged_row(a.c, page, kvh) + (key & pmask) : 0;
+        struct Pages {
+            uint32_t id[C::SUBS];
+        };
+        auto pages_at = [&](int i) {
+            Pages p;
+#pragma unroll
+            for (int b = 0; b < C::SUBS; ++b) {
+                const int key = key_of(i) + PD_SUB * b;
+                p.id[b] = i < nst && key < R.len ? __ldg(&table[key >> a.c.tshift]) : PG_NO_PAGE;
+            }
+            return p;
+        };
+        uint32_t there = 0;  // bit (i SUBS + b) % 32: that piece's page exists
+        const uint64_t head_row = (uint64_t)kvh << a.c.tshift;
+        auto load = [&](int i, Pages page) {
+#pragma unroll
+            for (int b = 0; i < nst && b < C::SUBS; ++b) {
+                const int key = key_of(i) + PD_SUB * b;
+                const bool ok = page.id[b] < a.c.pages;
+                const uint32_t bit = (i * C::SUBS + b) & 31;
+                there = (there & ~(1u << bit)) | ((uint32_t)ok << bit);
+                const uint64_t r = ok ? page.id[b] * a.c.page_rows + head_row + (key & pmask) : 0;
                 const uint8_t *kp = a.c.k + r * C::RB, *vp = a.c.v + r * C::RB;
-                const uint32_t dst = ring + (i % C::STAGES) * C::STEP_BYTES;
+                const uint32_t dst = ring + (i % C::STAGES) * C::STEP_BYTES + b * C::SUB_BYTES;
                 // only visible keys are read; the others are zero
                 auto copy = [&](auto bytes_of) {
 #pragma unroll
@@ -279,10 +313,10 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                         const int vpos = C::CPR == 4 ? ((kr >> 1) << 3) + ((((kr & 1) << 2) | c) ^ (((kr >> 1) & 3) << 1))
                                                      : kr * C::CPR + (c ^ (((kr >> 1) & 3) << 1));
                         cp16(dst + (kr * C::CPR + kc) * 16, kp + n * 16, bytes);
-                        cp16(dst + PD_STEP * C::RB + vpos * 16, vp + n * 16, bytes);
+                        cp16(dst + PD_SUB * C::RB + vpos * 16, vp + n * 16, bytes);
                     }
                     if constexpr (KV8)
-                        cp4(dst + 2 * PD_STEP * C::RB + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + r + (lane & 15),
+                        cp4(dst + 2 * PD_SUB * C::RB + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + r + (lane & 15),
                             bytes_of(lane & 15, 4));
                 };
                 if (ok && key + 16 <= R.len && (key >= R.low || key + 16 <= R.first))
@@ -295,42 +329,31 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             }
             cp_commit();
         };
-        uint32_t next = page_at(0);
+        Pages next;
+        {
+            Pages start[C::STAGES - 1];
 #pragma unroll
-        for (int i = 0; i < C::STAGES - 1; ++i) {
-            const uint32_t page = next;
-            next = page_at(i + 1);
-            load(i, page);
+            for (int i = 0; i < C::STAGES - 1; ++i) start[i] = pages_at(i);
+            next = pages_at(C::STAGES - 1);
+#pragma unroll
+            for (int i = 0; i < C::STAGES - 1; ++i) load(i, start[i]);
         }
 
-        // ---- the query heads as B fragments: head 8 hblk + g, dims by the
-        // permutation that the key rows' 16-byte chunks give the first product
+        // ---- the query heads as B fragments
         uint32_t qf[KS][2];
         float fac[2];
         {
-            const uint32_t hl = hblk * PD_HEADS + g;
-            const bool live = hl < w.group;
-            const uint16_t *qp = a.q + row * a.q_stride + (uint64_t)(kvh * w.group + (live ? hl : 0)) * DIM;
+            const bool live = hblk * PD_HEADS + g < w.group;
             if constexpr (KV8) {
                 float x[KS][4], amax = 0.f;
 #pragma unroll
-                for (int j = 0; j < KS / 4; ++j) {  // chunk t + 4 j: dims 16 (t + 4 j) .. + 15
-                    uint4 v[2];
-                    v[0] = reinterpret_cast<const uint4 *>(qp + 16 * (t + 4 * j))[0];
-                    v[1] = reinterpret_cast<const uint4 *>(qp + 16 * (t + 4 * j))[1];
-                    const uint32_t word[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        x[4 * j + k][0] = bflo(word[2 * k]);
-                        x[4 * j + k][1] = bfhi(word[2 * k]);
-                        x[4 * j + k][2] = bflo(word[2 * k + 1]);
-                        x[4 * j + k][3] = bfhi(word[2 * k + 1]);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
+                for (int k = 0; k < KS; ++k) {
+                    const uint4 v = qraw[k >> 1];
+                    const uint32_t w0 = k & 1 ? v.z : v.x, w1 = k & 1 ? v.w : v.y;
+                    x[k][0] = bflo(w0), x[k][1] = bfhi(w0), x[k][2] = bflo(w1), x[k][3] = bfhi(w1);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
+                }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 // 2^(14 - e): the largest |q| lands in [2^14, 2^15); values 2^-28 of it and smaller lose bits
@@ -346,9 +369,8 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 fac[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
             } else {
 #pragma unroll
-                for (int j = 0; j < KS / 2; ++j) {  // chunk t + 4 j: dims 8 (t + 4 j) .. + 7
-                    uint4 v = *reinterpret_cast<const uint4 *>(qp + 8 * (t + 4 * j));
-                    if (!live) v = make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < KS / 2; ++j) {
+                    const uint4 v = live ? qraw[j] : make_uint4(0, 0, 0, 0);
                     qf[2 * j][0] = v.x;
                     qf[2 * j][1] = v.y;
                     qf[2 * j + 1][0] = v.z;
@@ -364,68 +386,81 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
 
         for (int i = 0; i < nst; ++i) {
             {
-                const uint32_t page = next;
-                next = page_at(i + C::STAGES);
+                const Pages page = next;
+                next = pages_at(i + C::STAGES);
                 load(i + C::STAGES - 1, page);
             }
             cp_wait<C::STAGES - 1>();
             __syncwarp();
-            const uint32_t buf = ring + (i % C::STAGES) * C::STEP_BYTES;
-            // ---- scores of 16 keys (rows g, g + 8) x 8 heads (columns 2t, 2t + 1)
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (KV8) {
+            const uint32_t stage = ring + (i % C::STAGES) * C::STEP_BYTES;
+            const int key0 = key_of(i);
+            float s[C::SUBS][4], vs[C::SUBS][2];
 #pragma unroll
-                for (int j = 0; j < C::CPR / 4; ++j) {
-                    const int c = t + 4 * j, x = C::CPR == 4 ? 0 : (g & 1) << 2;
-                    const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
-                    const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
-                    const uint32_t wl4[4] = {lo.x, lo.y, lo.z, lo.w}, wh4[4] = {hi.x, hi.y, hi.z, hi.w};
+            for (int b = 0; b < C::SUBS; ++b) {
+                const uint32_t buf = stage + b * C::SUB_BYTES;
+                // ---- scores of 16 keys (rows g, g + 8) x 8 heads (columns 2t, 2t + 1)
+                float (&sb)[4] = s[b];
+                sb[0] = sb[1] = sb[2] = sb[3] = 0.f;
+                if constexpr (KV8) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t a0, a1, a2, a3;
-                        codes4_to_f16(wl4[k], a0, a2);
-                        codes4_to_f16(wh4[k], a1, a3);
-                        mma16816<true>(s, a0, a1, a2, a3, qf[4 * j + k][0], qf[4 * j + k][1]);
+                    for (int j = 0; j < C::CPR / 4; ++j) {
+                        const int c = t + 4 * j, x = C::CPR == 4 ? 0 : (g & 1) << 2;
+                        const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
+                        const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
+                        const uint32_t wl4[4] = {lo.x, lo.y, lo.z, lo.w}, wh4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t a0, a1, a2, a3;
+                            codes4_to_f16(wl4[k], a0, a2);
+                            codes4_to_f16(wh4[k], a1, a3);
+                            mma16816<true>(sb, a0, a1, a2, a3, qf[4 * j + k][0], qf[4 * j + k][1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C::CPR / 4; ++j) {
+                        const int c = t + 4 * j, x = (g & 1) << 2;
+                        const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
+                        const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
+                        mma16816<false>(sb, lo.x, hi.x, lo.y, hi.y, qf[2 * j][0], qf[2 * j][1]);
+                        mma16816<false>(sb, lo.z, hi.z, lo.w, hi.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
                     }
                 }
-            } else {
+                if constexpr (KV8) {
+                    const uint32_t sc = buf + 2 * PD_SUB * C::RB;
+                    const float k0 = lds32f(sc + g * 4), k1 = lds32f(sc + g * 4 + 32);
+                    vs[b][0] = lds32f(sc + 64 + g * 4);
+                    vs[b][1] = lds32f(sc + 96 + g * 4);
+                    sb[0] *= k0 * fac[0];
+                    sb[1] *= k0 * fac[1];
+                    sb[2] *= k1 * fac[0];
+                    sb[3] *= k1 * fac[1];
+                } else {
 #pragma unroll
-                for (int j = 0; j < C::CPR / 4; ++j) {
-                    const int c = t + 4 * j, x = (g & 1) << 2;
-                    const uint4 lo = lds128(buf + (g * C::CPR + (c ^ x)) * 16);
-                    const uint4 hi = lds128(buf + ((g + 8) * C::CPR + (c ^ x)) * 16);
-                    mma16816<false>(s, lo.x, hi.x, lo.y, hi.y, qf[2 * j][0], qf[2 * j][1]);
-                    mma16816<false>(s, lo.z, hi.z, lo.w, hi.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+                    for (int k = 0; k < 4; ++k) sb[k] *= fac0;
                 }
-            }
-            float vs[2] = {1.f, 1.f};
-            if constexpr (KV8) {
-                const uint32_t sc = buf + 2 * PD_STEP * C::RB;
-                const float k0 = lds32f(sc + g * 4), k1 = lds32f(sc + g * 4 + 32);
-                vs[0] = lds32f(sc + 64 + g * 4);
-                vs[1] = lds32f(sc + 96 + g * 4);
-                s[0] *= k0 * fac[0];
-                s[1] *= k0 * fac[1];
-                s[2] *= k1 * fac[0];
-                s[3] *= k1 * fac[1];
-            } else {
+                const int key = key0 + PD_SUB * b;
+                const bool ok = there >> ((i * C::SUBS + b) & 31) & 1;
+                if (!ok || key + 16 > R.len || (key < R.low && key + 16 > R.first)) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[k] *= fac0;
-            }
-            const int key = key_of(i);
-            if (!(there >> (i & 31) & 1) || key + 16 > R.len || (key < R.low && key + 16 > R.first)) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int kr = key + g + 8 * h;
-                    if (!(there >> (i & 31) & 1) || kr >= R.len || (kr < R.low && kr >= R.first))
-                        s[2 * h] = s[2 * h + 1] = -INFINITY;
+                    for (int h = 0; h < 2; ++h) {
+                        const int kr = key + g + 8 * h;
+                        if (!ok || kr >= R.len || (kr < R.low && kr >= R.first))
+                            sb[2 * h] = sb[2 * h + 1] = -INFINITY;
+                    }
                 }
             }
             // ---- the maximum, raised only where a score passes it by 2^8
-            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m[0] + 8.f || fmaxf(s[1], s[3]) > m[1] + 8.f)) {
+            float top[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
+#pragma unroll
+            for (int b = 1; b < C::SUBS; ++b) {
+                top[0] = fmaxf(top[0], fmaxf(s[b][0], s[b][2]));
+                top[1] = fmaxf(top[1], fmaxf(s[b][1], s[b][3]));
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float x = fmaxf(s[h], s[h + 2]);
+                    float x = top[h];
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     x = fmaxf(x, m[h]);
@@ -440,78 +475,82 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 }
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-            float p[4] = {ex2(s[0] - m0), ex2(s[1] - m1), ex2(s[2] - m0), ex2(s[3] - m1)};
-            l[0] += p[0] + p[2];
-            l[1] += p[1] + p[3];
-            if constexpr (KV8) {
-                p[0] *= vs[0];
-                p[1] *= vs[0];
-                p[2] *= vs[1];
-                p[3] *= vs[1];
-            }
-            // ---- weights as hi + lo, transposed to (keys x heads) B fragments
-            const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
-            const uint32_t b0 = movmatrix(h0), b1 = movmatrix(h1);
-            const uint32_t c0 = movmatrix(pack_bf16(p[0] - bflo(h0), p[1] - bfhi(h0)));
-            const uint32_t c1 = movmatrix(pack_bf16(p[2] - bflo(h1), p[3] - bfhi(h1)));
-            // ---- O^T += V^T P^T: tile j holds dims D0(g) + 2 j (row g) and + 1 (row g + 8)
-            const uint32_t vb = buf + PD_STEP * C::RB;
-            const int ra = 2 * t, rb = 2 * t + 8;  // keys 2t, 2t + 1 and 2t + 8, 2t + 9
-            if constexpr (KV8 && DIM == 64) {
-                uint2 v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int kr = (k < 2 ? ra : rb) + (k & 1);
-                    const int pos = ((kr >> 1) << 3) + ((((kr & 1) << 2) | (g >> 1)) ^ (((kr >> 1) & 3) << 1));
-                    v[k] = lds64(vb + pos * 16 + (g & 1) * 8);
+            for (int b = 0; b < C::SUBS; ++b) {
+                const uint32_t buf = stage + b * C::SUB_BYTES;
+                float p[4] = {ex2(s[b][0] - m0), ex2(s[b][1] - m1), ex2(s[b][2] - m0), ex2(s[b][3] - m1)};
+                l[0] += p[0] + p[2];
+                l[1] += p[1] + p[3];
+                if constexpr (KV8) {
+                    p[0] *= vs[b][0];
+                    p[1] *= vs[b][0];
+                    p[2] *= vs[b][1];
+                    p[3] *= vs[b][1];
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t x0 = j < 2 ? v[0].x : v[0].y, x1 = j < 2 ? v[1].x : v[1].y,
-                                   x2 = j < 2 ? v[2].x : v[2].y, x3 = j < 2 ? v[3].x : v[3].y;
-                    uint32_t a0, a1, a2, a3;
-                    if (j & 1) {
-                        a0 = codes_pair_bf16<2>(x0, x1), a1 = codes_pair_bf16<3>(x0, x1);
-                        a2 = codes_pair_bf16<2>(x2, x3), a3 = codes_pair_bf16<3>(x2, x3);
-                    } else {
-                        a0 = codes_pair_bf16<0>(x0, x1), a1 = codes_pair_bf16<1>(x0, x1);
-                        a2 = codes_pair_bf16<0>(x2, x3), a3 = codes_pair_bf16<1>(x2, x3);
-                    }
-                    mma16816<false>(o[j], a0, a1, a2, a3, b0, b1);
-                    mma16816<false>(o[j], a0, a1, a2, a3, c0, c1);
-                }
-            } else {
-                constexpr int NC = KV8 ? 1 : DIM / 64;  // 16-byte chunks of a key that this lane's dims take
-#pragma unroll
-                for (int q = 0; q < NC; ++q) {
-                    uint4 v[4];
+                // ---- weights as hi + lo, transposed to (keys x heads) B fragments
+                const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
+                const uint32_t b0 = movmatrix(h0), b1 = movmatrix(h1);
+                const uint32_t c0 = movmatrix(pack_bf16(p[0] - bflo(h0), p[1] - bfhi(h0)));
+                const uint32_t c1 = movmatrix(pack_bf16(p[2] - bflo(h1), p[3] - bfhi(h1)));
+                // ---- O^T += V^T P^T: tile j holds dims D0(g) + 2 j (row g) and + 1 (row g + 8)
+                const uint32_t vb = buf + PD_SUB * C::RB;
+                const int ra = 2 * t, rb = 2 * t + 8;  // keys 2t, 2t + 1 and 2t + 8, 2t + 9
+                if constexpr (KV8 && DIM == 64) {
+                    uint2 v[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int kr = (k < 2 ? ra : rb) + (k & 1);
-                        v[k] = lds128(vb + (kr * C::CPR + ((g + 8 * q) ^ (((kr >> 1) & 3) << 1))) * 16);
+                        const int pos = ((kr >> 1) << 3) + ((((kr & 1) << 2) | (g >> 1)) ^ (((kr >> 1) & 3) << 1));
+                        v[k] = lds64(vb + pos * 16 + (g & 1) * 8);
                     }
-                    const uint32_t x[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
-                                              {v[1].x, v[1].y, v[1].z, v[1].w},
-                                              {v[2].x, v[2].y, v[2].z, v[2].w},
-                                              {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {  // word k of the chunks
-                        if constexpr (KV8) {
-                            uint32_t a0 = codes_pair_bf16<0>(x[0][k], x[1][k]), a1 = codes_pair_bf16<1>(x[0][k], x[1][k]);
-                            uint32_t a2 = codes_pair_bf16<0>(x[2][k], x[3][k]), a3 = codes_pair_bf16<1>(x[2][k], x[3][k]);
-                            mma16816<false>(o[2 * k], a0, a1, a2, a3, b0, b1);
-                            mma16816<false>(o[2 * k], a0, a1, a2, a3, c0, c1);
-                            a0 = codes_pair_bf16<2>(x[0][k], x[1][k]), a1 = codes_pair_bf16<3>(x[0][k], x[1][k]);
-                            a2 = codes_pair_bf16<2>(x[2][k], x[3][k]), a3 = codes_pair_bf16<3>(x[2][k], x[3][k]);
-                            mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, b0, b1);
-                            mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, c0, c1);
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x0 = j < 2 ? v[0].x : v[0].y, x1 = j < 2 ? v[1].x : v[1].y,
+                                       x2 = j < 2 ? v[2].x : v[2].y, x3 = j < 2 ? v[3].x : v[3].y;
+                        uint32_t a0, a1, a2, a3;
+                        if (j & 1) {
+                            a0 = codes_pair_bf16<2>(x0, x1), a1 = codes_pair_bf16<3>(x0, x1);
+                            a2 = codes_pair_bf16<2>(x2, x3), a3 = codes_pair_bf16<3>(x2, x3);
                         } else {
-                            const uint32_t a0 = __byte_perm(x[0][k], x[1][k], 0x5410),
-                                           a1 = __byte_perm(x[0][k], x[1][k], 0x7632);
-                            const uint32_t a2 = __byte_perm(x[2][k], x[3][k], 0x5410),
-                                           a3 = __byte_perm(x[2][k], x[3][k], 0x7632);
-                            mma16816<false>(o[4 * q + k], a0, a1, a2, a3, b0, b1);
-                            mma16816<false>(o[4 * q + k], a0, a1, a2, a3, c0, c1);
+                            a0 = codes_pair_bf16<0>(x0, x1), a1 = codes_pair_bf16<1>(x0, x1);
+                            a2 = codes_pair_bf16<0>(x2, x3), a3 = codes_pair_bf16<1>(x2, x3);
+                        }
+                        mma16816<false>(o[j], a0, a1, a2, a3, b0, b1);
+                        mma16816<false>(o[j], a0, a1, a2, a3, c0, c1);
+                    }
+                } else {
+                    constexpr int NC = KV8 ? 1 : DIM / 64;  // 16-byte chunks of a key that this lane's dims take
+#pragma unroll
+                    for (int q = 0; q < NC; ++q) {
+                        uint4 v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int kr = (k < 2 ? ra : rb) + (k & 1);
+                            v[k] = lds128(vb + (kr * C::CPR + ((g + 8 * q) ^ (((kr >> 1) & 3) << 1))) * 16);
+                        }
+                        const uint32_t x[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
+                                                  {v[1].x, v[1].y, v[1].z, v[1].w},
+                                                  {v[2].x, v[2].y, v[2].z, v[2].w},
+                                                  {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // word k of the chunks
+                            if constexpr (KV8) {
+                                uint32_t a0 = codes_pair_bf16<0>(x[0][k], x[1][k]), a1 = codes_pair_bf16<1>(x[0][k], x[1][k]);
+                                uint32_t a2 = codes_pair_bf16<0>(x[2][k], x[3][k]), a3 = codes_pair_bf16<1>(x[2][k], x[3][k]);
+                                mma16816<false>(o[2 * k], a0, a1, a2, a3, b0, b1);
+                                mma16816<false>(o[2 * k], a0, a1, a2, a3, c0, c1);
+                                a0 = codes_pair_bf16<2>(x[0][k], x[1][k]), a1 = codes_pair_bf16<3>(x[0][k], x[1][k]);
+                                a2 = codes_pair_bf16<2>(x[2][k], x[3][k]), a3 = codes_pair_bf16<3>(x[2][k], x[3][k]);
+                                mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, b0, b1);
+                                mma16816<false>(o[2 * k + 1], a0, a1, a2, a3, c0, c1);
+                            } else {
+                                const uint32_t a0 = __byte_perm(x[0][k], x[1][k], 0x5410),
+                                               a1 = __byte_perm(x[0][k], x[1][k], 0x7632);
+                                const uint32_t a2 = __byte_perm(x[2][k], x[3][k], 0x5410),
+                                               a3 = __byte_perm(x[2][k], x[3][k], 0x7632);
+                                mma16816<false>(o[4 * q + k], a0, a1, a2, a3, b0, b1);
+                                mma16816<false>(o[4 * q + k], a0, a1, a2, a3, c0, c1);
+                            }
                         }
                     }
                 }
@@ -542,16 +581,20 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 os[(warp * PD_HEADS + 2 * t + (k & 1)) * (DIM + 1) + d + (k >> 1)] = o[j][k];
         }
         __syncthreads();
-        const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
-        float *piece = DIRECT ? fin : w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
         if (tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
             const int h = tid % PD_HEADS, i = tid / PD_HEADS;
             float M = -INFINITY;
 #pragma unroll
             for (int k = 0; k < PD_WARPS; ++k) M = fmaxf(M, wm[k][h]);
             wf[i][h] = ex2(0.5f * (wm[i][h] - (M == -INFINITY ? 0.f : M)));
+            if (i == 0) wM[h] = M;
         }
         __syncthreads();
+        const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
+        float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
+        const uint32_t part = DIRECT ? blockIdx.x % w.parts : 0;
+        if constexpr (DIRECT)
+            if (w.parts > 1) pd_cluster_wait();  // every CTA of the cluster has started
         for (int x = tid; x < PD_HEADS * DIM; x += PD_THREADS) {
             const int h = x / DIM, d = x % DIM;
             float L = 0.f, O = 0.f;
@@ -565,43 +608,42 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             if (whole) {
                 if (hl < w.group)
                     a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
+            } else if constexpr (DIRECT) {
+                // head h is joined by CTA h % parts, from slot `part` of its shared memory
+                const uint32_t slot = (part * (PD_HEADS / w.parts) + h / w.parts) * (DIM + 2);
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(fin + slot);
+                pd_dsmem_store(to + 4 * (2 + d), h % w.parts, O);
+                if (d == 0) {
+                    pd_dsmem_store(to, h % w.parts, wM[h]);
+                    pd_dsmem_store(to + 4, h % w.parts, L);
+                }
             } else {
                 piece[2 * PD_HEADS + x] = O;
                 if (d == 0) {
-                    float M = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < PD_WARPS; ++k) M = fmaxf(M, wm[k][h]);
-                    piece[h] = M;
+                    piece[h] = wM[h];
                     piece[PD_HEADS + h] = L;
                 }
             }
         }
         if constexpr (DIRECT) {
             if (w.parts > 1) {
-                // every CTA of the cluster joins its share of the (head, dim) values
                 tc::cluster_sync();
-                const uint32_t part = blockIdx.x % w.parts;
-                const uint32_t fs = (uint32_t)__cvta_generic_to_shared(fin);
-                for (uint32_t x = (part * PD_THREADS + tid) * 4; x < PD_HEADS * DIM; x += w.parts * PD_THREADS * 4) {
-                    const uint32_t h = x / DIM;
-                    float M = -INFINITY, L = 0.f;
-                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, pd_dsmem(fs + 4 * h, i));
+                const uint32_t mine = PD_HEADS / w.parts;  // heads joined here: part, part + parts, ..
+                for (uint32_t x = tid; x < mine * DIM; x += PD_THREADS) {
+                    const uint32_t k = x / DIM, d = x % DIM;
+                    float M = -INFINITY, L = 0.f, O = 0.f;
+                    for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, fin[(i * mine + k) * (DIM + 2)]);
                     const float M0 = M == -INFINITY ? 0.f : M;
                     for (uint32_t i = 0; i < w.parts; ++i) {
-                        const float f = ex2(0.5f * (pd_dsmem(fs + 4 * h, i) - M0));
-                        L += pd_dsmem(fs + 4 * (PD_HEADS + h), i) * f * f;
-                        const float4 o4 = tc::ld_dsmem_f4(fs + 4 * (2 * PD_HEADS + x), i);
-                        O.x += o4.x * f * f, O.y += o4.y * f * f, O.z += o4.z * f * f, O.w += o4.w * f * f;
+                        const float *p = fin + (i * mine + k) * (DIM + 2);
+                        const float f = ex2(0.5f * (p[0] - M0));
+                        L += p[1] * f * f;
+                        O += p[2 + d] * f * f;
                     }
-                    const uint32_t hl = hblk * PD_HEADS + h;
-                    if (hl < w.group) {
-                        uint2 v = make_uint2(pack_bf16(O.x / L, O.y / L), pack_bf16(O.z / L, O.w / L));
-                        if (L == 0.f) v = make_uint2(0, 0);
-                        *reinterpret_cast<uint2 *>(a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + x % DIM) = v;
-                    }
+                    const uint32_t hl = hblk * PD_HEADS + part + k * w.parts;
+                    if (hl < w.group)
+                        a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
                 }
-                tc::cluster_sync();  // no CTA leaves while its values are read
             }
             return;
         }
@@ -718,7 +760,7 @@ int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     w.items = a.c.hkv * w.hb;
     // units are counted in 32 bits
     if ((uint64_t)a.rows * w.items * PD_HEADS >= 1ull << 31) return -1;
-    if ((uint64_t)a.rows * w.items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 2) >= 1ull << 32) return -1;
+    if ((uint64_t)a.rows * w.items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 3) >= 1ull << 32) return -1;
     w.prefix = (uint32_t *)ws;
     w.pieces = reinterpret_cast<float *>((char *)ws + pd_prefix_bytes(a.rows));
     const int n = sms < PD_MAX_SMS ? sms : PD_MAX_SMS;
