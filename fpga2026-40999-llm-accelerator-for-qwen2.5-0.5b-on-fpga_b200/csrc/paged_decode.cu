@@ -8,13 +8,15 @@
 // fp32. KV8: the key's scale multiplies its score and the value's scale its
 // weight, so both products run on the codes.
 //
-// Work: the unit is 16 keys of one (row, block of up to 8 query heads that
-// share a KV head). All units of the batch are numbered in a row and CTA c of G takes
-// the c-th equal run of them, whatever the lengths, windows and empty rows
-// (every CTA derives the numbering from the lengths, so the launch does not
-// depend on them and can be captured). A run that covers an item alone writes ctx; pieces
-// go to the workspace (at most two per CTA) and the join kernel, launched
-// behind with programmatic serialisation, adds them in CTA order.
+// Work: an item is a row with a block of up to 8 query heads that share a KV
+// head. Usually one CTA, or a cluster of up to 16 that split the context evenly
+// and join over distributed shared memory, takes an item: one launch, nothing
+// in the workspace. Where that would leave the GPU idle (few items, long contexts), steps of
+// 16 or 32 keys of all items are numbered in a row and CTA c of G takes the c-th equal run (every CTA derives the
+// numbering from the lengths, so the launch does not depend on them and can be
+// captured); a run that covers an item alone writes ctx, pieces go to the
+// workspace (at most two per CTA) and a join kernel, launched behind with
+// programmatic serialisation, adds them in CTA order.
 //
 // Bound by HBM (the cache is read once: 8 heads share each key): keys are
 // copied to shared memory by 16-byte cp.async, every warp with a ring of its
@@ -33,8 +35,10 @@
 namespace qb {
 
 constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_SUB = 16, PD_HEADS = 8;
+constexpr uint32_t PD_MAX_PARTS = 16;  // CTAs of a cluster
 constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
 constexpr uint32_t PD_PART_KEYS = 512;  // keys that a CTA of a cluster has at least to be worth its join
+constexpr uint32_t PD_PART_MOST = 2048; // and at most where the clusters leave most of the GPU idle
 constexpr uint32_t PD_MIN_UNITS = 8;  // a CTA takes at least 8 steps (1 per warp)
 
 template <bool KV8, int DIM>
@@ -139,6 +143,8 @@ __device__ __forceinline__ void pd_dsmem_store(uint32_t local_saddr, uint32_t ra
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_saddr), "r"(rank));
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
+// Heads that a CTA of a cluster joins at most (CTA c those with h % parts == c).
+__device__ __forceinline__ uint32_t pd_heads_here(uint32_t parts) { return (PD_HEADS + parts - 1) / parts; }
 __device__ __forceinline__ void pd_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pd_cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS], wM[PD_HEADS];
-    __shared__ float fin[DIRECT ? PD_HEADS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
+    __shared__ float fin[DIRECT ? PD_MAX_PARTS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     // 16-byte chunks of a lane's query head: head 8 hblk + g, dims by the permutation that the key rows' chunks
     // give the first product (chunk t + 4 j of a row of keys)
@@ -610,7 +616,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                     a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
             } else if constexpr (DIRECT) {
                 // head h is joined by CTA h % parts, from slot `part` of its shared memory
-                const uint32_t slot = (part * (PD_HEADS / w.parts) + h / w.parts) * (DIM + 2);
+                const uint32_t slot = (part * pd_heads_here(w.parts) + h / w.parts) * (DIM + 2);
                 const uint32_t to = (uint32_t)__cvta_generic_to_shared(fin + slot);
                 pd_dsmem_store(to + 4 * (2 + d), h % w.parts, O);
                 if (d == 0) {
@@ -628,8 +634,8 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         if constexpr (DIRECT) {
             if (w.parts > 1) {
                 tc::cluster_sync();
-                const uint32_t mine = PD_HEADS / w.parts;  // heads joined here: part, part + parts, ..
-                for (uint32_t x = tid; x < mine * DIM; x += PD_THREADS) {
+                const uint32_t mine = pd_heads_here(w.parts);  // part, part + parts, .. as far as there are heads
+                for (uint32_t x = tid; x < mine * DIM && part + x / DIM * w.parts < PD_HEADS; x += PD_THREADS) {
                     const uint32_t k = x / DIM, d = x % DIM;
                     float M = -INFINITY, L = 0.f, O = 0.f;
                     for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, fin[(i * mine + k) * (DIM + 2)]);
@@ -723,24 +729,63 @@ size_t paged_decode_ws(uint32_t, uint32_t, uint32_t dim, uint32_t rows) {
     return pd_prefix_bytes(rows) + (size_t)2 * PD_MAX_SMS * 2 * (2 * PD_HEADS + PD_HEADS * dim) * 4;
 }
 
+// Whether the current device holds `units` clusters of `parts` CTAs (9 to 16) at once; asked once per device and size.
+template <bool KV8, int DIM>
+static bool pd_fits(uint32_t parts, uint32_t units) {
+    using C = PdCfg<KV8, DIM>;
+    static int known[64][PD_MAX_PARTS + 1];  // 1 + the answer, written with the same value by every thread that finds 0
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int n = __atomic_load_n(&known[dev][parts], __ATOMIC_RELAXED);
+    if (!n) {
+        auto *kernel = paged_decode_kernel<KV8, DIM, true>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(parts);
+        cfg.blockDim = dim3(PD_THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = parts;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            clusters = 0;
+        }
+        n = 1 + clusters;
+        __atomic_store_n(&known[dev][parts], n, __ATOMIC_RELAXED);
+    }
+    return n - 1 >= (int)units;
+}
+
 template <bool KV8, int DIM>
 static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM>;
-    // Which way: a CTA or cluster per (row, item) where those fill the GPU, or where no context can be long
-    // (the host knows the table's width and the window only); else equal runs of units and a join kernel.
+    // Which way: a CTA or cluster per (row, item) where those fill a third of the GPU, or where no context can be
+    // longer than its CTAs are worth (the host knows the table's width and the window only); else equal runs of
+    // units and a join kernel. Measured, first way against second: 64 rows x 2 KV heads x 2048 keys KV8 14.9 and
+    // 24.9 us, one row x 8 heads x 32768 keys bf16 28.9 and 37.7 us, one row x 2 heads KV8 8192 keys 8.5 and 11.4,
+    // 32768 keys 16.2 and 15.2, 131072 keys 41.7 and 22.4 us.
     const uint32_t slots = (uint32_t)(sms * C::MINB), units = a.rows * w.items;
     uint64_t most = (uint64_t)a.c.max_pages << a.c.tshift;
     if (a.window) {
         const uint64_t seen = (uint64_t)a.window + a.sinks;
         most = most < seen ? most : seen;
     }
-    const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS;
-    const uint32_t room = units < slots ? slots / units : 1;
-    w.parts = 1;
-    while (w.parts < 8 && 2 * w.parts <= room && w.parts < want) w.parts *= 2;
-    if ((uint64_t)units * w.parts * 2 >= slots || want <= 8) {
+    const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;
+    uint64_t parts = want < room ? want : room;
+    parts = parts < 1 ? 1 : parts < PD_MAX_PARTS ? parts : PD_MAX_PARTS;
+    while (parts > 8 && !pd_fits<KV8, DIM>((uint32_t)parts, units)) --parts;
+    w.parts = (uint32_t)parts;
+    if (units * parts * 3 >= slots || most <= parts * PD_PART_MOST) {
         auto *kernel = paged_decode_kernel<KV8, DIM, true>;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
+        if (parts > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return -3;
         return launch_pdl(kernel, dim3(units * w.parts), dim3(PD_THREADS), C::SMEM, st, w.parts, a, w);
     }
     auto *kernel = paged_decode_kernel<KV8, DIM, false>;
