@@ -12,7 +12,7 @@ int paged_check(const qwen_b200_paged_kv *kv) {
     const uint32_t t = kv->page_tokens;
     if (t < 16 || t > 256 || (t & (t - 1))) return QWEN_B200_EINVAL;
     if (!kv->layers || !kv->pages || !kv->kv_heads || !kv->seqs || !kv->max_pages) return QWEN_B200_EINVAL;
-    if (kv->pages >= 1u << 31 || kv->seqs > 65536 || kv->layers > 65536 || kv->kv_heads > 65536)
+    if (kv->pages >= 1u << 31 || kv->seqs > 65536 || kv->layers > 65536 || kv->kv_heads > 16384)
         return QWEN_B200_EINVAL;
     if ((uint64_t)kv->max_pages * t >= 1ull << 31) return QWEN_B200_EINVAL;
     uintptr_t align = (uintptr_t)kv->k | (uintptr_t)kv->v;

@@ -11,66 +11,76 @@
 namespace qb {
 
 // ---------------------------------------------------------------- append
-// K and V rows of new tokens -> pages. DIM / 8 threads hold one (row, head):
-// a 16-byte load of 8 bf16 values each, the row's largest magnitude over the
-// threads by shuffles, one 16-byte (bf16) or 8-byte (codes) store. Bound by
-// HBM for prompts and by the launch for single tokens.
+// K and V rows of new tokens -> pages. DIM / 8 threads hold one (row, head) of
+// K or V (blockIdx.y): a 16-byte load of 8 bf16 values each, the row's largest
+// magnitude over the threads by shuffles, one 16-byte (bf16) or 8-byte (codes)
+// store. A thread takes ROWS rows at a time, so that as many chains of
+// sequence -> length -> page -> row are in flight. Bound by HBM for prompts
+// (11k rows x 8 heads of 128 bf16: 14.2 us, 6.4 TB/s) and by that chain for single tokens.
 // KV8: scale = amax / 127, code = clamp(rne(x / scale), +-127), every step one
 // IEEE fp32 operation, the same bits as kv8_append_kernel.
+constexpr int PA_THREADS = 256, PA_ROWS = 4;
 template <bool KV8, int DIM>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(PA_THREADS)
     paged_append_kernel(PagedView c, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v,
                         uint64_t row_stride, uint32_t rows, const uint32_t *__restrict__ seqs,
                         const uint32_t *__restrict__ positions) {
-    constexpr int TPR = DIM / 8;
-    const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / TPR;
+    constexpr int TPR = DIM / 8, RPB = PA_THREADS / TPR;  // threads of a row, rows of a block at a time
     const int part = threadIdx.x % TPR;
-    const uint64_t per_row = 2ull * c.hkv;
-    const uint32_t r = (uint32_t)min(item / per_row, (uint64_t)rows), j = (uint32_t)(item % per_row);
-    const bool is_v = j >= c.hkv;
-    const uint32_t head = is_v ? j - c.hkv : j;
-    bool live = r < rows;
-    uint64_t dst = 0;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (live) {
-        const uint32_t seq = seqs[r], pos = positions[r];
-        live = pos < (uint32_t)paged_length(c, seq);
-        if (live) {
-            const uint32_t page = c.table[(uint64_t)seq * c.max_pages + (pos >> c.tshift)];
-            live = page < c.pages;
-            if (live) {
-                dst = paged_row(c, page, head) + (pos & ((1u << c.tshift) - 1));
-                w = *reinterpret_cast<const uint4 *>((is_v ? v : k) + (uint64_t)r * row_stride + head * DIM + 8 * part);
-            }
+    const bool is_v = blockIdx.y >= c.hkv;
+    const uint32_t head = is_v ? blockIdx.y - c.hkv : blockIdx.y;
+    const uint16_t *src = (is_v ? v : k) + head * DIM + 8 * part;
+    uint32_t seq[PA_ROWS], pos[PA_ROWS], page[PA_ROWS];
+    uint4 w[PA_ROWS];
+    const uint64_t first = (uint64_t)blockIdx.x * (RPB * PA_ROWS) + threadIdx.x / TPR;
+#pragma unroll
+    for (int i = 0; i < PA_ROWS; ++i) {
+        const uint64_t r = first + i * RPB;
+        seq[i] = pos[i] = 0xffffffffu;
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+            seq[i] = seqs[r];
+            pos[i] = positions[r];
+            w[i] = *reinterpret_cast<const uint4 *>(src + r * row_stride);
         }
     }
+#pragma unroll
+    for (int i = 0; i < PA_ROWS; ++i) {
+        page[i] = PG_NO_PAGE;
+        if (pos[i] < (uint32_t)paged_length(c, seq[i])) page[i] = c.table[(uint64_t)seq[i] * c.max_pages + (pos[i] >> c.tshift)];
+    }
     uint8_t *pool = const_cast<uint8_t *>(is_v ? c.v : c.k);
-    if constexpr (!KV8) {
-        if (live) *reinterpret_cast<uint4 *>(pool + (dst * DIM + 8 * part) * 2) = w;
-    } else {
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-        float x[8], amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = bflo(ww[i]);
-            x[2 * i + 1] = bfhi(ww[i]);
-        }
+    for (int i = 0; i < PA_ROWS; ++i) {
+        const bool live = page[i] < c.pages;
+        const uint64_t dst = live ? paged_row(c, page[i], head) + (pos[i] & ((1u << c.tshift) - 1)) : 0;
+        if constexpr (!KV8) {
+            if (live) *reinterpret_cast<uint4 *>(pool + (dst * DIM + 8 * part) * 2) = w[i];
+        } else {
+            const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            float x[8], amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-#pragma unroll
-        for (int o = TPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (!live) return;
-        const float s = __fdiv_rn(amax, 127.0f);
-        uint32_t b[2] = {0u, 0u};
-        if (s > 0.f) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int code = (int)fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f);
-                b[i >> 2] |= ((uint32_t)code & 0xffu) << (8 * (i & 3));
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = bflo(ww[j]);
+                x[2 * j + 1] = bfhi(ww[j]);
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
+#pragma unroll
+            for (int o = TPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if (!live) continue;  // (a row's threads agree, and the shuffles stay within it)
+            const float s = __fdiv_rn(amax, 127.0f);
+            uint32_t b[2] = {0u, 0u};
+            if (s > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int code = (int)fminf(fmaxf(rintf(__fdiv_rn(x[j], s)), -127.f), 127.f);
+                    b[j >> 2] |= ((uint32_t)code & 0xffu) << (8 * (j & 3));
+                }
+            }
+            *reinterpret_cast<uint2 *>(pool + dst * DIM + 8 * part) = make_uint2(b[0], b[1]);
+            if (part == 0) const_cast<float *>(is_v ? c.vs : c.ks)[dst] = s;
         }
-        *reinterpret_cast<uint2 *>(pool + dst * DIM + 8 * part) = make_uint2(b[0], b[1]);
-        if (part == 0) const_cast<float *>(is_v ? c.vs : c.ks)[dst] = s;
     }
 }
 
@@ -78,12 +88,12 @@ int launch_paged_append(const qwen_b200_paged_kv &kv, uint32_t layer, const uint
                         uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
                         cudaStream_t st) {
     const PagedView c = paged_view(kv, layer);
-    const uint64_t threads = (uint64_t)rows * 2 * kv.kv_heads * (kv.head_dim / 8), blocks = (threads + 255) / 256;
-    if (blocks >= 1ull << 31) return -1;
+    const uint32_t per = PA_THREADS / (kv.head_dim / 8) * PA_ROWS;
+    const dim3 grid((rows + per - 1) / per, 2 * kv.kv_heads);
     auto *kernel = kv.format == QWEN_B200_KV8
                        ? (kv.head_dim == 64 ? paged_append_kernel<true, 64> : paged_append_kernel<true, 128>)
                        : (kv.head_dim == 64 ? paged_append_kernel<false, 64> : paged_append_kernel<false, 128>);
-    kernel<<<(unsigned)blocks, 256, 0, st>>>(c, k, v, row_stride, rows, seqs, positions);
+    kernel<<<grid, PA_THREADS, 0, st>>>(c, k, v, row_stride, rows, seqs, positions);
     return QB_LAUNCH_CHECK();
 }
 
@@ -439,10 +449,10 @@ __global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(PageCopyArgs a) 
     const uint32_t segs = (page_bytes + PC_SEG - 1) / PC_SEG;
     const uint64_t work = (uint64_t)count * a.layers * 2 * segs;
     for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const uint32_t seg = (uint32_t)(w % segs);
-        const uint64_t item = w / segs;
-        const uint32_t which = (uint32_t)(item & 1), layer = (uint32_t)((item >> 1) % a.layers);
-        const uint32_t e = (uint32_t)((item >> 1) / a.layers);
+        unsigned long long item, seg64, e64, layer64;
+        div64(w, segs, item, seg64);
+        div64(item >> 1, a.layers, e64, layer64);
+        const uint32_t seg = (uint32_t)seg64, which = (uint32_t)(item & 1), layer = (uint32_t)layer64, e = (uint32_t)e64;
         const uint4 m = a.list ? a.list[e] : make_uint4(a.src[e], a.dst[e], 1u << a.tshift, 0);
         if (m.x >= a.pages || m.y >= a.pages) continue;
         const bool whole = m.z == 1u << a.tshift;

@@ -428,7 +428,7 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
  * Requirements (QWEN_B200_EINVAL otherwise): head_dim 64 or 128; page_tokens
  * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables
  * 4-byte aligned; strides multiples of 16 rows that keep pages and layers
- * apart; pages < 2^31, seqs <= 65536, max_pages * page_tokens < 2^31; the
+ * apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages * page_tokens < 2^31; the
  * pool on the current device. The page ids, lengths and indexes in device
  * memory are not seen by the host: a sequence index >= seqs (for example
  * QWEN_B200_NO_SEQ in a padded batch) is no sequence, a length beyond the
