@@ -5,10 +5,10 @@
 //
 // Mathematics, per (row, query head), over its visible keys j in blocks of 128:
 //   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
-// m is a reference near the running maximum: the maximum of the row's first
-// 64 keys, and a new one only where 64 keys' weights sum to more than 2^15 (so
-// most keys need no comparison at all and the accumulator is rarely rescaled;
-// fp32 and bf16 keep their relative precision far above and below 1). The weights
+// m is a reference for 2^x in place of the running maximum: fp32 and bf16 keep
+// their relative precision far above and below 1, so it only moves where the
+// weights of some keys sum to more than 2^15 (or the first ones to less than
+// 2^-20), and most keys need no comparison and no rescaling. The weights
 // are rounded to bf16 for the second product (half a step is 2^-8 of a weight, unbiased);
 // everything else is fp32. KV8: codes become bf16 exactly on the way to
 // shared memory, the key's scale multiplies its column of scores and the
@@ -421,8 +421,10 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             const int all_last = m_end == mt + 127 ? g.pos0 + (int)(mt / w.group) : -1;
             const int all_first = key_span(max(all_last, 0), a.window, a.sinks).first;
             const int all_low = key_span(max(g.pos0 + (int)(m_end / w.group), 0), a.window, a.sinks).low;
-            // a row that sees nothing needs no maximum
-            float m = pos < 0 ? 0.f : -INFINITY, l = 0.f;
+            // The reference starts at 0 and stands if the weights of the row's first keys sum to something in
+            // [2^-20, 2^15] (scores within some 15 of 0, the usual case); else it becomes their maximum.
+            float m = 0.f, l = 0.f;
+            bool fresh = true;  // no key seen yet
             const uint32_t steps = 2 * g.nblk;
             uint32_t st = 0;
             int kb = 0;
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         float sum;
                         pp_ld_wait();
                         auto weights = [&](float mu) {
-                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                            unsigned long long part[2] = {0ull, 0ull};
 #pragma unroll
                             for (int j = 0; j < CW; j += 4) {
                                 float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
@@ -480,25 +482,30 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     const float4 k4 = kc[j >> 2];
                                     f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
                                 }
+                                float y[4];
+                                unpk2(fma2(pk2(s[j], s[j + 1]), pk2(f[0], f[1]), dup2(-mu)), y[0], y[1]);
+                                unpk2(fma2(pk2(s[j + 2], s[j + 3]), pk2(f[2], f[3]), dup2(-mu)), y[2], y[3]);
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
-                                    float y = fmaf(s[j + k], f[k], -mu);
-                                    if constexpr (masked.value) y = bt & (1u << (j + k)) ? y : -INFINITY;
-                                    e[k] = pp_ex2(y);
-                                    part[k] += e[k];
+                                    if constexpr (masked.value) y[k] = bt & (1u << (j + k)) ? y[k] : -INFINITY;
+                                    e[k] = pp_ex2(y[k]);
                                 }
+                                part[0] = add2(part[0], pk2(e[0], e[1]));
+                                part[1] = add2(part[1], pk2(e[2], e[3]));
                                 if constexpr (KV8) {
                                     const float4 v4 = vf[CW / 4 * c + (j >> 2)];
-                                    e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
+                                    unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
+                                    unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
                                 }
                                 p[j / 2] = pp_pack(e[0], e[1]);
                                 p[j / 2 + 1] = pp_pack(e[2], e[3]);
                             }
-                            sum = (part[0] + part[1]) + (part[2] + part[3]);
+                            float a0, a1;
+                            unpk2(add2(part[0], part[1]), a0, a1);
+                            sum = a0 + a1;
                         };
-                        bool lift = m == -INFINITY && bt != 0;
-                        weights(m == -INFINITY ? 0.f : m);
-                        lift |= sum > 32768.f;
+                        weights(m);
+                        const bool lift = sum > 32768.f || (fresh && bt != 0 && sum < 0x1p-20f);
                         if (__builtin_expect(__any_sync(0xffffffffu, lift), 0)) {
                             float top = -INFINITY;
 #pragma unroll
@@ -510,7 +517,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             float f = 1.f, f2 = 1.f;
                             if (lift) {
                                 const float by = ceilf(top - m);
-                                if (m == -INFINITY || by > 252.f) {
+                                if (fresh || by > 252.f) {
                                     f = 0.f;
                                     m = top;
                                 } else if (by > 0.f) {
@@ -547,8 +554,9 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                 for (int k = 0; k < 8; ++k) o[k] = pp_pack(bflo(o[k]) * f * f2, bfhi(o[k]) * f * f2);
                                 pp_st8(sh + j, o);
                             }
-                            weights(m == -INFINITY ? 0.f : m);
+                            weights(m);
                         }
+                        fresh = fresh && bt == 0;
                         l += sum;
                         pp_st8(sh + CW / 2 * c, p);  // over columns whose scores have been read
                     }
@@ -558,7 +566,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     // two warps of a scheduler are not enough to hide that loop's latencies: 64 columns at once
                     // (630 us against 554 for the benchmark's longest prompts; at 64 dims, with four warps, the
                     // unrolled code is the slower one, 594 against 391 us)
-                    if (full && !__any_sync(0xffffffffu, m == -INFINITY)) {
+                    if (full && !__any_sync(0xffffffffu, fresh)) {
                         float s[64], part[4] = {0.f, 0.f, 0.f, 0.f};
                         uint32_t p[32];
                         pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
@@ -644,7 +652,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             } else {
                 float *piece = w.pieces + (uint64_t)g.piece * C::PIECE;
                 const int t = 128 * x + r;
-                piece[t] = m;
+                piece[t] = l == 0.f ? -INFINITY : m;
                 piece[C::TILE + t] = l;
                 float *po = piece + 2 * C::TILE + (uint64_t)t * DIM;
 #pragma unroll 1
