@@ -65,15 +65,16 @@ struct PpCfg {
     static constexpr int HALVES = DIM / 64;
     static constexpr int TILE_BYTES = 128 * 128 * HALVES;  // 128 rows of DIM bf16, 64 dims per swizzled half
     // K and V tiles in flight (K0 V0 K1 V1 ..), and KV8 tiles as codes in front of them
-    static constexpr int SLOTS = DIM == 64 ? 6 : KV8 ? 3 : 4;
-    static constexpr int RAW = KV8 ? (DIM == 64 ? 4 : 2) : SLOTS / 2, RAW_BYTES = KV8 ? 128 * DIM : 0;
-    static constexpr int Q = 0, RING = TILES * TILE_BYTES;
+    static constexpr int SLOTS = DIM == 64 ? 4 : KV8 ? 3 : 4;
+    static constexpr int RAW = KV8 ? 2 : SLOTS / 2, RAW_BYTES = KV8 ? 128 * DIM : 0;
+    static constexpr int QBUFS = DIM == 64 ? 2 : 1;        // the next segment's queries load behind the current one
+    static constexpr int Q = 0, RING = QBUFS * TILES * TILE_BYTES;
     static constexpr int CODES = RING + SLOTS * TILE_BYTES;  // [RAW][128][DIM] codes
     static constexpr int SC = CODES + RAW * RAW_BYTES;       // [PP_SC][ks 128 | vs 128] floats, [PP_SC][4] mask words
     static constexpr int MASK = SC + PP_SC * 256 * 4;
     static constexpr int SEG = MASK + PP_SC * 16;
     static constexpr int BARS = SEG + PP_SEG * 64;
-    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 11 + 2 * RAW;
+    static constexpr int NBARS = 2 * SLOTS + 2 * PP_SC + 2 * PP_SEG + 13 + 2 * RAW;
     static constexpr int SLOT = BARS + NBARS * 8;
     static constexpr int TOTAL = SLOT + 16;
     static constexpr int ALLOC = TOTAL + 1024;
@@ -310,8 +311,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BARS);
     uint64_t *kv_full = bars, *kv_empty = kv_full + C::SLOTS, *sc_full = kv_empty + C::SLOTS, *sc_empty = sc_full + PP_SC;
     uint64_t *seg_full = sc_empty + PP_SC, *seg_empty = seg_full + PP_SEG;
-    uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 1, *s_full = q_full + 2, *p_ready = q_full + 6,
-             *mdone = q_full + 10, *raw_full = mdone + 1, *raw_empty = raw_full + C::RAW;
+    uint64_t *q_full = seg_empty + PP_SEG, *q_empty = q_full + 2, *s_full = q_full + 4, *p_ready = q_full + 8,
+             *mdone = q_full + 12, *raw_full = mdone + 1, *raw_empty = raw_full + C::RAW;
     uint32_t *slot_p = reinterpret_cast<uint32_t *>(sm + C::SLOT);
     float *scales = reinterpret_cast<float *>(sm + C::SC);
     uint32_t *masks = reinterpret_cast<uint32_t *>(sm + C::MASK);
@@ -332,8 +333,10 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             tc::mbar_init(&seg_full[i], 1);
             tc::mbar_init(&seg_empty[i], 7 + C::SW);  // 4 tile warps, the copy warp, 2 issuers, the softmax warps
         }
-        tc::mbar_init(q_full, 4);
-        tc::mbar_init(q_empty, 2);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&q_full[i], 4);
+            tc::mbar_init(&q_empty[i], 2);
+        }
         for (int i = 0; i < 4; ++i) {  // [tile][score buffer]
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_ready[i], 4);
@@ -473,6 +476,14 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         uint32_t p[CW / 2];
                         float sum;
                         pp_ld_wait();
+                        if constexpr (masked.value) {
+                            if (!__any_sync(0xffffffffu, bt != 0)) {
+#pragma unroll
+                                for (int j = 0; j < CW / 2; ++j) p[j] = 0;
+                                pp_st8(sh + CW / 2 * c, p);
+                                continue;
+                            }
+                        }
                         auto weights = [&](float mu) {
                             unsigned long long part[2] = {0ull, 0ull};
 #pragma unroll
@@ -724,32 +735,33 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 page = page_of(i + 2);
                 if (i == 0) {
                     // queries: flattened row m of the tile is token m / group, head m % group of this KV
-                    // head; lane = row, its address handed to the lanes that copy it
-                    if (nseg > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty, (nseg - 1) & 1, w.err, 64));
+                    // head; lane = row, its address handed to the lanes that copy it (rows of whole lines)
+                    const uint32_t qb = nseg % C::QBUFS, use = nseg / C::QBUFS;
+                    if (use > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_empty[qb], (use - 1) & 1, w.err, 64));
                     if (!ok) break;
                     ++nseg;
 #pragma unroll 1
                     for (int x = 0; x < C::TILES; ++x) {
                         if (g.m0 + 128 * x >= g.mrows) break;
-                        const uint32_t mr = g.m0 + 128 * x + 32 * lw + lane;
+                        const uint32_t mr = g.m0 + 128 * x + 32 * lw + lane, token = mr / w.group;
                         const bool live = mr < g.mrows;
-                        const uint64_t mine = live ? (g.row0 + (uint64_t)(mr / w.group)) * a.q_stride +
-                                                         (uint64_t)(g.kvh * w.group + mr % w.group) * DIM
+                        const uint64_t mine = live ? (g.row0 + (uint64_t)token) * a.q_stride +
+                                                         (uint64_t)(g.kvh * w.group + mr - token * w.group) * DIM
                                                    : 0;
                         const uint32_t lives = __ballot_sync(0xffffffffu, live);
+                        const uint32_t dst = sbase + C::Q + (qb * C::TILES + x) * C::TILE_BYTES;
 #pragma unroll 4
                         for (int j = 0; j < CPR; ++j) {
                             const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
                             const uint64_t src = __shfl_sync(0xffffffffu, mine, rl);
-                            pp_cp16(sbase + C::Q + x * C::TILE_BYTES + pp_off(32 * lw + rl, c), a.q + src + 8 * c,
-                                    lives >> rl & 1 ? 16 : 0);
+                            pp_cp16(dst + pp_off(32 * lw + rl, c), a.q + src + 8 * c, lives >> rl & 1 ? 16 : 0);
                         }
                     }
                     pp_cp_commit();
                     pp_cp_wait<0>();
                     tc::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(q_full);
+                    if (lane == 0) tc::mbar_arrive(&q_full[qb]);
                 }
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++tiles) {
@@ -828,7 +840,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     };
                     // step n: the weights' product of step n - NB, then the scores of step n over its
                     // columns; descriptors differ in their address field only
-                    ok = tc::mbar_wait(q_full, nseg & 1, w.err, 68);
+                    const uint32_t qb = nseg % C::QBUFS;
+                    ok = tc::mbar_wait(&q_full[qb], (nseg / C::QBUFS) & 1, w.err, 68);
                     for (int n = 0; n < steps + C::NB && ok; ++n) {
                         const int pn = n - C::NB, h = n & 1, ph = pn & 1;
                         const bool scores = n < steps, product = pn >= 0;
@@ -851,7 +864,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     pp_mma_ts(tmem + 256 + x * DIM, sc + 8 * j, vd + j * (2048 >> 4), id_pv, pn > 0 || j > 0);
                             }
                             if (scores) {
-                                const uint64_t qd = q_desc + ((x * C::TILE_BYTES) >> 4),
+                                const uint64_t qd = q_desc + (((qb * C::TILES + x) * C::TILE_BYTES) >> 4),
                                                kd = k_desc + (((kt % C::SLOTS) * C::TILE_BYTES + h * 8192) >> 4);
 #pragma unroll
                                 for (int j = 0; j < DIM / 16; ++j) {
@@ -865,7 +878,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         if (ok && product && ph == 1) tc::mma_commit(&kv_empty[vt % C::SLOTS]);
                         if (ok && scores && h == 1) {
                             tc::mma_commit(&kv_empty[kt % C::SLOTS]);
-                            if (n + 1 == steps) tc::mma_commit(q_empty);
+                            if (n + 1 == steps) tc::mma_commit(&q_empty[qb]);
                         }
                     }
                 }
