@@ -78,8 +78,6 @@ struct UnitSplit {
 
 // Host side: 0, or the status of a descriptor that cannot be used.
 int paged_check(const qwen_b200_paged_kv *kv);
-// Whether p is memory of the current device (QWEN_B200_OK / EINVAL / EDEVICE).
-int paged_check_device(const void *p);
 PagedView paged_view(const qwen_b200_paged_kv &kv, uint32_t layer);
 inline uint32_t paged_row_bytes(const qwen_b200_paged_kv &kv) {
     return kv.format == QWEN_B200_KV8 ? kv.head_dim : 2 * kv.head_dim;

@@ -1,4 +1,6 @@
 // C entry points of the paged KV cache: argument checks, then one launcher.
+#include <initializer_list>
+
 #include "paged.cuh"
 
 using namespace qb;
@@ -14,7 +16,7 @@ int paged_check(const qwen_b200_paged_kv *kv) {
     if (!kv->layers || !kv->pages || !kv->kv_heads || !kv->seqs || !kv->max_pages) return QWEN_B200_EINVAL;
     if (kv->pages >= 1u << 31 || kv->seqs > 65536 || kv->layers > 65536 || kv->kv_heads > 16384)
         return QWEN_B200_EINVAL;
-    if ((uint64_t)kv->max_pages * t >= 1ull << 31) return QWEN_B200_EINVAL;
+    if ((uint64_t)kv->max_pages * t > 1ull << 30) return QWEN_B200_EINVAL;
     uintptr_t align = (uintptr_t)kv->k | (uintptr_t)kv->v;
     if (kv->format == QWEN_B200_KV8) {
         if (!kv->kscales || !kv->vscales) return QWEN_B200_EINVAL;
@@ -24,9 +26,9 @@ int paged_check(const qwen_b200_paged_kv *kv) {
         return QWEN_B200_EINVAL;
     // pages of one layer and layers of one page apart: one of the two strides
     // spans the other's whole range
-    const uint64_t block = (uint64_t)kv->kv_heads * t, most = 1ull << 32;  // strides below 2^40 bytes (tensor maps)
+    const uint64_t block = (uint64_t)kv->kv_heads * t;
     if ((kv->layer_stride | kv->page_stride) & 15) return QWEN_B200_EINVAL;
-    if (kv->layer_stride > most || kv->page_stride > most) return QWEN_B200_EINVAL;
+    if (kv->layer_stride > 1ull << 40 || kv->page_stride > 1ull << 31) return QWEN_B200_EINVAL;  // (a tensor map's stride is below 2^40 bytes)
     if (kv->pages > 1 && kv->page_stride < block) return QWEN_B200_EINVAL;
     if (kv->layers > 1 && kv->layer_stride < block) return QWEN_B200_EINVAL;
     const unsigned __int128 pspan = (unsigned __int128)(kv->pages - 1) * kv->page_stride + block;
@@ -37,15 +39,22 @@ int paged_check(const qwen_b200_paged_kv *kv) {
     return QWEN_B200_OK;
 }
 
-int paged_check_device(const void *p) {
+int paged_check_device(std::initializer_list<const void *> pointers) {
     int dev = 0;
-    cudaPointerAttributes a;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         return QWEN_B200_EDEVICE;
     }
-    if (a.type == cudaMemoryTypeManaged) return QWEN_B200_OK;
-    return a.type == cudaMemoryTypeDevice && a.device == dev ? QWEN_B200_OK : QWEN_B200_EINVAL;
+    for (const void *p : pointers) {
+        cudaPointerAttributes a;
+        if (!p) continue;
+        if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+            cudaGetLastError();
+            return QWEN_B200_EDEVICE;
+        }
+        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != dev)) return QWEN_B200_EINVAL;
+    }
+    return QWEN_B200_OK;
 }
 
 PagedView paged_view(const qwen_b200_paged_kv &kv, uint32_t layer) {
@@ -116,7 +125,7 @@ static int pages_check(const qwen_b200_paged_kv *kv, uint32_t *status, void *ws,
     if (int rc = paged_check(kv)) return rc;
     if (!kv->refs || !status || ((uintptr_t)status & 3) || !ws || ((uintptr_t)ws & 15)) return QWEN_B200_EINVAL;
     if (ws_bytes < pages_ws(kv->pages)) return QWEN_B200_EINVAL;
-    return paged_check_device(kv->k);
+    return paged_check_device({kv->k, kv->v, kv->table, kv->lengths, kv->refs, status, ws});
 }
 
 }  // namespace qb
@@ -131,7 +140,7 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
     if (row_stride < (uint64_t)kv->kv_heads * kv->head_dim || (row_stride & 7) || row_stride > 1ull << 40)
         return QWEN_B200_EINVAL;
     if (((uintptr_t)k | (uintptr_t)v) & 15) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(kv->k)) return rc;
+    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, k, v, seqs, positions})) return rc;
     return launch_paged_append(*kv, layer, k, v, row_stride, rows, seqs, positions, (cudaStream_t)stream);
 }
 
@@ -146,7 +155,7 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
                               size_t workspace_bytes, void *stream) {
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
     if (rows > 65536) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(kv->k)) return rc;
+    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, q, seqs, ctx, workspace})) return rc;
     if (workspace_bytes < paged_decode_ws(kv->kv_heads, q_heads, kv->head_dim, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, window, sinks, scale, ctx, ctx_stride);
     a.rows = rows;
@@ -166,7 +175,7 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
     if (!starts || !n || n > 65536 || rows > 1u << 24) return QWEN_B200_EINVAL;
     if ((uint64_t)rows * (q_heads / kv->kv_heads) >= 1ull << 31) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(kv->k)) return rc;
+    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, q, seqs, starts, ctx, workspace})) return rc;
     if (workspace_bytes < paged_prefill_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, window, sinks, scale, ctx, ctx_stride);
     a.rows = rows;
@@ -211,7 +220,7 @@ int qwen_b200_op_pages_copy(const qwen_b200_paged_kv *kv, const uint32_t *src, c
                             void *stream) {
     if (int rc = paged_check(kv)) return rc;
     if (!src || !dst || !n) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(kv->k)) return rc;
+    if (int rc = paged_check_device({kv->k, kv->v, src, dst})) return rc;
     return launch_pages_copy(*kv, src, dst, n, (cudaStream_t)stream);
 }
 

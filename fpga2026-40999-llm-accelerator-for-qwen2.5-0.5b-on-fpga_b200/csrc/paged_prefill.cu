@@ -9,8 +9,9 @@
 // their relative precision far above and below 1, so it only moves where the
 // weights of some keys sum to more than 2^15 (or the first ones to less than
 // 2^-20), and most keys need no comparison and no rescaling. The weights
-// are rounded to bf16 for the second product (half a step is 2^-8 of a weight, unbiased);
-// everything else is fp32. KV8: codes become bf16 exactly on the way to
+// are rounded to bf16 for the second product (half a step is 2^-8 of a weight,
+// unbiased); bf16 pools sum the rounded ones, so that a row's dominant key
+// cancels exactly. Everything else is fp32. KV8: codes become bf16 exactly on the way to
 // shared memory, the key's scale multiplies its column of scores and the
 // value's scale its column of weights.
 //
@@ -501,15 +502,19 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     if constexpr (masked.value) y[k] = bt & (1u << (j + k)) ? y[k] : -INFINITY;
                                     e[k] = pp_ex2(y[k]);
                                 }
-                                part[0] = add2(part[0], pk2(e[0], e[1]));
-                                part[1] = add2(part[1], pk2(e[2], e[3]));
                                 if constexpr (KV8) {
+                                    part[0] = add2(part[0], pk2(e[0], e[1]));
+                                    part[1] = add2(part[1], pk2(e[2], e[3]));
                                     const float4 v4 = vf[CW / 4 * c + (j >> 2)];
                                     unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
                                     unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
                                 }
                                 p[j / 2] = pp_pack(e[0], e[1]);
                                 p[j / 2 + 1] = pp_pack(e[2], e[3]);
+                                if constexpr (!KV8) {  // the rounded weights: what dominates a row cancels exactly
+                                    part[0] = add2(part[0], pk2(bflo(p[j / 2]), bfhi(p[j / 2])));
+                                    part[1] = add2(part[1], pk2(bflo(p[j / 2 + 1]), bfhi(p[j / 2 + 1])));
+                                }
                             }
                             float a0, a1;
                             unpk2(add2(part[0], part[1]), a0, a1);
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 e[k] = pp_ex2(fmaf(s[j + k], f[k], -m));
-                                part[k] += e[k];
+                                if constexpr (KV8) part[k] += e[k];
                             }
                             if constexpr (KV8) {
                                 const float4 v4 = vf[j >> 2];
@@ -601,6 +606,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             }
                             p[j / 2] = pp_pack(e[0], e[1]);
                             p[j / 2 + 1] = pp_pack(e[2], e[3]);
+                            if constexpr (!KV8) {
+                                part[0] += bflo(p[j / 2]);
+                                part[1] += bfhi(p[j / 2]);
+                                part[2] += bflo(p[j / 2 + 1]);
+                                part[3] += bfhi(p[j / 2 + 1]);
+                            }
                         }
                         const float sum = (part[0] + part[1]) + (part[2] + part[3]);
                         done = !__any_sync(0xffffffffu, sum > 32768.f);

@@ -428,8 +428,8 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
  * Requirements (QWEN_B200_EINVAL otherwise): head_dim 64 or 128; page_tokens
  * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables
  * 4-byte aligned; strides multiples of 16 rows that keep pages and layers
- * apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages * page_tokens < 2^31; the
- * pool on the current device. The page ids, lengths and indexes in device
+ * apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages * page_tokens <= 2^30; the
+ * pool and every other device pointer of a call on the current device. The page ids, lengths and indexes in device
  * memory are not seen by the host: a sequence index >= seqs (for example
  * QWEN_B200_NO_SEQ in a padded batch) is no sequence, a length beyond the
  * table is cut to it, and tokens on a page id >= pages are not there. */
@@ -468,14 +468,15 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * visible). Query head h reads KV head h / (q_heads / kv_heads); q_heads is a
  * multiple of kv_heads. A row with no key (length 0, no sequence) is zero.
  * Unlike qwen_b200_op_attention this is not the oracle's bit-exact order: the
- * weights are not rounded to bf16, sums are fp32, ctx is rounded once, and the
- * result does not depend on anything but the inputs, the batch and the GPU's
- * number of SMs. Only visible keys are read: what a page holds beyond the
+ * weights are held in 16 bits (two bf16 halves), sums are fp32, ctx is rounded
+ * once; the order of the sums, and so the last bits, depends on the sizes in the call and
+ * the GPU's number of SMs, and on nothing that varies from run to run. Only visible keys are read: what a page holds beyond the
  * length or outside the window does not matter, NaN included. ctx rows are
  * ctx_stride elements apart; q, ctx 16-byte aligned, strides multiples of 8
  * and at least q_heads * head_dim. The context is split over the GPU and
  * joined in the workspace (contents do not matter before or after; calls that
- * overlap on the GPU need one each). */
+ * overlap on the GPU need one each). rows * KV heads * blocks of 8 query heads
+ * * (max_pages * page_tokens / 16 + 3) < 2^32. */
 size_t qwen_b200_paged_decode_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t rows);
 int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
                               uint32_t q_heads, uint32_t rows, const uint32_t *seqs, uint32_t window, uint32_t sinks,
@@ -490,8 +491,11 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * left as they were. Rows before the sequence's first token (more rows than
  * its length) and rows of no sequence are zero. Keys that no row of the
  * sequence in this call sees may hold anything; a NaN or infinity in a value
- * that some row sees may reach the rows around it. Softmax weights are rounded to bf16 for the second
- * product, with the rounded weights in the sum; the other sums are fp32. */
+ * that some row sees may reach the rows around it. Softmax weights are rounded to
+ * bf16 for the second product (with bf16 pools the rounded ones are summed
+ * too); sums are fp32. The workspace's contents do not matter, but its first 4 bytes become
+ * non-zero if a bounded device wait expired (ctx is then not valid): a caller
+ * that wants to know zeroes them before. */
 size_t qwen_b200_paged_prefill_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
 int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
                                uint32_t q_heads, uint32_t n, const uint32_t *seqs, const uint32_t *starts,

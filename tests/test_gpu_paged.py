@@ -9,7 +9,7 @@ import pytest
 
 import qwen_b200
 from gpu_util import Keep, dev, host, stream, sync, torch_cuda, vp
-from paged_ref import Cache, bits, ref, unbits
+from paged_ref import BF16_HALF, U, Cache, bits, ref, unbits
 from qwen_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -308,6 +308,49 @@ def test_rows_past_32_bit_offsets():
     assert_within(got, exact, tol)
 
 
+@FORMATS
+@DIMS
+@pytest.mark.parametrize('keys', [513, 1025, 1537, 2600, 3600, 4097, 4700, 6200, 7700, 8200])
+def test_decode_clusters_of_every_size(fmt, dim, keys):
+    """One row and KV head: the table's width lets 2 to 16 CTAs share it, some of them without a key."""
+    c = cache(keys, fmt, dim, 64, [keys, 70], kv_heads=1)
+    keep = Keep()
+    kv = c.upload(keep)
+    check_decode(c, kv, keep, c.rand(2, 7, dim), None)
+    check_decode(c, kv, keep, c.rand(1, 3, dim), [1])
+    check_decode(c, kv, keep, c.rand(1, 3, dim), [0], window=keys - 500, sinks=33)
+
+
+def steep(c, s, q_dir, slope):
+    """Keys of sequence s along one direction: token t scores slope[t] (before the softmax scale) with q_dir."""
+    n = int(c.lengths[s])
+    k = np.repeat((slope[:n, None] * q_dir / np.dot(q_dir, q_dir))[:, None], c.hkv, 1)
+    c.write(0, s, np.arange(n), unbits(bits(k.astype(np.float32))), c.rand(n, c.hkv, c.dim))
+
+
+@FORMATS
+@DIMS
+@pytest.mark.parametrize('shape', ['rising', 'falling', 'low', 'jumps', 'late'])
+def test_scores_far_from_each_other(fmt, dim, shape):
+    """The reference of the softmax has to move, up to hundreds of powers of two at a time, and the sums so far with it."""
+    n = 700
+    c = cache(ord(shape[0]), fmt, dim, 32, [n, 300])
+    r = np.random.default_rng(2)
+    slope = {'rising': np.linspace(-400, 400, n), 'falling': np.linspace(400, -400, n), 'low': -500 + r.standard_normal(n),
+             'jumps': 300 * r.standard_normal(n), 'late': np.where(np.arange(n) < 650, -200.0, 90.0)}[shape]
+    u = np.ones(dim)
+    for s in range(2):
+        steep(c, s, u, slope)
+    keep = Keep()
+    kv = c.upload(keep)
+    # scores are slope * scale * the query's factor, which differs by row and head
+    q = unbits(bits((u * r.uniform(0.2, 1.5, (2, 14, 1))).astype(np.float32)))
+    check_decode(c, kv, keep, q, None, scale=1.0)
+    p = unbits(bits((u * r.uniform(0.2, 1.5, (500, 14, 1))).astype(np.float32)))
+    check_prefill(c, kv, keep, p, None, [0, 400, 500], scale=1.0)
+    check_prefill(c, kv, keep, p, None, [0, 400, 500], 200, 5, scale=1.0)
+
+
 # ---------------------------------------------------------------- prefill
 def runs(c, rows):
     return np.concatenate([[0], np.cumsum(rows)]).tolist()
@@ -430,6 +473,65 @@ def test_a_decode_row_equals_a_prompt_of_one_row(fmt):
     q = c.rand(3, 14, 64)
     check_decode(c, kv, keep, q, None, 90, 3)
     check_prefill(c, kv, keep, q, None, [0, 1, 2, 3], 90, 3)
+
+
+@FORMATS
+@DIMS
+def test_prefill_of_many_tiles(fmt, dim):
+    """More tiles than CTAs, so that a CTA walks several segments; against 64 bits on the GPU, with the host's bound."""
+    torch = torch_cuda()
+    lens, rows, heads, hkv, window, sinks = [2500, 1800], [2500, 900], 32, 8, 700, 130
+    c = cache(77, fmt, dim, 64, lens, kv_heads=hkv)
+    keep = Keep()
+    kv = c.upload(keep)
+    starts = runs(c, rows)
+    q = c.rand(starts[-1], heads, dim) * 2
+    got = prefill(c, kv, keep, 0, q, None, starts, window, sinks)
+    scale = dim ** -0.5
+    for i in range(2):
+        k, v = (torch.from_numpy(x).cuda() for x in c.read(0, i, np.arange(lens[i])))
+        pos = torch.arange(lens[i] - rows[i], lens[i], device='cuda')[:, None]
+        t = torch.arange(lens[i], device='cuda')[None]
+        seen = (t <= pos) & ((pos - t < window) | (t < sinks))
+        qi = torch.from_numpy(q[starts[i]:starts[i + 1]].astype(np.float64)).cuda()
+        for h in range(heads):
+            kh, vh = k[:, h // (heads // hkv)], v[:, h // (heads // hkv)]
+            x = (qi[:, h] @ kh.T * scale).masked_fill(~seen, -np.inf)
+            mag = (qi[:, h].abs() @ kh.abs().T * scale).masked_fill(~seen, 0).amax(1)
+            w = torch.softmax(x, 1)
+            out = w @ vh
+            size = w @ vh.abs() + out.abs()
+            e = PREFILL_W + 2 * (dim + 4) * U * mag + 2.0 ** -21 + 2 * lens[i] * U
+            tol = BF16_HALF * (out.abs() + e[:, None] * size) + e[:, None] * size
+            assert_within(got[starts[i]:starts[i + 1], h], out.cpu().numpy(), tol.cpu().numpy(), f'sequence {i} head {h}')
+
+
+@FORMATS
+@DIMS
+def test_prefill_waits_do_not_expire(fmt, dim):
+    """The workspace's first word stays zero; two calls on two streams, a workspace each, at the same time."""
+    torch = torch_cuda()
+    lens = [900, 300, 5]
+    c = cache(78, fmt, dim, 16, lens)
+    keep = Keep()
+    kv = c.upload(keep)
+    starts = [0, 500, 800, 805]
+    q = c.rand(805, 14, dim)
+    want = prefill(c, kv, keep, 0, q, None, starts)
+    qd, sd = keep(bits(q).view(np.int16)), keep(u32(starts))
+    n = L().qwen_b200_paged_prefill_workspace(ref(kv), 14, 3, 805)
+    ws = [torch.zeros(n, dtype=torch.uint8, device='cuda') for _ in range(2)]
+    out = [dev(np.zeros((805, 14, dim), np.int16)) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sync()
+    for _ in range(5):
+        for w, o, st in zip(ws, out, streams):
+            assert L().qwen_b200_op_paged_prefill(ref(kv), 0, qd, 14 * dim, 14, 3, None, sd, 805, 0, 0, dim ** -0.5, vp(o),
+                                                  14 * dim, vp(w), n, st.cuda_stream) == 0
+    sync()
+    for w, o in zip(ws, out):
+        assert int(host(w)[:4].view(np.uint32)[0]) == 0, 'a bounded wait expired'
+        assert np.array_equal(unbits(host(o)), want)
 
 
 # ---------------------------------------------------------------- pages
@@ -718,6 +820,23 @@ def test_same_inputs_same_bits(fmt):
     for _ in range(3):
         assert np.array_equal(first, decode(c, kv, keep, 0, q, None))
         assert np.array_equal(pfirst, prefill(c, kv, keep, 0, p, [2, 0], [0, 200, 300]))
+
+
+def test_host_memory_is_refused():
+    """A host pointer in any place of a call that the host can look at."""
+    c = cache(43, KV8, 64, 64, [300])
+    keep = Keep()
+    kv = c.upload(keep)
+    q, i = keep(np.zeros((4, 896), np.int16)), keep(u32([0, 4]))
+    bad = (ctypes.c_uint8 * 8192)()
+    at = ctypes.c_void_p((ctypes.addressof(bad) + 255) & ~255)
+    ws, n = workspace(keep, L().qwen_b200_paged_prefill_workspace(ref(kv), 14, 1, 4))
+    for x in range(4):
+        a, b, w, s = (at if x == y else z for y, z in enumerate((q, q, ws, i)))
+        assert L().qwen_b200_op_paged_decode(ref(kv), 0, a, 896, 14, 1, s, 0, 0, 0.125, b, 896, w, n, stream()) == _lib.EINVAL
+        assert L().qwen_b200_op_paged_prefill(ref(kv), 0, a, 896, 14, 1, None, s, 4, 0, 0, 0.125, b, 896, w, n,
+                                              stream()) == _lib.EINVAL
+        assert L().qwen_b200_op_paged_append(ref(kv), 0, a, b, 896, 1, s if x != 2 else at, i, stream()) == _lib.EINVAL
 
 
 def test_a_workspace_too_small_is_refused():
