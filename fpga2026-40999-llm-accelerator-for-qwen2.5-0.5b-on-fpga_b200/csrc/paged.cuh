@@ -40,15 +40,17 @@ __host__ __device__ __forceinline__ KeySpan key_span(int pos, uint32_t window, u
     return {(int)(sinks < (uint32_t)low ? sinks : (uint32_t)low), low};
 }
 
-// n / d and n % d, by 32-bit division where both fit (a 64-bit one is over 100
-// instructions).
+// n / d and n % d, by 32-bit division where both fit; a 64-bit one is several
+// hundred instructions, kept out of line (the kernels' loops share the
+// instruction cache with everything that is inlined around them).
+static __device__ __noinline__ unsigned long long div64_wide(unsigned long long n, unsigned long long d) { return n / d; }
 __device__ __forceinline__ void div64(unsigned long long n, unsigned long long d, unsigned long long &q,
                                       unsigned long long &r) {
     if (((n | d) >> 32) == 0) {
         q = (uint32_t)n / (uint32_t)d;
         r = (uint32_t)n - (uint32_t)q * (uint32_t)d;
     } else {
-        q = n / d;
+        q = div64_wide(n, d);
         r = n - q * d;
     }
 }

@@ -284,6 +284,16 @@ __device__ __forceinline__ bool pp_elect() {
     return r != 0;
 }
 
+// tc::mbar_wait in few instructions: the compiler unrolls its loop, and the
+// kernel has some 50 of them (147 KB of text in all with them unrolled, 95 KB so).
+__device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, unsigned *err, unsigned code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 21); ++i)
+        if (tc::mbar_try_wait(bar, parity)) return true;
+    atomicExch(err, code);
+    return false;
+}
+
 // The reading side of the segment ring.
 struct PpReader {
     const PpSeg *ring;
@@ -292,7 +302,7 @@ struct PpReader {
     // Copies the next segment; every lane of the warp calls it. false: a wait ran out.
     __device__ __forceinline__ bool next(PpSeg &s, unsigned *err) {
         const uint32_t d = n % PP_SEG;
-        const bool ok = tc::mbar_wait(&full[d], (n / PP_SEG) & 1, err, 60);
+        const bool ok = pp_wait(&full[d], (n / PP_SEG) & 1, err, 60);
         s = ring[d];
         __syncwarp();
         if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&empty[d]);
@@ -411,7 +421,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             const uint32_t mt = g.m0 + 128 * x;  // this MMA tile's first flattened row
             if (mt >= g.mrows) {                 // no rows: only let the scales go
                 for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
-                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sc_full[bc % PP_SC], (bc / PP_SC) & 1, w.err, 61));
+                    ok = __all_sync(0xffffffffu, pp_wait(&sc_full[bc % PP_SC], (bc / PP_SC) & 1, w.err, 61));
                     if (lane == 0) tc::mbar_arrive(&sc_empty[bc % PP_SC]);
                 }
                 continue;
@@ -438,10 +448,10 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     const int vb = g.b0 + (int)(n >> 1);
                     kb = (vb < g.s128 ? vb : vb - g.s128 + g.low128) * PP_BLK;
                     st = bc % PP_SC;
-                    ok = tc::mbar_wait(&sc_full[st], (bc / PP_SC) & 1, w.err, 61);
+                    ok = pp_wait(&sc_full[st], (bc / PP_SC) & 1, w.err, 61);
                 }
                 const uint32_t buf = n % C::NB, sh = s_base + 64 * buf;
-                ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&s_bar[buf], (round + n / C::NB) & 1, w.err, 62));
+                ok = __all_sync(0xffffffffu, ok && pp_wait(&s_bar[buf], (round + n / C::NB) & 1, w.err, 62));
                 if (!ok) break;
                 tc::tc_fence_after();
                 const int k0 = kb + 64 * h;
@@ -548,7 +558,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                 // every product into the context so far is complete: those over this buffer precede
                                 // its scores, that over the other buffer precedes that buffer's next scores
                                 if (C::NB == 2)
-                                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
+                                    ok = __all_sync(0xffffffffu, pp_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
                                 tc::tc_fence_after();
 #pragma unroll 1
                                 for (int j = 0; j < DIM; j += 16) {
@@ -643,7 +653,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             if (!ok) break;
             // the last products: one more round of each barrier
             round += steps / C::NB;
-            for (int b = 0; b < C::NB; ++b) ok = ok && tc::mbar_wait(&s_bar[b], round & 1, w.err, 63);
+            for (int b = 0; b < C::NB; ++b) ok = ok && pp_wait(&s_bar[b], round & 1, w.err, 63);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ++round;
@@ -732,7 +742,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 // scales and the mask of keys that are there
                 const uint32_t st = bc % PP_SC;
                 if (bc >= PP_SC)
-                    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sc_empty[st], ((bc / PP_SC) & 1) ^ 1, w.err, 65));
+                    ok = __all_sync(0xffffffffu, pp_wait(&sc_empty[st], ((bc / PP_SC) & 1) ^ 1, w.err, 65));
                 if (!ok) break;
                 if constexpr (KV8) {
                     scales[st * 256 + 32 * lw + lane] = w.negate ? -ksc * w.fac : ksc * w.fac;
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     // queries: flattened row m of the tile is token m / group, head m % group of this KV
                     // head; lane = row, its address handed to the lanes that copy it (rows of whole lines)
                     const uint32_t qb = nseg % C::QBUFS, use = nseg / C::QBUFS;
-                    if (use > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_empty[qb], (use - 1) & 1, w.err, 64));
+                    if (use > 0) ok = __all_sync(0xffffffffu, pp_wait(&q_empty[qb], (use - 1) & 1, w.err, 64));
                     if (!ok) break;
                     ++nseg;
 #pragma unroll 1
@@ -781,8 +791,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         // codes -> bf16, exactly; a code that is not visible is some code, and its
                         // scale and weight are 0
                         const uint32_t rs = tiles % C::RAW;
-                        ok = tc::mbar_wait(&raw_full[rs], (tiles / C::RAW) & 1, w.err, 58) &&
-                             (tiles < C::SLOTS || tc::mbar_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 66));
+                        ok = pp_wait(&raw_full[rs], (tiles / C::RAW) & 1, w.err, 58) &&
+                             (tiles < C::SLOTS || pp_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 66));
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         constexpr int NL = DIM / 16;
@@ -812,7 +822,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     } else if (kv == 1) {
                         // values that are not visible become 0 (a weight of 0 times NaN would not be)
                         const uint32_t vt = tiles / 2, rs = vt % C::RAW;
-                        ok = __all_sync(0xffffffffu, tc::mbar_wait(&raw_full[rs], (vt / C::RAW) & 1, w.err, 58));
+                        ok = __all_sync(0xffffffffu, pp_wait(&raw_full[rs], (vt / C::RAW) & 1, w.err, 58));
                         if (!ok) break;
                         if (now != 0xffffffffu) {
                             if (!(now >> lane & 1))
@@ -847,12 +857,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 const int tiles = (all_tiles + 1 - who) / 2, steps = 2 * g.nblk;  // this issuer's
                 if (pp_elect()) {
                     auto wait_tile = [&](uint32_t n) {
-                        return tc::mbar_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
+                        return pp_wait(&kv_full[n % C::SLOTS], (n / C::SLOTS) & 1, w.err, 67);
                     };
                     // step n: the weights' product of step n - NB, then the scores of step n over its
                     // columns; descriptors differ in their address field only
                     const uint32_t qb = nseg % C::QBUFS;
-                    ok = tc::mbar_wait(&q_full[qb], (nseg / C::QBUFS) & 1, w.err, 68);
+                    ok = pp_wait(&q_full[qb], (nseg / C::QBUFS) & 1, w.err, 68);
                     for (int n = 0; n < steps + C::NB && ok; ++n) {
                         const int pn = n - C::NB, h = n & 1, ph = pn & 1;
                         const bool scores = n < steps, product = pn >= 0;
@@ -865,7 +875,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             if (t >= tiles || !ok) break;
                             const int x = 2 * t + who;
                             const uint32_t sc = tmem + 64 * (x * C::NB + buf);
-                            if (product) ok = tc::mbar_wait(&p_ready[x * C::NB + buf], (round[t] + pn / C::NB) & 1, w.err, 69);
+                            if (product) ok = pp_wait(&p_ready[x * C::NB + buf], (round[t] + pn / C::NB) & 1, w.err, 69);
                             if (!ok) break;
                             tc::tc_fence_after();
                             if (product) {
@@ -903,7 +913,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             // every MMA is complete before TMEM is freed
             if (lane == 0) {
                 tc::mma_commit(mdone);
-                tc::mbar_wait(mdone, 0, w.err, 69);
+                pp_wait(mdone, 0, w.err, 69);
             }
             __syncwarp();
         } else if (warp == C::SW + 7) {
@@ -938,11 +948,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         if constexpr (KV8) {
                             slot = tiles % C::RAW;
                             bar = &raw_full[slot];
-                            if (tiles >= C::RAW) ok = tc::mbar_wait(&raw_empty[slot], ((tiles / C::RAW) & 1) ^ 1, w.err, 57);
+                            if (tiles >= C::RAW) ok = pp_wait(&raw_empty[slot], ((tiles / C::RAW) & 1) ^ 1, w.err, 57);
                         } else {
                             slot = tiles % C::SLOTS;
                             bar = kv ? &raw_full[tiles / 2 % C::RAW] : &kv_full[slot];
-                            if (tiles >= C::SLOTS) ok = tc::mbar_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 57);
+                            if (tiles >= C::SLOTS) ok = pp_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 57);
                         }
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
@@ -1027,7 +1037,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             g.piece = cnt == bl.n ? -1 : (int)(2 * blockIdx.x + (first_segment ? 0 : 1));
                             const uint32_t dd = n % PP_SEG;
                             if (n >= PP_SEG)
-                                ok = __all_sync(0xffffffffu, tc::mbar_wait(&seg_empty[dd], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
+                                ok = __all_sync(0xffffffffu, pp_wait(&seg_empty[dd], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
                             if (!ok) break;
                             if (lane == 0) {
                                 ring[dd] = g;
@@ -1058,7 +1068,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     }
                     continue;
                 }
-                if (n >= PP_SEG) ok = __all_sync(0xffffffffu, tc::mbar_wait(&seg_empty[d], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
+                if (n >= PP_SEG) ok = __all_sync(0xffffffffu, pp_wait(&seg_empty[d], ((n / PP_SEG) & 1) ^ 1, w.err, 60));
                 if (ok && lane == 0) {
                     ring[d] = g;  // nblk 0: the end
                     tc::mbar_arrive(&seg_full[d]);
