@@ -6,14 +6,14 @@
 // Mathematics, per (row, query head), over its visible keys j in blocks of 128:
 //   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
 // m is a reference for 2^x in place of the running maximum: fp32 and bf16 keep
-// their relative precision far above and below 1, so it only moves where the
-// weights of some keys sum to more than 2^15 (or the first ones to less than
-// 2^-20), and most keys need no comparison and no rescaling. The weights
-// are rounded to bf16 for the second product (half a step is 2^-8 of a weight,
-// unbiased); bf16 pools sum the rounded ones, so that a row's dominant key
-// cancels exactly. Everything else is fp32. KV8: codes become bf16 exactly on the way to
-// shared memory, the key's scale multiplies its column of scores and the
-// value's scale its column of weights.
+// their relative precision far above and below 1, so it starts at 0 and only
+// moves where the weights of some keys sum to more than 2^15 (or the first ones
+// to less than 2^-20), and most keys need no comparison and no rescaling. The
+// weights are rounded to bf16 for the second product (half a step is 2^-8 of a
+// weight, unbiased); bf16 pools sum the rounded ones, so that a row's dominant
+// key cancels exactly. Everything else is fp32. KV8: codes become bf16 exactly
+// on the way to shared memory, the key's scale multiplies its column of scores
+// and the value's scale its column of weights.
 //
 // Tiles: the rows of a sequence and the query heads that share a KV head are one
 // axis (row-major: token, head), cut into tiles of 512 (64 dims) or 256 (128
@@ -29,7 +29,8 @@
 // weights (bf16) back over them, second product into the tile's context
 // columns. At 64 dims TMEM holds four tiles with one score buffer each, at 128
 // dims two tiles with two each: either way four steps are in flight and the
-// tensor cores work on three while the softmax has one.
+// tensor cores work on three while the softmax has one. (64 dims with two buffers
+// of 32 keys for each tile: 390 us where this takes 336, the first case below.)
 //
 // Warps (one CTA per SM, registers moved to the softmax warps):
 //   0 ..      four softmax warps per MMA tile, one thread per row
@@ -42,8 +43,14 @@
 //   1         walks the units and publishes segments (tile, KV head, block
 //             range), then zeroes the rows in front of a sequence's first token
 //   1         copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
-// Bound by the exponentials at 64 dims (16 per clock and SM), by them and the
-// tensor cores alike at 128. Every wait is bounded (error codes 57-69).
+// Measured: 8 prompts of 4096 rows, window 1024, 14 heads on 2 of 64 dims, KV8:
+// 307 us, 344 TF/s (the exponentials alone, 16 per clock and SM, take 117 us, the
+// products 64). 3 prompts of up to 8192 rows, window 4096, 32 heads on 8 of 128
+// dims, bf16: 526 us, 750 TF/s (45 % of the GEMM rate). Bound by the chain from
+// scores to weights to product within a tile: without any softmax work the two
+// still take 230 and 434 us, and issue slots (47 and 38 % busy), exponentials
+// (27 and 37 %) and tensor cores (15 and 38 %) all have room.
+// Every wait is bounded (error codes 57-69).
 #include <type_traits>
 
 #include "kernels.h"
@@ -439,6 +446,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             // [2^-20, 2^15] (scores within some 15 of 0, the usual case); else it becomes their maximum.
             float m = 0.f, l = 0.f;
             bool fresh = true;  // no key seen yet
+            bool far = false;   // some row's reference is so large that x has to be rounded before it is subtracted
             const uint32_t steps = 2 * g.nblk;
             uint32_t st = 0;
             int kb = 0;
@@ -471,51 +479,41 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         bits[k] &= below(pos + 1) & (~below(low) | below(first));
                     }
                 }
-                // The weights, CW columns at a time in a loop whose code stays in the instruction cache. A row takes
-                // the maximum of CW keys only until it has a reference: 2^(x - m) may pass 1 by far, and below it keeps
-                // its relative precision in bf16 and fp32 alike; only where CW weights sum to more than 2^15 the
-                // reference goes up, by a whole number, so that what is done is rescaled exactly.
-                constexpr int CW = 16;
-                auto step = [&](auto masked) {
+                // 64 at once at 64 dims: 323 us against 307 for the first case above; 32 at 128 dims: 539 us against
+                // 526 for the second. A second copy of this code behind the test, for the rows that fail it,
+                // in place of the path below: 338 and 543 us.
+                constexpr int COLS = DIM == 64 ? 32 : 64;
+                int c = 0;  // keys done
+                if (full && !far) {
+                    // every key counts: the weights as they are with the row's reference, unless they sum to more
+                    // than 2^15 or a row's first ones to less than 2^-20
 #pragma unroll 1
-                    for (int c = 0; c < 64 / CW; ++c) {
-                        float s[CW];
-                        pp_ld16(sh + CW * c, reinterpret_cast<uint32_t *>(s));
-                        const float4 *kc = kf + CW / 4 * c;
-                        uint32_t bt = 0xffffffffu;
-                        if constexpr (masked.value) bt = (c < 2 ? bits[0] : bits[1]) >> (16 * (c & 1)) & 0xffffu;
-                        uint32_t p[CW / 2];
-                        float sum;
-                        pp_ld_wait();
-                        if constexpr (masked.value) {
-                            if (!__any_sync(0xffffffffu, bt != 0)) {
+                    for (; c < 64; c += COLS) {
+                        uint32_t p[COLS / 2];
+                        const float4 *kc = kf + c / 4, *vc = vf + c / 4;
+                        unsigned long long part[2] = {0ull, 0ull};
+                        const unsigned long long mu = dup2(-m);
 #pragma unroll
-                                for (int j = 0; j < CW / 2; ++j) p[j] = 0;
-                                pp_st8(sh + CW / 2 * c, p);
-                                continue;
-                            }
-                        }
-                        auto weights = [&](float mu) {
-                            unsigned long long part[2] = {0ull, 0ull};
+                        for (int b = 0; b < COLS; b += 8) {  // (16 or 32 at a time: 1 % slower)
+                            float s[8];
+                            pp_ld8(sh + c + b, reinterpret_cast<uint32_t *>(s));
+                            pp_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < CW; j += 4) {
+                            for (int i = 0; i < 8; i += 4) {
+                                const int j = b + i;
                                 float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
                                 if constexpr (KV8) {
                                     const float4 k4 = kc[j >> 2];
                                     f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
                                 }
-                                float y[4];
-                                unpk2(fma2(pk2(s[j], s[j + 1]), pk2(f[0], f[1]), dup2(-mu)), y[0], y[1]);
-                                unpk2(fma2(pk2(s[j + 2], s[j + 3]), pk2(f[2], f[3]), dup2(-mu)), y[2], y[3]);
+                                unpk2(fma2(pk2(s[i], s[i + 1]), pk2(f[0], f[1]), mu), e[0], e[1]);
+                                unpk2(fma2(pk2(s[i + 2], s[i + 3]), pk2(f[2], f[3]), mu), e[2], e[3]);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if constexpr (masked.value) y[k] = bt & (1u << (j + k)) ? y[k] : -INFINITY;
-                                    e[k] = pp_ex2(y[k]);
-                                }
+                                for (int k = 0; k < 4; ++k) e[k] = pp_ex2(e[k]);
                                 if constexpr (KV8) {
                                     part[0] = add2(part[0], pk2(e[0], e[1]));
                                     part[1] = add2(part[1], pk2(e[2], e[3]));
-                                    const float4 v4 = vf[CW / 4 * c + (j >> 2)];
+                                    const float4 v4 = vc[j >> 2];
                                     unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
                                     unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
                                 }
@@ -526,18 +524,90 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     part[1] = add2(part[1], pk2(bflo(p[j / 2 + 1]), bfhi(p[j / 2 + 1])));
                                 }
                             }
+                        }
+                        float a0, a1;
+                        unpk2(add2(part[0], part[1]), a0, a1);
+                        const float sum = a0 + a1;
+                        if (__builtin_expect(__any_sync(0xffffffffu, sum > 32768.f || (fresh && sum < 0x1p-20f)), 0)) break;
+                        fresh = false;
+                        l += sum;
+                        // over columns whose scores have been read
+                        if constexpr (COLS == 64)
+                            pp_st32(sh, p);
+                        else
+                            pp_st16(sh + c / 2, p);
+                    }
+                }
+                if (c == 64) {
+                } else if (__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
+                    // The same for some of the keys, 32 at a time. Where it does not do, the reference moves to the
+                    // largest of them and their weights are formed anew (the scores are still in TMEM): for a row that
+                    // has summed something by a whole number, so that what is done is rescaled exactly.
+#pragma unroll 1
+                    for (; c < 64; c += 32) {
+                        const uint32_t sc = sh + c, bt = c == 0 ? bits[0] : bits[1];
+                        const float4 *kc = kf + c / 4, *vc = vf + c / 4;
+                        uint32_t p[16];
+                        if (!__any_sync(0xffffffffu, bt != 0)) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) p[j] = 0;
+                            pp_st16(sh + c / 2, p);
+                            continue;
+                        }
+                        float sum;
+#pragma unroll 1
+                        for (bool again = false;; again = true) {
+                            unsigned long long part[2] = {0ull, 0ull};
+#pragma unroll
+                            for (int b = 0; b < 32; b += 8) {
+                                float s[8];
+                                pp_ld8(sc + b, reinterpret_cast<uint32_t *>(s));
+                                pp_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 8; i += 4) {
+                                    const int j = b + i;
+                                    float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
+                                    if constexpr (KV8) {
+                                        const float4 k4 = kc[j >> 2];
+                                        f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
+                                    }
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {  // x rounded before m is subtracted, as below
+                                        const float y = __fadd_rn(__fmul_rn(s[i + k], f[k]), -m);
+                                        e[k] = pp_ex2(bt & (1u << (j + k)) ? y : -INFINITY);
+                                    }
+                                    if constexpr (KV8) {
+                                        part[0] = add2(part[0], pk2(e[0], e[1]));
+                                        part[1] = add2(part[1], pk2(e[2], e[3]));
+                                        const float4 v4 = vc[j >> 2];
+                                        unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
+                                        unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
+                                    }
+                                    p[j / 2] = pp_pack(e[0], e[1]);
+                                    p[j / 2 + 1] = pp_pack(e[2], e[3]);
+                                    if constexpr (!KV8) {
+                                        part[0] = add2(part[0], pk2(bflo(p[j / 2]), bfhi(p[j / 2])));
+                                        part[1] = add2(part[1], pk2(bflo(p[j / 2 + 1]), bfhi(p[j / 2 + 1])));
+                                    }
+                                }
+                            }
                             float a0, a1;
                             unpk2(add2(part[0], part[1]), a0, a1);
                             sum = a0 + a1;
-                        };
-                        weights(m);
-                        const bool lift = sum > 32768.f || (fresh && bt != 0 && sum < 0x1p-20f);
-                        if (__builtin_expect(__any_sync(0xffffffffu, lift), 0)) {
+                            const bool lift = sum > 32768.f || (fresh && bt != 0 && sum < 0x1p-20f);
+                            // once more at most: then the largest weight is in (1/2, 1] and the sum at most 32 (or NaN)
+                            if (again || !__any_sync(0xffffffffu, lift)) break;
                             float top = -INFINITY;
+#pragma unroll 1
+                            for (int j = 0; j < 32; j += 8) {
+                                uint32_t o[8];
+                                pp_ld8(sc + j, o);
+                                pp_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < CW; ++j) {
-                                const float f = KV8 ? reinterpret_cast<const float *>(kc)[j] : w.fac;
-                                top = fmaxf(top, bt & (1u << j) ? s[j] * f : -INFINITY);
+                                for (int k = 0; k < 8; ++k) {
+                                    const float f = KV8 ? reinterpret_cast<const float *>(kc)[j + k] : w.fac;
+                                    if (bt >> (j + k) & 1) top = fmaxf(top, __fmul_rn(__uint_as_float(o[k]), f));
+                                }
                             }
                             // 2^-by in two factors (nothing that counts is that far below: 0 beyond 2^-252)
                             float f = 1.f, f2 = 1.f;
@@ -554,6 +624,9 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                 }
                             }
                             l = l * f * f2;
+                            // scores so large that their own rounding shows: an fma would weigh equal ones
+                            // differently here and above, by 2^-12 at this size and without bound beyond
+                            far = far || __any_sync(0xffffffffu, fabsf(m) > 4096.f);
                             if (n > 0) {
                                 // every product into the context so far is complete: those over this buffer precede
                                 // its scores, that over the other buffer precedes that buffer's next scores
@@ -561,17 +634,17 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     ok = __all_sync(0xffffffffu, pp_wait(&s_bar[buf ^ 1], (round + (n + 1) / C::NB) & 1, w.err, 63));
                                 tc::tc_fence_after();
 #pragma unroll 1
-                                for (int j = 0; j < DIM; j += 16) {
-                                    uint32_t o[16];
-                                    pp_ld16(o_addr + j, o);
+                                for (int j = 0; j < DIM; j += 8) {
+                                    uint32_t o[8];
+                                    pp_ld8(o_addr + j, o);
                                     pp_ld_wait();
 #pragma unroll
-                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f * f2);
-                                    pp_st16(o_addr + j, o);
+                                    for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f * f2);
+                                    pp_st8(o_addr + j, o);
                                 }
                             }
 #pragma unroll 1
-                            for (int j = 0; j < CW / 2 * c; j += 8) {  // this step's weights so far
+                            for (int j = 0; j < c / 2; j += 8) {  // this step's weights so far
                                 uint32_t o[8];
                                 pp_st_wait();
                                 pp_ld8(sh + j, o);
@@ -580,62 +653,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                 for (int k = 0; k < 8; ++k) o[k] = pp_pack(bflo(o[k]) * f * f2, bfhi(o[k]) * f * f2);
                                 pp_st8(sh + j, o);
                             }
-                            weights(m);
+                            if (!ok) break;
                         }
                         fresh = fresh && bt == 0;
                         l += sum;
-                        pp_st8(sh + CW / 2 * c, p);  // over columns whose scores have been read
+                        pp_st16(sh + c / 2, p);
                     }
-                };
-                bool done = false;
-                if constexpr (DIM == 128) {
-                    // two warps of a scheduler are not enough to hide that loop's latencies: 64 columns at once
-                    // (630 us against 554 for the benchmark's longest prompts; at 64 dims, with four warps, the
-                    // unrolled code is the slower one, 594 against 391 us)
-                    if (full && !__any_sync(0xffffffffu, fresh)) {
-                        float s[64], part[4] = {0.f, 0.f, 0.f, 0.f};
-                        uint32_t p[32];
-                        pp_ld32(sh, reinterpret_cast<uint32_t *>(s));
-                        pp_ld32(sh + 32, reinterpret_cast<uint32_t *>(s) + 32);
-                        pp_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 64; j += 4) {
-                            float e[4], f[4] = {w.fac, w.fac, w.fac, w.fac};
-                            if constexpr (KV8) {
-                                const float4 k4 = kf[j >> 2];
-                                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                e[k] = pp_ex2(fmaf(s[j + k], f[k], -m));
-                                if constexpr (KV8) part[k] += e[k];
-                            }
-                            if constexpr (KV8) {
-                                const float4 v4 = vf[j >> 2];
-                                e[0] *= v4.x, e[1] *= v4.y, e[2] *= v4.z, e[3] *= v4.w;
-                            }
-                            p[j / 2] = pp_pack(e[0], e[1]);
-                            p[j / 2 + 1] = pp_pack(e[2], e[3]);
-                            if constexpr (!KV8) {
-                                part[0] += bflo(p[j / 2]);
-                                part[1] += bfhi(p[j / 2]);
-                                part[2] += bflo(p[j / 2 + 1]);
-                                part[3] += bfhi(p[j / 2 + 1]);
-                            }
-                        }
-                        const float sum = (part[0] + part[1]) + (part[2] + part[3]);
-                        done = !__any_sync(0xffffffffu, sum > 32768.f);
-                        if (done) {
-                            l += sum;
-                            pp_st32(sh, p);
-                        }
-                    }
-                }
-                if (done) {
-                } else if (DIM == 64 && full) {
-                    step(std::false_type{});
-                } else if (__any_sync(0xffffffffu, (bits[0] | bits[1]) != 0)) {
-                    step(std::true_type{});
                 } else {
                     const uint32_t zero[32] = {};
                     pp_st32(sh, zero);

@@ -351,6 +351,41 @@ def test_scores_far_from_each_other(fmt, dim, shape):
     check_prefill(c, kv, keep, p, None, [0, 400, 500], 200, 5, scale=1.0)
 
 
+@FORMATS
+@DIMS
+@pytest.mark.parametrize('log', [20, 27, 34, 66])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_equal_scores_of_any_size_weigh_the_same(fmt, dim, log, sign):
+    """All keys are alike, so every score of a row is the same number, of a size whose fp32 steps pass 1 by far: the
+    result is the mean of the visible values.
+
+    Tolerance: a weight is 1 (times the value's scale) rounded by half a step of its type at most, W; the sum of n
+    products and n weights in fp32 errs by n U each; the result is rounded to bf16."""
+    n = 300
+    c = cache(log, fmt, dim, 32, [n, n])
+    k = np.full((n, c.hkv, dim), 1.34375, np.float32)
+    v = c.rand(n, c.hkv, dim)
+    for s in range(2):
+        c.write(0, s, np.arange(n), k, v)
+    keep = Keep()
+    kv = c.upload(keep)
+    heads = 7 * c.hkv
+    # scores of log2 size `log` or a little above, and no power of two
+    q = unbits(bits((sign * 2.0 ** log / dim * np.linspace(1, 1.9, heads)[:, None] * np.ones(dim)).astype(np.float32)))
+    values = c.read(0, 0, np.arange(n))[1].astype(np.float64).repeat(7, axis=1)
+    count = np.arange(1, n + 1)[:, None, None]
+    mean, size = values.cumsum(0) / count, abs(values).cumsum(0) / count
+
+    def check(got, at, w):
+        bound = (2 * w + 4 * n * U) * size[at]
+        bound = bound + BF16_HALF * (abs(mean[at]) + bound)
+        assert (abs(got - mean[at]) <= bound).all()
+
+    check(decode(c, kv, keep, 0, np.stack([q, q]), None, scale=1.0), [n - 1, n - 1], DECODE_W)
+    got = prefill(c, kv, keep, 0, np.stack([q] * (n + 20)), None, [0, n, n + 20], scale=1.0)
+    check(got, list(range(n)) + list(range(n - 20, n)), PREFILL_W)
+
+
 # ---------------------------------------------------------------- prefill
 def runs(c, rows):
     return np.concatenate([[0], np.cumsum(rows)]).tolist()
