@@ -39,22 +39,38 @@ int paged_check(const qwen_b200_paged_kv *kv) {
     return QWEN_B200_OK;
 }
 
-int paged_check_device(std::initializer_list<const void *> pointers) {
+// The cache's memory and every other device pointer of a call (NULL: not given) have
+// to be the current device's.
+static int paged_check_device(const qwen_b200_paged_kv &kv, std::initializer_list<const void *> more) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         return QWEN_B200_EDEVICE;
     }
-    for (const void *p : pointers) {
+    auto check = [&](const void *p) {
         cudaPointerAttributes a;
-        if (!p) continue;
+        if (!p) return QWEN_B200_OK;
         if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
             cudaGetLastError();
             return QWEN_B200_EDEVICE;
         }
-        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != dev)) return QWEN_B200_EINVAL;
-    }
+        const bool ours = a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev);
+        return ours ? QWEN_B200_OK : QWEN_B200_EINVAL;
+    };
+    const bool scales = kv.format == QWEN_B200_KV8;
+    const void *pool[] = {kv.k, kv.v, scales ? kv.kscales : nullptr, scales ? kv.vscales : nullptr, kv.table, kv.lengths};
+    for (const void *p : pool)
+        if (int rc = check(p)) return rc;
+    for (const void *p : more)
+        if (int rc = check(p)) return rc;
     return QWEN_B200_OK;
+}
+
+// Lists of 32-bit indexes and counts in device memory.
+static bool words_aligned(std::initializer_list<const uint32_t *> lists) {
+    uintptr_t bits = 0;
+    for (const uint32_t *p : lists) bits |= (uintptr_t)p;
+    return (bits & 3) == 0;
 }
 
 PagedView paged_view(const qwen_b200_paged_kv &kv, uint32_t layer) {
@@ -120,12 +136,16 @@ static PagedAttnArgs attn_args(const qwen_b200_paged_kv &kv, uint32_t layer, con
     return a;
 }
 
-// Checks shared by the page management calls (list pointers checked by the caller).
-static int pages_check(const qwen_b200_paged_kv *kv, uint32_t *status, void *ws, size_t ws_bytes) {
+// Checks shared by the page management calls.
+static int pages_check(const qwen_b200_paged_kv *kv, std::initializer_list<const uint32_t *> lists, uint32_t n,
+                       uint32_t *status, void *ws, size_t ws_bytes) {
     if (int rc = paged_check(kv)) return rc;
+    if (!words_aligned(lists) || n >= 1u << 31) return QWEN_B200_EINVAL;
     if (!kv->refs || !status || ((uintptr_t)status & 3) || !ws || ((uintptr_t)ws & 15)) return QWEN_B200_EINVAL;
     if (ws_bytes < pages_ws(kv->pages)) return QWEN_B200_EINVAL;
-    return paged_check_device({kv->k, kv->v, kv->table, kv->lengths, kv->refs, status, ws});
+    for (const uint32_t *p : lists)
+        if (int rc = paged_check_device(*kv, {p})) return rc;
+    return paged_check_device(*kv, {kv->refs, status, ws});
 }
 
 }  // namespace qb
@@ -139,8 +159,8 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
     if (!k || !v || !rows || !seqs || !positions || layer >= kv->layers || rows >= 1u << 31) return QWEN_B200_EINVAL;
     if (row_stride < (uint64_t)kv->kv_heads * kv->head_dim || (row_stride & 7) || row_stride > 1ull << 40)
         return QWEN_B200_EINVAL;
-    if (((uintptr_t)k | (uintptr_t)v) & 15) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, k, v, seqs, positions})) return rc;
+    if ((((uintptr_t)k | (uintptr_t)v) & 15) || !words_aligned({seqs, positions})) return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {k, v, seqs, positions})) return rc;
     return launch_paged_append(*kv, layer, k, v, row_stride, rows, seqs, positions, (cudaStream_t)stream);
 }
 
@@ -154,8 +174,8 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
                               float scale, uint16_t *ctx, uint64_t ctx_stride, void *workspace,
                               size_t workspace_bytes, void *stream) {
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
-    if (rows > 65536) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, q, seqs, ctx, workspace})) return rc;
+    if (rows > 65536 || !words_aligned({seqs})) return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {q, seqs, ctx, workspace})) return rc;
     if (workspace_bytes < paged_decode_ws(kv->kv_heads, q_heads, kv->head_dim, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, window, sinks, scale, ctx, ctx_stride);
     a.rows = rows;
@@ -173,9 +193,9 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
                                uint32_t rows, uint32_t window, uint32_t sinks, float scale, uint16_t *ctx,
                                uint64_t ctx_stride, void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
-    if (!starts || !n || n > 65536 || rows > 1u << 24) return QWEN_B200_EINVAL;
+    if (!starts || !n || n > 65536 || rows > 1u << 24 || !words_aligned({seqs, starts})) return QWEN_B200_EINVAL;
     if ((uint64_t)rows * (q_heads / kv->kv_heads) >= 1ull << 31) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device({kv->k, kv->v, kv->table, kv->lengths, q, seqs, starts, ctx, workspace})) return rc;
+    if (int rc = paged_check_device(*kv, {q, seqs, starts, ctx, workspace})) return rc;
     if (workspace_bytes < paged_prefill_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, window, sinks, scale, ctx, ctx_stride);
     a.rows = rows;
@@ -191,7 +211,7 @@ size_t qwen_b200_pages_workspace(const qwen_b200_paged_kv *kv) {
 int qwen_b200_op_pages_reserve(const qwen_b200_paged_kv *kv, const uint32_t *seqs, const uint32_t *tokens, uint32_t n,
                                uint32_t *status, void *workspace, size_t workspace_bytes, void *stream) {
     if (!seqs || !tokens || !n) return QWEN_B200_EINVAL;
-    if (int rc = pages_check(kv, status, workspace, workspace_bytes)) return rc;
+    if (int rc = pages_check(kv, {seqs, tokens}, n, status, workspace, workspace_bytes)) return rc;
     return launch_pages_reserve(*kv, seqs, tokens, n, status, workspace, (cudaStream_t)stream);
 }
 
@@ -199,28 +219,28 @@ int qwen_b200_op_pages_fork(const qwen_b200_paged_kv *kv, const uint32_t *parent
                             const uint32_t *prefix, uint32_t n, uint32_t *status, void *workspace,
                             size_t workspace_bytes, void *stream) {
     if (!parents || !children || !prefix || !n) return QWEN_B200_EINVAL;
-    if (int rc = pages_check(kv, status, workspace, workspace_bytes)) return rc;
+    if (int rc = pages_check(kv, {parents, children, prefix}, n, status, workspace, workspace_bytes)) return rc;
     return launch_pages_fork(*kv, parents, children, prefix, n, status, workspace, (cudaStream_t)stream);
 }
 
 int qwen_b200_op_pages_free(const qwen_b200_paged_kv *kv, const uint32_t *seqs, uint32_t n, uint32_t *status,
                             void *workspace, size_t workspace_bytes, void *stream) {
     if (!seqs || !n) return QWEN_B200_EINVAL;
-    if (int rc = pages_check(kv, status, workspace, workspace_bytes)) return rc;
+    if (int rc = pages_check(kv, {seqs}, n, status, workspace, workspace_bytes)) return rc;
     return launch_pages_free(*kv, seqs, n, status, (cudaStream_t)stream);
 }
 
 int qwen_b200_op_pages_compact(const qwen_b200_paged_kv *kv, uint32_t *status, void *workspace,
                                size_t workspace_bytes, void *stream) {
-    if (int rc = pages_check(kv, status, workspace, workspace_bytes)) return rc;
+    if (int rc = pages_check(kv, {}, 0, status, workspace, workspace_bytes)) return rc;
     return launch_pages_compact(*kv, status, workspace, (cudaStream_t)stream);
 }
 
 int qwen_b200_op_pages_copy(const qwen_b200_paged_kv *kv, const uint32_t *src, const uint32_t *dst, uint32_t n,
                             void *stream) {
     if (int rc = paged_check(kv)) return rc;
-    if (!src || !dst || !n) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device({kv->k, kv->v, src, dst})) return rc;
+    if (!src || !dst || !n || n >= 1u << 31 || !words_aligned({src, dst})) return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {src, dst})) return rc;
     return launch_pages_copy(*kv, src, dst, n, (cudaStream_t)stream);
 }
 

@@ -426,13 +426,14 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
  * qwen_b200_op_pages_* calls read it, and it may be NULL for the others.
  *
  * Requirements (QWEN_B200_EINVAL otherwise): head_dim 64 or 128; page_tokens
- * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables
- * 4-byte aligned; strides multiples of 16 rows that keep pages and layers
- * apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages * page_tokens <= 2^30; the
- * pool and every other device pointer of a call on the current device. The page ids, lengths and indexes in device
- * memory are not seen by the host: a sequence index >= seqs (for example
- * QWEN_B200_NO_SEQ in a padded batch) is no sequence, a length beyond the
- * table is cut to it, and tokens on a page id >= pages are not there. */
+ * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables and
+ * index lists 4-byte aligned; strides multiples of 16 rows that keep pages and
+ * layers apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages *
+ * page_tokens <= 2^30; the pool and every other device pointer of a call on the
+ * current device. The page ids, lengths and indexes in device memory are not
+ * seen by the host: a sequence index >= seqs (for example QWEN_B200_NO_SEQ in a
+ * padded batch) is no sequence, a length beyond the table is cut to it, and
+ * tokens on a page id >= pages are not there. */
 #define QWEN_B200_KV8 0u
 #define QWEN_B200_KV_BF16 1u
 #define QWEN_B200_NO_SEQ 0xffffffffu
@@ -469,11 +470,12 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * multiple of kv_heads. A row with no key (length 0, no sequence) is zero.
  * Unlike qwen_b200_op_attention this is not the oracle's bit-exact order: the
  * weights are held in 16 bits (two bf16 halves), sums are fp32, ctx is rounded
- * once; the order of the sums, and so the last bits, depends on the sizes in the call and
- * the GPU's number of SMs, and on nothing that varies from run to run. Only visible keys are read: what a page holds beyond the
- * length or outside the window does not matter, NaN included. ctx rows are
- * ctx_stride elements apart; q, ctx 16-byte aligned, strides multiples of 8
- * and at least q_heads * head_dim. The context is split over the GPU and
+ * once; the order of the sums, and so the last bits, depends on the sizes in
+ * the call and the GPU's number of SMs, and on nothing that varies from run to
+ * run. Only visible keys are read: what a page holds beyond the length or
+ * outside the window does not matter, NaN included. ctx rows are ctx_stride
+ * elements apart and do not overlap q; q, ctx 16-byte aligned, strides
+ * multiples of 8 and at least q_heads * head_dim. The context is split over the GPU and
  * joined in the workspace (contents do not matter before or after; calls that
  * overlap on the GPU need one each). rows * KV heads * blocks of 8 query heads
  * * (max_pages * page_tokens / 16 + 3) < 2^32. */
@@ -485,17 +487,17 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
 /* The same attention for the newest rows of n sequences (prompts and prompt
  * chunks): rows starts[i] .. starts[i + 1] - 1 of q are the last tokens of
  * sequence seqs[i] (seqs NULL: sequence i), the last of them at position
- * lengths - 1, their keys already in the cache; each row sees the keys up to its own position
- * under the window and first tokens. starts is [n + 1] on the device, not
+ * lengths - 1, their keys already in the cache; each row sees the keys up to
+ * its own position under the window and first tokens. starts is [n + 1] on the device, not
  * decreasing; q and ctx hold `rows` rows, and those at or behind starts[n] are
  * left as they were. Rows before the sequence's first token (more rows than
  * its length) and rows of no sequence are zero. Keys that no row of the
  * sequence in this call sees may hold anything; a NaN or infinity in a value
- * that some row sees may reach the rows around it. Softmax weights are rounded to
- * bf16 for the second product (with bf16 pools the rounded ones are summed
- * too); sums are fp32. The workspace's contents do not matter, but its first 4 bytes become
- * non-zero if a bounded device wait expired (ctx is then not valid): a caller
- * that wants to know zeroes them before. */
+ * that some row sees may reach the rows around it. Softmax weights are rounded
+ * to bf16 for the second product (with bf16 pools the rounded ones are summed
+ * too); sums are fp32. The workspace's contents do not matter, but its first 4
+ * bytes become non-zero if a bounded device wait expired (ctx is then not
+ * valid): a caller that wants to know zeroes them before. */
 size_t qwen_b200_paged_prefill_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
 int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
                                uint32_t q_heads, uint32_t n, const uint32_t *seqs, const uint32_t *starts,
@@ -511,7 +513,8 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * call changed nothing else. Free pages are taken lowest id first, in the
  * order of the list, so tables do not depend on timing. Calls on one cache
  * run one after the other; each needs qwen_b200_pages_workspace bytes
- * (16-byte aligned, contents do not matter). */
+ * (16-byte aligned, contents do not matter). Lists have fewer than 2^31
+ * entries. */
 #define QWEN_B200_PAGES_OK 0u
 #define QWEN_B200_PAGES_FULL 1u
 #define QWEN_B200_PAGES_BAD 2u

@@ -885,3 +885,35 @@ def test_a_workspace_too_small_is_refused():
     n = L().qwen_b200_paged_prefill_workspace(ref(kv), 14, 1, 4)
     assert L().qwen_b200_op_paged_prefill(ref(kv), 0, q, 896, 14, 1, None, keep(u32([0, 4])), 4, 0, 0, 0.125, q, 896,
                                           keep(np.zeros(16, np.uint8)), n - 1, stream()) == _lib.EINVAL
+
+
+@pytest.mark.parametrize('field', ['k', 'v', 'kscales', 'vscales', 'table', 'lengths', 'refs'])
+def test_a_cache_in_host_memory_is_refused(field):
+    c = cache(44, KV8, 64, 64, [300])
+    keep = Keep()
+    kv = c.upload(keep)
+    bad = (ctypes.c_uint8 * 8192)()
+    setattr(kv, field, (ctypes.addressof(bad) + 255) & ~255)
+    x, i = keep(np.zeros((4, 896), np.int16)), keep(u32([0, 4]))
+    ws, n = keep(np.zeros(1 << 22, np.uint8)), 1 << 22
+    if field != 'refs':
+        assert L().qwen_b200_op_paged_decode(ref(kv), 0, x, 896, 14, 1, None, 0, 0, 0.125, x, 896, ws, n, stream()) == _lib.EINVAL
+        assert L().qwen_b200_op_paged_append(ref(kv), 0, x, x, 896, 1, i, i, stream()) == _lib.EINVAL
+    assert L().qwen_b200_op_pages_free(ref(kv), i, 1, i, ws, n, stream()) == _lib.EINVAL
+    assert L().qwen_b200_op_pages_compact(ref(kv), i, ws, n, stream()) == _lib.EINVAL
+
+
+def test_lists_in_host_memory_are_refused():
+    c = cache(45, KV8, 64, 64, [300, 20])
+    keep = Keep()
+    kv = c.upload(keep)
+    bad = (ctypes.c_uint8 * 8192)()
+    at = (ctypes.addressof(bad) + 255) & ~255
+    i, ws, n, st = keep(u32([0, 4])), keep(np.zeros(1 << 16, np.uint8)), 1 << 16, keep(u32([0, 0]))
+    for x in range(3):
+        a, b, d = (at if x == y else i for y in range(3))
+        assert L().qwen_b200_op_pages_fork(ref(kv), a, b, d, 1, st, ws, n, stream()) == _lib.EINVAL
+        if x < 2:
+            assert L().qwen_b200_op_pages_reserve(ref(kv), a, b, 1, st, ws, n, stream()) == _lib.EINVAL
+            assert L().qwen_b200_op_pages_copy(ref(kv), a, b, 1, stream()) == _lib.EINVAL
+    assert L().qwen_b200_op_pages_free(ref(kv), at, 1, st, ws, n, stream()) == _lib.EINVAL

@@ -107,3 +107,22 @@ def test_both_pool_orders_pass_the_stride_check():
     for c in (kv(), kv(layer_stride=2 * 64, page_stride=4 * 2 * 64), kv(layers=1, layer_stride=0), kv(format=_lib.KV_BF16,
                                                                                                       kscales=None)):
         assert L.qwen_b200_pages_workspace(ctypes.byref(c)) > 0
+
+
+@pytest.mark.parametrize('op', ['append', 'prefill', 'reserve', 'fork', 'free', 'copy'])
+def test_index_lists_are_aligned(op):
+    assert calls(kv(), idx=A + 2)[op]() == _lib.EINVAL
+
+
+def test_index_lists_of_decode_are_aligned():
+    L = qwen_b200.lib()
+    assert L.qwen_b200_op_paged_decode(ctypes.byref(kv()), 0, A, 896, 14, 2, A + 1, 0, 0, 0.125, A, 896, A, 1 << 40,
+                                       None) == _lib.EINVAL
+    assert L.qwen_b200_op_paged_prefill(ctypes.byref(kv()), 0, A, 896, 14, 2, A + 3, A, 2, 0, 0, 0.125, A, 896, A, 1 << 40,
+                                        None) == _lib.EINVAL
+
+
+@pytest.mark.parametrize('op', ['reserve', 'fork', 'free', 'copy'])
+def test_lists_too_long_for_31_bits_are_refused(op):
+    assert calls(kv(), n=1 << 31)[op]() == _lib.EINVAL
+    assert calls(kv(), n=(1 << 32) - 1)[op]() == _lib.EINVAL
