@@ -512,6 +512,19 @@ def test_a_decode_row_equals_a_prompt_of_one_row(fmt):
 
 @FORMATS
 @DIMS
+@pytest.mark.parametrize('n', [1, 3, 26])
+def test_prefill_tiles_in_several_pieces(fmt, dim, n):
+    """Chunks of a few rows over hundreds of keys: every tile is split over CTAs, for few tiles and for many."""
+    lens = [1500 - 370 * (i % 4) + i for i in range(n)]
+    rows = [9 - i % 3 for i in range(n)]
+    c = cache(60 + n, fmt, dim, 64, lens)
+    keep = Keep()
+    kv = c.upload(keep)
+    check_prefill(c, kv, keep, c.rand(sum(rows), 14, dim) * 2, None, runs(c, rows))
+
+
+@FORMATS
+@DIMS
 def test_prefill_of_many_tiles(fmt, dim):
     """More tiles than CTAs, so that a CTA walks several segments; against 64 bits on the GPU, with the host's bound."""
     torch = torch_cuda()
