@@ -48,8 +48,9 @@
 // products 64). 3 prompts of up to 8192 rows, window 4096, 32 heads on 8 of 128
 // dims, bf16: 526 us, 750 TF/s (45 % of the GEMM rate). Bound by the chain from
 // scores to weights to product within a tile: without any softmax work the two
-// still take 230 and 434 us, and issue slots (47 and 38 % busy), exponentials
-// (27 and 37 %) and tensor cores (15 and 38 %) all have room.
+// still take 230 and 456 us, and issue slots (47 and 43 % busy), exponentials
+// (29 and 42 %) and tensor cores (17 and 44 %) all have room. 16 rows on 1000
+// keys take 19 us, the latency of two launches and of a CTA's one pass.
 // Every wait is bounded (error codes 57-69).
 #include <type_traits>
 
@@ -61,7 +62,7 @@ namespace qb {
 
 constexpr int PP_BLK = 128;
 constexpr int PP_MAX_SMS = 192;
-constexpr uint32_t PP_MIN_UNITS = 1;  // blocks a CTA takes at least (16 rows on 276 keys: 21.0 us, 23.2 with 2, 27.0 with 4)
+constexpr uint32_t PP_MIN_UNITS = 1;  // blocks a CTA takes at least (16 rows on 276 keys: 2 us more with 2, 6 us more with 4)
 constexpr int PP_SC = 4;              // blocks of scales and key masks in flight
 constexpr int PP_SEG = 2;             // segments published ahead
 
