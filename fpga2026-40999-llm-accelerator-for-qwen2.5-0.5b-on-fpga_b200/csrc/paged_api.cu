@@ -39,31 +39,30 @@ int paged_check(const qwen_b200_paged_kv *kv) {
     return QWEN_B200_OK;
 }
 
-// The cache's memory and every other device pointer of a call (NULL: not given) have
-// to be the current device's.
-static int paged_check_device(const qwen_b200_paged_kv &kv, std::initializer_list<const void *> more) {
+// Every device pointer of a call (NULL: not given) has to be the current device's.
+static int check_pointers(std::initializer_list<const void *> pointers) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         return QWEN_B200_EDEVICE;
     }
-    auto check = [&](const void *p) {
+    for (const void *p : pointers) {
         cudaPointerAttributes a;
-        if (!p) return QWEN_B200_OK;
+        if (!p) continue;
         if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
             cudaGetLastError();
             return QWEN_B200_EDEVICE;
         }
-        const bool ours = a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev);
-        return ours ? QWEN_B200_OK : QWEN_B200_EINVAL;
-    };
-    const bool scales = kv.format == QWEN_B200_KV8;
-    const void *pool[] = {kv.k, kv.v, scales ? kv.kscales : nullptr, scales ? kv.vscales : nullptr, kv.table, kv.lengths};
-    for (const void *p : pool)
-        if (int rc = check(p)) return rc;
-    for (const void *p : more)
-        if (int rc = check(p)) return rc;
+        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != dev)) return QWEN_B200_EINVAL;
+    }
     return QWEN_B200_OK;
+}
+static int paged_check_device(const qwen_b200_paged_kv &kv, std::initializer_list<const void *> more) {
+    const bool scales = kv.format == QWEN_B200_KV8;
+    if (int rc = check_pointers({kv.k, kv.v, scales ? kv.kscales : nullptr, scales ? kv.vscales : nullptr, kv.table,
+                                 kv.lengths}))
+        return rc;
+    return check_pointers(more);
 }
 
 // Lists of 32-bit indexes and counts in device memory.
@@ -144,7 +143,7 @@ static int pages_check(const qwen_b200_paged_kv *kv, std::initializer_list<const
     if (!kv->refs || !status || ((uintptr_t)status & 3) || !ws || ((uintptr_t)ws & 15)) return QWEN_B200_EINVAL;
     if (ws_bytes < pages_ws(kv->pages)) return QWEN_B200_EINVAL;
     for (const uint32_t *p : lists)
-        if (int rc = paged_check_device(*kv, {p})) return rc;
+        if (int rc = check_pointers({p})) return rc;
     return paged_check_device(*kv, {kv->refs, status, ws});
 }
 
