@@ -583,6 +583,9 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                         const float4 v4 = vc[j >> 2];
                                         unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
                                         unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
+#pragma unroll
+                                        for (int k = 0; k < 4; ++k)  // 0 whatever the scale of a value that the row does not see
+                                            e[k] = bt & (1u << (j + k)) ? e[k] : 0.f;
                                     }
                                     p[j / 2] = pp_pack(e[0], e[1]);
                                     p[j / 2 + 1] = pp_pack(e[2], e[3]);

@@ -492,8 +492,9 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * decreasing; q and ctx hold `rows` rows, and those at or behind starts[n] are
  * left as they were. Rows before the sequence's first token (more rows than
  * its length) and rows of no sequence are zero. Keys that no row of the
- * sequence in this call sees may hold anything; a NaN or infinity in a value
- * that some row sees may reach the rows around it. Softmax weights are rounded
+ * sequence in this call sees may hold anything. In KV8 pools that goes for each
+ * row by itself; in bf16 pools a NaN or infinity in a value that some row sees
+ * may reach the rows around it. Softmax weights are rounded
  * to bf16 for the second product (with bf16 pools the rounded ones are summed
  * too); sums are fp32. The workspace's contents do not matter, but its first 4
  * bytes become non-zero if a bounded device wait expired (ctx is then not

@@ -510,6 +510,26 @@ def test_a_decode_row_equals_a_prompt_of_one_row(fmt):
     check_prefill(c, kv, keep, q, None, [0, 1, 2, 3], 90, 3)
 
 
+@DIMS
+@pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize('what', ['ks', 'vs'])
+def test_prefill_rows_before_a_broken_scale_do_not_see_it(dim, bad, what):
+    """KV8: a key's or value's scale that is no number reaches the rows that see the token, and no other."""
+    n, at = 300, 170
+    c = cache(88, KV8, dim, 64, [n])
+    q = c.rand(n, 14, dim)
+    exact, tol = c.attention(0, q, [0] * n, range(n), 60, 3, dim ** -0.5, PREFILL_W)
+    p, t = c.at(0, at)
+    getattr(c, what)[0, p, :, t] = bad
+    keep = Keep()
+    kv = c.upload(keep)
+    got = prefill(c, kv, keep, 0, q, None, [0, n], 60, 3)
+    sees = (np.arange(n) >= at) & (np.arange(n) - at < 60)
+    assert_within(got[~sees], exact[~sees], tol[~sees])
+    if what == 'vs':
+        assert not np.isfinite(got[sees]).any()
+
+
 @FORMATS
 @DIMS
 @pytest.mark.parametrize('n', [1, 3, 26])
