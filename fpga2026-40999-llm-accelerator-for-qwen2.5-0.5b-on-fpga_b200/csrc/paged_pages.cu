@@ -156,12 +156,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, 
 struct PlanShared {
     uint32_t warp_sums[32];
     uint32_t seen[65536 / 32];  // one bit per sequence: named in this call
+    unsigned long long need;    // pages that the call wants
     uint32_t bad;
 };
 
 __device__ __forceinline__ void plan_begin(const PagesState &s, PlanShared &sh) {
     for (uint32_t i = threadIdx.x; i < (s.seqs + 31) / 32; i += PP_THREADS) sh.seen[i] = 0;
-    if (threadIdx.x == 0) sh.bad = 0;
+    if (threadIdx.x == 0) {
+        sh.bad = 0;
+        sh.need = 0;
+    }
     __syncthreads();
 }
 // Marks sequence q as named; false where it is out of range or was named before.
@@ -212,29 +216,28 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
     const int lane = threadIdx.x & 31;
     plan_begin(s, sh);
     const uint64_t cap = (uint64_t)s.max_pages << s.tshift;
-    uint32_t need = 0;  // pages taken; a call that wants 2^32 or more is too long for the table anyway
-    for (uint32_t base = 0; base < n; base += PP_THREADS) {
-        const uint32_t i = base + threadIdx.x;
-        uint32_t mine = 0;
-        if (i < n) {
-            const uint32_t q = seqs[i];
-            const bool ok = plan_name(s, sh, q);
-            const uint64_t len = ok ? s.lengths[q] : 0, next = len + tokens[i];
-            if (!ok || len > cap || next > cap)
-                sh.bad = 1;
-            else
-                mine = pages_of((uint32_t)next, s.tshift) - pages_of((uint32_t)len, s.tshift);
-        }
-        uint32_t total;
-        block_scan(mine, sh.warp_sums, total);
-        need = total > 0xffffffffu - need ? 0xffffffffu : need + total;
+    // 64 bits: a sequence may want 2^26 pages, and there are up to 65536 of them
+    unsigned long long want = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += PP_THREADS) {
+        const uint32_t q = seqs[i];
+        const bool ok = plan_name(s, sh, q);
+        const uint64_t len = ok ? s.lengths[q] : 0, next = len + tokens[i];
+        if (!ok || len > cap || next > cap)
+            sh.bad = 1;
+        else
+            want += pages_of((uint32_t)next, s.tshift) - pages_of((uint32_t)len, s.tshift);
     }
-    const uint32_t have = free_pages(s, sh, need);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) want += __shfl_xor_sync(0xffffffffu, want, o);
+    if (lane == 0 && want) atomicAdd(&sh.need, want);
+    __syncthreads();
+    const unsigned long long need = sh.need;
+    const uint32_t have = free_pages(s, sh, (uint32_t)min(need, (unsigned long long)s.pages));
     if (sh.bad || need > have) {
         plan_status(s, sh.bad ? QWEN_B200_PAGES_BAD : QWEN_B200_PAGES_FULL, have);
         return;
     }
-    uint32_t taken = 0;
+    uint32_t taken = 0;  // (need <= have: the sums below fit 32 bits)
     for (uint32_t base = 0; base < n; base += PP_THREADS) {
         const uint32_t i = base + threadIdx.x;
         uint32_t q = 0, held = 0, mine = 0;
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
             }
         }
     }
-    plan_status(s, QWEN_B200_PAGES_OK, have - need);
+    plan_status(s, QWEN_B200_PAGES_OK, have - (uint32_t)need);
 }
 
 __global__ void __launch_bounds__(PP_THREADS, 1)
