@@ -101,6 +101,8 @@ struct PagedAttnArgs {
 size_t paged_decode_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t rows);
 int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 size_t paged_prefill_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);
+// Whether the blocks of a KV head that such a call can have are counted in 32 bits.
+bool paged_prefill_fits(const PagedAttnArgs &a);
 int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 int launch_paged_append(const qwen_b200_paged_kv &kv, uint32_t layer, const uint16_t *k, const uint16_t *v,
                         uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,

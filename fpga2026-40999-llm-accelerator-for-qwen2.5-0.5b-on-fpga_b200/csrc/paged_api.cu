@@ -194,12 +194,13 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
     if (!starts || !n || n > 65536 || rows > 1u << 24 || !words_aligned({seqs, starts})) return QWEN_B200_EINVAL;
     if ((uint64_t)rows * (q_heads / kv->kv_heads) >= 1ull << 31) return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(*kv, {q, seqs, starts, ctx, workspace})) return rc;
-    if (workspace_bytes < paged_prefill_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, window, sinks, scale, ctx, ctx_stride);
     a.rows = rows;
     a.n = n;
     a.starts = starts;
+    if (!paged_prefill_fits(a)) return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {q, seqs, starts, ctx, workspace})) return rc;
+    if (workspace_bytes < paged_prefill_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     return launch_paged_prefill(a, workspace, (cudaStream_t)stream);
 }
 

@@ -1231,6 +1231,20 @@ size_t paged_prefill_ws(uint32_t, uint32_t, uint32_t dim, uint32_t, uint32_t) {
     return 256 + (size_t)PP_MAX_SMS * (sizeof(PpRec) + 2 * (2 * tile + tile * dim) * 4);
 }
 
+// From what the host knows: the tiles that the rows can be cut into, times the
+// blocks that a tile can see in the widest table row, or in its window (that of
+// all its tokens, cut at both ends) and the first tokens.
+bool paged_prefill_fits(const PagedAttnArgs &a) {
+    const uint64_t tile = a.dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE, group = a.qh / a.c.hkv;
+    const uint64_t tiles = a.rows * group / tile + a.n;
+    uint64_t blocks = (((uint64_t)a.c.max_pages << a.c.tshift) + PP_BLK - 1) / PP_BLK;
+    if (a.window) {
+        const uint64_t seen = (a.window + tile / group + 1) / PP_BLK + 2 + ((uint64_t)a.sinks + PP_BLK - 1) / PP_BLK;
+        blocks = blocks < seen ? blocks : seen;
+    }
+    return tiles * blocks < 1ull << 32;
+}
+
 template <bool KV8, int DIM>
 static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t st) {
     using C = PpCfg<KV8, DIM>;

@@ -488,7 +488,10 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * chunks): rows starts[i] .. starts[i + 1] - 1 of q are the last tokens of
  * sequence seqs[i] (seqs NULL: sequence i), the last of them at position
  * lengths - 1, their keys already in the cache; each row sees the keys up to
- * its own position under the window and first tokens. starts is [n + 1] on the device, not
+ * its own position under the window and first tokens. n <= 65536, rows <= 2^24,
+ * rows * (q_heads / kv_heads) < 2^31, and (rows * (q_heads / kv_heads) / t + n) *
+ * ceil(max_pages * page_tokens / 128) < 2^32 with t = 512 at 64 dims and 256 at 128
+ * (a window narrower than the table counts in its place). starts is [n + 1] on the device, not
  * decreasing; q and ctx hold `rows` rows, and those at or behind starts[n] are
  * left as they were. Rows before the sequence's first token (more rows than
  * its length) and rows of no sequence are zero. Keys that no row of the
