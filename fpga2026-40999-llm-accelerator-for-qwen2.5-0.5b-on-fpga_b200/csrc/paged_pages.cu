@@ -375,6 +375,35 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
 __global__ void __launch_bounds__(PP_THREADS, 1) pages_compact_kernel(PagesState s) {
     __shared__ PlanShared sh;
     pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) sh.bad = 0;
+    __syncthreads();
+    // Every sequence's length and pages, before anything changes: a page that a table names and refs counts as free
+    // would be overwritten by one that moves. A warp has 32 sequences' lengths at a time, and four of them in flight.
+    const uint64_t cap = (uint64_t)s.max_pages << s.tshift;
+    bool bad = false;
+    for (uint32_t base = warp; base < s.seqs; base += PP_THREADS) {
+        const uint32_t mine = base + 32 * lane, len = mine < s.seqs ? s.lengths[mine] : 0;
+        bad |= len > cap;
+        const uint32_t held = len > cap ? 0 : pages_of(len, s.tshift);
+        for (int k = 0; k < 32 && base + 32 * k < s.seqs; k += 4) {
+            uint32_t h[4], most = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = __shfl_sync(0xffffffffu, held, k + i);
+                most = max(most, h[i]);
+            }
+            for (uint32_t j = lane; j < most; j += 32) {
+                uint32_t page[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    page[i] = j < h[i] ? s.table[(uint64_t)(base + 32 * (k + i)) * s.max_pages + j] : PG_NO_PAGE;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bad |= j < h[i] && (page[i] >= s.pages || s.refs[page[i]] == 0);
+            }
+        }
+    }
+    if (bad) sh.bad = 1;  // (read behind the scans' barriers)
     uint32_t live = 0;
     for (uint32_t base = 0; base < s.pages; base += 4 * PP_THREADS) {
         uint32_t mine = 0, total;
@@ -385,6 +414,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) pages_compact_kernel(PagesState
         }
         block_scan(mine, sh.warp_sums, total);
         live += total;
+    }
+    if (sh.bad) {
+        if (threadIdx.x == 0) *s.count = 0;
+        plan_status(s, QWEN_B200_PAGES_BAD, s.pages - live);
+        return;
     }
     uint32_t holes = 0, movers = 0;
     for (uint32_t base = 0; base < s.pages; base += 4 * PP_THREADS) {
@@ -485,7 +519,7 @@ __global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(PageCopyArgs a) 
                 if ((u & ((1u << a.tshift) - 1)) < m.z) a.scales[which][to + u] = a.scales[which][from + u];
         }
     }
-    if (!a.remap) return;
+    if (!a.remap || count == 0) return;  // (no page moves: the tables stand)
     const uint32_t warps = gridDim.x * (PC_THREADS / 32);
     for (uint32_t q = blockIdx.x * (PC_THREADS / 32) + (threadIdx.x >> 5); q < a.seqs; q += warps) {
         const uint32_t held = min(pages_of(a.lengths[q], a.tshift), a.max_pages);

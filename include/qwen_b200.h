@@ -538,7 +538,8 @@ int qwen_b200_op_pages_free(const qwen_b200_paged_kv *kv, const uint32_t *seqs, 
                             void *workspace, size_t workspace_bytes, void *stream);
 /* Moves pages in use to the front of the pool: with L pages in use, the i-th
  * free page below L takes the i-th used page at or above L, in every layer,
- * and tables and refs follow. After it pages 0 .. L-1 are in use. */
+ * and tables and refs follow. After it pages 0 .. L-1 are in use. A held page
+ * that refs counts as free is _BAD too: another would be moved onto it. */
 int qwen_b200_op_pages_compact(const qwen_b200_paged_kv *kv, uint32_t *status, void *workspace,
                                size_t workspace_bytes, void *stream);
 /* Copies whole pages in every layer: dst[i] = src[i]. No tables change. A

@@ -7,9 +7,9 @@ import pytest
 
 import qwen_b200
 from gpu_util import Keep, dev, host, stream, sync, torch_cuda, vp
-from paged_ref import ref
+from paged_ref import Cache, ref
 from qwen_b200 import _lib
-from test_gpu_paged import u32, workspace
+from test_gpu_paged import Book, DevicePages, u32, workspace
 
 pytestmark = pytest.mark.gpu
 L = qwen_b200.lib
@@ -36,3 +36,39 @@ def test_a_request_of_more_than_32_bits_of_pages_is_full(more):
     sync()
     assert host(status).tolist() == [_lib.PAGES_FULL, pages]
     assert not host(lengths).any() and not host(refs).any()
+
+
+FORMATS = pytest.mark.parametrize('fmt', [_lib.KV8, _lib.KV_BF16], ids=['kv8', 'bf16'])
+
+
+def broken_caches(c):
+    """(what, the arrays changed) of caches whose tables, lengths and counts do not belong together, one at a time; c is
+    put back after each."""
+    last = c.seqs - 1
+    n = -(-int(c.lengths[last]) // c.T)
+    for what, array, at, value in (('a length beyond the table', c.lengths, 2, c.max_pages * c.T + 1),
+                                   ('the largest length', c.lengths, last, 0xffffffff),
+                                   ('a page id behind the pool', c.table, (0, 1), c.pages),
+                                   ('an id of no page', c.table, (last, n - 1), 0xffffffff),
+                                   ('a held page that counts as free', c.refs, int(c.table[last, n - 1]), 0)):
+        was = array[at].copy()
+        array[at] = value
+        yield what
+        array[at] = was
+
+
+@FORMATS
+@pytest.mark.parametrize('seqs', [3, 70, 1100])
+def test_compaction_of_a_broken_cache_is_refused(fmt, seqs):
+    lens = [40 + (7 * i) % 60 for i in range(seqs)]
+    c = Cache(seqs, fmt, 2, 64, 16, sum(-(-n // 16) for n in lens) + 200, seqs, 40).give(lens)
+    for what in broken_caches(c):
+        keep = Keep()
+        d = DevicePages(c, c.upload(keep), keep)
+        assert d('compact') == [_lib.PAGES_BAD, int((c.refs == 0).sum())], what
+        c.assert_same()
+    keep = Keep()
+    d, b = DevicePages(c, c.upload(keep), keep), Book(c)
+    for _ in range(2):  # the second finds nothing to move
+        assert d('compact') == b.compact()
+        c.assert_same()
