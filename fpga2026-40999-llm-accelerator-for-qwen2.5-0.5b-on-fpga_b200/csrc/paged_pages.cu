@@ -271,30 +271,28 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
     __shared__ PlanShared sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     plan_begin(s, sh);
+    bool bad = false;
     for (uint32_t i = threadIdx.x; i < n; i += PP_THREADS) {
         const uint32_t q = seqs[i];
-        if (!plan_name(s, sh, q) || s.lengths[q] > (uint64_t)s.max_pages << s.tshift) sh.bad = 1;
+        bad |= !plan_name(s, sh, q) || s.lengths[q] > (uint64_t)s.max_pages << s.tshift;
     }
-    __syncthreads();
-    bool bad = sh.bad;
-    __syncthreads();  // everybody has read it
-    if (!bad) {  // every held id, before anything changes
+    bad = __syncthreads_or(bad);
+    // f(page) for every page that the sequences hold, a warp for each of them; whether one was true
+    auto any_page = [&](auto f) {
+        bool any = false;
         for (uint32_t i = warp; i < n; i += PP_THREADS / 32) {
             const uint32_t q = seqs[i], held = pages_of(s.lengths[q], s.tshift);
-            for (uint32_t j = lane; j < held; j += 32)
-                if (s.table[(uint64_t)q * s.max_pages + j] >= s.pages) sh.bad = 1;
+            for (uint32_t j = lane; j < held; j += 32) any |= f(s.table[(uint64_t)q * s.max_pages + j]);
         }
-        __syncthreads();
-        bad = sh.bad;
-    }
+        return __syncthreads_or(any) != 0;
+    };
+    if (!bad) bad = any_page([&](uint32_t page) { return page >= s.pages; });  // before anything changes
     if (!bad) {
-        for (uint32_t i = warp; i < n; i += PP_THREADS / 32) {
-            const uint32_t q = seqs[i], held = pages_of(s.lengths[q], s.tshift);
-            for (uint32_t j = lane; j < held; j += 32)
-                atomicSub(&s.refs[s.table[(uint64_t)q * s.max_pages + j]], 1u);
-            __syncwarp();
-            if (lane == 0) s.lengths[q] = 0;
-        }
+        bad = any_page([&](uint32_t page) { return atomicSub(&s.refs[page], 1u) == 0; });
+        if (bad)  // more holders than counted: what was taken goes back
+            any_page([&](uint32_t page) { return atomicAdd(&s.refs[page], 1u), false; });
+        else
+            for (uint32_t i = threadIdx.x; i < n; i += PP_THREADS) s.lengths[seqs[i]] = 0;
     }
     __syncthreads();
     const uint32_t have = free_pages(s, sh, 0);
@@ -326,11 +324,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
         need += total;
     }
     __syncthreads();
-    if (!sh.bad) {  // every id of the prefixes, before anything changes
+    if (!sh.bad) {  // every id of the prefixes, before anything changes; a page that counts as free may be handed out
         for (uint32_t i = warp; i < n; i += PP_THREADS / 32) {
             const uint32_t p = parents[i], held = pages_of(prefix[i], s.tshift);
-            for (uint32_t j = lane; j < held; j += 32)
-                if (s.table[(uint64_t)p * s.max_pages + j] >= s.pages) sh.bad = 1;
+            for (uint32_t j = lane; j < held; j += 32) {
+                const uint32_t page = s.table[(uint64_t)p * s.max_pages + j];
+                if (page >= s.pages || s.refs[page] == 0) sh.bad = 1;
+            }
         }
     }
     const uint32_t have = free_pages(s, sh, need);

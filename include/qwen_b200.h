@@ -512,7 +512,10 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * that it can be captured with the steps around it. Each call writes
  * status[0] = QWEN_B200_PAGES_OK, _FULL (not enough free pages) or _BAD (an
  * index out of range or named twice, a child that is not empty, a prefix
- * longer than its parent, a length beyond the table, a held page id >= pages),
+ * longer than its parent, a length beyond the table; where the call follows the
+ * pages of a sequence (free, those of a prefix in fork, all of them in compact) a
+ * held page id >= pages, or a held page whose refs are 0; in free, also one with
+ * fewer refs than sequences named that hold it),
  * and status[1] = the free pages after the call. When status[0] is not OK the
  * call changed nothing else. Free pages are taken lowest id first, in the
  * order of the list, so tables do not depend on timing. Calls on one cache
@@ -538,8 +541,7 @@ int qwen_b200_op_pages_free(const qwen_b200_paged_kv *kv, const uint32_t *seqs, 
                             void *workspace, size_t workspace_bytes, void *stream);
 /* Moves pages in use to the front of the pool: with L pages in use, the i-th
  * free page below L takes the i-th used page at or above L, in every layer,
- * and tables and refs follow. After it pages 0 .. L-1 are in use. A held page
- * that refs counts as free is _BAD too: another would be moved onto it. */
+ * and tables and refs follow. After it pages 0 .. L-1 are in use. */
 int qwen_b200_op_pages_compact(const qwen_b200_paged_kv *kv, uint32_t *status, void *workspace,
                                size_t workspace_bytes, void *stream);
 /* Copies whole pages in every layer: dst[i] = src[i]. No tables change. A

@@ -48,7 +48,7 @@ def broken_caches(c):
     n = -(-int(c.lengths[last]) // c.T)
     for what, array, at, value in (('a length beyond the table', c.lengths, 2, c.max_pages * c.T + 1),
                                    ('the largest length', c.lengths, last, 0xffffffff),
-                                   ('a page id behind the pool', c.table, (0, 1), c.pages),
+                                   ('a page id behind the pool', c.table, (1, 1), c.pages),
                                    ('an id of no page', c.table, (last, n - 1), 0xffffffff),
                                    ('a held page that counts as free', c.refs, int(c.table[last, n - 1]), 0)):
         was = array[at].copy()
@@ -72,3 +72,46 @@ def test_compaction_of_a_broken_cache_is_refused(fmt, seqs):
     for _ in range(2):  # the second finds nothing to move
         assert d('compact') == b.compact()
         c.assert_same()
+
+
+def refused(c, what, *lists):
+    """Runs a call on a fresh copy of c that has to change nothing."""
+    keep = Keep()
+    d = DevicePages(c, c.upload(keep), keep)
+    assert d(what, *lists) == [_lib.PAGES_BAD, int((c.refs == 0).sum())], (what, lists)
+    c.assert_same()
+
+
+@FORMATS
+@pytest.mark.parametrize('seqs', [3, 70])
+def test_sequences_of_a_broken_cache_are_not_freed_or_forked(fmt, seqs):
+    lens = [0] + [40 + (7 * i) % 60 for i in range(1, seqs)]
+    c = Cache(seqs, fmt, 2, 64, 16, sum(-(-n // 16) for n in lens) + 20, seqs, 40).give(lens)
+    last = seqs - 1
+    c.table[0, 1] = c.pages  # (not held: sequence 0 is empty)
+    for what in broken_caches(c):
+        refused(c, 'free', list(range(seqs)))
+        if what.startswith('a held page'):
+            refused(c, 'free', [last])
+            refused(c, 'fork', [last], [0], [int(c.lengths[last])])  # the page in question ends the prefix
+            c.lengths[last] = 16 * (int(c.lengths[last]) // 16)
+            keep = Keep()
+            d, b = DevicePages(c, c.upload(keep), keep), Book(c)
+            assert d('fork', [last], [0], [int(c.lengths[last])]) == b.fork([last], [0], [int(c.lengths[last])])
+            c.assert_same()
+
+
+@FORMATS
+def test_a_page_of_more_holders_than_its_count_is_not_freed(fmt):
+    """Two sequences on the same pages, counted once: freed together they would take a count below 0; one of them alone
+    is freed, and the other is then refused."""
+    c = Cache(4, fmt, 2, 64, 16, 80, 40, 12).give([100, 0, 35] + [16] * 37)
+    c.table[1], c.lengths[1] = c.table[0], 100
+    refused(c, 'free', [2, 0, 3, 1])
+    refused(c, 'free', list(range(40)))
+    keep = Keep()
+    d, b = DevicePages(c, c.upload(keep), keep), Book(c)
+    assert d('free', [2, 0]) == b.free([2, 0])
+    c.assert_same()
+    refused(c, 'free', [1])
+    refused(c, 'compact')
