@@ -127,7 +127,7 @@ struct PpMaps {  // bf16 pools
 };
 
 struct PpSeqInfo {
-    uint32_t row0, seq, mrows;
+    uint32_t row0, seq, rows, mrows;
     int pos0, nt;
 };
 __device__ __forceinline__ PpSeqInfo pp_seq(const PagedAttnArgs &a, const PpWork &w, uint32_t i) {
@@ -135,12 +135,21 @@ __device__ __forceinline__ PpSeqInfo pp_seq(const PagedAttnArgs &a, const PpWork
     const uint32_t s0 = min(a.starts[i], a.rows), s1 = min(max(a.starts[i + 1], s0), a.rows);
     s.row0 = s0;
     s.seq = a.seqs ? a.seqs[i] : i;
-    s.mrows = (s1 - s0) * w.group;
+    s.rows = s1 - s0;
+    s.mrows = s.rows * w.group;
     const int len = paged_length(a.c, s.seq);
-    s.pos0 = len - (int)(s1 - s0);
+    s.pos0 = len - (int)s.rows;
     s.nt = len > 0 ? (int)((s.mrows + w.tile - 1) / w.tile) : 0;
     return s;
 }
+// Rows of a sequence in front of its first token (all of them, where there is no token or no sequence): zero.
+__device__ __forceinline__ uint32_t pp_dead(const PpSeqInfo &s) {
+    return s.pos0 >= 0 ? 0u : min((uint32_t)-s.pos0, s.rows);
+}
+// The most of them that one CTA's warp writes alone; more are shared by all CTAs, each of which then looks at each such
+// sequence: 14 heads of 64 dims, alone against shared, one sequence of 4096 rows 842 and 17 us, 256 of 200 rows 92 and
+// 129, 256 of 48 rows 29 and 70, 4096 of 40 rows 254 and 794.
+__device__ __forceinline__ uint32_t pp_dead_alone(const PagedAttnArgs &a) { return max(32u, a.n); }
 struct PpBlocks {
     int s128, low128, first, low, last, n;
 };
@@ -163,13 +172,15 @@ __device__ __forceinline__ uint32_t pp_units_warp(const PagedAttnArgs &a, const 
     for (int k = threadIdx.x & 31; k < nt; k += 32) u += pp_blocks(a, w, pos0, mrows, k).n;
     return __reduce_add_sync(0xffffffffu, u);
 }
-// Blocks of the sequences base + lane < end, one per lane.
-__device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const PpWork &w, uint32_t base, uint32_t end) {
+// Blocks of the sequences base + lane < end, one per lane; `dead` is set where the rows of one are zeroed by all CTAs.
+__device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const PpWork &w, uint32_t base, uint32_t end,
+                                                  bool &dead) {
     const uint32_t i = base + (threadIdx.x & 31);
     PpSeqInfo s = {};
     uint32_t u = 0;
     if (i < end) {
         s = pp_seq(a, w, i);
+        if (pp_dead(s) > pp_dead_alone(a)) dead = true;
         if (s.nt <= 4)
             for (int k = 0; k < s.nt; ++k) u += pp_blocks(a, w, s.pos0, s.mrows, k).n;
     }
@@ -324,7 +335,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     using C = PpCfg<KV8, DIM>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ unsigned long long wsum[C::WARPS], at_prefix;
-    __shared__ uint32_t at_seq;
+    __shared__ uint32_t at_seq, wdead[C::WARPS];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = tc::smem_u32(sm);
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + C::BARS);
@@ -372,8 +383,13 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     // ---- numbering of the units: a warp takes a run of sequences
     const uint32_t per = (a.n + C::WARPS - 1) / C::WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
     unsigned long long mine = 0;
-    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane(a, w, b, i1));
-    if (lane == 0) wsum[warp] = mine;
+    bool dead = false;
+    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane(a, w, b, i1, dead));
+    dead = __any_sync(0xffffffffu, dead);
+    if (lane == 0) {
+        wsum[warp] = mine;
+        wdead[warp] = dead;
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -389,7 +405,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     if (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv) {
         unsigned long long p = before;
         for (uint32_t b = i0; b < i1; b += 32) {
-            uint32_t u = pp_units_lane(a, w, b, i1), x = u;
+            uint32_t u = pp_units_lane(a, w, b, i1, dead), x = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -1106,13 +1122,27 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     }
     if (warp == C::SW + 6) {  // (behind its segments)
         // ---------------- rows in front of the first token, and of no sequence
+        const uint32_t chunks = a.qh * (DIM / 8);
+        auto zero = [&](uint32_t row0, uint32_t n, uint32_t r0, uint32_t step) {
+            for (uint32_t r = r0; r < n; r += step)
+                for (uint32_t c = lane; c < chunks; c += 32)
+                    *reinterpret_cast<uint4 *>(a.ctx + (row0 + (uint64_t)r) * a.ctx_stride + 8 * c) = make_uint4(0, 0, 0, 0);
+        };
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
             const PpSeqInfo s = pp_seq(a, w, i);
-            const uint32_t nrows = s.mrows / w.group, zero = s.pos0 >= 0 ? 0 : min((uint32_t)-s.pos0, nrows);
-            const uint32_t chunks = a.qh * (DIM / 8);
-            for (uint32_t r = 0; r < zero; ++r)
-                for (uint32_t c = lane; c < chunks; c += 32)
-                    *reinterpret_cast<uint4 *>(a.ctx + (s.row0 + (uint64_t)r) * a.ctx_stride + 8 * c) = make_uint4(0, 0, 0, 0);
+            if (pp_dead(s) <= pp_dead_alone(a)) zero(s.row0, pp_dead(s), 0, 1);
+        }
+        // the runs of sequences in which the numbering met more rows (padded prompts)
+        for (uint32_t runs = __ballot_sync(0xffffffffu, lane < C::WARPS && wdead[lane]); runs; runs &= runs - 1) {
+            for (uint32_t b = min((__ffs(runs) - 1) * per, a.n), e = min(b + per, a.n); b < e; b += 32) {
+                const PpSeqInfo s = pp_seq(a, w, min(b + lane, e - 1));
+                const uint32_t n = b + lane < e ? pp_dead(s) : 0;
+                for (uint32_t todo = __ballot_sync(0xffffffffu, n > pp_dead_alone(a)); todo; todo &= todo - 1) {
+                    const int l = __ffs(todo) - 1;
+                    zero(__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, n, l), (blockIdx.x + b + l) % gridDim.x,
+                         gridDim.x);
+                }
+            }
         }
     }
     tc::tc_fence_before();
