@@ -953,8 +953,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     if (t < tiles) round[t] += steps / C::NB;
                 ++nseg;
             }
-            // every MMA is complete before TMEM is freed
-            if (lane == 0) {
+            // every MMA is complete before TMEM is freed (the commit is the thread's that issued them)
+            if (pp_elect()) {
                 tc::mma_commit(mdone);
                 pp_wait(mdone, 0, w.err, 69);
             }
@@ -964,8 +964,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             // of it); KV8 pages as runs of codes, bf16 pages as swizzled boxes
             PpReader rd{ring, seg_full, seg_empty};
             const int per = min(1 << a.c.tshift, PP_BLK), npages = PP_BLK / per;  // tokens of a copy, copies of a block
-            constexpr uint32_t RB = KV8 ? DIM : 2 * DIM;
+            constexpr uint32_t RB = KV8 ? DIM : 2 * DIM, RING = KV8 ? C::RAW : C::SLOTS;
             uint32_t tiles = 0;
+            auto full_of = [&](uint32_t t) {  // what the copies of tile t (K and V in turn) complete on
+                return KV8 ? &raw_full[t % C::RAW] : t & 1 ? &raw_full[t / 2 % C::RAW] : &kv_full[t % C::SLOTS];
+            };
             PpSeg g;
             while (ok) {
                 ok = rd.next(g, w.err);
@@ -986,17 +989,10 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     const int row = ((int)g.kvh << a.c.tshift) + (key & ((1 << a.c.tshift) - 1));  // within the page
 #pragma unroll 1
                     for (int kv = 0; kv < 2; ++kv, ++tiles) {
-                        uint64_t *bar;
-                        uint32_t slot;
-                        if constexpr (KV8) {
-                            slot = tiles % C::RAW;
-                            bar = &raw_full[slot];
-                            if (tiles >= C::RAW) ok = pp_wait(&raw_empty[slot], ((tiles / C::RAW) & 1) ^ 1, w.err, 57);
-                        } else {
-                            slot = tiles % C::SLOTS;
-                            bar = kv ? &raw_full[tiles / 2 % C::RAW] : &kv_full[slot];
-                            if (tiles >= C::SLOTS) ok = pp_wait(&kv_empty[slot], ((tiles / C::SLOTS) & 1) ^ 1, w.err, 57);
-                        }
+                        uint64_t *bar = full_of(tiles);
+                        const uint32_t slot = tiles % RING;
+                        if (tiles >= RING)
+                            ok = pp_wait(KV8 ? &raw_empty[slot] : &kv_empty[slot], ((tiles / RING) & 1) ^ 1, w.err, 57);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         if (lane == 0) tc::mbar_arrive_expect_tx(bar, bytes);
@@ -1015,6 +1011,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     }
                 }
             }
+            // No copy is in flight when the CTA ends, also where a wait ran out and nobody waits for the last ones.
+            for (uint32_t t = tiles > RING ? tiles - RING : 0; t < tiles; ++t) pp_wait(full_of(t), (t / RING) & 1, w.err, 57);
         } else if (warp == C::SW + 6) {
             // ---------------- segments
             uint32_t n = 0;
