@@ -1307,8 +1307,7 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     w.max_ctas = (uint32_t)(sms < PP_MAX_SMS ? sms : PP_MAX_SMS);
     w.tile = a.dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
     w.negate = a.scale < 0.f;
-    const float f = fabsf(a.scale) * 1.44269504f;
-    w.fac = f > 1e-30f ? f : 1e-30f;  // a scale of 0 leaves masked scores at -inf
+    w.fac = fabsf(a.scale) * 1.44269504f;
     w.err = (unsigned *)ws;
     w.recs = reinterpret_cast<PpRec *>((char *)ws + 256);
     w.pieces = reinterpret_cast<float *>((char *)ws + 256 + PP_MAX_SMS * sizeof(PpRec));
