@@ -111,7 +111,7 @@ static int attn_check(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16
     if (q_stride < width || ctx_stride < width || ((q_stride | ctx_stride) & 7)) return QWEN_B200_EINVAL;
     if (q_stride > 1ull << 40 || ctx_stride > 1ull << 40) return QWEN_B200_EINVAL;
     if (((uintptr_t)q | (uintptr_t)ctx | (uintptr_t)ws) & 15) return QWEN_B200_EINVAL;
-    if (!(scale > -3.0e38f && scale < 3.0e38f)) return QWEN_B200_EINVAL;
+    if (!(fabsf(scale) <= 2.0e38f)) return QWEN_B200_EINVAL;  // log2(e) scale is finite
     return QWEN_B200_OK;
 }
 

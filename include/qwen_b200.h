@@ -466,8 +466,8 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  *     ctx[r][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j - max),
  * over the keys j < len with window == 0, or len - 1 - j < window (a sliding
  * window that counts the token itself), or j < sinks (first tokens that stay
- * visible). Query head h reads KV head h / (q_heads / kv_heads); q_heads is a
- * multiple of kv_heads. A row with no key (length 0, no sequence) is zero.
+ * visible). |scale| <= 2e38. Query head h reads KV head h / (q_heads / kv_heads); q_heads is a
+ * multiple of kv_heads, at most 65536. A row with no key (length 0, no sequence) is zero.
  * Unlike qwen_b200_op_attention this is not the oracle's bit-exact order: the
  * weights are held in 16 bits (two bf16 halves), sums are fp32, ctx is rounded
  * once; the order of the sums, and so the last bits, depends on the sizes in

@@ -1,5 +1,5 @@
 """Sizes that the paged prompt attention can count in 32 bits are taken, larger
-ones are refused. Runs without a GPU: a call that passes the checks of its
+ones are refused; so are softmax scales whose product with log2(e) is not finite. Runs without a GPU: a call that passes the checks of its
 numbers goes on to look at its (made-up) pointers, which EDEVICE shows there;
 on a machine with a GPU those are refused with EINVAL too, so only the refusals
 are told apart there."""
@@ -9,7 +9,7 @@ import pytest
 
 import qwen_b200
 from qwen_b200 import _lib
-from test_paged_refusals import A, kv
+from test_paged_refusals import A, calls, kv
 
 
 def has_gpu():
@@ -70,3 +70,16 @@ def test_the_bound_holds_every_block_that_a_tile_visits():
                         low = span(first, window, sinks)[1]
                         lead = min((span(last, window, sinks)[0] + 127) >> 7, low >> 7)
                         assert lead + (last >> 7) + 1 - (low >> 7) <= bound
+
+
+@pytest.mark.parametrize('op', ['decode', 'prefill'])
+@pytest.mark.parametrize('scale', [2.4e38, -2.4e38, 2.99e38])
+def test_scales_whose_factor_would_be_infinite_are_refused(op, scale):
+    assert calls(kv(), scale=scale)[op]() == _lib.EINVAL
+
+
+@pytest.mark.skipif('has_gpu()')
+@pytest.mark.parametrize('op', ['decode', 'prefill'])
+@pytest.mark.parametrize('scale', [2.0e38, -2.0e38, 0.0, 1e-44])
+def test_scales_that_can_be_used_pass(op, scale):
+    assert calls(kv(), scale=scale)[op]() == _lib.EDEVICE
