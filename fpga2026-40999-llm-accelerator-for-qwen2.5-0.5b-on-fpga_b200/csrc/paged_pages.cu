@@ -286,11 +286,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1)
         }
         return __syncthreads_or(any) != 0;
     };
-    if (!bad) bad = any_page([&](uint32_t page) { return page >= s.pages; });  // before anything changes
     if (!bad) {
-        bad = any_page([&](uint32_t page) { return atomicSub(&s.refs[page], 1u) == 0; });
-        if (bad)  // more holders than counted: what was taken goes back
-            any_page([&](uint32_t page) { return atomicAdd(&s.refs[page], 1u), false; });
+        bad = any_page([&](uint32_t page) { return page >= s.pages || atomicSub(&s.refs[page], 1u) == 0; });
+        if (bad)  // an id that is no page, or more holders than counted: what was taken goes back
+            any_page([&](uint32_t page) { return page < s.pages && (atomicAdd(&s.refs[page], 1u), false); });
         else
             for (uint32_t i = threadIdx.x; i < n; i += PP_THREADS) s.lengths[seqs[i]] = 0;
     }
