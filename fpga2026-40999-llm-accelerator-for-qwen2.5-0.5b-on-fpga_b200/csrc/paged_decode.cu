@@ -24,8 +24,9 @@
 // instruction issue and the start's chain of length, page and key), one row over
 // 96 keys 6.3 us (that chain alone).
 //
-// The cache is read once (8 heads share each key); keys are copied to shared
-// memory by 16-byte cp.async, every warp with a ring of its own, so no barrier stands between the loads and the products. Both products
+// 8 query heads share each key that is read; a KV head of more is read once for
+// each block of 8. Keys are copied to shared memory by 16-byte cp.async, every warp with
+// a ring of its own, so no barrier stands between the loads and the products. Both products
 // are mma.sync m16n8k16 with the keys (then the dims) as the 16-row side and the
 // heads as the 8-column side: a row has up to 8 useful columns, where a
 // 128-row tcgen05 tile would be 6 % full, and per byte of cache these

@@ -481,7 +481,7 @@ constexpr uint32_t PC_SEG = PC_THREADS * 4 * 16;
 __global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(PageCopyArgs a) {
     pdl_wait();
     const uint32_t count = a.list ? *a.count : a.n;
-    const uint32_t page_bytes = (a.hkv * a.row_bytes) << a.tshift;  // at most 2^16 heads * 256 B * 256: checked on the host
+    const uint32_t page_bytes = (a.hkv * a.row_bytes) << a.tshift;  // at most 2^14 heads * 2^8 tokens * 2^8 bytes
     const uint32_t segs = (page_bytes + PC_SEG - 1) / PC_SEG;
     const uint64_t work = (uint64_t)count * a.layers * 2 * segs;
     for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
@@ -550,7 +550,6 @@ static PageCopyArgs copy_args(const qwen_b200_paged_kv &kv) {
 
 static int launch_copy(const qwen_b200_paged_kv &kv, const PageCopyArgs &a, uint64_t most, cudaStream_t st) {
     const uint64_t page_bytes = (uint64_t)kv.kv_heads * kv.page_tokens * a.row_bytes;
-    if (page_bytes >= 1ull << 31) return -1;
     const uint64_t segs = (page_bytes + PC_SEG - 1) / PC_SEG;
     const int sms = paged_sms();
     if (!sms) return -3;

@@ -30,7 +30,8 @@
 // columns. At 64 dims TMEM holds four tiles with one score buffer each, at 128
 // dims two tiles with two each: either way four steps are in flight and the
 // tensor cores work on three while the softmax has one. (64 dims with two buffers
-// of 32 keys for each tile: 390 us where this takes 336, the first case below.)
+// of 32 keys for each tile: 390 us for the first case below, against 336 with the
+// softmax code of that time.)
 //
 // Warps (one CTA per SM, registers moved to the softmax warps):
 //   0 ..      four softmax warps per MMA tile, one thread per row
@@ -44,13 +45,14 @@
 //             range), then zeroes the rows in front of a sequence's first token
 //   1         copies pages into shared memory: KV8 codes by bulk copies, bf16 rows by TMA
 // Measured: 8 prompts of 4096 rows, window 1024, 14 heads on 2 of 64 dims, KV8:
-// 307 us, 344 TF/s (the exponentials alone, 16 per clock and SM, take 117 us, the
+// 303 us, 350 TF/s (the exponentials alone, 16 per clock and SM, take 117 us, the
 // products 64). 3 prompts of up to 8192 rows, window 4096, 32 heads on 8 of 128
-// dims, bf16: 526 us, 750 TF/s (45 % of the GEMM rate). Bound by the chain from
+// dims, bf16: 517 us, 764 TF/s on the same inputs again and again, 545 us, 725
+// TF/s (44 % of the GEMM rate) on new ones each time. Bound by the chain from
 // scores to weights to product within a tile: without any softmax work the two
-// still take 230 and 456 us, and issue slots (47 and 43 % busy), exponentials
-// (29 and 42 %) and tensor cores (17 and 44 %) all have room. 16 rows on 1000
-// keys take 19 us, the latency of two launches and of a CTA's one pass.
+// still take 230 and 456 us, and issue slots (47 and 41 % busy), exponentials
+// (32 and 42 %) and tensor cores (19 and 44 %) all have room. 16 rows on 1000
+// keys take 18.6 us, the latency of two launches and of a CTA's one pass.
 // Every wait is bounded (error codes 57-69).
 #include <type_traits>
 
@@ -227,13 +229,6 @@ __device__ __forceinline__ uint64_t pp_desc_mn(uint32_t saddr) {
 }
 #define PP_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define PP_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
-__device__ __forceinline__ void pp_ld32(uint32_t addr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : PP_R8(r, 0), PP_R8(r, 8), PP_R8(r, 16), PP_R8(r, 24)
-        : "r"(addr));
-}
 __device__ __forceinline__ void pp_st32(uint32_t addr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -496,8 +491,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         bits[k] &= below(pos + 1) & (~below(low) | below(first));
                     }
                 }
-                // 64 at once at 64 dims: 323 us against 307 for the first case above; 32 at 128 dims: 539 us against
-                // 526 for the second. A second copy of this code behind the test, for the rows that fail it,
+                // 64 at once at 64 dims: 336 us against 303 for the first case above; 32 at 128 dims: 535 us against
+                // 517 for the second. A second copy of this code behind the test, for the rows that fail it,
                 // in place of the path below: 338 and 543 us.
                 constexpr int COLS = DIM == 64 ? 32 : 64;
                 int c = 0;  // keys done

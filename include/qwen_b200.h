@@ -428,7 +428,7 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
  * Requirements (QWEN_B200_EINVAL otherwise): head_dim 64 or 128; page_tokens
  * 16, 32, 64, 128 or 256; k, v, kscales, vscales 16-byte and the tables and
  * index lists 4-byte aligned; strides multiples of 16 rows that keep pages and
- * layers apart; pages < 2^31, seqs <= 65536, kv_heads <= 16384, max_pages *
+ * layers apart; pages < 2^31, seqs and layers <= 65536, kv_heads <= 16384, max_pages *
  * page_tokens <= 2^30; the pool and every other device pointer of a call on the
  * current device. The page ids, lengths and indexes in device memory are not
  * seen by the host: a sequence index >= seqs (for example QWEN_B200_NO_SEQ in a
@@ -472,7 +472,7 @@ int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * weights are held in 16 bits (two bf16 halves), sums are fp32, ctx is rounded
  * once; the order of the sums, and so the last bits, depends on the sizes in
  * the call and the GPU's number of SMs, and on nothing that varies from run to
- * run. Only visible keys are read: what a page holds beyond the length or
+ * run. The sums are not scaled to the values: those above 2^80 may overflow them. Only visible keys are read: what a page holds beyond the length or
  * outside the window does not matter, NaN included. ctx rows are ctx_stride
  * elements apart and do not overlap q; q, ctx 16-byte aligned, strides
  * multiples of 8 and at least q_heads * head_dim. The context is split over the GPU and
@@ -497,9 +497,11 @@ int qwen_b200_op_paged_decode(const qwen_b200_paged_kv *kv, uint32_t layer, cons
  * its length) and rows of no sequence are zero. Keys that no row of the
  * sequence in this call sees may hold anything. In KV8 pools that goes for each
  * row by itself; in bf16 pools a NaN or infinity in a value that some row sees
- * may reach the rows around it. Softmax weights are rounded
- * to bf16 for the second product (with bf16 pools the rounded ones are summed
- * too); sums are fp32. The workspace's contents do not matter, but its first 4
+ * may reach the rows around it. Softmax weights (KV8: times the value's scale)
+ * are rounded to bf16 for the second product. The denominator sums the rounded
+ * ones in bf16 pools and the unrounded ones in KV8 pools: there a row that sees one
+ * key, or one that outweighs the rest, is off by up to half a bf16 step, 2^-8, in
+ * all its dims alike, besides the rounding of the result. Sums are fp32. The workspace's contents do not matter, but its first 4
  * bytes become non-zero if a bounded device wait expired (ctx is then not
  * valid): a caller that wants to know zeroes them before. */
 size_t qwen_b200_paged_prefill_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
