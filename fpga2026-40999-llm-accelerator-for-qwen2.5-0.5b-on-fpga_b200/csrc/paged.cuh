@@ -3,6 +3,8 @@
 // is checked here before it is used, so no table, length or sequence list can
 // take an access out of the pool.
 #pragma once
+#include <initializer_list>
+
 #include "common.cuh"
 #include "qwen_b200.h"
 
@@ -86,6 +88,9 @@ inline uint32_t paged_row_bytes(const qwen_b200_paged_kv &kv) {
 }
 // SMs of the current device, looked up once per device.
 int paged_sms();
+// Whether every pointer (NULL: not given) is the current device's memory, and whether lists of 32-bit words are aligned.
+int check_pointers(std::initializer_list<const void *> pointers);
+bool words_aligned(std::initializer_list<const void *> lists);
 
 struct PagedAttnArgs {
     PagedView c;
@@ -107,6 +112,35 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 int launch_paged_append(const qwen_b200_paged_kv &kv, uint32_t layer, const uint16_t *k, const uint16_t *v,
                         uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
                         cudaStream_t st);
+// Attention of one token a row, rows starts[g] .. of group g sharing their first prefix[g] tokens.
+struct PagedSharedArgs {
+    PagedView c;
+    const uint16_t *q;
+    uint64_t q_stride, ctx_stride;
+    uint16_t *ctx;
+    const uint32_t *seqs, *starts, *prefix;
+    uint32_t qh, rows, n;
+    float scale;
+    uint32_t format, dim;
+};
+size_t paged_shared_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);
+int launch_paged_shared(const PagedSharedArgs &a, void *ws, cudaStream_t st);
+
+struct RotaryView {
+    const float *table;
+    uint32_t positions, rotated, pairs;
+};
+struct AppendRotary {
+    const uint16_t *q, *k, *v;
+    uint16_t *q_out;
+    uint64_t q_stride, q_out_stride, kv_stride;
+    uint32_t q_heads, rows;
+    const uint32_t *seqs, *positions;
+};
+int launch_rotary(const RotaryView &t, const uint16_t *x, uint64_t x_stride, uint32_t heads, uint32_t dim, uint32_t rows,
+                  const uint32_t *positions, uint16_t *out, uint64_t out_stride, cudaStream_t st);
+int launch_paged_append_rotary(const qwen_b200_paged_kv &kv, uint32_t layer, const RotaryView &t, const AppendRotary &a,
+                               cudaStream_t st);
 size_t pages_ws(uint32_t pages);
 int launch_pages_reserve(const qwen_b200_paged_kv &kv, const uint32_t *seqs, const uint32_t *tokens, uint32_t n,
                          uint32_t *status, void *ws, cudaStream_t st);

@@ -1,7 +1,7 @@
-// C entry points of the paged KV cache: argument checks, then one launcher.
-#include <initializer_list>
-
+// C entry points of the paged KV cache, of rotary positions and of sampling:
+// argument checks, then one launcher.
 #include "paged.cuh"
+#include "sample.cuh"
 
 using namespace qb;
 
@@ -40,7 +40,7 @@ int paged_check(const qwen_b200_paged_kv *kv) {
 }
 
 // Every device pointer of a call (NULL: not given) has to be the current device's.
-static int check_pointers(std::initializer_list<const void *> pointers) {
+int check_pointers(std::initializer_list<const void *> pointers) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
@@ -66,9 +66,9 @@ static int paged_check_device(const qwen_b200_paged_kv &kv, std::initializer_lis
 }
 
 // Lists of 32-bit indexes and counts in device memory.
-static bool words_aligned(std::initializer_list<const uint32_t *> lists) {
+bool words_aligned(std::initializer_list<const void *> lists) {
     uintptr_t bits = 0;
-    for (const uint32_t *p : lists) bits |= (uintptr_t)p;
+    for (const void *p : lists) bits |= (uintptr_t)p;
     return (bits & 3) == 0;
 }
 
@@ -135,11 +135,24 @@ static PagedAttnArgs attn_args(const qwen_b200_paged_kv &kv, uint32_t layer, con
     return a;
 }
 
+static int rotary_check(const qwen_b200_rotary *r, uint32_t head_dim) {
+    if (!r || !r->table || !r->positions || r->positions > QWEN_B200_ROTARY_POSITIONS) return QWEN_B200_EINVAL;
+    if (!r->rotated || r->rotated % 16 || r->rotated > head_dim || r->rotated > QWEN_B200_ROTARY_DIMS) return QWEN_B200_EINVAL;
+    if (r->layout != QWEN_B200_ROTARY_HALVES && r->layout != QWEN_B200_ROTARY_PAIRS) return QWEN_B200_EINVAL;
+    if ((uintptr_t)r->table & 15) return QWEN_B200_EINVAL;
+    return QWEN_B200_OK;
+}
+static RotaryView rotary_view(const qwen_b200_rotary &r) {
+    return {r.table, r.positions, r.rotated, r.layout == QWEN_B200_ROTARY_PAIRS};
+}
+
 // Checks shared by the page management calls.
 static int pages_check(const qwen_b200_paged_kv *kv, std::initializer_list<const uint32_t *> lists, uint32_t n,
                        uint32_t *status, void *ws, size_t ws_bytes) {
     if (int rc = paged_check(kv)) return rc;
-    if (!words_aligned(lists) || n >= 1u << 31) return QWEN_B200_EINVAL;
+    for (const uint32_t *p : lists)
+        if (!words_aligned({p})) return QWEN_B200_EINVAL;
+    if (n >= 1u << 31) return QWEN_B200_EINVAL;
     if (!kv->refs || !status || ((uintptr_t)status & 3) || !ws || ((uintptr_t)ws & 15)) return QWEN_B200_EINVAL;
     if (ws_bytes < pages_ws(kv->pages)) return QWEN_B200_EINVAL;
     for (const uint32_t *p : lists)
@@ -202,6 +215,92 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
     if (int rc = paged_check_device(*kv, {q, seqs, starts, ctx, workspace})) return rc;
     if (workspace_bytes < paged_prefill_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     return launch_paged_prefill(a, workspace, (cudaStream_t)stream);
+}
+
+size_t qwen_b200_paged_decode_shared_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows) {
+    if (paged_check(kv) || !q_heads || q_heads % kv->kv_heads || q_heads > 65536 || rows > 65536 || n > 65536) return 0;
+    return paged_shared_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows);
+}
+
+int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
+                                     uint32_t q_heads, uint32_t n, const uint32_t *starts, const uint32_t *prefix,
+                                     uint32_t rows, const uint32_t *seqs, float scale, uint16_t *ctx,
+                                     uint64_t ctx_stride, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
+    if (!starts || !prefix || !n || n > 65536 || rows > 65536 || !words_aligned({seqs, starts, prefix}))
+        return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {q, seqs, starts, prefix, ctx, workspace})) return rc;
+    if (workspace_bytes < paged_shared_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
+    PagedSharedArgs a;
+    a.c = paged_view(*kv, layer);
+    a.q = q;
+    a.q_stride = q_stride;
+    a.ctx_stride = ctx_stride;
+    a.ctx = ctx;
+    a.seqs = seqs;
+    a.starts = starts;
+    a.prefix = prefix;
+    a.qh = q_heads;
+    a.rows = rows;
+    a.n = n;
+    a.scale = scale;
+    a.format = kv->format;
+    a.dim = kv->head_dim;
+    return launch_paged_shared(a, workspace, (cudaStream_t)stream);
+}
+
+int qwen_b200_op_rotary(const qwen_b200_rotary *rotary, const uint16_t *x, uint64_t x_stride, uint32_t heads,
+                        uint32_t head_dim, uint32_t rows, const uint32_t *positions, uint16_t *out, uint64_t out_stride,
+                        void *stream) {
+    if (!head_dim || head_dim % 16 || head_dim > QWEN_B200_ROTARY_DIMS) return QWEN_B200_EINVAL;
+    if (int rc = rotary_check(rotary, head_dim)) return rc;
+    if (!x || !out || !positions || !rows || rows >= 1u << 31 || !heads || heads > 65536) return QWEN_B200_EINVAL;
+    const uint64_t width = (uint64_t)heads * head_dim;
+    if (x_stride < width || out_stride < width || ((x_stride | out_stride) & 7)) return QWEN_B200_EINVAL;
+    if (x_stride > 1ull << 32 || out_stride > 1ull << 32) return QWEN_B200_EINVAL;
+    if ((((uintptr_t)x | (uintptr_t)out) & 15) || !words_aligned({positions})) return QWEN_B200_EINVAL;
+    if (x == out && x_stride != out_stride) return QWEN_B200_EINVAL;
+    if (int rc = check_pointers({rotary->table, x, positions, out})) return rc;
+    return launch_rotary(rotary_view(*rotary), x, x_stride, heads, head_dim, rows, positions, out, out_stride,
+                         (cudaStream_t)stream);
+}
+
+int qwen_b200_op_paged_append_rotary(const qwen_b200_paged_kv *kv, uint32_t layer, const qwen_b200_rotary *rotary,
+                                     const uint16_t *q, uint64_t q_stride, uint32_t q_heads, uint16_t *q_out,
+                                     uint64_t q_out_stride, const uint16_t *k, const uint16_t *v, uint64_t row_stride,
+                                     uint32_t rows, const uint32_t *seqs, const uint32_t *positions, void *stream) {
+    if (int rc = paged_check(kv)) return rc;
+    if (int rc = rotary_check(rotary, kv->head_dim)) return rc;
+    if (!k || !v || !rows || !seqs || !positions || layer >= kv->layers || rows >= 1u << 31) return QWEN_B200_EINVAL;
+    if (row_stride < (uint64_t)kv->kv_heads * kv->head_dim || (row_stride & 7) || row_stride > 1ull << 32)
+        return QWEN_B200_EINVAL;
+    if ((((uintptr_t)k | (uintptr_t)v) & 15) || !words_aligned({seqs, positions})) return QWEN_B200_EINVAL;
+    if (q_heads) {
+        const uint64_t width = (uint64_t)q_heads * kv->head_dim;
+        if (!q || !q_out || q_heads > 65536 || q_stride < width || q_out_stride < width) return QWEN_B200_EINVAL;
+        if (((q_stride | q_out_stride) & 7) || q_stride > 1ull << 32 || q_out_stride > 1ull << 32) return QWEN_B200_EINVAL;
+        if (((uintptr_t)q | (uintptr_t)q_out) & 15) return QWEN_B200_EINVAL;
+        if (q == q_out && q_stride != q_out_stride) return QWEN_B200_EINVAL;
+    }
+    if (int rc = paged_check_device(*kv, {rotary->table, k, v, seqs, positions})) return rc;
+    if (q_heads)
+        if (int rc = check_pointers({q, q_out})) return rc;
+    return launch_paged_append_rotary(*kv, layer, rotary_view(*rotary),
+                                      {q, k, v, q_out, q_stride, q_out_stride, row_stride, q_heads, rows, seqs, positions},
+                                      (cudaStream_t)stream);
+}
+
+int qwen_b200_op_sample(const uint16_t *logits, uint64_t stride, uint32_t rows, uint32_t vocab, const float *temperature,
+                        const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *tokens,
+                        float *probs, void *stream) {
+    if (!logits || !u || !tokens || !rows || rows > 65536 || !vocab || vocab > SM_MAX_VOCAB) return QWEN_B200_EINVAL;
+    if (stride < vocab || stride > 1ull << 32 || ((uintptr_t)logits & 1)) return QWEN_B200_EINVAL;
+    if (!words_aligned({temperature, top_k, top_p, min_p, u, tokens, probs})) return QWEN_B200_EINVAL;
+    if (int rc = check_pointers({logits, temperature, top_k, top_p, min_p, u, tokens, probs})) return rc;
+    const int sms = paged_sms();
+    if (sms <= 0) return QWEN_B200_EDEVICE;
+    return launch_sample({logits, stride, rows, vocab, temperature, top_p, min_p, u, top_k, tokens, probs, 0, 0, 0}, sms,
+                         (cudaStream_t)stream);
 }
 
 size_t qwen_b200_pages_workspace(const qwen_b200_paged_kv *kv) {

@@ -1,0 +1,22 @@
+// What the host side of qwen_b200_op_sample hands to its kernel.
+#pragma once
+#include "common.cuh"
+
+namespace qb {
+
+constexpr uint32_t SM_MAX_VOCAB = 8 * 8191 * 8 - 8;  // 8 CTAs of 65528 elements, less the row's misalignment
+
+struct SampleArgs {
+    const uint16_t *logits;
+    uint64_t stride;
+    uint32_t rows, vocab;
+    const float *temperature, *top_p, *min_p, *u;
+    const uint32_t *top_k;
+    uint32_t *tokens;
+    float *probs;
+    uint32_t ctas, part;  // CTAs of a row; 16-byte groups that each counts
+    int unit;             // weights are whole multiples of 2^-unit
+};
+int launch_sample(SampleArgs a, int sms, cudaStream_t st);
+
+}  // namespace qb

@@ -4,7 +4,7 @@ The library is the product: there is no Python or CPU fallback. Importing this
 module fails loudly when the in-tree shared object has not been built.
 """
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_size_t, c_uint, c_uint16, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_size_t, c_uint, c_uint16, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parents[1] / 'libqwen_b200.so'
@@ -14,6 +14,9 @@ NOALLOC_SCRATCH_BYTES = 16 << 20
 FLAG_RTL_KV = 1
 KV8, KV_BF16, NO_SEQ = 0, 1, 0xffffffff
 PAGES_OK, PAGES_FULL, PAGES_BAD = 0, 1, 2
+ROTARY_HALVES, ROTARY_PAIRS = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
+NO_TOKEN = 0xffffffff
 VOCAB, HIDDEN, FFN, LAYERS = 151936, 896, 4864, 24
 
 
@@ -30,11 +33,23 @@ class PagedKV(ctypes.Structure):
                 ('page_tokens', c_uint32), ('head_dim', c_uint32), ('seqs', c_uint32), ('max_pages', c_uint32)]
 
 
+class Rotary(ctypes.Structure):
+    """qwen_b200_rotary: a device table of angles and the dims that it turns."""
+    _fields_ = [('table', c_void_p), ('positions', c_uint32), ('rotated', c_uint32), ('layout', c_uint32)]
+
+
+class RotaryAngles(ctypes.Structure):
+    """qwen_b200_rotary_angles: what a table of angles is made from."""
+    _fields_ = [('theta', c_double), ('factor', c_double), ('fast', c_double), ('slow', c_double), ('size', c_double),
+                ('rotated', c_uint32), ('scaling', c_uint32), ('trained', c_uint32)]
+
+
 _P8 = POINTER(ctypes.c_int8)
 _P16 = POINTER(c_uint16)
 _P32 = POINTER(c_uint32)
 _PF = POINTER(c_float)
 _PKV = POINTER(PagedKV)
+_PROT = POINTER(Rotary)
 
 _SIGNATURES = {
     'qwen_b200_default_config': (None, [POINTER(Config)]),
@@ -116,6 +131,17 @@ _SIGNATURES = {
     'qwen_b200_op_paged_prefill': (c_int, [_PKV, c_uint32, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_void_p,
                                            c_uint32, c_uint32, c_uint32, c_float, c_void_p, c_uint64, c_void_p,
                                            c_size_t, c_void_p]),
+    'qwen_b200_paged_decode_shared_workspace': (c_size_t, [_PKV, c_uint32, c_uint32, c_uint32]),
+    'qwen_b200_op_paged_decode_shared': (c_int, [_PKV, c_uint32, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p,
+                                                 c_void_p, c_uint32, c_void_p, c_float, c_void_p, c_uint64, c_void_p,
+                                                 c_size_t, c_void_p]),
+    'qwen_b200_op_paged_append_rotary': (c_int, [_PKV, c_uint32, _PROT, c_void_p, c_uint64, c_uint32, c_void_p, c_uint64,
+                                                 c_void_p, c_void_p, c_uint64, c_uint32, c_void_p, c_void_p, c_void_p]),
+    'qwen_b200_rotary_table': (c_int, [POINTER(RotaryAngles), c_uint32, _PF]),
+    'qwen_b200_op_rotary': (c_int, [_PROT, c_void_p, c_uint64, c_uint32, c_uint32, c_uint32, c_void_p, c_void_p, c_uint64,
+                                    c_void_p]),
+    'qwen_b200_op_sample': (c_int, [c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p]),
     'qwen_b200_pages_workspace': (c_size_t, [_PKV]),
     'qwen_b200_op_pages_reserve': (c_int, [_PKV, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
     'qwen_b200_op_pages_fork': (c_int, [_PKV, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_size_t,

@@ -407,6 +407,80 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
                                 const int8_t *w, const float *scale, uint32_t vocab, uint16_t *logits,
                                 uint32_t *tokens, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- sampling --------------------------------------------------------------- */
+/* One token per row of bf16 logits (those of qwen_b200_op_lm_head_argmax, or any
+ * others; rows `stride` elements apart, 2-byte aligned) from the uniform random
+ * number u[r] in [0, 1). The candidates in the order of their logits, the lowest
+ * id first among equal ones (both zeros are equal), have the weights
+ * w = exp((logit - largest) / temperature[r]). Kept are the top_k[r] first (0:
+ * all); of these, those with less than top_p[r] of their weight before them
+ * (1 and more: all); of these, those with w >= min_p[r], that is a probability of
+ * at least min_p times the largest one's. The first is always kept. tokens[r] is
+ * the first kept candidate whose running sum of weights passes u[r] times the
+ * kept sum, probs[r] (probs nullable) its share of the kept weight. NULL for
+ * temperature, top_k, top_p or min_p: 1, 0, 1 and 0 in every row. All arrays are
+ * on the device, and all parameters of a row are read there, so a call can be
+ * captured and replayed as the settings of its rows change.
+ * A temperature that is not above 0 (0, NaN) gives the greedy token of
+ * qwen_b200_op_lm_head_argmax, the highest id of equal ones, with probability 1.
+ * NaN and -infinity are no candidates; a row without any gives
+ * QWEN_B200_NO_TOKEN with probability 0. Next to a logit of +infinity the
+ * others weigh nothing. u outside of [0, 1) counts as its nearer end (NaN as 0), a NaN in
+ * top_p or min_p keeps the first candidate only. Weights are rounded to whole
+ * multiples of 2^-(63 - bits of vocab) and summed exactly, so the result depends on the
+ * row alone. vocab <= 524216, rows <= 65536. */
+#define QWEN_B200_NO_TOKEN 0xffffffffu
+int qwen_b200_op_sample(const uint16_t *logits, uint64_t stride, uint32_t rows, uint32_t vocab, const float *temperature,
+                        const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *tokens,
+                        float *probs, void *stream);
+
+/* ---- rotary positions ------------------------------------------------------- */
+/* Rotation of head dims by position, for any head size and both pairings,
+ * where qwen_b200_op_rope is the model's own (64 dims in halves, rounded as the
+ * reference rounds). Pair i of a head at position p turns by p f_i: dims (i, i +
+ * rotated / 2) in QWEN_B200_ROTARY_HALVES, (2 i, 2 i + 1) in
+ * QWEN_B200_ROTARY_PAIRS; dims from `rotated` on stay. The angles are a table
+ * that a program makes once: device fp32 [positions][rotated], each row the
+ * cosines of rotated / 2 angles, then their sines. rotated is a multiple of 16,
+ * at most head_dim; the table 16-byte aligned. A token whose position is not in
+ * the table is left out: nothing is written for it. */
+#define QWEN_B200_ROTARY_HALVES 0u
+#define QWEN_B200_ROTARY_PAIRS 1u
+#define QWEN_B200_ROTARY_POSITIONS (1u << 24)
+#define QWEN_B200_ROTARY_DIMS 512u
+typedef struct qwen_b200_rotary {
+    const float *table;
+    uint32_t positions, rotated, layout;
+} qwen_b200_rotary;
+/* The table on the host, angles in 64 bits, f_i = theta^(-2i / rotated) scaled
+ * for contexts `factor` times as long as the model was trained on:
+ *   PLAIN   as they are
+ *   LINEAR  f_i / factor
+ *   NTK     theta * factor^(rotated / (rotated - 2)) in place of theta
+ *   YARN    f_i for pairs that turn more than `fast` times in the `trained`
+ *           positions, f_i / factor for those that turn less than `slow` times, a
+ *           ramp over the pairs between (Peng et al. 2023; usually 32 and 1)
+ * cos and sin are multiplied by `size`; 0 stands for 1, with YARN for 0.1
+ * ln(factor) + 1. EINVAL for values that give no table. */
+#define QWEN_B200_ROTARY_PLAIN 0u
+#define QWEN_B200_ROTARY_LINEAR 1u
+#define QWEN_B200_ROTARY_NTK 2u
+#define QWEN_B200_ROTARY_YARN 3u
+typedef struct qwen_b200_rotary_angles {
+    double theta, factor, fast, slow, size;
+    uint32_t rotated, scaling, trained;
+} qwen_b200_rotary_angles;
+int qwen_b200_rotary_table(const qwen_b200_rotary_angles *angles, uint32_t positions, float *table);
+/* out[r][h] = x[r][h] turned to positions[r]: rows x_stride and out_stride
+ * elements apart, heads of head_dim (a multiple of 16, at most 512) side by
+ * side in a row, so query and key heads of a fused q|k|v row are one call. x and
+ * out 16-byte aligned, strides multiples of 8; out may be x (with the same
+ * stride) and overlaps it in no other way. Products and sums are fp32, each
+ * rounded, the result rounded once to bf16. */
+int qwen_b200_op_rotary(const qwen_b200_rotary *rotary, const uint16_t *x, uint64_t x_stride, uint32_t heads,
+                        uint32_t head_dim, uint32_t rows, const uint32_t *positions, uint16_t *out, uint64_t out_stride,
+                        void *stream);
+
 /* ---- paged KV cache: operator level ---------------------------------------- */
 /* A cache whose sequences hold pages of page_tokens tokens out of one pool,
  * instead of a contiguous slot each. The reference has one contiguous cache
@@ -459,6 +533,19 @@ typedef struct qwen_b200_paged_kv {
 int qwen_b200_op_paged_append(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *k, const uint16_t *v,
                               uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
                               void *stream);
+/* The same with the rotation on the way, in one pass over a fused q|k|v row:
+ * keys are turned to positions[r] (qwen_b200_rotary above) and written like the
+ * values, which are not; q_heads query heads of q (rows q_stride apart) are
+ * turned into q_out (rows q_out_stride apart; q_out may be q with the same
+ * stride, and overlaps it in no other way, nor k and v). The bits are those of qwen_b200_op_rotary and then
+ * qwen_b200_op_paged_append. q_heads 0 (q, q_out not looked at): keys and
+ * values only. A row that writes no key (no sequence, a position at or beyond its
+ * length or the table of angles, a page id >= pages) leaves its row of q_out as it
+ * was. */
+int qwen_b200_op_paged_append_rotary(const qwen_b200_paged_kv *kv, uint32_t layer, const qwen_b200_rotary *rotary,
+                                     const uint16_t *q, uint64_t q_stride, uint32_t q_heads, uint16_t *q_out,
+                                     uint64_t q_out_stride, const uint16_t *k, const uint16_t *v, uint64_t row_stride,
+                                     uint32_t rows, const uint32_t *seqs, const uint32_t *positions, void *stream);
 /* Attention of one token per sequence (the last one, whose key is in the
  * cache): row r of q ([q_heads][head_dim] bf16, rows q_stride elements apart)
  * attends to sequence seqs[r] (seqs NULL: sequence r) of `layer`, len =
@@ -509,6 +596,27 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
                                uint32_t q_heads, uint32_t n, const uint32_t *seqs, const uint32_t *starts,
                                uint32_t rows, uint32_t window, uint32_t sinks, float scale, uint16_t *ctx,
                                uint64_t ctx_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same attention where groups of sequences share their first tokens (one
+ * prompt's samples after qwen_b200_op_pages_fork, requests behind one system
+ * prompt), which are read once for a group instead of once for a sequence: rows
+ * starts[g] .. starts[g + 1] - 1 of q (one token each, of sequences seqs[r] as in
+ * qwen_b200_op_paged_decode) are group g, whose sequences hold the same keys and
+ * values in their first prefix[g] tokens, in shared pages or in copies. Those
+ * are read from the pages of the group's first row; a prefix longer than that
+ * sequence is cut to it, so a group whose first row is no sequence shares
+ * nothing. Tokens from prefix[g] on are each sequence's own. A sequence may be
+ * shorter than the prefix. There is no window: under one, a shared prefix soon
+ * lies behind it, and qwen_b200_op_paged_decode reads no more than the window.
+ * n groups (1 .. 65536, empty ones allowed), rows <= 65536. starts is [n + 1]
+ * on the device, not decreasing; rows in front of starts[0] and at or behind
+ * starts[n] are left as they were, rows with no key are zero. Workspace from
+ * qwen_b200_paged_decode_shared_workspace. */
+size_t qwen_b200_paged_decode_shared_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
+int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
+                                     uint32_t q_heads, uint32_t n, const uint32_t *starts, const uint32_t *prefix,
+                                     uint32_t rows, const uint32_t *seqs, float scale, uint16_t *ctx,
+                                     uint64_t ctx_stride, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Page management, all on the device (index lists and counts included), so
  * that it can be captured with the steps around it. Each call writes
