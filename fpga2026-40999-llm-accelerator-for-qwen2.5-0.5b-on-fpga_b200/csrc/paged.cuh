@@ -97,11 +97,37 @@ struct PagedAttnArgs {
     const uint16_t *q;
     uint64_t q_stride, ctx_stride;
     uint16_t *ctx;
-    const uint32_t *seqs, *starts;  // starts: prefill only
-    uint32_t qh, rows, n;           // rows of q; n sequences (prefill)
+    const uint32_t *seqs, *starts;  // starts: prefill and shared decode
+    uint32_t qh, rows, n;           // rows of q; n sequences (prefill) or groups (shared decode)
     uint32_t window, sinks;
     float scale;
     uint32_t format, dim;
+    const uint32_t *prefix = nullptr;  // shared decode: tokens that a group's sequences share
+};
+// A group of sequences that share their first tokens: its rows of q, and how many tokens of its first row's sequence
+// the tile kernel takes for all of them (0: none, each row takes its whole context).
+struct SharedGroup {
+    uint32_t row0, rows, seq;
+    int keys;
+};
+constexpr uint32_t SHARED_ROWS = 2;  // rows and keys that are worth the tile kernel's piece
+constexpr int SHARED_KEYS = 128;
+__device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
+    SharedGroup s;
+    s.row0 = min(a.starts[g], a.rows);
+    s.rows = min(max(a.starts[g + 1], s.row0), a.rows) - s.row0;
+    s.seq = s.rows == 0 ? QWEN_B200_NO_SEQ : a.seqs ? a.seqs[s.row0] : s.row0;
+    s.keys = s.rows < SHARED_ROWS ? 0 : min((int)min(a.prefix[g], 0x7fffffffu), paged_length(a.c, s.seq));
+    if (s.keys < SHARED_KEYS) s.keys = 0;
+    return s;
+}
+// What the tile kernel leaves for the row kernel. Units (tile, KV head, block of 128 keys) are numbered group by group,
+// KV head by KV head, and split evenly over `ctas`; a tile's list of blocks is in pieces of the CTAs that have some of it
+// (two a CTA at most: [m tile][l tile][o tile x dim]), or whole, then by (row, head): [rows][qh] (m, l), [rows][qh][dim] o.
+struct SharedParts {
+    unsigned long long *base;  // [n + 1] units of one KV head in the groups before
+    float *pieces, *ml, *o;
+    uint32_t tile, ctas;
 };
 size_t paged_decode_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t rows);
 int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st);
@@ -112,19 +138,12 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 int launch_paged_append(const qwen_b200_paged_kv &kv, uint32_t layer, const uint16_t *k, const uint16_t *v,
                         uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
                         cudaStream_t st);
-// Attention of one token a row, rows starts[g] .. of group g sharing their first prefix[g] tokens.
-struct PagedSharedArgs {
-    PagedView c;
-    const uint16_t *q;
-    uint64_t q_stride, ctx_stride;
-    uint16_t *ctx;
-    const uint32_t *seqs, *starts, *prefix;
-    uint32_t qh, rows, n;
-    float scale;
-    uint32_t format, dim;
-};
-size_t paged_shared_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);
-int launch_paged_shared(const PagedSharedArgs &a, void *ws, cudaStream_t st);
+size_t paged_shared_ws(uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);
+int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st);
+// Its two halves: the shared tokens by tiles of query rows, then each row's own tokens joined with those.
+size_t paged_shared_pieces_bytes(uint32_t dim);
+int launch_shared_tiles(const PagedAttnArgs &a, SharedParts &parts, unsigned *err, cudaStream_t st);
+int launch_shared_rows(const PagedAttnArgs &a, const SharedParts &parts, bool tiles, cudaStream_t st);
 
 struct RotaryView {
     const float *table;

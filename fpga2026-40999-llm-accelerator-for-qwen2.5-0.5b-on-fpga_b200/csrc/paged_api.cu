@@ -219,7 +219,7 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
 
 size_t qwen_b200_paged_decode_shared_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows) {
     if (paged_check(kv) || !q_heads || q_heads % kv->kv_heads || q_heads > 65536 || rows > 65536 || n > 65536) return 0;
-    return paged_shared_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows);
+    return paged_shared_ws(q_heads, kv->head_dim, n, rows);
 }
 
 int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
@@ -230,22 +230,12 @@ int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t laye
     if (!starts || !prefix || !n || n > 65536 || rows > 65536 || !words_aligned({seqs, starts, prefix}))
         return QWEN_B200_EINVAL;
     if (int rc = paged_check_device(*kv, {q, seqs, starts, prefix, ctx, workspace})) return rc;
-    if (workspace_bytes < paged_shared_ws(kv->kv_heads, q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
-    PagedSharedArgs a;
-    a.c = paged_view(*kv, layer);
-    a.q = q;
-    a.q_stride = q_stride;
-    a.ctx_stride = ctx_stride;
-    a.ctx = ctx;
-    a.seqs = seqs;
-    a.starts = starts;
-    a.prefix = prefix;
-    a.qh = q_heads;
+    if (workspace_bytes < paged_shared_ws(q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
+    PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, 0, 0, scale, ctx, ctx_stride);
     a.rows = rows;
     a.n = n;
-    a.scale = scale;
-    a.format = kv->format;
-    a.dim = kv->head_dim;
+    a.starts = starts;
+    a.prefix = prefix;
     return launch_paged_shared(a, workspace, (cudaStream_t)stream);
 }
 

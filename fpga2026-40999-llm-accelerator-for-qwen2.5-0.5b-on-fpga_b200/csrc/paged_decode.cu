@@ -58,7 +58,7 @@ struct PdCfg {
     static constexpr int STAGES = 3;
     static constexpr int MINB = RB == 256 ? 1 : 2;  // CTAs per SM
     static constexpr int RING = PD_WARPS * STAGES * STEP_BYTES;
-    static constexpr int OUT = PD_WARPS * PD_HEADS * (DIM + 1) * 4;  // the warps' contexts, over the drained ring
+    static constexpr int OUT = PD_WARPS * PD_HEADS * (DIM + 1) * 4 + PD_HEADS * DIM * 4;  // the warps' contexts and a shared prefix's, over the drained ring
     static constexpr int SMEM = RING > OUT ? RING : OUT;
     static constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;  // floats of a partial result: m, l, o
 };
@@ -70,6 +70,8 @@ struct PdWork {
     uint32_t max_ctas;
     uint32_t *prefix;     // [rows + 1] units of one item in the rows before
     float *pieces;        // [CTA][2][PIECE]
+    SharedParts sh;       // shared prefixes: the tile kernel's results,
+    bool tiles;           // and whether it ran
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
@@ -162,10 +164,11 @@ struct PdRow {
     uint32_t steps;
 };
 template <int LOG>
-__device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
+__device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row, int from = 0) {
     PdRow r;
     r.len = paged_length(a.c, a.seqs ? a.seqs[row] : row);
-    const KeySpan k = key_span(r.len - 1, a.window, a.sinks);
+    // (keys in front of `from` are not this kernel's; there is no window then)
+    const KeySpan k = from > 0 ? KeySpan{0, min(from, r.len)} : key_span(r.len - 1, a.window, a.sinks);
     r.first = k.first;
     r.low = k.low;
     constexpr int up = (1 << LOG) - 1;
@@ -175,10 +178,53 @@ __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     return r;
 }
 
+// The group that a row belongs to, found by a whole warp in rounds of 32; false for none.
+__device__ __forceinline__ bool pd_group(const PagedAttnArgs &a, uint32_t row, uint32_t &g) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, n = a.n + 1;  // the first start above `row` is in starts[lo, lo + n), or there is none up to its end
+    while (n > 0) {
+        const uint32_t step = (n + 31) / 32, i = lo + min(lane * step + step - 1, n - 1);
+        const uint32_t above = __ballot_sync(0xffffffffu, a.starts[i] > row);
+        if (!above) {
+            lo += n;
+            break;
+        }
+        const uint32_t l = __ffs(above) - 1, at = min(l * step + step - 1, n - 1);
+        if (step == 1) {
+            lo += at;
+            break;
+        }
+        lo += l * step;
+        n = at - l * step + 1;
+    }
+    g = lo - 1;
+    return lo > 0 && lo <= a.n && a.starts[g] <= row;
+}
+
+// One query head's share of the tile kernel's results: n of them, the i-th at m[i], l[i], o[i].
+struct PdPieces {
+    uint32_t n, c0, slot0, t;
+    uint64_t whole;  // (row, head), n == 1
+};
+__device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t g, const SharedGroup &s,
+                                              uint32_t row, uint32_t kvh, uint32_t h) {
+    const uint32_t blocks = (uint32_t)(s.keys + 127) >> 7, m = (row - s.row0) * w.group + h, tiles = (s.rows * w.group + w.sh.tile - 1) / w.sh.tile;
+    const UnitSplit split(w.sh.base[a.n] * a.c.hkv, w.sh.ctas, 1);
+    const unsigned long long u0 = w.sh.base[g] * a.c.hkv + (unsigned long long)kvh * tiles * blocks + (unsigned long long)(m / w.sh.tile) * blocks;
+    PdPieces p;
+    p.c0 = split.cta_of(u0);
+    p.n = split.cta_of(u0 + blocks - 1) - p.c0 + 1;
+    p.slot0 = split.start(p.c0) < u0;
+    p.t = m % w.sh.tile;
+    p.whole = (uint64_t)row * a.qh + kvh * w.group + h;
+    return p;
+}
+
 // DIRECT: CTA (or cluster of `parts` CTAs) b has row b / items, item b % items;
 // its CTAs take equal parts of the context and join them over distributed
 // shared memory. Otherwise CTA c takes the c-th run of all units.
-template <bool KV8, int DIM, bool DIRECT>
+// SHARED (and DIRECT): the row's own keys, those behind its group's shared ones, joined with what the tile kernel left.
+template <bool KV8, int DIM, bool DIRECT, bool SHARED>
 __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decode_kernel(PagedAttnArgs a, PdWork w) {
     using C = PdCfg<KV8, DIM>;
     constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
@@ -199,17 +245,28 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     };
     uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
     UnitSplit split;
+    uint32_t grp = 0;
+    SharedGroup sg = {};
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
         if (w.parts > 1) pd_cluster_arrive();
         row = unit / w.items;
         load_q(row, unit % w.items);  // needs no length
-        const PdRow R = pd_row<C::LOG>(a, row);
+        if constexpr (SHARED) {
+            if (!pd_group(a, row, grp)) {  // (the whole cluster) the row stays
+                pdl_wait();
+                if (w.parts > 1) pd_cluster_wait();
+                return;
+            }
+            if (w.tiles) sg = shared_group(a, grp);
+        }
+        const PdRow R = pd_row<C::LOG>(a, row, sg.keys);
         base = 0;
         const uint32_t first = unit % w.items * R.steps;
         u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
         u_end = first + (uint32_t)((uint64_t)R.steps * (part + 1) / w.parts);
-        if (R.steps == 0) {  // no key (the whole cluster): zero
+        if (R.steps == 0 && (!SHARED || sg.keys == 0)) {  // no key (the whole cluster): zero
+            if constexpr (SHARED) pdl_wait();
             const uint32_t item = unit % w.items, kvh = item / w.hb, h0 = item % w.hb * PD_HEADS;
             const uint32_t heads = min(w.group - h0, (uint32_t)PD_HEADS);
             uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + h0) * DIM;
@@ -273,12 +330,12 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     const float fac0 = a.scale * 1.44269504f;
     bool first_segment = true;
     while (DIRECT || u < u_end) {  // DIRECT: once, also for a CTA of a cluster that has no step
-        const PdRow R = pd_row<C::LOG>(a, row);
+        const PdRow R = pd_row<C::LOG>(a, row, sg.keys);
         if (!DIRECT && R.steps == 0) {
             ++row;
             continue;
         }
-        const uint32_t item = (u - base) / R.steps, rem = u - base - item * R.steps;
+        const uint32_t item = SHARED ? blockIdx.x / w.parts % w.items : (u - base) / R.steps, rem = u - base - item * R.steps;
         const int cnt = (int)min(R.steps - rem, u_end - u);
         const uint32_t kvh = item / w.hb, hblk = item % w.hb;
         if constexpr (!DIRECT) load_q(row, item);
@@ -604,6 +661,71 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
         }
         __syncthreads();
         const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
+        // ---- the shared keys' results: a cluster's CTAs take them in turn
+        constexpr int MOST = SHARED ? PD_MAX_SMS : 1;
+        __shared__ PdPieces pp[PD_HEADS];
+        __shared__ float pf[PD_HEADS][MOST], ptop[PD_HEADS], psum[PD_HEADS];
+        if constexpr (SHARED) {
+            pdl_wait();
+            if (sg.keys > 0) {
+                const uint32_t part0 = blockIdx.x % w.parts;
+                auto at = [&](int h, uint32_t i) {
+                    const PdPieces &p = pp[h];
+                    return w.sh.pieces + ((uint64_t)(p.c0 + i) * 2 + (i == 0 ? p.slot0 : 0)) * ((uint64_t)w.sh.tile * (DIM + 2));
+                };
+                if (tid < PD_HEADS) {
+                    PdPieces p = {};
+                    if (hblk * PD_HEADS + tid < w.group) p = pd_pieces(a, w, grp, sg, row, kvh, hblk * PD_HEADS + tid);
+                    pp[tid] = p;
+                }
+                __syncthreads();
+                {  // warp h: head h
+                    const PdPieces p = pp[warp];
+                    float M = wM[warp], L = 0.f;
+                    for (uint32_t i = part0 + lane * w.parts; i < p.n; i += 32 * w.parts) {
+                        const float m1 = p.n == 1 ? w.sh.ml[2 * p.whole] : at(warp, i)[p.t];
+                        pf[warp][i] = m1;
+                        M = fmaxf(M, m1);
+                    }
+                    M = warp_max(M);
+                    const float M0 = M == -INFINITY ? 0.f : M;
+                    for (uint32_t i = part0 + lane * w.parts; i < p.n; i += 32 * w.parts) {
+                        const float f = ex2(0.5f * (pf[warp][i] - M0)), l1 = p.n == 1 ? w.sh.ml[2 * p.whole + 1] : at(warp, i)[w.sh.tile + p.t];
+                        pf[warp][i] = f;
+                        L += l1 * f * f;
+                    }
+                    L = warp_sum(L);
+                    if (lane < PD_WARPS) {  // the warps' factors anew
+                        const float f = ex2(0.5f * (wm[lane][warp] - M0));
+                        wf[lane][warp] = f;
+                    }
+                    if (lane == 0) {
+                        ptop[warp] = M;
+                        psum[warp] = L;
+                    }
+                }
+                __syncthreads();
+                // their contexts summed over the first warp's slot of a ninth row of `os`
+                float *po = os + PD_WARPS * PD_HEADS * (DIM + 1);
+                for (int x = tid; x < PD_HEADS * DIM / 4; x += PD_THREADS) {
+                    const int h = x / (DIM / 4), d = x % (DIM / 4) * 4;
+                    const PdPieces p = pp[h];
+                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (uint32_t i = part0; i < p.n; i += w.parts) {
+                        const float4 v = *reinterpret_cast<const float4 *>(
+                            p.n == 1 ? w.sh.o + p.whole * DIM + d : at(h, i) + 2 * w.sh.tile + (uint64_t)p.t * DIM + d);
+                        const float f = pf[h][i];
+                        O.x += v.x * f * f;
+                        O.y += v.y * f * f;
+                        O.z += v.z * f * f;
+                        O.w += v.w * f * f;
+                    }
+                    *reinterpret_cast<float4 *>(po + h * DIM + d) = O;
+                }
+                __syncthreads();
+            }
+        }
         float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
         const uint32_t part = DIRECT ? blockIdx.x % w.parts : 0;
         if constexpr (DIRECT)
@@ -617,6 +739,13 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 L += wl[i][h] * f * f;
                 O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f * f;
             }
+            float M = wM[h];
+            if constexpr (SHARED)
+                if (sg.keys > 0) {
+                    M = ptop[h];
+                    L += psum[h];
+                    O += os[PD_WARPS * PD_HEADS * (DIM + 1) + x];
+                }
             const uint32_t hl = hblk * PD_HEADS + h;
             if (whole) {
                 if (hl < w.group)
@@ -627,13 +756,13 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 const uint32_t to = (uint32_t)__cvta_generic_to_shared(fin + slot);
                 pd_dsmem_store(to + 4 * (2 + d), h % w.parts, O);
                 if (d == 0) {
-                    pd_dsmem_store(to, h % w.parts, wM[h]);
+                    pd_dsmem_store(to, h % w.parts, M);
                     pd_dsmem_store(to + 4, h % w.parts, L);
                 }
             } else {
                 piece[2 * PD_HEADS + x] = O;
                 if (d == 0) {
-                    piece[h] = wM[h];
+                    piece[h] = M;
                     piece[PD_HEADS + h] = L;
                 }
             }
@@ -737,7 +866,7 @@ size_t paged_decode_ws(uint32_t, uint32_t, uint32_t dim, uint32_t rows) {
 }
 
 // Whether the current device holds `units` clusters of `parts` CTAs (9 to 16) at once; asked once per device and size.
-template <bool KV8, int DIM>
+template <bool KV8, int DIM, bool SHARED>
 static bool pd_fits(uint32_t parts, uint32_t units) {
     using C = PdCfg<KV8, DIM>;
     static int known[64][PD_MAX_PARTS + 1];  // 1 + the answer, written with the same value by every thread that finds 0
@@ -745,7 +874,7 @@ static bool pd_fits(uint32_t parts, uint32_t units) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
     int n = __atomic_load_n(&known[dev][parts], __ATOMIC_RELAXED);
     if (!n) {
-        auto *kernel = paged_decode_kernel<KV8, DIM, true>;
+        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED>;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(parts);
         cfg.blockDim = dim3(PD_THREADS);
@@ -769,7 +898,7 @@ static bool pd_fits(uint32_t parts, uint32_t units) {
     return n - 1 >= (int)units;
 }
 
-template <bool KV8, int DIM>
+template <bool KV8, int DIM, bool SHARED = false>
 static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM>;
     // Which way: a CTA or cluster per (row, item) where those fill a third of the GPU, or where no context can be
@@ -786,16 +915,16 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
     const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;
     uint64_t parts = want < room ? want : room;
     parts = parts < 1 ? 1 : parts < PD_MAX_PARTS ? parts : PD_MAX_PARTS;
-    while (parts > 8 && !pd_fits<KV8, DIM>((uint32_t)parts, units)) --parts;
+    while (parts > 8 && !pd_fits<KV8, DIM, SHARED>((uint32_t)parts, units)) --parts;
     w.parts = (uint32_t)parts;
-    if (units * parts * 3 >= slots || most <= parts * PD_PART_MOST) {
-        auto *kernel = paged_decode_kernel<KV8, DIM, true>;
+    if (SHARED || units * parts * 3 >= slots || most <= parts * PD_PART_MOST) {
+        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED>;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
         if (parts > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return -3;
         return launch_pdl(kernel, dim3(units * w.parts), dim3(PD_THREADS), C::SMEM, st, w.parts, a, w);
     }
-    auto *kernel = paged_decode_kernel<KV8, DIM, false>;
+    auto *kernel = paged_decode_kernel<KV8, DIM, false, false>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
     w.max_ctas = slots;
     PdlChain chain;
@@ -819,6 +948,24 @@ int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     if (a.format == QWEN_B200_KV8)
         return a.dim == 64 ? launch_decode<true, 64>(a, w, n, st) : launch_decode<true, 128>(a, w, n, st);
     return a.dim == 64 ? launch_decode<false, 64>(a, w, n, st) : launch_decode<false, 128>(a, w, n, st);
+}
+
+// `tiles`: whether the tile kernel was launched in front (in the same PdlChain).
+int launch_shared_rows(const PagedAttnArgs &a, const SharedParts &parts, bool tiles, cudaStream_t st) {
+    const int sms = paged_sms();
+    if (sms <= 0) return -3;
+    PdWork w = {};
+    w.group = a.qh / a.c.hkv;
+    w.hb = (w.group + PD_HEADS - 1) / PD_HEADS;
+    w.items = a.c.hkv * w.hb;
+    w.sh = parts;
+    w.tiles = tiles;
+    if ((uint64_t)a.rows * w.items * PD_HEADS >= 1ull << 31) return -1;
+    if ((uint64_t)a.rows * w.items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 3) >= 1ull << 32) return -1;
+    const int n = sms < PD_MAX_SMS ? sms : PD_MAX_SMS;
+    if (a.format == QWEN_B200_KV8)
+        return a.dim == 64 ? launch_decode<true, 64, true>(a, w, n, st) : launch_decode<true, 128, true>(a, w, n, st);
+    return a.dim == 64 ? launch_decode<false, 64, true>(a, w, n, st) : launch_decode<false, 128, true>(a, w, n, st);
 }
 
 }  // namespace qb

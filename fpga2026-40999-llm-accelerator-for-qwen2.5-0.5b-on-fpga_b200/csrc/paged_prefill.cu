@@ -122,6 +122,7 @@ struct PpWork {
     unsigned *err;
     PpRec *recs;     // [max_ctas]
     float *pieces;   // [max_ctas][2][PIECE]
+    SharedParts sh;  // shared prefixes: what is left for the row kernel
 };
 
 struct PpMaps {  // bf16 pools
@@ -132,8 +133,19 @@ struct PpSeqInfo {
     uint32_t row0, seq, rows, mrows;
     int pos0, nt;
 };
+template <bool SHARED>
 __device__ __forceinline__ PpSeqInfo pp_seq(const PagedAttnArgs &a, const PpWork &w, uint32_t i) {
     PpSeqInfo s;
+    if constexpr (SHARED) {  // every row is at the shared keys' end
+        const SharedGroup g = shared_group(a, i);
+        s.row0 = g.row0;
+        s.seq = g.seq;
+        s.rows = g.rows;
+        s.mrows = g.rows * w.group;
+        s.pos0 = g.keys - 1;
+        s.nt = g.keys > 0 ? (int)((s.mrows + w.tile - 1) / w.tile) : 0;
+        return s;
+    }
     const uint32_t s0 = min(a.starts[i], a.rows), s1 = min(max(a.starts[i + 1], s0), a.rows);
     s.row0 = s0;
     s.seq = a.seqs ? a.seqs[i] : i;
@@ -155,7 +167,9 @@ __device__ __forceinline__ uint32_t pp_dead_alone(const PagedAttnArgs &a) { retu
 struct PpBlocks {
     int s128, low128, first, low, last, n;
 };
+template <bool SHARED>
 __device__ __forceinline__ PpBlocks pp_blocks(const PagedAttnArgs &a, const PpWork &w, int pos0, uint32_t mrows, int k) {
+    if constexpr (SHARED) return {0, 0, 0, 0, pos0, (pos0 + PP_BLK) / PP_BLK};
     PpBlocks b;
     const uint32_t m0 = (uint32_t)k * w.tile, m1 = min(m0 + w.tile, mrows) - 1;
     const int pmin = max(pos0 + (int)(m0 / w.group), 0);
@@ -168,27 +182,32 @@ __device__ __forceinline__ PpBlocks pp_blocks(const PagedAttnArgs &a, const PpWo
     return b;
 }
 // Blocks of a sequence's tiles, summed by a whole warp.
+template <bool SHARED>
 __device__ __forceinline__ uint32_t pp_units_warp(const PagedAttnArgs &a, const PpWork &w, int pos0, uint32_t mrows,
                                                   int nt) {
+    if constexpr (SHARED) return (uint32_t)nt * pp_blocks<true>(a, w, pos0, mrows, 0).n;
     uint32_t u = 0;
-    for (int k = threadIdx.x & 31; k < nt; k += 32) u += pp_blocks(a, w, pos0, mrows, k).n;
+    for (int k = threadIdx.x & 31; k < nt; k += 32) u += pp_blocks<false>(a, w, pos0, mrows, k).n;
     return __reduce_add_sync(0xffffffffu, u);
 }
 // Blocks of the sequences base + lane < end, one per lane; `dead` is set where the rows of one are zeroed by all CTAs.
+template <bool SHARED>
 __device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const PpWork &w, uint32_t base, uint32_t end,
                                                   bool &dead) {
     const uint32_t i = base + (threadIdx.x & 31);
     PpSeqInfo s = {};
     uint32_t u = 0;
     if (i < end) {
-        s = pp_seq(a, w, i);
+        s = pp_seq<SHARED>(a, w, i);
+        if constexpr (SHARED) return (uint32_t)s.nt * pp_blocks<true>(a, w, s.pos0, s.mrows, 0).n;
         if (pp_dead(s) > pp_dead_alone(a)) dead = true;
         if (s.nt <= 4)
-            for (int k = 0; k < s.nt; ++k) u += pp_blocks(a, w, s.pos0, s.mrows, k).n;
+            for (int k = 0; k < s.nt; ++k) u += pp_blocks<false>(a, w, s.pos0, s.mrows, k).n;
     }
+    if constexpr (SHARED) return 0;
     for (uint32_t todo = __ballot_sync(0xffffffffu, s.nt > 4); todo; todo &= todo - 1) {
         const int l = __ffs(todo) - 1;
-        const uint32_t x = pp_units_warp(a, w, __shfl_sync(0xffffffffu, s.pos0, l), __shfl_sync(0xffffffffu, s.mrows, l),
+        const uint32_t x = pp_units_warp<false>(a, w, __shfl_sync(0xffffffffu, s.pos0, l), __shfl_sync(0xffffffffu, s.mrows, l),
                                          __shfl_sync(0xffffffffu, s.nt, l));
         if ((int)(threadIdx.x & 31) == l) u = x;
     }
@@ -325,7 +344,9 @@ struct PpReader {
     }
 };
 
-template <bool KV8, int DIM>
+// SHARED: the "sequences" are groups whose rows all see the group's shared keys (as far as their own length goes), and
+// every tile's result is left for the row kernel.
+template <bool KV8, int DIM, bool SHARED>
 __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ PpMaps maps, PagedAttnArgs a, PpWork w) {
     using C = PpCfg<KV8, DIM>;
     extern __shared__ uint8_t smem_raw[];
@@ -379,7 +400,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     const uint32_t per = (a.n + C::WARPS - 1) / C::WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
     unsigned long long mine = 0;
     bool dead = false;
-    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane(a, w, b, i1, dead));
+    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane<SHARED>(a, w, b, i1, dead));
     dead = __any_sync(0xffffffffu, dead);
     if (lane == 0) {
         wsum[warp] = mine;
@@ -397,10 +418,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     const UnitSplit split(all * a.c.hkv, w.max_ctas, PP_MIN_UNITS);
     const bool active = blockIdx.x < split.g && all > 0;
     const unsigned long long u0 = split.start(blockIdx.x), u1 = split.start(blockIdx.x + 1);
-    if (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv) {
+    const bool books = SHARED && blockIdx.x == 0;  // this CTA writes down every group's first unit
+    if (books && tid == 0) w.sh.base[a.n] = all;
+    if (books || (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv)) {
         unsigned long long p = before;
         for (uint32_t b = i0; b < i1; b += 32) {
-            uint32_t u = pp_units_lane(a, w, b, i1, dead), x = u;
+            uint32_t u = pp_units_lane<SHARED>(a, w, b, i1, dead), x = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -411,7 +434,8 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 at_seq = b + lane;
                 at_prefix = p + x - u;
             }
-            if (__any_sync(0xffffffffu, here)) break;
+            if (books && b + lane < i1) w.sh.base[b + lane] = p + x - u;
+            if (!books && __any_sync(0xffffffffu, here)) break;
             p += __shfl_sync(0xffffffffu, x, 31);
         }
     }
@@ -420,7 +444,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
 
     if (!active) {
         // ---------------- nothing to compute
-        if (tid == 0) w.recs[blockIdx.x].valid = 0;
+        if (!SHARED && tid == 0) w.recs[blockIdx.x].valid = 0;
     } else if (warp < C::SW) {
         // ---------------- softmax: thread = row r of MMA tile `x`
         if constexpr (DIM == 64)
@@ -446,14 +470,21 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 continue;
             }
             const uint32_t m_row = mt + r, row_i = m_row / w.group;
-            const int pos = m_row < g.mrows ? g.pos0 + (int)row_i : -1;
-            const KeySpan ks = key_span(max(pos, 0), a.window, a.sinks);
+            int pos = m_row < g.mrows ? g.pos0 + (int)row_i : -1;
+            if constexpr (SHARED) {  // the shared keys, or as many as the row has; what is no row is not written
+                pos = g.pos0;
+                if (m_row < g.mrows) {
+                    const uint32_t row = g.row0 + row_i;
+                    pos = min(pos, paged_length(a.c, a.seqs ? a.seqs[row] : row) - 1);
+                }
+            }
+            const KeySpan ks = SHARED ? KeySpan{0, 0} : key_span(max(pos, 0), a.window, a.sinks);
             const int first = pos < 0 ? 0 : ks.first, low = ks.low;
             // keys seen by every row of the MMA tile: [0, all_first) and [all_low, all_last]
             const uint32_t m_end = min(mt + 128, g.mrows) - 1;
-            const int all_last = m_end == mt + 127 ? g.pos0 + (int)(mt / w.group) : -1;
-            const int all_first = key_span(max(all_last, 0), a.window, a.sinks).first;
-            const int all_low = key_span(max(g.pos0 + (int)(m_end / w.group), 0), a.window, a.sinks).low;
+            const int all_last = SHARED ? __reduce_min_sync(0xffffffffu, pos) : m_end == mt + 127 ? g.pos0 + (int)(mt / w.group) : -1;
+            const int all_first = SHARED ? 0 : key_span(max(all_last, 0), a.window, a.sinks).first;
+            const int all_low = SHARED ? 0 : key_span(max(g.pos0 + (int)(m_end / w.group), 0), a.window, a.sinks).low;
             // The reference starts at 0 and stands if the weights of the row's first keys sum to something in
             // [2^-20, 2^15] (scores within some 15 of 0, the usual case); else it becomes their maximum.
             float m = 0.f, l = 0.f;
@@ -697,7 +728,21 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             ++round;
             tc::tc_fence_after();
             const bool live = m_row < g.mrows && pos >= 0;
-            if (g.piece < 0) {
+            if (SHARED && g.piece < 0) {
+                const uint64_t at = (g.row0 + (uint64_t)row_i) * a.qh + g.kvh * w.group + m_row % w.group;
+                if (m_row < g.mrows) *reinterpret_cast<float2 *>(w.sh.ml + 2 * at) = make_float2(l == 0.f ? -INFINITY : m, l);
+#pragma unroll 1
+                for (int j = 0; j < DIM; j += 16) {
+                    uint32_t o[16];
+                    pp_ld16(o_addr + j, o);
+                    pp_ld_wait();
+                    if (m_row < g.mrows) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4)
+                            *reinterpret_cast<uint4 *>(w.sh.o + at * DIM + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    }
+                }
+            } else if (g.piece < 0) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 uint16_t *out = a.ctx + (g.row0 + (uint64_t)row_i) * a.ctx_stride +
                                 (uint64_t)(g.kvh * w.group + m_row % w.group) * DIM;
@@ -1014,13 +1059,13 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             uint32_t i = at_seq;
             unsigned long long u = u0, base = at_prefix * a.c.hkv;  // units before sequence i
             bool first_segment = true;
-            if (lane == 0) w.recs[blockIdx.x].valid = 0;
+            if (!SHARED && lane == 0) w.recs[blockIdx.x].valid = 0;
             while (ok) {
                 const uint32_t d = n % PP_SEG;
                 PpSeg g = {};
                 if (u < u1) {
-                    const PpSeqInfo s = pp_seq(a, w, i);
-                    const uint32_t units = pp_units_warp(a, w, s.pos0, s.mrows, s.nt);
+                    const PpSeqInfo s = pp_seq<SHARED>(a, w, i);
+                    const uint32_t units = pp_units_warp<SHARED>(a, w, s.pos0, s.mrows, s.nt);
                     if (units == 0 || u >= base + (unsigned long long)units * a.c.hkv) {
                         base += (unsigned long long)units * a.c.hkv;
                         ++i;
@@ -1034,7 +1079,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     int k = 0, b0 = 0;
                     PpBlocks bl = {};
                     for (int kb = 0;; kb += 32) {
-                        const PpBlocks mine_b = pp_blocks(a, w, s.pos0, s.mrows, min(kb + lane, s.nt - 1));
+                        const PpBlocks mine_b = pp_blocks<SHARED>(a, w, s.pos0, s.mrows, min(kb + lane, s.nt - 1));
                         const uint32_t cnt = kb + lane < s.nt ? mine_b.n : 0;
                         uint32_t xs = cnt;
 #pragma unroll
@@ -1054,7 +1099,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     // this tile and those behind it in the KV head: one segment each
                     bool more = true;
                     while (more && ok) {
-                        bl = pp_blocks(a, w, s.pos0, s.mrows, k);
+                        bl = pp_blocks<SHARED>(a, w, s.pos0, s.mrows, k);
                         const int cnt = (int)min((unsigned long long)(bl.n - b0), u1 - u);
                         if (cnt > 0) {
                             g.seq = s.seq;
@@ -1081,7 +1126,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             }
                             __syncwarp();
                             ++n;
-                            if (first_segment && b0 > 0 && lane == 0) {
+                            if (!SHARED && first_segment && b0 > 0 && lane == 0) {
                                 PpRec rec = {};
                                 const unsigned long long t0 = u - b0;
                                 rec.valid = 1;
@@ -1113,7 +1158,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             }
         }
     }
-    if (warp == C::SW + 6) {  // (behind its segments)
+    if (!SHARED && warp == C::SW + 6) {  // (behind its segments)
         // ---------------- rows in front of the first token, and of no sequence
         const uint32_t chunks = a.qh * (DIM / 8);
         auto zero = [&](uint32_t row0, uint32_t n, uint32_t r0, uint32_t step) {
@@ -1122,13 +1167,13 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     *reinterpret_cast<uint4 *>(a.ctx + (row0 + (uint64_t)r) * a.ctx_stride + 8 * c) = make_uint4(0, 0, 0, 0);
         };
         for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-            const PpSeqInfo s = pp_seq(a, w, i);
+            const PpSeqInfo s = pp_seq<false>(a, w, i);
             if (pp_dead(s) <= pp_dead_alone(a)) zero(s.row0, pp_dead(s), 0, 1);
         }
         // the runs of sequences in which the numbering met more rows (padded prompts)
         for (uint32_t runs = __ballot_sync(0xffffffffu, lane < C::WARPS && wdead[lane]); runs; runs &= runs - 1) {
             for (uint32_t b = min((__ffs(runs) - 1) * per, a.n), e = min(b + per, a.n); b < e; b += 32) {
-                const PpSeqInfo s = pp_seq(a, w, min(b + lane, e - 1));
+                const PpSeqInfo s = pp_seq<false>(a, w, min(b + lane, e - 1));
                 const uint32_t n = b + lane < e ? pp_dead(s) : 0;
                 for (uint32_t todo = __ballot_sync(0xffffffffu, n > pp_dead_alone(a)); todo; todo &= todo - 1) {
                     const int l = __ffs(todo) - 1;
@@ -1268,10 +1313,10 @@ bool paged_prefill_fits(const PagedAttnArgs &a) {
     return tiles * blocks < 1ull << 32;
 }
 
-template <bool KV8, int DIM>
+template <bool KV8, int DIM, bool SHARED = false>
 static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t st) {
     using C = PpCfg<KV8, DIM>;
-    auto *kernel = paged_prefill_kernel<KV8, DIM>;
+    auto *kernel = paged_prefill_kernel<KV8, DIM, SHARED>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::ALLOC) != cudaSuccess) return -3;
     PpMaps maps = {};
     if (!KV8) {
@@ -1282,6 +1327,7 @@ static int launch_prefill(const PagedAttnArgs &a, const PpWork &w, cudaStream_t 
     }
     PdlChain chain;
     if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(C::THREADS), C::ALLOC, st, 1, maps, a, w)) return rc;
+    if constexpr (SHARED) return 0;
     // Few tiles are in many pieces: first way against second, 14 heads on 2 of 64 dims KV8, 128 rows on 4000 keys 35.1
     // and 41.7 us, 8 x 64 rows on 2000 keys 37.2 and 39.2, 16 x 64 47.7 and 47.2, 32 x 64 70.0 and 67.5; 32 heads on 8
     // of 128 dims bf16, 4 x 32 rows on 8000 keys 41.7 and 45.6.
@@ -1309,6 +1355,31 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     if (a.format == QWEN_B200_KV8)
         return a.dim == 64 ? launch_prefill<true, 64>(a, w, st) : launch_prefill<true, 128>(a, w, st);
     return a.dim == 64 ? launch_prefill<false, 64>(a, w, st) : launch_prefill<false, 128>(a, w, st);
+}
+
+size_t paged_shared_pieces_bytes(uint32_t dim) {
+    const size_t tile = dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
+    return (size_t)PP_MAX_SMS * 2 * (2 * tile + tile * dim) * 4;
+}
+
+int launch_shared_tiles(const PagedAttnArgs &a, SharedParts &parts, unsigned *err, cudaStream_t st) {
+    const int sms = paged_sms();
+    if (sms <= 0) return -3;
+    PpWork w;
+    w.group = a.qh / a.c.hkv;
+    w.max_ctas = (uint32_t)(sms < PP_MAX_SMS ? sms : PP_MAX_SMS);
+    w.tile = a.dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
+    w.negate = a.scale < 0.f;
+    w.fac = fabsf(a.scale) * 1.44269504f;
+    w.err = err;
+    w.recs = nullptr;
+    w.pieces = parts.pieces;
+    parts.tile = w.tile;
+    parts.ctas = w.max_ctas;
+    w.sh = parts;
+    if (a.format == QWEN_B200_KV8)
+        return a.dim == 64 ? launch_prefill<true, 64, true>(a, w, st) : launch_prefill<true, 128, true>(a, w, st);
+    return a.dim == 64 ? launch_prefill<false, 64, true>(a, w, st) : launch_prefill<false, 128, true>(a, w, st);
 }
 
 }  // namespace qb

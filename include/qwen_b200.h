@@ -610,8 +610,15 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * lies behind it, and qwen_b200_op_paged_decode reads no more than the window.
  * n groups (1 .. 65536, empty ones allowed), rows <= 65536. starts is [n + 1]
  * on the device, not decreasing; rows in front of starts[0] and at or behind
- * starts[n] are left as they were, rows with no key are zero. Workspace from
- * qwen_b200_paged_decode_shared_workspace. */
+ * starts[n] are left as they were, rows with no key are zero. rows * (q_heads /
+ * kv_heads) and blocks are limited as in qwen_b200_op_paged_prefill, rows and keys as
+ * in qwen_b200_op_paged_decode. Softmax weights of shared tokens are rounded as in the
+ * former, those of a sequence's own as in the latter; NaN and infinities in
+ * values of a prefix that some row sees may reach the rows of its group. The
+ * workspace (qwen_b200_paged_decode_shared_workspace; calls that overlap need one
+ * each) may hold anything, but its first 4 bytes become non-zero if a bounded
+ * device wait expired (ctx is then not valid): a caller that wants to know
+ * zeroes them before. */
 size_t qwen_b200_paged_decode_shared_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);
 int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t layer, const uint16_t *q, uint64_t q_stride,
                                      uint32_t q_heads, uint32_t n, const uint32_t *starts, const uint32_t *prefix,
