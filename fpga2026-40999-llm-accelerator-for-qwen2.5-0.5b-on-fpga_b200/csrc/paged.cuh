@@ -121,14 +121,26 @@ __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint
     if (s.keys < SHARED_KEYS) s.keys = 0;
     return s;
 }
+// The group that a row belongs to; false for none. starts is not decreasing.
+__device__ __forceinline__ bool shared_find(const PagedAttnArgs &a, uint32_t row, uint32_t &g) {
+    uint32_t lo = 0, hi = a.n;  // the last start at or before the row
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (a.starts[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    g = lo;
+    return lo < a.n && a.starts[lo] <= row && row < a.starts[lo + 1];
+}
 // What the tile kernel leaves for the row kernel. Units (tile, KV head, block of 128 keys) are numbered group by group,
 // KV head by KV head, and split evenly over `ctas`; a tile's list of blocks is in pieces of the CTAs that have some of it
 // (two a CTA at most: [m tile][l tile][o tile x dim]), or whole, then by (row, head): [rows][qh] (m, l), [rows][qh][dim] o.
 struct SharedParts {
     unsigned long long *base;  // [n + 1] units of one KV head in the groups before
+    uint4 *rows;               // [rows] shared keys (SHARED_NO_GROUP: the row has none), length, group, row of the group
     float *pieces, *ml, *o;
     uint32_t tile, ctas;
 };
+constexpr uint32_t SHARED_NO_GROUP = 0xffffffffu;
 size_t paged_decode_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t rows);
 int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 size_t paged_prefill_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);

@@ -41,24 +41,27 @@
 
 namespace qb {
 
-constexpr int PD_WARPS = 8, PD_THREADS = 32 * PD_WARPS, PD_SUB = 16, PD_HEADS = 8;
+constexpr int PD_SUB = 16, PD_HEADS = 8;
 constexpr uint32_t PD_MAX_PARTS = 16;  // CTAs of a cluster
 constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
 constexpr uint32_t PD_PART_KEYS = 512;  // keys that a CTA of a cluster has at least to be worth its join
 constexpr uint32_t PD_PART_MOST = 2048; // and at most where the clusters leave most of the GPU idle
 constexpr uint32_t PD_MIN_UNITS = 8;  // steps that a CTA takes at least (1 per warp)
 
-template <bool KV8, int DIM>
+template <bool KV8, int DIM, int NW = 8>  // NW warps
 struct PdCfg {
+    static constexpr int WARPS = NW, THREADS = 32 * NW;
     static constexpr int RB = KV8 ? DIM : 2 * DIM;  // bytes of a row
     static constexpr int CPR = RB / 16;             // 16-byte chunks of a row
     static constexpr int SUBS = RB == 64 ? 2 : 1, STEP = SUBS * PD_SUB;  // 16-key pieces of a step; its keys
     static constexpr int LOG = STEP == 32 ? 5 : 4;
     static constexpr int SUB_BYTES = 2 * PD_SUB * RB + (KV8 ? 2 * PD_SUB * 4 : 0), STEP_BYTES = SUBS * SUB_BYTES;
     static constexpr int STAGES = 3;
-    static constexpr int MINB = RB == 256 ? 1 : 2;  // CTAs per SM
-    static constexpr int RING = PD_WARPS * STAGES * STEP_BYTES;
-    static constexpr int OUT = PD_WARPS * PD_HEADS * (DIM + 1) * 4 + PD_HEADS * DIM * 4;  // the warps' contexts and a shared prefix's, over the drained ring
+    static constexpr int MINB = (RB == 256 ? 8 : 16) / NW;  // CTAs per SM
+    static constexpr int RING = NW * STAGES * STEP_BYTES;
+    // over the drained ring: the warps' contexts, a shared prefix's, and the maxima (then factors) and sums of its pieces
+    static constexpr int OS = NW * PD_HEADS * (DIM + 1), PO = PD_HEADS * DIM, PF = PD_HEADS * PD_MAX_SMS;
+    static constexpr int OUT = (OS + PO + 2 * PF) * 4;
     static constexpr int SMEM = RING > OUT ? RING : OUT;
     static constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;  // floats of a partial result: m, l, o
 };
@@ -164,11 +167,10 @@ struct PdRow {
     uint32_t steps;
 };
 template <int LOG>
-__device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row, int from = 0) {
+__device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     PdRow r;
     r.len = paged_length(a.c, a.seqs ? a.seqs[row] : row);
-    // (keys in front of `from` are not this kernel's; there is no window then)
-    const KeySpan k = from > 0 ? KeySpan{0, min(from, r.len)} : key_span(r.len - 1, a.window, a.sinks);
+    const KeySpan k = key_span(r.len - 1, a.window, a.sinks);
     r.first = k.first;
     r.low = k.low;
     constexpr int up = (1 << LOG) - 1;
@@ -178,45 +180,41 @@ __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row, in
     return r;
 }
 
-// The group that a row belongs to, found by a whole warp in rounds of 32; false for none.
-__device__ __forceinline__ bool pd_group(const PagedAttnArgs &a, uint32_t row, uint32_t &g) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t lo = 0, n = a.n + 1;  // the first start above `row` is in starts[lo, lo + n), or there is none up to its end
-    while (n > 0) {
-        const uint32_t step = (n + 31) / 32, i = lo + min(lane * step + step - 1, n - 1);
-        const uint32_t above = __ballot_sync(0xffffffffu, a.starts[i] > row);
-        if (!above) {
-            lo += n;
-            break;
-        }
-        const uint32_t l = __ffs(above) - 1, at = min(l * step + step - 1, n - 1);
-        if (step == 1) {
-            lo += at;
-            break;
-        }
-        lo += l * step;
-        n = at - l * step + 1;
-    }
-    g = lo - 1;
-    return lo > 0 && lo <= a.n && a.starts[g] <= row;
+// The same for a row's keys behind the shared ones (there is no window).
+template <int LOG>
+__device__ __forceinline__ PdRow pd_own(uint4 rec) {
+    PdRow r;
+    r.len = (int)rec.y;
+    r.first = r.nfirst = 0;
+    r.low = (int)min(rec.x, rec.y);
+    r.nlow = r.low >> LOG;
+    r.steps = r.len > r.low ? (uint32_t)(((r.len + (1 << LOG) - 1) >> LOG) - r.nlow) : 0u;
+    return r;
 }
 
-// One query head's share of the tile kernel's results: n of them, the i-th at m[i], l[i], o[i].
+// One query head's share of the tile kernel's results: n of them. The first's maximum, sum and context are at m0, l0 and
+// o0; those of the CTAs behind the first follow `next`, two pieces apart.
 struct PdPieces {
-    uint32_t n, c0, slot0, t;
-    uint64_t whole;  // (row, head), n == 1
+    const float *m0, *l0, *o0, *next;
+    uint32_t n, t;
 };
-__device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t g, const SharedGroup &s,
-                                              uint32_t row, uint32_t kvh, uint32_t h) {
-    const uint32_t blocks = (uint32_t)(s.keys + 127) >> 7, m = (row - s.row0) * w.group + h, tiles = (s.rows * w.group + w.sh.tile - 1) / w.sh.tile;
-    const UnitSplit split(w.sh.base[a.n] * a.c.hkv, w.sh.ctas, 1);
-    const unsigned long long u0 = w.sh.base[g] * a.c.hkv + (unsigned long long)kvh * tiles * blocks + (unsigned long long)(m / w.sh.tile) * blocks;
+template <int DIM>
+__device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t row, uint4 rec, uint32_t kvh,
+                                              uint32_t h) {
+    const uint32_t blocks = (rec.x + 127) >> 7, m = rec.w * w.group + h, size = w.sh.tile * (DIM + 2);
+    const unsigned long long all = w.sh.base[a.n], b0 = w.sh.base[rec.z], units = w.sh.base[rec.z + 1] - b0;  // of a KV head
+    const UnitSplit split(all * a.c.hkv, w.sh.ctas, 1);
+    const unsigned long long u0 = b0 * a.c.hkv + kvh * units + (unsigned long long)(m / w.sh.tile) * blocks;
+    const uint32_t c0 = split.cta_of(u0);
     PdPieces p;
-    p.c0 = split.cta_of(u0);
-    p.n = split.cta_of(u0 + blocks - 1) - p.c0 + 1;
-    p.slot0 = split.start(p.c0) < u0;
+    p.n = split.cta_of(u0 + blocks - 1) - c0 + 1;
     p.t = m % w.sh.tile;
-    p.whole = (uint64_t)row * a.qh + kvh * w.group + h;
+    const float *first = w.sh.pieces + ((uint64_t)c0 * 2 + (split.start(c0) < u0)) * size;
+    const uint64_t whole = (uint64_t)row * a.qh + kvh * w.group + h;
+    p.m0 = p.n == 1 ? w.sh.ml + 2 * whole : first + p.t;
+    p.l0 = p.n == 1 ? p.m0 + 1 : p.m0 + w.sh.tile;
+    p.o0 = p.n == 1 ? w.sh.o + whole * DIM : first + 2 * w.sh.tile + (uint64_t)p.t * DIM;
+    p.next = w.sh.pieces + ((uint64_t)c0 * 2 + 2) * size;
     return p;
 }
 
@@ -224,13 +222,16 @@ __device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWo
 // its CTAs take equal parts of the context and join them over distributed
 // shared memory. Otherwise CTA c takes the c-th run of all units.
 // SHARED (and DIRECT): the row's own keys, those behind its group's shared ones, joined with what the tile kernel left.
-template <bool KV8, int DIM, bool DIRECT, bool SHARED>
-__global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decode_kernel(PagedAttnArgs a, PdWork w) {
-    using C = PdCfg<KV8, DIM>;
+template <bool KV8, int DIM, bool DIRECT, bool SHARED, int NW>
+__global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_decode_kernel(PagedAttnArgs a, PdWork w) {
+    using C = PdCfg<KV8, DIM, NW>;
+    constexpr int PD_WARPS = NW, PD_THREADS = 32 * NW;
     constexpr int KS = DIM / 16;  // k-steps of the first product, and 16-dim tiles of the second
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS], wM[PD_HEADS];
-    __shared__ float fin[DIRECT ? PD_MAX_PARTS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
+    __shared__ float fin[DIRECT && NW == 8 ? PD_MAX_PARTS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
+    __shared__ PdPieces pp[SHARED ? PD_HEADS : 1];
+    __shared__ float psum[SHARED ? PD_HEADS : 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     // 16-byte chunks of a lane's query head: head 8 hblk + g, dims by the permutation that the key rows' chunks
     // give the first product (chunk t + 4 j of a row of keys)
@@ -245,28 +246,32 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     };
     uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
     UnitSplit split;
-    uint32_t grp = 0;
-    SharedGroup sg = {};
+    uint4 rec = make_uint4(0, 0, 0, 0);  // SHARED: see SharedParts
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
         if (w.parts > 1) pd_cluster_arrive();
         row = unit / w.items;
         load_q(row, unit % w.items);  // needs no length
         if constexpr (SHARED) {
-            if (!pd_group(a, row, grp)) {  // (the whole cluster) the row stays
+            if (w.tiles) {
                 pdl_wait();
+                rec = w.sh.rows[row];
+            } else {
+                uint32_t g;
+                rec.x = shared_find(a, row, g) ? 0 : SHARED_NO_GROUP;
+                rec.y = paged_length(a.c, a.seqs ? a.seqs[row] : row);
+            }
+            if (rec.x == SHARED_NO_GROUP) {  // (the whole cluster) the row stays
                 if (w.parts > 1) pd_cluster_wait();
                 return;
             }
-            if (w.tiles) sg = shared_group(a, grp);
         }
-        const PdRow R = pd_row<C::LOG>(a, row, sg.keys);
+        const PdRow R = SHARED ? pd_own<C::LOG>(rec) : pd_row<C::LOG>(a, row);
         base = 0;
         const uint32_t first = unit % w.items * R.steps;
         u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
         u_end = first + (uint32_t)((uint64_t)R.steps * (part + 1) / w.parts);
-        if (R.steps == 0 && (!SHARED || sg.keys == 0)) {  // no key (the whole cluster): zero
-            if constexpr (SHARED) pdl_wait();
+        if (R.steps == 0 && (!SHARED || rec.x == 0)) {  // no key (the whole cluster): zero
             const uint32_t item = unit % w.items, kvh = item / w.hb, h0 = item % w.hb * PD_HEADS;
             const uint32_t heads = min(w.group - h0, (uint32_t)PD_HEADS);
             uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + h0) * DIM;
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
     const float fac0 = a.scale * 1.44269504f;
     bool first_segment = true;
     while (DIRECT || u < u_end) {  // DIRECT: once, also for a CTA of a cluster that has no step
-        const PdRow R = pd_row<C::LOG>(a, row, sg.keys);
+        const PdRow R = SHARED ? pd_own<C::LOG>(rec) : pd_row<C::LOG>(a, row);
         if (!DIRECT && R.steps == 0) {
             ++row;
             continue;
@@ -407,6 +412,14 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             next = pages_at(C::STAGES - 1);
 #pragma unroll
             for (int i = 0; i < C::STAGES - 1; ++i) load(i, start[i]);
+        }
+
+        if constexpr (SHARED) {  // (behind the first loads; read behind the loop's barrier)
+            if (rec.x > 0 && tid < PD_HEADS) {
+                PdPieces p = {};
+                if (hblk * PD_HEADS + tid < w.group) p = pd_pieces<DIM>(a, w, row, rec, kvh, hblk * PD_HEADS + tid);
+                pp[tid] = p;
+            }
         }
 
         // ---- the query heads as B fragments
@@ -650,8 +663,51 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             for (int k = 0; k < 4; ++k)
                 os[(warp * PD_HEADS + 2 * t + (k & 1)) * (DIM + 1) + d + (k >> 1)] = o[j][k];
         }
+        // ---- the shared keys' results: a cluster's CTAs take them in turn, [head][piece]
+        float *pf = os + C::OS + C::PO, *pl = pf + C::PF;
+        const uint32_t part0 = DIRECT ? blockIdx.x % w.parts : 0, stride2 = SHARED ? 2 * w.sh.tile * (DIM + 2) : 0;
+        const bool joins = SHARED && rec.x > 0;
+        if constexpr (SHARED) {
+            if (joins) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int h = 0; h < PD_HEADS; ++h) most = max(most, pp[h].n);
+                const uint32_t h = tid % PD_HEADS;
+                const PdPieces p = pp[h];
+#pragma unroll 4
+                for (uint32_t i = part0 + tid / PD_HEADS * w.parts; i < most; i += PD_THREADS / PD_HEADS * w.parts) {
+                    const float *q = p.next + (uint64_t)(i - 1) * stride2 + p.t;
+                    if (i < p.n) {
+                        pf[h * PD_MAX_SMS + i] = i == 0 ? *p.m0 : q[0];
+                        pl[h * PD_MAX_SMS + i] = i == 0 ? *p.l0 : q[w.sh.tile];
+                    }
+                }
+            }
+        }
         __syncthreads();
-        if (tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+        if constexpr (SHARED) {
+            if (joins) {
+                for (int h = warp; h < PD_HEADS; h += PD_WARPS) {
+                    const uint32_t n = pp[h].n;
+                    float M = lane < PD_WARPS ? wm[lane][h] : -INFINITY, L = 0.f;
+                    for (uint32_t i = part0 + lane * w.parts; i < n; i += 32 * w.parts) M = fmaxf(M, pf[h * PD_MAX_SMS + i]);
+                    M = warp_max(M);
+                    const float M0 = M == -INFINITY ? 0.f : M;
+                    for (uint32_t i = part0 + lane * w.parts; i < n; i += 32 * w.parts) {
+                        const float f = ex2(0.5f * (pf[h * PD_MAX_SMS + i] - M0));  // applied twice, as below
+                        pf[h * PD_MAX_SMS + i] = f;
+                        L += pl[h * PD_MAX_SMS + i] * f * f;
+                    }
+                    L = warp_sum(L);
+                    if (lane < PD_WARPS) wf[lane][h] = ex2(0.5f * (wm[lane][h] - M0));
+                    if (lane == 0) {
+                        wM[h] = M;
+                        psum[h] = L;
+                    }
+                }
+            }
+        }
+        if (!joins && tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
             const int h = tid % PD_HEADS, i = tid / PD_HEADS;
             float M = -INFINITY;
 #pragma unroll
@@ -660,72 +716,52 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
             if (i == 0) wM[h] = M;
         }
         __syncthreads();
-        const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
-        // ---- the shared keys' results: a cluster's CTAs take them in turn
-        constexpr int MOST = SHARED ? PD_MAX_SMS : 1;
-        __shared__ PdPieces pp[PD_HEADS];
-        __shared__ float pf[PD_HEADS][MOST], ptop[PD_HEADS], psum[PD_HEADS];
         if constexpr (SHARED) {
-            pdl_wait();
-            if (sg.keys > 0) {
-                const uint32_t part0 = blockIdx.x % w.parts;
-                auto at = [&](int h, uint32_t i) {
-                    const PdPieces &p = pp[h];
-                    return w.sh.pieces + ((uint64_t)(p.c0 + i) * 2 + (i == 0 ? p.slot0 : 0)) * ((uint64_t)w.sh.tile * (DIM + 2));
-                };
-                if (tid < PD_HEADS) {
-                    PdPieces p = {};
-                    if (hblk * PD_HEADS + tid < w.group) p = pd_pieces(a, w, grp, sg, row, kvh, hblk * PD_HEADS + tid);
-                    pp[tid] = p;
-                }
-                __syncthreads();
-                {  // warp h: head h
-                    const PdPieces p = pp[warp];
-                    float M = wM[warp], L = 0.f;
-                    for (uint32_t i = part0 + lane * w.parts; i < p.n; i += 32 * w.parts) {
-                        const float m1 = p.n == 1 ? w.sh.ml[2 * p.whole] : at(warp, i)[p.t];
-                        pf[warp][i] = m1;
-                        M = fmaxf(M, m1);
+            if (joins) {
+                // a thread has CPT columns of four dims, and eight of their loads in flight
+                constexpr int COLS = PD_HEADS * DIM / 4, CPT = COLS > PD_THREADS ? COLS / PD_THREADS : 1, BATCH = 8 / CPT;
+                if (tid < COLS) {
+                    PdPieces p[CPT];
+                    float4 O[CPT];
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int c = 0; c < CPT; ++c) {
+                        const int x = tid + c * PD_THREADS;
+                        p[c] = pp[x / (DIM / 4)];
+                        p[c].o0 += x % (DIM / 4) * 4;
+                        p[c].next += 2 * w.sh.tile + (uint64_t)p[c].t * DIM + x % (DIM / 4) * 4;
+                        O[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        most = max(most, p[c].n);
                     }
-                    M = warp_max(M);
-                    const float M0 = M == -INFINITY ? 0.f : M;
-                    for (uint32_t i = part0 + lane * w.parts; i < p.n; i += 32 * w.parts) {
-                        const float f = ex2(0.5f * (pf[warp][i] - M0)), l1 = p.n == 1 ? w.sh.ml[2 * p.whole + 1] : at(warp, i)[w.sh.tile + p.t];
-                        pf[warp][i] = f;
-                        L += l1 * f * f;
+                    for (uint32_t i0 = part0; i0 < most; i0 += BATCH * w.parts) {
+                        float4 v[BATCH][CPT];
+#pragma unroll
+                        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                            for (int c = 0; c < CPT; ++c) {
+                                const uint32_t i = i0 + k * w.parts;
+                                const float *q = i == 0 ? p[c].o0 : p[c].next + (uint64_t)(i - 1) * stride2;
+                                v[k][c] = i < p[c].n ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            }
+#pragma unroll
+                        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                            for (int c = 0; c < CPT; ++c) {
+                                const uint32_t i = i0 + k * w.parts;
+                                const float f = i < p[c].n ? pf[(tid + c * PD_THREADS) / (DIM / 4) * PD_MAX_SMS + i] : 0.f;
+                                O[c].x += v[k][c].x * f * f;
+                                O[c].y += v[k][c].y * f * f;
+                                O[c].z += v[k][c].z * f * f;
+                                O[c].w += v[k][c].w * f * f;
+                            }
                     }
-                    L = warp_sum(L);
-                    if (lane < PD_WARPS) {  // the warps' factors anew
-                        const float f = ex2(0.5f * (wm[lane][warp] - M0));
-                        wf[lane][warp] = f;
-                    }
-                    if (lane == 0) {
-                        ptop[warp] = M;
-                        psum[warp] = L;
-                    }
-                }
-                __syncthreads();
-                // their contexts summed over the first warp's slot of a ninth row of `os`
-                float *po = os + PD_WARPS * PD_HEADS * (DIM + 1);
-                for (int x = tid; x < PD_HEADS * DIM / 4; x += PD_THREADS) {
-                    const int h = x / (DIM / 4), d = x % (DIM / 4) * 4;
-                    const PdPieces p = pp[h];
-                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (uint32_t i = part0; i < p.n; i += w.parts) {
-                        const float4 v = *reinterpret_cast<const float4 *>(
-                            p.n == 1 ? w.sh.o + p.whole * DIM + d : at(h, i) + 2 * w.sh.tile + (uint64_t)p.t * DIM + d);
-                        const float f = pf[h][i];
-                        O.x += v.x * f * f;
-                        O.y += v.y * f * f;
-                        O.z += v.z * f * f;
-                        O.w += v.w * f * f;
-                    }
-                    *reinterpret_cast<float4 *>(po + h * DIM + d) = O;
+#pragma unroll
+                    for (int c = 0; c < CPT; ++c) *reinterpret_cast<float4 *>(os + C::OS + (tid + c * PD_THREADS) * 4) = O[c];
                 }
                 __syncthreads();
             }
         }
+        const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
         float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
         const uint32_t part = DIRECT ? blockIdx.x % w.parts : 0;
         if constexpr (DIRECT)
@@ -739,12 +775,11 @@ __global__ void __launch_bounds__(PD_THREADS, PdCfg<KV8, DIM>::MINB) paged_decod
                 L += wl[i][h] * f * f;
                 O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f * f;
             }
-            float M = wM[h];
+            const float M = wM[h];
             if constexpr (SHARED)
-                if (sg.keys > 0) {
-                    M = ptop[h];
+                if (joins) {
                     L += psum[h];
-                    O += os[PD_WARPS * PD_HEADS * (DIM + 1) + x];
+                    O += os[C::OS + x];
                 }
             const uint32_t hl = hblk * PD_HEADS + h;
             if (whole) {
@@ -874,10 +909,10 @@ static bool pd_fits(uint32_t parts, uint32_t units) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
     int n = __atomic_load_n(&known[dev][parts], __ATOMIC_RELAXED);
     if (!n) {
-        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED>;
+        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED, 8>;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(parts);
-        cfg.blockDim = dim3(PD_THREADS);
+        cfg.blockDim = dim3(C::THREADS);
         cfg.dynamicSmemBytes = C::SMEM;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
@@ -912,23 +947,34 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
         const uint64_t seen = (uint64_t)a.window + a.sinks;
         most = most < seen ? most : seen;
     }
+    if constexpr (SHARED) {
+        // Many rows with little of their own: two warps an item, so that an SM has 8 (4) items' chains of length, page and
+        // key in flight.
+        if (units >= 2 * (uint32_t)sms) {
+            using C2 = PdCfg<KV8, DIM, 2>;
+            auto *kernel = paged_decode_kernel<KV8, DIM, true, true, 2>;
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C2::SMEM) != cudaSuccess) return -3;
+            w.parts = 1;
+            return launch_pdl(kernel, dim3(units), dim3(C2::THREADS), C2::SMEM, st, 1, a, w);
+        }
+    }
     const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;
     uint64_t parts = want < room ? want : room;
     parts = parts < 1 ? 1 : parts < PD_MAX_PARTS ? parts : PD_MAX_PARTS;
     while (parts > 8 && !pd_fits<KV8, DIM, SHARED>((uint32_t)parts, units)) --parts;
     w.parts = (uint32_t)parts;
     if (SHARED || units * parts * 3 >= slots || most <= parts * PD_PART_MOST) {
-        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED>;
+        auto *kernel = paged_decode_kernel<KV8, DIM, true, SHARED, 8>;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
         if (parts > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return -3;
-        return launch_pdl(kernel, dim3(units * w.parts), dim3(PD_THREADS), C::SMEM, st, w.parts, a, w);
+        return launch_pdl(kernel, dim3(units * w.parts), dim3(C::THREADS), C::SMEM, st, w.parts, a, w);
     }
-    auto *kernel = paged_decode_kernel<KV8, DIM, false, false>;
+    auto *kernel = paged_decode_kernel<KV8, DIM, false, false, 8>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
     w.max_ctas = slots;
     PdlChain chain;
-    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(PD_THREADS), C::SMEM, st, 1, a, w)) return rc;
+    if (int rc = launch_pdl(kernel, dim3(w.max_ctas), dim3(C::THREADS), C::SMEM, st, 1, a, w)) return rc;
     return launch_pdl(paged_join_kernel<DIM>, dim3(units * PD_HEADS), dim3(DIM * PJ_GROUPS), 0, st, 1, a, w);
 }
 

@@ -1158,6 +1158,18 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             }
         }
     }
+    if (SHARED && warp == C::SW + 6) {
+        // ---------------- what the row kernel needs to know of each row
+        for (uint32_t r = blockIdx.x * 32 + lane; r < a.rows; r += gridDim.x * 32) {
+            uint32_t grp;
+            uint4 rec = make_uint4(SHARED_NO_GROUP, 0, 0, 0);
+            if (shared_find(a, r, grp)) {
+                const SharedGroup sg = shared_group(a, grp);
+                rec = make_uint4(sg.keys, paged_length(a.c, a.seqs ? a.seqs[r] : r), grp, r - sg.row0);
+            }
+            w.sh.rows[r] = rec;
+        }
+    }
     if (!SHARED && warp == C::SW + 6) {  // (behind its segments)
         // ---------------- rows in front of the first token, and of no sequence
         const uint32_t chunks = a.qh * (DIM / 8);
