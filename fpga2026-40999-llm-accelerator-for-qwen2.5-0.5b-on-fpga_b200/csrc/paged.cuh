@@ -133,14 +133,14 @@ __device__ __forceinline__ bool shared_find(const PagedAttnArgs &a, uint32_t row
 }
 // What the tile kernel leaves for the row kernel. Units (tile, KV head, block of 128 keys) are numbered group by group,
 // KV head by KV head, and split evenly over `ctas`; a tile's list of blocks is in pieces of the CTAs that have some of it
-// (two a CTA at most: [m tile][l tile][o tile x dim]), or whole, then by (row, head): [rows][qh] (m, l), [rows][qh][dim] o.
+// (two a CTA at most: [m tile][l tile][o dim / 4][tile][4]), or whole, then by flattened row of a KV head:
+// [hkv][rows * group] (m, l), [hkv][dim / 4][rows * group][4] o. (A thread of the tile kernel has a row: with four dims of
+// all rows side by side its stores are whole lines; [row][dim] took 3 us more.)
 struct SharedParts {
     unsigned long long *base;  // [n + 1] units of one KV head in the groups before
-    uint4 *rows;               // [rows] shared keys (SHARED_NO_GROUP: the row has none), length, group, row of the group
     float *pieces, *ml, *o;
     uint32_t tile, ctas;
 };
-constexpr uint32_t SHARED_NO_GROUP = 0xffffffffu;
 size_t paged_decode_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t rows);
 int launch_paged_decode(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 size_t paged_prefill_ws(uint32_t kv_heads, uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);

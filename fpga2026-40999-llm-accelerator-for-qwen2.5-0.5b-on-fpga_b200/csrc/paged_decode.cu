@@ -59,9 +59,9 @@ struct PdCfg {
     static constexpr int STAGES = 3;
     static constexpr int MINB = (RB == 256 ? 8 : 16) / NW;  // CTAs per SM
     static constexpr int RING = NW * STAGES * STEP_BYTES;
-    // over the drained ring: the warps' contexts, a shared prefix's, and the maxima (then factors) and sums of its pieces
-    static constexpr int OS = NW * PD_HEADS * (DIM + 1), PO = PD_HEADS * DIM, PF = PD_HEADS * PD_MAX_SMS;
-    static constexpr int OUT = (OS + PO + 2 * PF) * 4;
+    // over the drained ring: the warps' contexts, and the maxima (then factors) and sums of a shared prefix's pieces
+    static constexpr int OS = NW * PD_HEADS * (DIM + 1), PF = PD_HEADS * PD_MAX_SMS;
+    static constexpr int OUT = (OS + 2 * PF) * 4;
     static constexpr int SMEM = RING > OUT ? RING : OUT;
     static constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;  // floats of a partial result: m, l, o
 };
@@ -180,29 +180,34 @@ __device__ __forceinline__ PdRow pd_row(const PagedAttnArgs &a, uint32_t row) {
     return r;
 }
 
+// A row's group, and how many of its keys the tile kernel takes.
+struct PdShare {
+    uint32_t keys, group, at;  // at: the row's place in the group
+};
 // The same for a row's keys behind the shared ones (there is no window).
 template <int LOG>
-__device__ __forceinline__ PdRow pd_own(uint4 rec) {
+__device__ __forceinline__ PdRow pd_own(const PagedAttnArgs &a, uint32_t row, uint32_t keys) {
     PdRow r;
-    r.len = (int)rec.y;
+    r.len = paged_length(a.c, a.seqs ? a.seqs[row] : row);
     r.first = r.nfirst = 0;
-    r.low = (int)min(rec.x, rec.y);
+    r.low = min((int)keys, r.len);
     r.nlow = r.low >> LOG;
     r.steps = r.len > r.low ? (uint32_t)(((r.len + (1 << LOG) - 1) >> LOG) - r.nlow) : 0u;
     return r;
 }
 
 // One query head's share of the tile kernel's results: n of them. The first's maximum, sum and context are at m0, l0 and
-// o0; those of the CTAs behind the first follow `next`, two pieces apart.
+// o0; those of the CTAs behind the first follow `next`, two pieces apart. Four dims are `step` from the next four.
 struct PdPieces {
     const float *m0, *l0, *o0, *next;
+    uint64_t step;
     uint32_t n, t;
 };
 template <int DIM>
-__device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t row, uint4 rec, uint32_t kvh,
+__device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t row, const PdShare &share, uint32_t kvh,
                                               uint32_t h) {
-    const uint32_t blocks = (rec.x + 127) >> 7, m = rec.w * w.group + h, size = w.sh.tile * (DIM + 2);
-    const unsigned long long all = w.sh.base[a.n], b0 = w.sh.base[rec.z], units = w.sh.base[rec.z + 1] - b0;  // of a KV head
+    const uint32_t blocks = (share.keys + 127) >> 7, m = share.at * w.group + h, size = w.sh.tile * (DIM + 2);
+    const unsigned long long all = w.sh.base[a.n], b0 = w.sh.base[share.group], units = w.sh.base[share.group + 1] - b0;  // of a KV head
     const UnitSplit split(all * a.c.hkv, w.sh.ctas, 1);
     const unsigned long long u0 = b0 * a.c.hkv + kvh * units + (unsigned long long)(m / w.sh.tile) * blocks;
     const uint32_t c0 = split.cta_of(u0);
@@ -210,12 +215,166 @@ __device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWo
     p.n = split.cta_of(u0 + blocks - 1) - c0 + 1;
     p.t = m % w.sh.tile;
     const float *first = w.sh.pieces + ((uint64_t)c0 * 2 + (split.start(c0) < u0)) * size;
-    const uint64_t whole = (uint64_t)row * a.qh + kvh * w.group + h;
-    p.m0 = p.n == 1 ? w.sh.ml + 2 * whole : first + p.t;
+    const uint64_t flat = (uint64_t)a.rows * w.group, at = (uint64_t)row * w.group + h;
+    p.m0 = p.n == 1 ? w.sh.ml + 2 * (kvh * flat + at) : first + p.t;
     p.l0 = p.n == 1 ? p.m0 + 1 : p.m0 + w.sh.tile;
-    p.o0 = p.n == 1 ? w.sh.o + whole * DIM : first + 2 * w.sh.tile + (uint64_t)p.t * DIM;
+    p.o0 = p.n == 1 ? w.sh.o + (kvh * (DIM / 4) * flat + at) * 4 : first + 2 * w.sh.tile + 4 * p.t;
+    p.step = 4 * (p.n == 1 ? flat : w.sh.tile);
     p.next = w.sh.pieces + ((uint64_t)c0 * 2 + 2) * size;
     return p;
+}
+
+// Behind the CTAs' pushes into `fin`: each joins the heads that are its own.
+template <int DIM>
+__device__ __forceinline__ void pd_cluster_join(const PagedAttnArgs &a, const PdWork &w, uint32_t row, uint32_t kvh, uint32_t hblk,
+                                                const float *fin) {
+    const uint32_t part = blockIdx.x % w.parts;
+    tc::cluster_sync();
+    const uint32_t mine = pd_heads_here(w.parts);  // part, part + parts, .. as far as there are heads
+    for (uint32_t x = threadIdx.x; x < mine * DIM && part + x / DIM * w.parts < PD_HEADS; x += blockDim.x) {
+        const uint32_t k = x / DIM, d = x % DIM;
+        float M = -INFINITY, L = 0.f, O = 0.f;
+        for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, fin[(i * mine + k) * (DIM + 2)]);
+        const float M0 = M == -INFINITY ? 0.f : M;
+        for (uint32_t i = 0; i < w.parts; ++i) {
+            const float *p = fin + (i * mine + k) * (DIM + 2);
+            const float f = ex2(0.5f * (p[0] - M0));
+            L += p[1] * f * f;
+            O += p[2 + d] * f * f;
+        }
+        const uint32_t hl = hblk * PD_HEADS + part + k * w.parts;
+        if (hl < w.group)
+            a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
+    }
+}
+
+// A row's own results (os, wm, wl: by warp) and its group's shared ones joined. The CTAs of a cluster take the pieces of the
+// shared ones in turn.
+template <bool KV8, int DIM, int NW>
+__device__ __forceinline__ void pd_join(const PagedAttnArgs &a, const PdWork &w, const PdShare &share, uint32_t row, uint32_t kvh,
+                                        uint32_t hblk, float *os, const float (*wm)[PD_HEADS], const float (*wl)[PD_HEADS],
+                                        float *fin) {
+    using C = PdCfg<KV8, DIM, NW>;
+    constexpr int THREADS = C::THREADS, LPH = THREADS / PD_HEADS;  // threads of a head at the factors
+    __shared__ PdPieces pp[PD_HEADS];
+    __shared__ float wf[NW][PD_HEADS], wM[PD_HEADS], wL[PD_HEADS];
+    float *pf = os + C::OS, *pl = pf + C::PF;  // maxima (then factors) and sums of the pieces: [head][piece]
+    const uint32_t tid = threadIdx.x, part = blockIdx.x % w.parts, stride2 = 2 * w.sh.tile * (DIM + 2);
+    if (w.tiles) pdl_wait();
+    if (tid < PD_HEADS) {
+        PdPieces p = {};
+        if (share.keys > 0 && hblk * PD_HEADS + tid < w.group) p = pd_pieces<DIM>(a, w, row, share, kvh, hblk * PD_HEADS + tid);
+        pp[tid] = p;
+    }
+    __syncthreads();
+    // a thread has CPT columns of four dims of a head (head x % 8, dims 4 (x / 8) ..), and eight loads of them in flight
+    constexpr int COLS = PD_HEADS * DIM / 4, CPT = COLS > THREADS ? COLS / THREADS : 1, BATCH = 8 / CPT;
+    PdPieces p[CPT];
+    float4 O[CPT], v[BATCH][CPT];
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+        const uint32_t x = tid + c * THREADS;
+        p[c] = pp[x % PD_HEADS];
+        if (x >= COLS) p[c].n = 0;
+        p[c].o0 += x / PD_HEADS * p[c].step;
+        p[c].next += 2 * w.sh.tile + 4 * p[c].t + x / PD_HEADS * p[c].step;
+        O[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        most = max(most, p[c].n);
+    }
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int c = 0; c < CPT; ++c) {
+                const uint32_t i = i0 + k * w.parts;
+                const float *q = i == 0 ? p[c].o0 : p[c].next + (uint64_t)(i - 1) * stride2;
+                v[k][c] = i < p[c].n ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    };
+    {
+        const uint32_t h = tid / LPH, sub = tid % LPH;
+        const PdPieces q = pp[h];
+        float M = -INFINITY, L = 0.f;
+        load(part);  // (needs no factor)
+        for (uint32_t i = part + sub * w.parts; i < q.n; i += LPH * w.parts) {
+            const float *at = q.next + (uint64_t)(i - 1) * stride2 + q.t;
+            const float m1 = __ldcg(i == 0 ? q.m0 : at), l1 = __ldcg(i == 0 ? q.l0 : at + w.sh.tile);
+            pf[h * PD_MAX_SMS + i] = m1;
+            pl[h * PD_MAX_SMS + i] = l1;
+            M = fmaxf(M, m1);
+        }
+#pragma unroll
+        for (uint32_t i = sub; i < NW; i += LPH) M = fmaxf(M, wm[i][h]);
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float M0 = M == -INFINITY ? 0.f : M;
+        for (uint32_t i = part + sub * w.parts; i < q.n; i += LPH * w.parts) {
+            const float f = ex2(0.5f * (pf[h * PD_MAX_SMS + i] - M0));  // applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+            pf[h * PD_MAX_SMS + i] = f;
+            L += pl[h * PD_MAX_SMS + i] * f * f;
+        }
+#pragma unroll
+        for (uint32_t i = sub; i < NW; i += LPH) {
+            const float f = ex2(0.5f * (wm[i][h] - M0));
+            wf[i][h] = f;
+            L += wl[i][h] * f * f;
+        }
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (sub == 0) {
+            wM[h] = M;
+            wL[h] = L;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i0 = part; i0 < most; i0 += BATCH * w.parts) {
+        if (i0 > part) load(i0);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int c = 0; c < CPT; ++c) {
+                const uint32_t i = i0 + k * w.parts;
+                const float f = i < p[c].n ? pf[(tid + c * THREADS) % PD_HEADS * PD_MAX_SMS + i] : 0.f;
+                O[c].x += v[k][c].x * f * f;
+                O[c].y += v[k][c].y * f * f;
+                O[c].z += v[k][c].z * f * f;
+                O[c].w += v[k][c].w * f * f;
+            }
+    }
+    if (w.parts > 1) pd_cluster_wait();  // every CTA of the cluster has started
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+        const uint32_t x = tid + c * THREADS, h = x % PD_HEADS, d = x / PD_HEADS * 4, hl = hblk * PD_HEADS + h;
+        if (x >= COLS) break;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float f = wf[i][h], *o = os + (i * PD_HEADS + h) * (DIM + 1) + d;
+            O[c].x += o[0] * f * f;
+            O[c].y += o[1] * f * f;
+            O[c].z += o[2] * f * f;
+            O[c].w += o[3] * f * f;
+        }
+        const float L = wL[h];
+        if (w.parts == 1) {
+            uint2 out = make_uint2(pack_bf16(O[c].x / L, O[c].y / L), pack_bf16(O[c].z / L, O[c].w / L));
+            if (L == 0.f) out = make_uint2(0, 0);
+            if (hl < w.group)
+                *reinterpret_cast<uint2 *>(a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d) = out;
+        } else {  // head h is joined by CTA h % parts, from slot `part` of its shared memory
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(fin + (part * pd_heads_here(w.parts) + h / w.parts) * (DIM + 2));
+            const uint32_t rank = h % w.parts;
+            pd_dsmem_store(to + 4 * (2 + d), rank, O[c].x);
+            pd_dsmem_store(to + 4 * (3 + d), rank, O[c].y);
+            pd_dsmem_store(to + 4 * (4 + d), rank, O[c].z);
+            pd_dsmem_store(to + 4 * (5 + d), rank, O[c].w);
+            if (d == 0) {
+                pd_dsmem_store(to, rank, wM[h]);
+                pd_dsmem_store(to + 4, rank, L);
+            }
+        }
+    }
+    if (w.parts > 1) pd_cluster_join<DIM>(a, w, row, kvh, hblk, fin);
 }
 
 // DIRECT: CTA (or cluster of `parts` CTAs) b has row b / items, item b % items;
@@ -230,8 +389,6 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float wm[PD_WARPS][PD_HEADS], wl[PD_WARPS][PD_HEADS], wf[PD_WARPS][PD_HEADS], wM[PD_HEADS];
     __shared__ float fin[DIRECT && NW == 8 ? PD_MAX_PARTS * (DIM + 2) : 1];  // m, l, o of the heads that this CTA joins, from every CTA of the cluster
-    __shared__ PdPieces pp[SHARED ? PD_HEADS : 1];
-    __shared__ float psum[SHARED ? PD_HEADS : 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     // 16-byte chunks of a lane's query head: head 8 hblk + g, dims by the permutation that the key rows' chunks
     // give the first product (chunk t + 4 j of a row of keys)
@@ -246,32 +403,32 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
     };
     uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
     UnitSplit split;
-    uint4 rec = make_uint4(0, 0, 0, 0);  // SHARED: see SharedParts
+    PdShare share = {};
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
         if (w.parts > 1) pd_cluster_arrive();
         row = unit / w.items;
         load_q(row, unit % w.items);  // needs no length
         if constexpr (SHARED) {
-            if (w.tiles) {
+            // (nothing here depends on the tile kernel, whose end this one need not wait for before its join)
+            if (!shared_find(a, row, share.group)) {  // (the whole cluster) the row stays
                 pdl_wait();
-                rec = w.sh.rows[row];
-            } else {
-                uint32_t g;
-                rec.x = shared_find(a, row, g) ? 0 : SHARED_NO_GROUP;
-                rec.y = paged_length(a.c, a.seqs ? a.seqs[row] : row);
-            }
-            if (rec.x == SHARED_NO_GROUP) {  // (the whole cluster) the row stays
                 if (w.parts > 1) pd_cluster_wait();
                 return;
             }
+            if (w.tiles) {
+                const SharedGroup sg = shared_group(a, share.group);
+                share.keys = (uint32_t)sg.keys;
+                share.at = row - sg.row0;
+            }
         }
-        const PdRow R = SHARED ? pd_own<C::LOG>(rec) : pd_row<C::LOG>(a, row);
+        const PdRow R = SHARED ? pd_own<C::LOG>(a, row, share.keys) : pd_row<C::LOG>(a, row);
         base = 0;
         const uint32_t first = unit % w.items * R.steps;
         u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
         u_end = first + (uint32_t)((uint64_t)R.steps * (part + 1) / w.parts);
-        if (R.steps == 0 && (!SHARED || rec.x == 0)) {  // no key (the whole cluster): zero
+        if (R.steps == 0 && (!SHARED || share.keys == 0)) {  // no key (the whole cluster): zero
+            if constexpr (SHARED) pdl_wait();
             const uint32_t item = unit % w.items, kvh = item / w.hb, h0 = item % w.hb * PD_HEADS;
             const uint32_t heads = min(w.group - h0, (uint32_t)PD_HEADS);
             uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + h0) * DIM;
@@ -335,7 +492,7 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
     const float fac0 = a.scale * 1.44269504f;
     bool first_segment = true;
     while (DIRECT || u < u_end) {  // DIRECT: once, also for a CTA of a cluster that has no step
-        const PdRow R = SHARED ? pd_own<C::LOG>(rec) : pd_row<C::LOG>(a, row);
+        const PdRow R = SHARED ? pd_own<C::LOG>(a, row, share.keys) : pd_row<C::LOG>(a, row);
         if (!DIRECT && R.steps == 0) {
             ++row;
             continue;
@@ -412,14 +569,6 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
             next = pages_at(C::STAGES - 1);
 #pragma unroll
             for (int i = 0; i < C::STAGES - 1; ++i) load(i, start[i]);
-        }
-
-        if constexpr (SHARED) {  // (behind the first loads; read behind the loop's barrier)
-            if (rec.x > 0 && tid < PD_HEADS) {
-                PdPieces p = {};
-                if (hblk * PD_HEADS + tid < w.group) p = pd_pieces<DIM>(a, w, row, rec, kvh, hblk * PD_HEADS + tid);
-                pp[tid] = p;
-            }
         }
 
         // ---- the query heads as B fragments
@@ -663,51 +812,12 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
             for (int k = 0; k < 4; ++k)
                 os[(warp * PD_HEADS + 2 * t + (k & 1)) * (DIM + 1) + d + (k >> 1)] = o[j][k];
         }
-        // ---- the shared keys' results: a cluster's CTAs take them in turn, [head][piece]
-        float *pf = os + C::OS + C::PO, *pl = pf + C::PF;
-        const uint32_t part0 = DIRECT ? blockIdx.x % w.parts : 0, stride2 = SHARED ? 2 * w.sh.tile * (DIM + 2) : 0;
-        const bool joins = SHARED && rec.x > 0;
         if constexpr (SHARED) {
-            if (joins) {
-                uint32_t most = 0;
-#pragma unroll
-                for (int h = 0; h < PD_HEADS; ++h) most = max(most, pp[h].n);
-                const uint32_t h = tid % PD_HEADS;
-                const PdPieces p = pp[h];
-#pragma unroll 4
-                for (uint32_t i = part0 + tid / PD_HEADS * w.parts; i < most; i += PD_THREADS / PD_HEADS * w.parts) {
-                    const float *q = p.next + (uint64_t)(i - 1) * stride2 + p.t;
-                    if (i < p.n) {
-                        pf[h * PD_MAX_SMS + i] = i == 0 ? *p.m0 : q[0];
-                        pl[h * PD_MAX_SMS + i] = i == 0 ? *p.l0 : q[w.sh.tile];
-                    }
-                }
-            }
+            pd_join<KV8, DIM, NW>(a, w, share, row, kvh, hblk, os, wm, wl, fin);
+            return;
         }
         __syncthreads();
-        if constexpr (SHARED) {
-            if (joins) {
-                for (int h = warp; h < PD_HEADS; h += PD_WARPS) {
-                    const uint32_t n = pp[h].n;
-                    float M = lane < PD_WARPS ? wm[lane][h] : -INFINITY, L = 0.f;
-                    for (uint32_t i = part0 + lane * w.parts; i < n; i += 32 * w.parts) M = fmaxf(M, pf[h * PD_MAX_SMS + i]);
-                    M = warp_max(M);
-                    const float M0 = M == -INFINITY ? 0.f : M;
-                    for (uint32_t i = part0 + lane * w.parts; i < n; i += 32 * w.parts) {
-                        const float f = ex2(0.5f * (pf[h * PD_MAX_SMS + i] - M0));  // applied twice, as below
-                        pf[h * PD_MAX_SMS + i] = f;
-                        L += pl[h * PD_MAX_SMS + i] * f * f;
-                    }
-                    L = warp_sum(L);
-                    if (lane < PD_WARPS) wf[lane][h] = ex2(0.5f * (wm[lane][h] - M0));
-                    if (lane == 0) {
-                        wM[h] = M;
-                        psum[h] = L;
-                    }
-                }
-            }
-        }
-        if (!joins && tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
+        if (tid < PD_HEADS * PD_WARPS) {  // each warp's factor, applied twice: 2^(m - M) may underflow where o 2^(m - M) does not
             const int h = tid % PD_HEADS, i = tid / PD_HEADS;
             float M = -INFINITY;
 #pragma unroll
@@ -716,51 +826,6 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
             if (i == 0) wM[h] = M;
         }
         __syncthreads();
-        if constexpr (SHARED) {
-            if (joins) {
-                // a thread has CPT columns of four dims, and eight of their loads in flight
-                constexpr int COLS = PD_HEADS * DIM / 4, CPT = COLS > PD_THREADS ? COLS / PD_THREADS : 1, BATCH = 8 / CPT;
-                if (tid < COLS) {
-                    PdPieces p[CPT];
-                    float4 O[CPT];
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        const int x = tid + c * PD_THREADS;
-                        p[c] = pp[x / (DIM / 4)];
-                        p[c].o0 += x % (DIM / 4) * 4;
-                        p[c].next += 2 * w.sh.tile + (uint64_t)p[c].t * DIM + x % (DIM / 4) * 4;
-                        O[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        most = max(most, p[c].n);
-                    }
-                    for (uint32_t i0 = part0; i0 < most; i0 += BATCH * w.parts) {
-                        float4 v[BATCH][CPT];
-#pragma unroll
-                        for (int k = 0; k < BATCH; ++k)
-#pragma unroll
-                            for (int c = 0; c < CPT; ++c) {
-                                const uint32_t i = i0 + k * w.parts;
-                                const float *q = i == 0 ? p[c].o0 : p[c].next + (uint64_t)(i - 1) * stride2;
-                                v[k][c] = i < p[c].n ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            }
-#pragma unroll
-                        for (int k = 0; k < BATCH; ++k)
-#pragma unroll
-                            for (int c = 0; c < CPT; ++c) {
-                                const uint32_t i = i0 + k * w.parts;
-                                const float f = i < p[c].n ? pf[(tid + c * PD_THREADS) / (DIM / 4) * PD_MAX_SMS + i] : 0.f;
-                                O[c].x += v[k][c].x * f * f;
-                                O[c].y += v[k][c].y * f * f;
-                                O[c].z += v[k][c].z * f * f;
-                                O[c].w += v[k][c].w * f * f;
-                            }
-                    }
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) *reinterpret_cast<float4 *>(os + C::OS + (tid + c * PD_THREADS) * 4) = O[c];
-                }
-                __syncthreads();
-            }
-        }
         const bool whole = DIRECT ? w.parts == 1 : cnt == R.steps;
         float *piece = w.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * C::PIECE;
         const uint32_t part = DIRECT ? blockIdx.x % w.parts : 0;
@@ -775,12 +840,6 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
                 L += wl[i][h] * f * f;
                 O += os[(i * PD_HEADS + h) * (DIM + 1) + d] * f * f;
             }
-            const float M = wM[h];
-            if constexpr (SHARED)
-                if (joins) {
-                    L += psum[h];
-                    O += os[C::OS + x];
-                }
             const uint32_t hl = hblk * PD_HEADS + h;
             if (whole) {
                 if (hl < w.group)
@@ -791,36 +850,20 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
                 const uint32_t to = (uint32_t)__cvta_generic_to_shared(fin + slot);
                 pd_dsmem_store(to + 4 * (2 + d), h % w.parts, O);
                 if (d == 0) {
-                    pd_dsmem_store(to, h % w.parts, M);
+                    pd_dsmem_store(to, h % w.parts, wM[h]);
                     pd_dsmem_store(to + 4, h % w.parts, L);
                 }
             } else {
                 piece[2 * PD_HEADS + x] = O;
                 if (d == 0) {
-                    piece[h] = M;
+                    piece[h] = wM[h];
                     piece[PD_HEADS + h] = L;
                 }
             }
         }
         if constexpr (DIRECT) {
             if (w.parts > 1) {
-                tc::cluster_sync();
-                const uint32_t mine = pd_heads_here(w.parts);  // part, part + parts, .. as far as there are heads
-                for (uint32_t x = tid; x < mine * DIM && part + x / DIM * w.parts < PD_HEADS; x += PD_THREADS) {
-                    const uint32_t k = x / DIM, d = x % DIM;
-                    float M = -INFINITY, L = 0.f, O = 0.f;
-                    for (uint32_t i = 0; i < w.parts; ++i) M = fmaxf(M, fin[(i * mine + k) * (DIM + 2)]);
-                    const float M0 = M == -INFINITY ? 0.f : M;
-                    for (uint32_t i = 0; i < w.parts; ++i) {
-                        const float *p = fin + (i * mine + k) * (DIM + 2);
-                        const float f = ex2(0.5f * (p[0] - M0));
-                        L += p[1] * f * f;
-                        O += p[2 + d] * f * f;
-                    }
-                    const uint32_t hl = hblk * PD_HEADS + part + k * w.parts;
-                    if (hl < w.group)
-                        a.ctx[row * a.ctx_stride + (uint64_t)(kvh * w.group + hl) * DIM + d] = f2bf(L == 0.f ? 0.f : O / L);
-                }
+                pd_cluster_join<DIM>(a, w, row, kvh, hblk, fin);
             }
             return;
         }
@@ -933,6 +976,14 @@ static bool pd_fits(uint32_t parts, uint32_t units) {
     return n - 1 >= (int)units;
 }
 
+template <bool KV8, int DIM, int NW>
+static int launch_rows(const PagedAttnArgs &a, const PdWork &w, uint32_t units, cudaStream_t st) {
+    using C = PdCfg<KV8, DIM, NW>;
+    auto *kernel = paged_decode_kernel<KV8, DIM, true, true, NW>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
+    return launch_pdl(kernel, dim3(units), dim3(C::THREADS), C::SMEM, st, 1, a, w);
+}
+
 template <bool KV8, int DIM, bool SHARED = false>
 static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM>;
@@ -948,14 +999,11 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
         most = most < seen ? most : seen;
     }
     if constexpr (SHARED) {
-        // Many rows with little of their own: two warps an item, so that an SM has 8 (4) items' chains of length, page and
-        // key in flight.
+        // Many rows with little of their own: one or two warps an item, so that an SM has many items' chains of length,
+        // page and key in flight.
         if (units >= 2 * (uint32_t)sms) {
-            using C2 = PdCfg<KV8, DIM, 2>;
-            auto *kernel = paged_decode_kernel<KV8, DIM, true, true, 2>;
-            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C2::SMEM) != cudaSuccess) return -3;
             w.parts = 1;
-            return launch_pdl(kernel, dim3(units), dim3(C2::THREADS), C2::SMEM, st, 1, a, w);
+            return units >= 5 * (uint32_t)sms ? launch_rows<KV8, DIM, 1>(a, w, units, st) : launch_rows<KV8, DIM, 2>(a, w, units, st);
         }
     }
     const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;

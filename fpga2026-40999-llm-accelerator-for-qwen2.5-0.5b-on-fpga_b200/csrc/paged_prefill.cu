@@ -327,6 +327,27 @@ __device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, unsigned
     return false;
 }
 
+// Queries of 32 rows (quarter `part`) of the MMA tile from flattened row mt: row m is token m / group, head m % group of the
+// segment's KV head; lane = row, its address handed to the lanes that copy it (rows of whole lines).
+template <int DIM>
+__device__ __forceinline__ void pp_queries(const PagedAttnArgs &a, const PpWork &w, const PpSeg &g, uint32_t dst, uint32_t mt,
+                                           int part) {
+    constexpr int CPR = DIM / 8;  // 16-byte chunks of a bf16 row
+    const int lane = threadIdx.x & 31;
+    const uint32_t mr = mt + 32 * part + lane, token = mr / w.group;
+    const bool live = mr < g.mrows;
+    const uint64_t mine = live ? (g.row0 + (uint64_t)token) * a.q_stride +
+                                     (uint64_t)(g.kvh * w.group + mr - token * w.group) * DIM
+                               : 0;
+    const uint32_t lives = __ballot_sync(0xffffffffu, live);
+#pragma unroll 4
+    for (int j = 0; j < CPR; ++j) {
+        const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
+        const uint64_t src = __shfl_sync(0xffffffffu, mine, rl);
+        pp_cp16(dst + pp_off(32 * part + rl, c), a.q + src + 8 * c, lives >> rl & 1 ? 16 : 0);
+    }
+}
+
 // The reading side of the segment ring.
 struct PpReader {
     const PpSeg *ring;
@@ -380,7 +401,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             tc::mbar_init(&seg_empty[i], 7 + C::SW);  // 4 tile warps, the copy warp, 2 issuers, the softmax warps
         }
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&q_full[i], 4);
+            tc::mbar_init(&q_full[i], SHARED ? C::SW : 4);
             tc::mbar_init(&q_empty[i], 2);
         }
         for (int i = 0; i < 4; ++i) {  // [tile][score buffer]
@@ -456,12 +477,27 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
         const uint32_t s_base = lane_addr + x * (64 * C::NB), o_addr = lane_addr + 256 + x * DIM;
         uint64_t *const s_bar = s_full + x * C::NB, *const p_bar = p_ready + x * C::NB;
         PpReader rd{ring, seg_full, seg_empty};
+        uint32_t nseg = 0;
         uint32_t bc = 0, round = 0;  // blocks of the CTA; rounds of this tile's score barriers before the segment
         PpSeg g;
         while (ok) {
             ok = rd.next(g, w.err);
             if (!ok || g.nblk == 0) break;
             const uint32_t mt = g.m0 + 128 * x;  // this MMA tile's first flattened row
+            if constexpr (SHARED) {
+                // A CTA has one or two segments here, so there is little behind which the tile warps could load the next
+                // queries: each warp loads its own rows, with four times as many issuing (3.2 -> 1.5 us)
+                if (mt < g.mrows) pp_queries<DIM>(a, w, g, sbase + C::Q + ((nseg % C::QBUFS) * C::TILES + x) * C::TILE_BYTES, mt, warp & 3);
+                pp_cp_commit();
+                pp_cp_wait<0>();
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&q_full[nseg % C::QBUFS]);
+                // (a tile without rows waits for nothing else before its warps arrive again)
+                if (mt >= g.mrows) ok = __all_sync(0xffffffffu, pp_wait(&q_full[nseg % C::QBUFS], (nseg / C::QBUFS) & 1, w.err, 68));
+                if (!ok) break;
+                ++nseg;
+            }
             if (mt >= g.mrows) {                 // no rows: only let the scales go
                 for (int i = 0; i < g.nblk && ok; ++i, ++bc) {
                     ok = __all_sync(0xffffffffu, pp_wait(&sc_full[bc % PP_SC], (bc / PP_SC) & 1, w.err, 61));
@@ -728,18 +764,31 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
             ++round;
             tc::tc_fence_after();
             const bool live = m_row < g.mrows && pos >= 0;
-            if (SHARED && g.piece < 0) {
-                const uint64_t at = (g.row0 + (uint64_t)row_i) * a.qh + g.kvh * w.group + m_row % w.group;
-                if (m_row < g.mrows) *reinterpret_cast<float2 *>(w.sh.ml + 2 * at) = make_float2(l == 0.f ? -INFINITY : m, l);
+            if constexpr (SHARED) {
+                const bool whole = g.piece < 0;
+                const uint64_t flat = (uint64_t)a.rows * w.group, at = (g.row0 + (uint64_t)row_i) * w.group + m_row % w.group;
+                float *piece = w.pieces + (uint64_t)max(g.piece, 0) * C::PIECE, *po;
+                uint64_t step;  // from four dims to the next four
+                const float top = l == 0.f ? -INFINITY : m;
+                if (whole) {
+                    if (m_row < g.mrows) *reinterpret_cast<float2 *>(w.sh.ml + 2 * (g.kvh * flat + at)) = make_float2(top, l);
+                    po = w.sh.o + (g.kvh * (DIM / 4) * flat + at) * 4;
+                    step = 4 * flat;
+                } else {
+                    piece[128 * x + r] = top;
+                    piece[C::TILE + 128 * x + r] = l;
+                    po = piece + 2 * C::TILE + 4 * (128 * x + r);
+                    step = 4 * C::TILE;
+                }
 #pragma unroll 1
                 for (int j = 0; j < DIM; j += 16) {
                     uint32_t o[16];
                     pp_ld16(o_addr + j, o);
                     pp_ld_wait();
-                    if (m_row < g.mrows) {
+                    if (!whole || m_row < g.mrows) {
 #pragma unroll
                         for (int k = 0; k < 16; k += 4)
-                            *reinterpret_cast<uint4 *>(w.sh.o + at * DIM + j + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                            *reinterpret_cast<uint4 *>(po + (j + k) / 4 * step) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                 }
             } else if (g.piece < 0) {
@@ -837,9 +886,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 if (lane == 0) tc::mbar_arrive(&sc_full[st]);
                 scales_of(i + 1, page);
                 page = page_of(i + 2);
-                if (i == 0) {
-                    // queries: flattened row m of the tile is token m / group, head m % group of this KV
-                    // head; lane = row, its address handed to the lanes that copy it (rows of whole lines)
+                if (!SHARED && i == 0) {
                     const uint32_t qb = nseg % C::QBUFS, use = nseg / C::QBUFS;
                     if (use > 0) ok = __all_sync(0xffffffffu, pp_wait(&q_empty[qb], (use - 1) & 1, w.err, 64));
                     if (!ok) break;
@@ -847,19 +894,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
 #pragma unroll 1
                     for (int x = 0; x < C::TILES; ++x) {
                         if (g.m0 + 128 * x >= g.mrows) break;
-                        const uint32_t mr = g.m0 + 128 * x + 32 * lw + lane, token = mr / w.group;
-                        const bool live = mr < g.mrows;
-                        const uint64_t mine = live ? (g.row0 + (uint64_t)token) * a.q_stride +
-                                                         (uint64_t)(g.kvh * w.group + mr - token * w.group) * DIM
-                                                   : 0;
-                        const uint32_t lives = __ballot_sync(0xffffffffu, live);
-                        const uint32_t dst = sbase + C::Q + (qb * C::TILES + x) * C::TILE_BYTES;
-#pragma unroll 4
-                        for (int j = 0; j < CPR; ++j) {
-                            const int n = j * 32 + lane, rl = n / CPR, c = n % CPR;
-                            const uint64_t src = __shfl_sync(0xffffffffu, mine, rl);
-                            pp_cp16(dst + pp_off(32 * lw + rl, c), a.q + src + 8 * c, lives >> rl & 1 ? 16 : 0);
-                        }
+                        pp_queries<DIM>(a, w, g, sbase + C::Q + (qb * C::TILES + x) * C::TILE_BYTES, g.m0 + 128 * x, lw);
                     }
                     pp_cp_commit();
                     pp_cp_wait<0>();
@@ -1156,18 +1191,6 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 }
                 break;
             }
-        }
-    }
-    if (SHARED && warp == C::SW + 6) {
-        // ---------------- what the row kernel needs to know of each row
-        for (uint32_t r = blockIdx.x * 32 + lane; r < a.rows; r += gridDim.x * 32) {
-            uint32_t grp;
-            uint4 rec = make_uint4(SHARED_NO_GROUP, 0, 0, 0);
-            if (shared_find(a, r, grp)) {
-                const SharedGroup sg = shared_group(a, grp);
-                rec = make_uint4(sg.keys, paged_length(a.c, a.seqs ? a.seqs[r] : r), grp, r - sg.row0);
-            }
-            w.sh.rows[r] = rec;
         }
     }
     if (!SHARED && warp == C::SW + 6) {  // (behind its segments)

@@ -16,7 +16,7 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t paged_shared_ws(uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows) {
     const size_t heads = (size_t)rows * q_heads;
-    return 256 + up256(((size_t)n + 1) * 8) + up256((size_t)rows * 16) + paged_shared_pieces_bytes(dim) + up256(heads * 8) + heads * dim * 4;
+    return 256 + up256(((size_t)n + 1) * 8) + paged_shared_pieces_bytes(dim) + up256(heads * 8) + heads * dim * 4;
 }
 
 int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
@@ -26,8 +26,6 @@ int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     SharedParts parts = {};
     parts.base = reinterpret_cast<unsigned long long *>(p);
     p += up256(((size_t)a.n + 1) * 8);
-    parts.rows = reinterpret_cast<uint4 *>(p);
-    p += up256((size_t)a.rows * 16);
     parts.pieces = reinterpret_cast<float *>(p);
     p += paged_shared_pieces_bytes(a.dim);
     parts.ml = reinterpret_cast<float *>(p);
