@@ -110,15 +110,19 @@ struct SharedGroup {
     uint32_t row0, rows, seq;
     int keys;
 };
-constexpr uint32_t SHARED_ROWS = 2;  // rows and keys that are worth the tile kernel's piece
-constexpr int SHARED_KEYS = 128;
+// Whether a group is worth the tile kernel: rows * keys * KV heads * dims from 2^25 on. Its launch and the join of its
+// pieces take some 12 us whatever the size, and the row kernel finds shared pages in L2. Without and with the tiles: 14 heads
+// on 2 of 64 dims KV8, 64 rows on 2048 keys (2^24) 14.4 and 23.2 us, 256 rows on 4096 (2^27) 119 and 43; 32 heads on 8 of
+// 128 dims bf16, 32 rows on 512 keys (2^24) 16.1 and 20.8 us, 1024 (2^25) 21.6 and 23.0, 64 rows on 1024 (2^26) 28.9 and 22.4;
+// 4 groups of 8 rows on 2048 (2^24 each) 33.9 and 31.8.
+constexpr uint64_t SHARED_WORK = 1ull << 25;
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
     SharedGroup s;
     s.row0 = min(a.starts[g], a.rows);
     s.rows = min(max(a.starts[g + 1], s.row0), a.rows) - s.row0;
     s.seq = s.rows == 0 ? QWEN_B200_NO_SEQ : a.seqs ? a.seqs[s.row0] : s.row0;
-    s.keys = s.rows < SHARED_ROWS ? 0 : min((int)min(a.prefix[g], 0x7fffffffu), paged_length(a.c, s.seq));
-    if (s.keys < SHARED_KEYS) s.keys = 0;
+    s.keys = min((int)min(a.prefix[g], 0x7fffffffu), paged_length(a.c, s.seq));
+    if (s.rows < 2 || (uint64_t)s.rows * s.keys < (SHARED_WORK / a.dim + a.c.hkv - 1) / a.c.hkv) s.keys = 0;
     return s;
 }
 // The group that a row belongs to; false for none. starts is not decreasing.

@@ -46,6 +46,7 @@ constexpr uint32_t PD_MAX_PARTS = 16;  // CTAs of a cluster
 constexpr int PD_MAX_SMS = 192;  // sizes the workspace whatever the device
 constexpr uint32_t PD_PART_KEYS = 512;  // keys that a CTA of a cluster has at least to be worth its join
 constexpr uint32_t PD_PART_MOST = 2048; // and at most where the clusters leave most of the GPU idle
+constexpr uint32_t PD_SM_BYTES = 227 * 1024, PD_STATIC_BYTES = 4096;  // shared memory of an SM; what a CTA has beside its dynamic part, at most
 constexpr uint32_t PD_MIN_UNITS = 8;  // steps that a CTA takes at least (1 per warp)
 
 template <bool KV8, int DIM, int NW = 8>  // NW warps
@@ -267,8 +268,9 @@ __device__ __forceinline__ void pd_join(const PagedAttnArgs &a, const PdWork &w,
         pp[tid] = p;
     }
     __syncthreads();
-    // a thread has CPT columns of four dims of a head (head x % 8, dims 4 (x / 8) ..), and eight loads of them in flight
-    constexpr int COLS = PD_HEADS * DIM / 4, CPT = COLS > THREADS ? COLS / THREADS : 1, BATCH = 8 / CPT;
+    // a thread has CPT columns of four dims of a head (head x % 8, dims 4 (x / 8) ..), and 16 loads of them in flight
+    constexpr int COLS = PD_HEADS * DIM / 4, CPT = COLS > THREADS ? COLS / THREADS : 1;
+    constexpr int BATCH = 16 / CPT;
     PdPieces p[CPT];
     float4 O[CPT], v[BATCH][CPT];
     uint32_t most = 0;
@@ -403,12 +405,17 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
     };
     uint32_t row, u, u_end, base;  // units: u .. u_end, of the row's first one at `base`
     UnitSplit split;
+    uint32_t item0 = 0;
     PdShare share = {};
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
         if (w.parts > 1) pd_cluster_arrive();
-        row = unit / w.items;
-        load_q(row, unit % w.items);  // needs no length
+        // Blocks of two warps and fewer come several to an SM, neighbours together: neighbours are different rows there, or one
+        // SM would get all KV heads of a long one (1024 blocks with 1 to 512 keys: 47 us for the loop, not 27).
+        constexpr bool SPREAD = SHARED && NW < 8;
+        row = SPREAD ? unit % a.rows : unit / w.items;
+        item0 = SPREAD ? unit / a.rows : unit % w.items;
+        load_q(row, item0);  // needs no length
         if constexpr (SHARED) {
             // (nothing here depends on the tile kernel, whose end this one need not wait for before its join)
             if (!shared_find(a, row, share.group)) {  // (the whole cluster) the row stays
@@ -424,12 +431,12 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
         }
         const PdRow R = SHARED ? pd_own<C::LOG>(a, row, share.keys) : pd_row<C::LOG>(a, row);
         base = 0;
-        const uint32_t first = unit % w.items * R.steps;
+        const uint32_t first = item0 * R.steps;
         u = first + (uint32_t)((uint64_t)R.steps * part / w.parts);
         u_end = first + (uint32_t)((uint64_t)R.steps * (part + 1) / w.parts);
         if (R.steps == 0 && (!SHARED || share.keys == 0)) {  // no key (the whole cluster): zero
             if constexpr (SHARED) pdl_wait();
-            const uint32_t item = unit % w.items, kvh = item / w.hb, h0 = item % w.hb * PD_HEADS;
+            const uint32_t kvh = item0 / w.hb, h0 = item0 % w.hb * PD_HEADS;
             const uint32_t heads = min(w.group - h0, (uint32_t)PD_HEADS);
             uint16_t *out = a.ctx + row * a.ctx_stride + (uint64_t)(kvh * w.group + h0) * DIM;
             if (part == 0)
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
             ++row;
             continue;
         }
-        const uint32_t item = SHARED ? blockIdx.x / w.parts % w.items : (u - base) / R.steps, rem = u - base - item * R.steps;
+        const uint32_t item = SHARED ? item0 : (u - base) / R.steps, rem = u - base - item * R.steps;
         const int cnt = (int)min(R.steps - rem, u_end - u);
         const uint32_t kvh = item / w.hb, hblk = item % w.hb;
         if constexpr (!DIRECT) load_q(row, item);
@@ -977,11 +984,15 @@ static bool pd_fits(uint32_t parts, uint32_t units) {
 }
 
 template <bool KV8, int DIM, int NW>
-static int launch_rows(const PagedAttnArgs &a, const PdWork &w, uint32_t units, cudaStream_t st) {
+static int launch_rows(const PagedAttnArgs &a, const PdWork &w, uint32_t units, uint32_t sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM, NW>;
     auto *kernel = paged_decode_kernel<KV8, DIM, true, true, NW>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
-    return launch_pdl(kernel, dim3(units), dim3(C::THREADS), C::SMEM, st, 1, a, w);
+    // Blocks start as SMs come free of the tile kernel: without a limit the first ones would take as many as they hold
+    // and the others none. Shared memory that nothing uses keeps it at an even share.
+    const uint32_t share = (units + sms - 1) / sms, fair = (PD_SM_BYTES / (share ? share : 1) - PD_STATIC_BYTES) & ~15u;
+    const uint32_t smem = fair > C::SMEM ? fair : C::SMEM;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
+    return launch_pdl(kernel, dim3(units), dim3(C::THREADS), smem, st, 1, a, w);
 }
 
 template <bool KV8, int DIM, bool SHARED = false>
@@ -999,11 +1010,11 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
         most = most < seen ? most : seen;
     }
     if constexpr (SHARED) {
-        // Many rows with little of their own: one or two warps an item, so that an SM has many items' chains of length,
+        // Many rows with little of their own: two warps an item, so that an SM has many items' chains of length,
         // page and key in flight.
         if (units >= 2 * (uint32_t)sms) {
             w.parts = 1;
-            return units >= 5 * (uint32_t)sms ? launch_rows<KV8, DIM, 1>(a, w, units, st) : launch_rows<KV8, DIM, 2>(a, w, units, st);
+            return launch_rows<KV8, DIM, 2>(a, w, units, sms, st);
         }
     }
     const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;

@@ -1,6 +1,7 @@
 // Attention of one token per sequence where groups of sequences share their
 // first tokens: the shared keys by tiles of query rows (paged_prefill.cu), then
-// each row's own keys joined with those (paged_decode.cu).
+// each row's own keys joined with those (paged_decode.cu). A group that is not
+// worth the tiles has each row read its whole context, shared pages from L2.
 //
 // Mathematics, per (row, query head), P the group's prefix, over keys j < len:
 //   x_j = log2(e) scale q.k_j,  p_j = 2^(x_j - m),  ctx = sum p_j v_j / sum p_j
@@ -30,9 +31,13 @@ int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     p += paged_shared_pieces_bytes(a.dim);
     parts.ml = reinterpret_cast<float *>(p);
     parts.o = reinterpret_cast<float *>(p + up256(heads * 8));
+    // The host knows no prefix, but no call can be worth the tile kernel that is too small with the widest table.
+    const uint64_t most = (uint64_t)a.c.max_pages << a.c.tshift;
+    const bool tiles = (unsigned __int128)a.rows * most * a.c.hkv * a.dim >= SHARED_WORK;
     PdlChain chain;
-    if (int rc = launch_shared_tiles(a, parts, (unsigned *)ws, st)) return rc;
-    return launch_shared_rows(a, parts, true, st);
+    if (tiles)
+        if (int rc = launch_shared_tiles(a, parts, (unsigned *)ws, st)) return rc;
+    return launch_shared_rows(a, parts, tiles, st);
 }
 
 }  // namespace qb

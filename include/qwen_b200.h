@@ -603,10 +603,10 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * starts[g] .. starts[g + 1] - 1 of q (one token each, of sequences seqs[r] as in
  * qwen_b200_op_paged_decode) are group g, whose sequences hold the same keys and
  * values in their first prefix[g] tokens, in shared pages or in copies. Those
- * are read from the pages of the group's first row; a prefix longer than that
- * sequence is cut to it, so a group whose first row is no sequence shares
- * nothing. Tokens from prefix[g] on are each sequence's own. A sequence may be
- * shorter than the prefix. There is no window: under one, a shared prefix soon
+ * are read from the pages of the group's first row (in groups too small for that to
+ * pay, from each sequence's own); a prefix longer than that sequence is cut to
+ * it, so a group whose first row is no sequence shares nothing. Tokens from
+ * prefix[g] on are each sequence's own. A sequence may be shorter than the prefix. There is no window: under one, a shared prefix soon
  * lies behind it, and qwen_b200_op_paged_decode reads no more than the window.
  * n groups (1 .. 65536, empty ones allowed), rows <= 65536. starts is [n + 1]
  * on the device, not decreasing; rows in front of starts[0] and at or behind

@@ -8,7 +8,7 @@ import pytest
 
 import qwen_b200
 from gpu_util import Keep, dev, host, stream, sync, torch_cuda, vp
-from paged_ref import Cache, bf16, bits, ref, unbits
+from paged_ref import BF16_HALF, U, Cache, bf16, bits, ref, unbits
 from qwen_b200 import _lib
 from test_gpu_paged import DIMS, FILL, FORMATS, PREFILL_W, assert_within, padded, u32, workspace
 
@@ -21,23 +21,26 @@ def shared_cache(seed, fmt, dim, page, groups, kv_heads=2, layers=1, copies=Fals
     """groups: [(tokens shared, lengths of the group's sequences)]. Full shared pages are one page in every table (or,
     with copies, pages of their own with the same contents); the page that a prefix ends in is always a copy."""
     lens = [t for _, members in groups for t in members]
-    pages = sum(-(-t // page) for t in lens) + 3
-    c = Cache(seed, fmt, kv_heads, dim, page, pages, len(lens), max(1, -(-max(lens) // page)) + 1, layers, **more).give(lens)
-    at = 0
-    for prefix, members in groups:
-        first = at
-        for i in range(at, at + len(members)):
-            n = min(prefix, lens[i], lens[first])
-            if i == first or not n:
-                continue
-            for a in [c.k, c.v] + ([c.ks, c.vs] if fmt == KV8 else []):
-                for j in range(-(-n // page)):
-                    t = min(page, n - j * page)
-                    a[:, c.table[i, j], :, :t] = a[:, c.table[first, j], :, :t]
-            if not copies:
-                for j in range(n // page):
-                    c.table[i, j] = c.table[first, j]
-        at += len(members)
+    agree = [min(prefix, t, members[0]) for prefix, members in groups for t in members]  # tokens that a sequence has of the first
+    first = [sum(len(m) for _, m in groups[:g]) for g, (_, members) in enumerate(groups) for _ in members]
+    own = [0 if copies or first[i] == i else agree[i] // page for i in range(len(lens))]  # pages that are the first's
+    c = Cache(seed, fmt, kv_heads, dim, page, sum(-(-t // page) for t in lens) - sum(own) + 3, len(lens),
+              max(1, -(-max(lens) // page)) + 1, layers, **more)
+    ids = iter(c.r.permutation(c.pages))
+    c.lengths[:] = lens
+    for i, t in enumerate(lens):
+        c.table[i, :own[i]] = c.table[first[i], :own[i]]
+        held = [next(ids) for _ in range(own[i], -(-t // page))]
+        c.table[i, own[i]:own[i] + len(held)] = held
+        c.refs[c.table[i, :-(-t // page)]] += 1
+        n = agree[i] if first[i] != i else 0
+        for a in [c.k, c.v] + ([c.ks, c.vs] if fmt == KV8 else []):
+            for j in range(own[i], -(-n // page)):
+                m = min(page, n - j * page)
+                a[:, c.table[i, j], :, :m] = a[:, c.table[first[i], j], :, :m]
+        for layer in range(layers):
+            if t > n:
+                c.write(layer, i, np.arange(n, t), c.rand(t - n, kv_heads, dim), c.rand(t - n, kv_heads, dim))
     return c
 
 
@@ -58,11 +61,42 @@ def shared(c, kv, keep, q, starts, prefix, seqs=None, scale=None, layer=0, extra
     return got[:, :heads * dim].reshape(q.shape)
 
 
+def attention(c, layer, q, seqs, scale):
+    """Cache.attention without a window, with weights rounded as in prompts: the same values and the same bound (which
+    its docstring derives), by matrix products of a row's heads."""
+    rows, heads, dim = q.shape
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for r in range(rows):
+        s = seqs[r]
+        t = np.arange(int(c.lengths[s])) if s < c.seqs else np.arange(0)
+        t = t[c.at(s, t)[0] < c.pages] if t.size else t
+        if not t.size:
+            continue
+        k, v = (x.transpose(1, 0, 2) for x in c.read(layer, s, t))  # [kv head][key][dim]
+        p = q[r].astype(np.float64).reshape(c.hkv, -1, dim)
+        x = p @ k.transpose(0, 2, 1) * scale
+        mag = (np.abs(p) @ np.abs(k).transpose(0, 2, 1) * abs(scale)).max(2)
+        w = np.exp(x - x.max(2, keepdims=True))
+        w /= w.sum(2, keepdims=True)
+        y = w @ v
+        size = w @ np.abs(v) + np.abs(y)
+        e = (PREFILL_W + 2 * (dim + 4) * U * mag + 2.0 ** -21 + 2 * t.size * U)[..., None]
+        out[r] = y.reshape(heads, dim)
+        tol[r] = (BF16_HALF * (np.abs(y) + e * size) + e * size).reshape(heads, dim)
+    return out, tol
+
+
+def test_the_bound_is_that_of_the_cache():
+    c = shared_cache(1, KV8, 64, 16, [(60, [70, 65, 0])])
+    q = bf16(c.rand(3, 4, 64))
+    for a, b in zip(attention(c, 0, q, np.arange(3), 0.3), c.attention(0, q, np.arange(3), [69, 64, -1], 0, 0, 0.3, PREFILL_W)):
+        assert np.allclose(a, b, rtol=1e-12, atol=1e-300)
+
+
 def check(c, kv, keep, q, starts, prefix, seqs=None, scale=None, layer=0, extra=0):
     got = shared(c, kv, keep, q, starts, prefix, seqs, scale, layer, extra)
     s = np.arange(len(q)) if seqs is None else np.asarray(seqs, np.int64)
-    pos = [int(c.lengths[i]) - 1 if i < c.seqs else -1 for i in s]
-    exact, tol = c.attention(layer, q, s, pos, 0, 0, q.shape[2] ** -0.5 if scale is None else scale, PREFILL_W)
+    exact, tol = attention(c, layer, q, s, q.shape[2] ** -0.5 if scale is None else scale)
     a, b = min(starts[0], len(q)), min(starts[-1], len(q))
     if a < b:
         assert_within(got[a:b], exact[a:b], tol[a:b])
@@ -328,7 +362,7 @@ def test_samples_of_one_prompt(fmt):
     """A prompt forked into samples that each go on with tokens of their own: fork, reserve, rotated append, shared
     attention, sampling, step after step, against the host cache."""
     from sample_ref import check as check_token
-    from test_gpu_rotary import append, make_table, rotation, turned  # noqa: F401
+    from test_gpu_paged_rotary import append, make_table, rotation, turned  # noqa: F401
     heads, hkv, dim, T, samples, prompt = 6, 2, 64, 16, 5, 75
     c = Cache(30, fmt, hkv, dim, T, 40, samples + 1, 10, 1).give([prompt] + [0] * samples)
     keep, table = Keep(), make_table(200, dim)
@@ -375,3 +409,186 @@ def test_samples_of_one_prompt(fmt):
         sync()
         for i in range(samples):
             check_token(int(host(tokens)[i]), host(probs)[i], logits[i], u[i], 0.8, 50, 0.95)
+
+
+# ---------------------------------------------------------------- groups large enough for tiles of query rows
+# (rows * shared keys * KV heads * dims of 2^25 and more)
+BIG = pytest.mark.parametrize('dim,rows,prefix', [(64, 130, 520), (128, 100, 333)])
+
+
+def big(seed, fmt, dim, rows, prefix, page=64, kv_heads=8, group=2, own=40, **more):
+    assert rows * prefix * kv_heads * dim >= 1 << 25
+    r = np.random.default_rng(seed)
+    return [(prefix, [prefix + int(x) for x in r.integers(0, own, rows)])], dict(kv_heads=kv_heads, group=group, **more)
+
+
+@FORMATS
+@BIG
+@pytest.mark.parametrize('page', [16, 64, 256])
+@pytest.mark.parametrize('copies', [False, True])
+def test_tiles_pages(fmt, dim, rows, prefix, page, copies):
+    groups, more = big(page, fmt, dim, rows, prefix, copies=copies)
+    run(page, fmt, dim, page, groups, **more)
+
+
+@FORMATS
+@DIMS
+@pytest.mark.parametrize('prefix', [513, 575, 576, 577, 639, 640, 641, 767, 768, 1024])
+def test_tiles_prefix_edges(fmt, dim, prefix):
+    groups, more = big(prefix, fmt, dim, 128, prefix)
+    run(prefix, fmt, dim, 32, groups, **more)
+
+
+@FORMATS
+@pytest.mark.parametrize('dim,kv_heads,group,rows,prefix', [
+    (64, 1, 1, 520, 1024), (64, 2, 7, 256, 1030), (64, 8, 1, 300, 260), (128, 4, 3, 171, 400), (128, 2, 8, 129, 1100),
+    (128, 1, 17, 260, 1025), (64, 3, 9, 400, 450), (128, 1, 70, 257, 1100), (64, 32, 5, 60, 300)])
+def test_tiles_head_layouts(fmt, dim, kv_heads, group, rows, prefix):
+    """Tiles that end inside a row's heads, at them, and rows over several tiles."""
+    groups, more = big(rows, fmt, dim, rows, prefix, kv_heads=kv_heads, group=group)
+    run(rows, fmt, dim, 128, groups, **more)
+
+
+@FORMATS
+@BIG
+def test_tiles_many_groups(fmt, dim, rows, prefix):
+    """Groups with and without tiles between one another, one of them empty, rows of no group around them."""
+    r = np.random.default_rng(dim)
+    sizes = [(0, 3), (prefix, rows), (prefix, 5), (prefix + 200, rows + 31), (90, 8), (2 * prefix, rows // 2 + 1), (0, 2)]
+    groups = [(p, [p + int(x) for x in r.integers(1, 30, n)]) for p, n in sizes]
+    c = shared_cache(dim, fmt, dim, 32, groups, kv_heads=8)
+    keep = Keep()
+    kv = c.upload(keep)
+    q = bf16(c.rand(c.seqs, 16, dim) * 2)
+    starts = np.cumsum([n for _, n in sizes])[:-1]
+    prefixes = [p for p, _ in sizes[1:-1]]
+    # an empty group in the middle, with a prefix of its own
+    starts, prefixes = np.insert(starts, 2, starts[2]), prefixes[:2] + [777] + prefixes[2:]
+    check(c, kv, keep, q, starts, prefixes, extra=16)
+
+
+@FORMATS
+@BIG
+def test_tiles_short_rows_no_sequences_and_missing_pages(fmt, dim, rows, prefix):
+    """Rows that end inside the prefix, rows of no sequence, a prefix cut to its first sequence, pages that are not there."""
+    groups, more = big(3, fmt, dim, rows, prefix)
+    lens = groups[0][1]
+    lens[0] = prefix + 9
+    lens[1:8] = [1, 0, 63, 64, 65, prefix - 1, 127]
+    c = shared_cache(4, fmt, dim, 32, groups, kv_heads=8)
+    seqs = np.arange(rows)
+    seqs[[9, 50]] = NO_SEQ
+    c.table[:, 3] = c.pages + 1
+    c.table[20, prefix // 32 + 1:] = c.pages
+    keep = Keep()
+    kv = c.upload(keep)
+    q = bf16(c.rand(rows, 16, dim) * 2)
+    got = check(c, kv, keep, q, [0, rows], [prefix], seqs)
+    assert not got[[2, 9, 50]].any() and got[1].any()
+    c.table[:] = c.pages
+    keep2 = Keep()
+    kv = c.upload(keep2)
+    assert not shared(c, kv, keep2, q, [0, rows], [prefix]).any()
+
+
+@FORMATS
+@BIG
+def test_tiles_a_prefix_longer_than_the_first_sequence(fmt, dim, rows, prefix):
+    """It is cut to the first sequence, in whose tokens the others agree; what they hold behind it is their own."""
+    groups, more = big(31, fmt, dim, rows, prefix)
+    groups[0][1][0] = prefix
+    c = shared_cache(31, fmt, dim, 32, [(prefix, groups[0][1])], kv_heads=8)
+    keep = Keep()
+    kv = c.upload(keep)
+    q = bf16(c.rand(rows, 16, dim) * 2)
+    for claim in (prefix + 1, 2 * prefix, 0xffffffff):
+        check(c, kv, keep, q, [0, rows], [claim])
+
+
+@FORMATS
+@BIG
+@pytest.mark.parametrize('scale', [-0.2, 0.0, 1e-30, 4.0])
+def test_tiles_scales(fmt, dim, rows, prefix, scale):
+    groups, more = big(9, fmt, dim, rows, prefix)
+    c = shared_cache(9, fmt, dim, 64, groups, kv_heads=8)
+    keep = Keep()
+    kv = c.upload(keep)
+    check(c, kv, keep, bf16(c.rand(rows, 16, dim)), [0, rows], [prefix], scale=scale)
+
+
+@FORMATS
+@BIG
+@pytest.mark.parametrize('where', ['prefix', 'own'])
+def test_tiles_one_key_outweighs_the_rest(fmt, dim, rows, prefix, where):
+    groups, more = big(12, fmt, dim, rows, prefix, own=2)
+    groups[0][1][:] = [prefix + 1 + i % 3 for i in range(rows)]
+    c = shared_cache(12, fmt, dim, 64, groups, kv_heads=8)
+    q = bf16(np.repeat(c.rand(1, 16, dim), rows, 0) * (1 + np.arange(rows) % 3)[:, None, None])
+    k = bf16(q[0].reshape(8, 2, dim)[:, 0][None] * 8)
+    for s in range(rows):
+        if where == 'own' or s == 0 or prefix % 64 > 0 and prefix - 5 >= prefix // 64 * 64:
+            c.write(0, s, [prefix - 5 if where == 'prefix' else prefix], k, bf16(np.ones((1, 8, dim)) * 3))
+    keep = Keep()
+    kv = c.upload(keep)
+    check(c, kv, keep, q, [0, rows], [prefix], scale=4.0)
+
+
+@FORMATS
+@DIMS
+def test_tiles_of_values_that_nobody_sees(fmt, dim):
+    """What the pages hold behind the prefix of the first sequence and behind each length does not matter (NaN there)."""
+    groups = [(577, [577] + [577 + i % 7 for i in range(127)])]
+    run(17, fmt, dim, 256, groups, kv_heads=8, group=1)
+
+
+def test_tiles_give_the_same_bits_again_and_with_two_streams():
+    torch = torch_cuda()
+    jobs, keep = [], Keep()
+    for fmt in (KV8, BF16):
+        groups, _ = big(21, fmt, 64, 300, 600)
+        c = shared_cache(21, fmt, 64, 64, groups, kv_heads=8)
+        kv = c.upload(keep)
+        q = bf16(c.rand(300, 16, 64) * 2)
+        first = check(c, kv, keep, q, [0, 300], [600])
+        ws = dev(np.zeros(L().qwen_b200_paged_decode_shared_workspace(ref(kv), 16, 1, 300), np.uint8))
+        jobs.append((kv, dev(bits(q).view(np.int16)), dev(np.zeros((300, 1024), np.int16)), ws, torch.cuda.Stream(), first, c))
+    starts, prefix = dev(u32([0, 300])), dev(u32([600]))
+    sync()
+    for _ in range(10):
+        for kv, qd, out, ws, st, _, _ in jobs:
+            assert L().qwen_b200_op_paged_decode_shared(ref(kv), 0, vp(qd), 1024, 16, 1, vp(starts), vp(prefix), 300, None, 0.125,
+                                                        vp(out), 1024, vp(ws), ws.numel(), ctypes.c_void_p(st.cuda_stream)) == 0
+    sync()
+    for kv, qd, out, ws, st, first, _ in jobs:
+        assert np.array_equal(host(out).view(np.uint16).reshape(first.shape), bits(first))
+        assert not host(ws)[:4].any()  # no wait ran out
+
+
+def test_tiles_captured_and_replayed_as_the_prefix_changes():
+    """A graph of the call answers for groups that are worth tiles and for those that are not."""
+    torch = torch_cuda()
+    groups, _ = big(22, KV8, 128, 100, 400)
+    c = shared_cache(22, KV8, 128, 64, groups, kv_heads=8)
+    keep = Keep()
+    kv = c.upload(keep)
+    q = bf16(c.rand(100, 16, 128) * 2)
+    qd, out = dev(bits(q).view(np.int16)), dev(np.zeros((100, 2048), np.int16))
+    starts, prefix = dev(u32([0, 100])), dev(u32([400]))
+    ws = dev(np.zeros(L().qwen_b200_paged_decode_shared_workspace(ref(kv), 16, 1, 100), np.uint8))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def call():
+        assert L().qwen_b200_op_paged_decode_shared(ref(kv), 0, vp(qd), 2048, 16, 1, vp(starts), vp(prefix), 100, None, 0.088,
+                                                    vp(out), 2048, vp(ws), ws.numel(), ctypes.c_void_p(side.cuda_stream)) == 0
+    call()
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    exact, tol = attention(c, 0, q, np.arange(100), 0.088)
+    for p in (400, 20, 399, 0, 350):
+        prefix.copy_(torch.from_numpy(u32([p])))
+        out.zero_()
+        sync()
+        graph.replay()
+        sync()
+        assert_within(unbits(host(out)).reshape(q.shape), exact, tol, str(p))
