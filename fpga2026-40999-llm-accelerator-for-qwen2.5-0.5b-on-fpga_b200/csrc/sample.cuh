@@ -4,7 +4,7 @@
 
 namespace qb {
 
-constexpr uint32_t SM_MAX_VOCAB = 8 * 8191 * 8 - 8;  // 8 CTAs of 65528 elements, less the row's misalignment
+constexpr uint32_t SM_MAX_VOCAB = 524216;
 
 struct SampleArgs {
     const uint16_t *logits;
@@ -14,8 +14,8 @@ struct SampleArgs {
     const uint32_t *top_k;
     uint32_t *tokens;
     float *probs;
-    uint32_t ctas, part;  // CTAs of a row; 16-byte groups that each counts
-    int unit;             // weights are whole multiples of 2^-unit
+    uint32_t part;  // 16-byte groups that each CTA of a row counts
+    int unit;       // weights are whole multiples of 2^-unit
 };
 int launch_sample(SampleArgs a, int sms, cudaStream_t st);
 
