@@ -21,8 +21,9 @@
 // 65536 values instead, counted anew at each step (about ten times slower).
 //
 // A cluster of C CTAs has a row: each counts a part of it, then takes 8192 / C
-// values, adds the CTAs' counts over distributed shared memory and scans;
-// borders are exchanged by the CTA that finds them.
+// values, adds the CTAs' counts over distributed shared memory, forms the weights
+// and sums them by warps of 512 / C values; the warp in which a border lies
+// finds it and tells the others.
 #include "kernels.h"
 #include "qwen_b200.h"
 #include "sample.cuh"
@@ -34,20 +35,22 @@ constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_MAX_CTAS = 8;
 constexpr uint32_t SM_BINS = 8192, SM_WINDOWS = 65536 / SM_BINS;
 // The usual window: magnitudes from SM_LOW on (as bf16 bits), SM_SIDE of them on each side of 0.
 constexpr uint32_t SM_LOW = 0x3400, SM_SIDE = 31 * 128;
+constexpr int SM_BATCH = 4;                // 16-byte loads of a thread in flight
+constexpr uint32_t SM_NONE = 0xff80ff80u;  // two logits of -infinity
 
 // What a cluster's CTAs tell one another; written by their peers.
 struct SmShared {
-    uint32_t first[SM_MAX_CTAS];            // lowest order (largest logit) of each CTA's part
-    uint32_t below[SM_MAX_CTAS];            // the same of its values below the usual window
-    uint32_t odd[SM_MAX_CTAS];              // whether it has values that the window's two sides do not hold
-    uint32_t count[SM_MAX_CTAS];            // candidates of its values
-    unsigned long long sum[SM_MAX_CTAS];    // and their weights
-    unsigned long long kept[SM_MAX_CTAS];   // weights up to its last kept candidate
-    unsigned long long top_k;               // weights of the k first
-    uint32_t bin, nth;                      // the token: nth occurrence of a value
-    uint32_t found;                         // in this window + 1
+    uint32_t first[SM_MAX_CTAS];           // lowest order (largest logit) of each CTA's part
+    uint32_t below[SM_MAX_CTAS];           // the same of its values below the usual window
+    uint32_t odd[SM_MAX_CTAS];             // whether it has values that the window's two sides do not hold
+    uint32_t count[SM_MAX_CTAS];           // candidates of its values
+    unsigned long long sum[SM_MAX_CTAS];   // their weights
+    unsigned long long high[SM_MAX_CTAS];  // and those of at least min_p
+    unsigned long long top_k, top_p;       // weights of the k first, and of those that top_p leaves
+    uint32_t bin, nth;                     // the token: nth occurrence of a value
+    uint32_t found;                        // in this window
     uint32_t wcount[SM_WARPS], wbelow[SM_WARPS], wodd;  // this CTA's own
-    unsigned long long wsum[SM_WARPS];
+    unsigned long long wsum[SM_WARPS], whigh[SM_WARPS];
 };
 
 __device__ __forceinline__ uint32_t sm_rank() {
@@ -65,11 +68,6 @@ __device__ __forceinline__ void sm_put32(void *p, uint32_t rank, uint32_t v) {
 }
 __device__ __forceinline__ void sm_put64(void *p, uint32_t rank, unsigned long long v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sm_remote(p, rank)), "l"(v) : "memory");
-}
-__device__ __forceinline__ uint2 sm_get64(const void *p, uint32_t rank) {
-    uint2 v;
-    asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(sm_remote(p, rank)) : "memory");
-    return v;
 }
 __device__ __forceinline__ uint32_t sm_get32(const void *p, uint32_t rank) {
     uint32_t v;
@@ -96,8 +94,8 @@ __device__ __forceinline__ bool sm_counts(uint32_t order) { return order >= 0x7f
 __device__ __forceinline__ int sm_bin(uint32_t b, uint32_t window) {
     const uint32_t mag = b & 0x7fffu;
     if (window == SM_WINDOWS) {
-        const uint32_t t = mag - SM_LOW;
-        if (t < SM_SIDE) return b & 0x8000u ? SM_SIDE + 1 + t : SM_SIDE - 1 - t;
+        const uint32_t t = mag - SM_LOW, negative = (uint32_t)((int)(b << 16) >> 31);
+        if (t < SM_SIDE) return (int)((t ^ ~negative) + SM_SIDE - negative);  // SM_SIDE - 1 - t, or SM_SIDE + 1 + t
         return mag == 0 ? (int)SM_SIDE : -1;
     }
     const uint32_t d = sm_order(b);
@@ -131,11 +129,42 @@ __device__ __forceinline__ uint32_t sm_half(const uint4 &v, int k) {
     return k & 1 ? w >> 16 : w & 0xffffu;
 }
 
+// Shared memory beside SmShared: the histogram, and of this CTA's values the counts of all CTAs and the weights.
 template <int C>
-__global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(SampleArgs a) {
-    constexpr int PER = SM_BINS / C / SM_THREADS;  // values of a thread
-    __shared__ __align__(16) uint32_t hist[SM_BINS];
+struct SmCfg {
+    static constexpr int SEG = SM_BINS / C, WS = SEG / SM_WARPS, STEPS = WS / 32;  // values of a CTA, of a warp
+    static constexpr int COUNTS = SM_BINS * 4, WEIGHTS = COUNTS + (C > 1 ? SEG * 4 : 0), BYTES = WEIGHTS + SEG * 8;
+};
+
+template <typename T>
+__device__ __forceinline__ T sm_warp_sum(T v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T sm_warp_scan(T v) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += y;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t sm_max2(uint32_t a, uint32_t b) {  // of two bf16 pairs; NaN counts as nothing
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+template <int C>
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
+    using K = SmCfg<C>;
+    extern __shared__ __align__(16) uint8_t smem[];
     __shared__ SmShared sh;
+    uint32_t *const hist = reinterpret_cast<uint32_t *>(smem);
+    uint32_t *const counts = reinterpret_cast<uint32_t *>(smem + (C > 1 ? K::COUNTS : 0));
+    unsigned long long *const weights = reinterpret_cast<unsigned long long *>(smem + K::WEIGHTS);
     const uint32_t rank = C > 1 ? sm_rank() : 0, row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + row * a.stride);
@@ -144,25 +173,43 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
     x.skew = (uint32_t)(at & 15) / 2;
     x.vocab = a.vocab;
     const uint32_t groups = (x.skew + a.vocab + 7) / 8, g0 = min(rank * a.part, groups), g1 = min(g0 + a.part, groups);
+    const float temperature = a.temperature ? a.temperature[row] : 1.f;
+    const bool greedy = !(temperature > 0.f);
+    const uint32_t k_of = a.top_k && !greedy ? a.top_k[row] : 0;
+    const float p = a.top_p && !greedy ? a.top_p[row] : 1.f, least = a.min_p && !greedy ? a.min_p[row] : 0.f, u = a.u[row];
 
     // ---- this CTA's part of the row, counted in the usual window
     auto clear = [&] {
         for (uint32_t i = tid; i < SM_BINS / 4; i += SM_THREADS) reinterpret_cast<uint4 *>(hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     };
+    // visit(16 bytes) for this CTA's part, SM_BATCH loads of a thread in flight
+    auto each_group = [&](auto &&visit) {
+        for (uint32_t g = g0 + tid; g < g1; g += SM_BATCH * SM_THREADS) {
+            uint4 v[SM_BATCH];
+#pragma unroll
+            for (int i = 0; i < SM_BATCH; ++i)
+                if (g + i * SM_THREADS < g1) v[i] = x.group(g + i * SM_THREADS);
+#pragma unroll
+            for (int i = 0; i < SM_BATCH; ++i)
+                if (g + i * SM_THREADS < g1) visit(v[i]);
+        }
+    };
     if (tid == 0) sh.wodd = 0, sh.found = 0;
     clear();
-    uint32_t first = 0xffffu, below = 0xffffu;
+    uint32_t top2 = SM_NONE, below = 0xffffu;
     bool odd = false;
-    for (uint32_t g = g0 + tid; g < g1; g += SM_THREADS) {
-        const uint4 v = x.group(g);
+    each_group([&](uint4 v) {
+        top2 = sm_max2(sm_max2(top2, sm_max2(v.x, v.y)), sm_max2(v.z, v.w));
+        const bool same = v.x == v.y && v.z == v.w && v.x == v.z && v.x >> 16 == (v.x & 0xffffu);
+        const uint32_t add = same ? 8 : 1;  // (a row of one value would add to one counter 32 times a warp)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
+            if (k > 0 && same) break;
             const uint32_t b = sm_half(v, k);
             const int bin = sm_bin(b, SM_WINDOWS);
             if (bin >= 0) {
-                atomicAdd(&hist[bin], 1);
-                first = min(first, (uint32_t)bin);
+                atomicAdd(&hist[bin], add);
             } else {
                 const uint32_t d = sm_order(b);
                 if (sm_counts(d)) {
@@ -170,13 +217,9 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
                 }
             }
         }
-    }
-    // (as orders: a bin of the window lies between 0x7fff - (SM_LOW + SM_SIDE - 1) and the values below it)
-    if (first != 0xffffu) {
-        const float v = sm_bin_value(first, SM_WINDOWS);
-        first = sm_order(__float_as_uint(v) >> 16);
-    }
-    first = __reduce_min_sync(0xffffffffu, min(first, below));
+    });
+    uint32_t first = min(sm_order(top2 & 0xffffu), sm_order(top2 >> 16));  // (-infinity: no candidate)
+    first = __reduce_min_sync(0xffffffffu, first);
     below = __reduce_min_sync(0xffffffffu, below);
     if (lane == 0) sh.wcount[warp] = first, sh.wbelow[warp] = below;
     if (odd) sh.wodd = 1;
@@ -192,90 +235,102 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
     }
     sm_sync<C>();
     first = below = 0xffffu;
+    odd = false;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         first = min(first, sh.first[c]);
         below = min(below, sh.below[c]);
-        odd = c == 0 ? sh.odd[0] != 0 : odd || sh.odd[c] != 0;
+        odd = odd || sh.odd[c] != 0;
     }
-
-    const float temperature = a.temperature ? a.temperature[row] : 1.f;
-    const bool greedy = !(temperature > 0.f);
-    const double T = temperature, unit = ldexp(1.0, a.unit);  // weights are whole numbers of 1 / unit
-    double top = 0.0;
-    auto weight_of = [&](double l) { return l == top ? 1.0 : greedy ? 0.0 : exp((l - top) / T); };
-    auto whole = [&](double w) { return (unsigned long long)__double2ull_rn(w * unit); };
-    uint32_t window = SM_WINDOWS;
-    if (odd) {  // the largest may be one of those: from its order, counted in the first windows
-        window = 0;
-    } else if (first == 0xffffu) {  // no candidate
+    if (!sm_counts(first)) {  // no candidate
         if (rank == 0 && tid == 0) {
             a.tokens[row] = QWEN_B200_NO_TOKEN;
             if (a.probs) a.probs[row] = 0.f;
         }
         return;  // (no CTA reads another's memory any more)
-    } else {
-        top = sm_value(first);
-        if (below != 0xffffu && whole(weight_of(sm_value(below)))) window = 0;
     }
-    const bool usual = window == SM_WINDOWS;
+    const double top = sm_value(first), T = temperature, unit = ldexp(1.0, a.unit);  // weights are whole numbers of 1 / unit
+    auto weight = [&](double l) {
+        return __double2ull_rn((l == top ? 1.0 : greedy ? 0.0 : exp((l - top) / T)) * unit);
+    };
+    const bool usual = !odd && (below == 0xffffu || weight(sm_value(below)) == 0);
+    // the least weight that min_p leaves (NaN: none)
+    const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;
 
-    // ---- the counts and weights of a window's values, PER neighbours a thread, and what is before them
-    uint32_t n[PER], cb = 0, cnt = 0, cw = 0;              // before; of the thread; of the window
-    unsigned long long w[PER], sb = 0, sum = 0, sw = 0;
-    const uint32_t bin0 = rank * (SM_BINS / C) + tid * PER;
+    // ---- a window's counts and weights; cb and sb: candidates and weights before this warp's values, cnt and sum of them,
+    // cw, sw and hw of the window (hw: of at least `floor`)
+    uint32_t window = SM_WINDOWS, cb = 0, cnt = 0, cw = 0;
+    unsigned long long sb = 0, sum = 0, sw = 0, hw = 0;
     auto scan = [&](uint32_t c_before, unsigned long long s_before) {
         cnt = 0, sum = 0;
+        unsigned long long high = 0;
+        uint32_t n[K::STEPS];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) n[j] = 0;
+        for (int i = 0; i < K::STEPS; ++i) {
+            const uint32_t at = warp * K::WS + 32 * i + lane;
+            n[i] = 0;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int j = 0; j < PER; j += 2) {
-                const uint2 v = C > 1 ? sm_get64(&hist[bin0 + j], c) : *reinterpret_cast<uint2 *>(&hist[bin0 + j]);
-                n[j] += v.x;
-                n[j + 1] += v.y;
-            }
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            w[j] = 0;
-            if (n[j]) {
-                w[j] = whole(weight_of(sm_bin_value(bin0 + j, window)));
-                cnt += n[j];
-                sum += n[j] * w[j];
-            }
+            for (int c = 0; c < C; ++c) n[i] += C > 1 ? sm_get32(&hist[rank * K::SEG + at], c) : hist[at];
+            if (C > 1) counts[at] = n[i];
         }
-        uint32_t ic = cnt;
-        unsigned long long is = sum;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t yc = __shfl_up_sync(0xffffffffu, ic, o);
-            const unsigned long long ys = __shfl_up_sync(0xffffffffu, is, o);
-            if (lane >= o) ic += yc, is += ys;
+        for (int i = 0; i < K::STEPS; ++i) {
+            const uint32_t at = warp * K::WS + 32 * i + lane;
+            if (!__any_sync(0xffffffffu, n[i])) continue;
+            const unsigned long long w = n[i] ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
+            weights[at] = w;
+            cnt += n[i];
+            sum += n[i] * w;
+            high += w >= floor ? n[i] * w : 0;
         }
-        if (lane == 31) sh.wcount[warp] = ic, sh.wsum[warp] = is;
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        sum = sm_warp_sum(sum);
+        high = sm_warp_sum(high);
+        if (lane == 0) sh.wcount[warp] = cnt, sh.wsum[warp] = sum, sh.whigh[warp] = high;
         __syncthreads();
         uint32_t call = 0;
-        unsigned long long sall = 0;
-        cb = c_before + ic - cnt, sb = s_before + is - sum;
+        unsigned long long sall = 0, hall = 0;
+        cb = c_before, sb = s_before;
 #pragma unroll
         for (int i = 0; i < SM_WARPS; ++i) {
             const uint32_t y = sh.wcount[i];
             const unsigned long long z = sh.wsum[i];
             if (i < warp) cb += y, sb += z;
-            call += y, sall += z;
+            call += y, sall += z, hall += sh.whigh[i];
         }
         if (tid < C) {
             sm_put32(&sh.count[rank], tid, call);
             sm_put64(&sh.sum[rank], tid, sall);
+            sm_put64(&sh.high[rank], tid, hall);
         }
         sm_sync<C>();
-        cw = 0, sw = 0;
+        cw = 0, sw = 0, hw = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (c < (int)rank) cb += sh.count[c], sb += sh.sum[c];
             cw += sh.count[c];
             sw += sh.sum[c];
+            hw += sh.high[c];
+        }
+    };
+    // The first value of this warp at which `there`(candidates, weights up to its end) holds: tell(its place in the CTA's
+    // values, its count and weight, weights and candidates before it) by one lane. All lanes of one warp call it.
+    auto find = [&](auto &&there, auto &&tell) {
+        uint32_t c = cb;
+        unsigned long long s = sb;
+        for (int i = 0; i < K::STEPS; ++i) {
+            const uint32_t at = warp * K::WS + 32 * i + lane, n = counts[at];
+            if (!__any_sync(0xffffffffu, n)) continue;
+            const unsigned long long w = n ? weights[at] : 0;
+            const uint32_t ic = sm_warp_scan(n);
+            const unsigned long long is = sm_warp_scan(n * w);
+            const uint32_t hit = __ballot_sync(0xffffffffu, n && there(c + ic, s + is));
+            if (hit) {
+                if (lane == __ffs(hit) - 1) tell(at, n, w, s + is - n * w, c + ic - n);
+                return;
+            }
+            c += __shfl_sync(0xffffffffu, ic, 31);
+            s += __shfl_sync(0xffffffffu, is, 31);
         }
     };
     // Moves on to a window (the usual one is there already).
@@ -283,17 +338,17 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
         window = to;
         sm_sync<C>();  // nobody reads the counts any more
         clear();
-        for (uint32_t g = g0 + tid; g < g1; g += SM_THREADS) {
-            const uint4 v = x.group(g);
+        each_group([&](uint4 v) {
 #pragma unroll 1
             for (int k = 0; k < 8; ++k) {
                 const int bin = sm_bin(sm_half(v, k), to);
                 if (bin >= 0) atomicAdd(&hist[bin], 1);
             }
-        }
+        });
         sm_sync<C>();
     };
     // Every value in falling order: visit() behind each window's scan, until it says so.
+    if (usual) scan(0, 0);
     auto sweep = [&](auto &&visit) {
         if (usual) {
             visit();
@@ -308,124 +363,59 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
             c += cw, s += sw;
         }
     };
-    if (usual) {
-        scan(0, 0);
-    } else {
-        // the largest logit: the first value of the first window that has one
-        first = 0xffffu;
-        for (uint32_t i = 0; i < SM_WINDOWS && first == 0xffffu; ++i) {
-            count_window(i);
-            uint32_t f = 0xffffu;
-            for (uint32_t j = tid; j < SM_BINS; j += SM_THREADS)
-                for (int c = 0; c < C; ++c)
-                    if (sm_get32(&hist[j], c)) f = min(f, i * SM_BINS + j);
-            f = __reduce_min_sync(0xffffffffu, f);
-            if (lane == 0) sh.wcount[warp] = f;
-            __syncthreads();
-            for (int k = 0; k < SM_WARPS; ++k) first = min(first, sh.wcount[k]);
-            __syncthreads();
-        }
-        top = sm_value(first);
-    }
 
-    // ---- the weights of the k first
-    const uint32_t k_of = a.top_k && !greedy ? a.top_k[row] : 0;
+    // ---- the weights of the k first, and of those with a weight of at least min_p
     uint32_t total = 0;
-    unsigned long long mass = 0;
+    unsigned long long mass = 0, high = 0;
     sweep([&] {
-        if (k_of && cb < k_of && k_of <= cb + cnt) {
-            uint32_t left = k_of - cb;
-            unsigned long long s = sb;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const uint32_t m = min(n[j], left);
-                s += m * w[j];
-                left -= m;
-            }
-            for (int c = 0; c < C; ++c) sm_put64(&sh.top_k, c, s);
-        }
-        total += cw;
-        mass += sw;
+        if (k_of && cb < k_of && k_of <= cb + cnt)
+            find([&](uint32_t c, unsigned long long) { return c >= k_of; },
+                 [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t c) {
+                     for (int i = 0; i < C; ++i) sm_put64(&sh.top_k, i, s + (k_of - c) * w);
+                 });
+        total += cw, mass += sw, high += hw;
         return false;
     });
-    const uint32_t k_first = k_of ? min(k_of, total) : total;
-    if (k_first < total) {
+    if (k_of && k_of < total) {
         sm_sync<C>();
         mass = sh.top_k;
     }
-    // ---- the kept candidates: the first one, and those of the k first with less than top_p before them and min_p themselves
-    const float p = a.top_p && !greedy ? a.top_p[row] : 1.f, least = a.min_p && !greedy ? a.min_p[row] : 0.f;
-    const bool cut = !(p >= 1.f), floor = !(least <= 0.f);
-    const unsigned long long share = cut ? __double2ull_ru(fmax((double)p, 0.0) * (double)mass) : 0;
-    auto keep = [&](int j, uint32_t i, unsigned long long s) {  // of value j, whose first candidate is the i-th, with s before it
-        uint32_t m = i < k_first ? min(n[j], k_first - i) : 0;
-        if (cut && m) {
-            if (s >= share)
-                m = 0;
-            else if (w[j])
-                m = (uint32_t)min((unsigned long long)m, (share - s + w[j] - 1) / w[j]);
+    // ---- the kept candidates: of the k first, those with less than top_p of their weights before them, and min_p themselves.
+    // Each leaves a prefix of the order, so the least sum is the shortest one's; the first candidate stays.
+    unsigned long long kept = min(mass, high);
+    if (!(p >= 1.f)) {
+        const unsigned long long share = __double2ull_ru(fmax((double)p, 0.0) * (double)mass);  // (at most mass)
+        if (share) {
+            sweep([&] {
+                if (sb < share && share <= sb + sum)
+                    find([&](uint32_t, unsigned long long s) { return s >= share; },
+                         [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t) {
+                             for (int i = 0; i < C; ++i) sm_put64(&sh.top_p, i, s + (share - s + w - 1) / w * w);
+                         });
+                return false;
+            });
+            sm_sync<C>();
+            kept = min(kept, sh.top_p);
+        } else {
+            kept = 0;
         }
-        if (floor && m && !(weight_of(sm_bin_value(bin0 + j, window)) >= (double)least)) m = 0;
-        return i == 0 && n[j] ? max(m, 1u) : m;
-    };
-    unsigned long long kept = mass;
-    if (cut || floor) {
-        kept = 0;
-        sweep([&] {
-            if (cnt) {
-                uint32_t i = cb;
-                unsigned long long s = sb;
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const uint32_t m = keep(j, i, s);
-                    if (m) kept = s + m * w[j];
-                    i += n[j];
-                    s += n[j] * w[j];
-                }
-            }
-            return false;
-        });
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long y = __shfl_xor_sync(0xffffffffu, kept, o);
-            kept = max(kept, y);
-        }
-        __syncthreads();
-        if (lane == 0) sh.wsum[warp] = kept;
-        __syncthreads();
-        if (tid < C) {
-            for (int i = 0; i < SM_WARPS; ++i) kept = max(kept, sh.wsum[i]);
-            sm_put64(&sh.kept[rank], tid, kept);
-        }
-        sm_sync<C>();
-        kept = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c) kept = max(kept, sh.kept[c]);
     }
+    kept = max(kept, (unsigned long long)unit);
 
     // ---- the token's value, and which of its occurrences
-    const float u = fminf(fmaxf(a.u[row], 0.f), 0x1.fffffep-1f);  // (NaN: 0)
-    const unsigned long long target = greedy ? 0 : (unsigned long long)((double)u * (double)kept);
+    const unsigned long long target = greedy ? 0 : (unsigned long long)((double)fminf(fmaxf(u, 0.f), 0x1.fffffep-1f) * (double)kept);  // (NaN: 0)
     sweep([&] {
-        if (cnt && sb <= target && target < sb + sum) {
-            uint32_t i = cb;
-            unsigned long long s = sb;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (target >= s && target < s + n[j] * w[j]) {
-                    const uint32_t nth = greedy ? n[j] - 1 : (uint32_t)((target - s) / w[j]);
-                    for (int c = 0; c < C; ++c) {
-                        sm_put32(&sh.bin, c, bin0 + j);
-                        sm_put32(&sh.nth, c, nth);
-                        sm_put32(&sh.found, c, 1);
-                    }
-                    if (a.probs)
-                        a.probs[row] = greedy ? 1.f : (float)(weight_of(sm_bin_value(bin0 + j, window)) * unit / (double)kept);
-                }
-                i += n[j];
-                s += n[j] * w[j];
-            }
-        }
+        if (sb <= target && target < sb + sum)
+            find([&](uint32_t, unsigned long long s) { return s > target; },
+                 [&](uint32_t at, uint32_t n, unsigned long long w, unsigned long long s, uint32_t) {
+                     const uint32_t nth = greedy ? n - 1 : (uint32_t)((target - s) / w);
+                     for (int i = 0; i < C; ++i) {
+                         sm_put32(&sh.bin, i, rank * K::SEG + at);
+                         sm_put32(&sh.nth, i, nth);
+                         sm_put32(&sh.found, i, 1);
+                     }
+                     if (a.probs) a.probs[row] = greedy ? 1.f : (float)((double)w / (double)kept);
+                 });
         sm_sync<C>();
         return sh.found != 0;
     });
@@ -442,60 +432,72 @@ __global__ void __launch_bounds__(SM_THREADS, C > 2 ? 2 : 1) sample_kernel(Sampl
         }
         nth -= here;
     }
-    if (mine) {
-        const uint32_t per_warp = (g1 - g0 + SM_WARPS - 1) / SM_WARPS, w0 = min(g0 + warp * per_warp, g1), w1 = min(w0 + per_warp, g1);
-        auto matches = [&](uint32_t g) {
-            uint32_t bits = 0;
-            if (g < w1) {
-                const uint4 v = x.group(g);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) bits |= (uint32_t)(sm_bin(sm_half(v, k), window) == (int)bin) << k;
-            }
-            return bits;
-        };
-        uint32_t m = 0;
-        for (uint32_t g = w0; g < w1; g += 32) m += __popc(matches(g + lane));
-        m = __reduce_add_sync(0xffffffffu, m);
-        if (lane == 0) sh.wcount[warp] = m;
-        __syncthreads();  // (the whole CTA is here)
-        for (int i = 0; i < warp; ++i) {
-            const uint32_t y = sh.wcount[i];
-            nth = nth < y ? 0xffffffffu : nth - y;  // an earlier warp has it
-            if (nth == 0xffffffffu) break;
-        }
-        if (nth < sh.wcount[warp])
-            for (uint32_t g = w0; g < w1; g += 32) {
-                const uint32_t bits = matches(g + lane), y = __popc(bits);
-                uint32_t incl = y;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t z = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += z;
-                }
-                if (nth >= incl - y && nth < incl)
-                    a.tokens[row] = 8 * (g + lane) + __fns(bits, 0, nth - (incl - y) + 1) - x.skew;
-                const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
-                if (nth < all) break;
-                nth -= all;
-            }
-    }
     if constexpr (C > 1) tc::cluster_sync();  // no CTA ends while its counters are read
+    if (!mine) return;
+    const uint32_t per_warp = (g1 - g0 + SM_WARPS - 1) / SM_WARPS, w0 = min(g0 + warp * per_warp, g1), w1 = min(w0 + per_warp, g1);
+    // bit k of byte i: whether element k of group g + 32 i + lane is one, SM_BATCH groups at a time
+    auto matches = [&](uint32_t g) {
+        uint4 v[SM_BATCH];
+#pragma unroll
+        for (int i = 0; i < SM_BATCH; ++i)
+            v[i] = g + 32 * i + lane < w1 ? x.group(g + 32 * i + lane) : make_uint4(SM_NONE, SM_NONE, SM_NONE, SM_NONE);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < SM_BATCH; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) bits |= (uint32_t)(sm_bin(sm_half(v[i], k), window) == (int)bin) << (8 * i + k);
+        return bits;
+    };
+    uint32_t m = 0;
+    for (uint32_t g = w0; g < w1; g += 32 * SM_BATCH) m += __popc(matches(g));
+    m = __reduce_add_sync(0xffffffffu, m);
+    if (lane == 0) sh.wcount[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) {
+        const uint32_t y = sh.wcount[i];
+        if (nth < y) return;  // an earlier warp has it
+        nth -= y;
+    }
+    if (nth >= m) return;
+    for (uint32_t g = w0;; g += 32 * SM_BATCH) {  // (it is there)
+        const uint32_t bits = matches(g);
+        const uint32_t all = __reduce_add_sync(0xffffffffu, __popc(bits));
+        if (nth >= all) {
+            nth -= all;
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < SM_BATCH; ++i) {
+            const uint32_t mine8 = bits >> (8 * i) & 0xffu, y = __popc(mine8);
+            uint32_t incl = y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t z = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += z;
+            }
+            if (nth >= incl - y && nth < incl)
+                a.tokens[row] = 8 * (g + 32 * i + lane) + __fns(mine8, 0, nth - (incl - y) + 1) - x.skew;
+            const uint32_t some = __shfl_sync(0xffffffffu, incl, 31);
+            if (nth < some) return;
+            nth -= some;
+        }
+    }
 }
 
 template <int C>
 static int launch_sample_ctas(SampleArgs a, uint32_t groups, cudaStream_t st) {
     a.part = (groups + C - 1) / C;
-    return launch_pdl(sample_kernel<C>, dim3(a.rows * C), dim3(SM_THREADS), 0, st, C, a);
+    if (cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmCfg<C>::BYTES) != cudaSuccess) return -3;
+    return launch_pdl(sample_kernel<C>, dim3(a.rows * C), dim3(SM_THREADS), SmCfg<C>::BYTES, st, C, a);
 }
 
 int launch_sample(SampleArgs a, int sms, cudaStream_t st) {
     const uint32_t groups = (a.vocab + 7 + 7) / 8;
     a.unit = __builtin_clz(a.vocab) + 31;  // 63 - bits of the vocabulary: the sums stay below 2^63
-    const uint32_t want = (2 * (uint32_t)sms + a.rows - 1) / a.rows, most = (groups + 511) / 512;
-    const uint32_t ctas = want < most ? want : most;
-    if (ctas >= 8) return launch_sample_ctas<8>(a, groups, st);
-    if (ctas >= 3 || (a.vocab > 32768 && most >= 4)) return launch_sample_ctas<4>(a, groups, st);
-    if (ctas == 2) return launch_sample_ctas<2>(a, groups, st);
+    const uint32_t slots = 2 * (uint32_t)sms, most = (groups + 511) / 512;  // (a CTA has work for its threads)
+    if (a.rows * 8 <= slots && most >= 8) return launch_sample_ctas<8>(a, groups, st);
+    if (a.rows * 4 <= slots && most >= 4) return launch_sample_ctas<4>(a, groups, st);
+    if (a.rows * 2 <= slots && most >= 2) return launch_sample_ctas<2>(a, groups, st);
     return launch_sample_ctas<1>(a, groups, st);
 }
 
