@@ -14,16 +14,17 @@
 // 2^-(63 - bits of the vocabulary), summed as 64-bit integers: exact in any
 // order, so the answer does not depend on the launch.
 //
-// The histogram has a window of 8192 values in shared memory. One window holds
-// 0 and every magnitude in [2^-23, 2^8), which is all of a row in practice: what
+// The histogram has a window of 12288 values in shared memory. One window holds
+// 0 and every magnitude in [2^-39, 2^8), which is all of a row in practice: what
 // lies below it (masks such as -1e4 or the lowest value) has no weight and is left
-// out. A row for which that does not hold goes through 8 windows of 8192 of the
+// out. A row for which that does not hold goes through 6 windows of 12288 of the
 // 65536 values instead, counted anew at each step (about ten times slower).
 //
-// A cluster of C CTAs has a row: each counts a part of it, then takes 8192 / C
-// values, adds the CTAs' counts over distributed shared memory, forms the weights
-// and sums them by warps of 512 / C values; the warp in which a border lies
-// finds it and tells the others.
+// A cluster of C CTAs has a row: each counts a part of it, then takes 12288 / C
+// values, 32 a step: a warp adds the CTAs' counts of a step over distributed
+// shared memory, forms the weights and sums them; a thread has the sums of a step,
+// and the one in whose step a border lies finds it with its warp and tells the
+// others.
 #include "kernels.h"
 #include "qwen_b200.h"
 #include "sample.cuh"
@@ -32,9 +33,9 @@
 namespace qb {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_MAX_CTAS = 8;
-constexpr uint32_t SM_BINS = 8192, SM_WINDOWS = 65536 / SM_BINS;
+constexpr uint32_t SM_BINS = 12288, SM_WINDOWS = (65536 + SM_BINS - 1) / SM_BINS;
 // The usual window: magnitudes from SM_LOW on (as bf16 bits), SM_SIDE of them on each side of 0.
-constexpr uint32_t SM_LOW = 0x3400, SM_SIDE = 31 * 128;
+constexpr uint32_t SM_LOW = 0x2c00, SM_SIDE = 47 * 128;
 constexpr int SM_BATCH = 4;                // 16-byte loads of a thread in flight
 constexpr uint32_t SM_NONE = 0xff80ff80u;  // two logits of -infinity
 
@@ -129,11 +130,13 @@ __device__ __forceinline__ uint32_t sm_half(const uint4 &v, int k) {
     return k & 1 ? w >> 16 : w & 0xffffu;
 }
 
-// Shared memory beside SmShared: the histogram, and of this CTA's values the counts of all CTAs and the weights.
+// Shared memory beside SmShared: the histogram, of this CTA's values the counts of all CTAs, and of its steps the weights,
+// those of at least min_p, and the counts.
 template <int C>
 struct SmCfg {
-    static constexpr int SEG = SM_BINS / C, WS = SEG / SM_WARPS, STEPS = WS / 32;  // values of a CTA, of a warp
-    static constexpr int COUNTS = SM_BINS * 4, WEIGHTS = COUNTS + (C > 1 ? SEG * 4 : 0), BYTES = WEIGHTS + SEG * 8;
+    static constexpr int SEG = SM_BINS / C, STEPS = SEG / 32;  // values and steps of a CTA
+    static constexpr int COUNTS = SM_BINS * 4, SUMS = COUNTS + (C > 1 ? SEG * 4 : 0), BYTES = SUMS + STEPS * 20;
+    static_assert(STEPS % SM_WARPS == 0 && STEPS <= SM_THREADS, "steps");
 };
 
 template <typename T>
@@ -164,7 +167,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     __shared__ SmShared sh;
     uint32_t *const hist = reinterpret_cast<uint32_t *>(smem);
     uint32_t *const counts = reinterpret_cast<uint32_t *>(smem + (C > 1 ? K::COUNTS : 0));
-    unsigned long long *const weights = reinterpret_cast<unsigned long long *>(smem + K::WEIGHTS);
+    unsigned long long *const step_sum = reinterpret_cast<unsigned long long *>(smem + K::SUMS), *const step_high = step_sum + K::STEPS;
+    uint32_t *const step_count = reinterpret_cast<uint32_t *>(step_high + K::STEPS);
     const uint32_t rank = C > 1 ? sm_rank() : 0, row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + row * a.stride);
@@ -185,11 +189,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     };
     // visit(16 bytes) for this CTA's part, SM_BATCH loads of a thread in flight
     auto each_group = [&](auto &&visit) {
-        for (uint32_t g = g0 + tid; g < g1; g += SM_BATCH * SM_THREADS) {
-            uint4 v[SM_BATCH];
+        uint4 v[SM_BATCH], next[SM_BATCH];
+        auto load = [&](uint32_t g) {
 #pragma unroll
             for (int i = 0; i < SM_BATCH; ++i)
-                if (g + i * SM_THREADS < g1) v[i] = x.group(g + i * SM_THREADS);
+                if (g + i * SM_THREADS < g1) next[i] = x.group(g + i * SM_THREADS);
+        };
+        load(g0 + tid);
+        for (uint32_t g = g0 + tid; g < g1; g += SM_BATCH * SM_THREADS) {
+#pragma unroll
+            for (int i = 0; i < SM_BATCH; ++i) v[i] = next[i];
+            load(g + SM_BATCH * SM_THREADS);
 #pragma unroll
             for (int i = 0; i < SM_BATCH; ++i)
                 if (g + i * SM_THREADS < g1) visit(v[i]);
@@ -199,22 +209,31 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     clear();
     uint32_t top2 = SM_NONE, below = 0xffffu;
     bool odd = false;
+    const uint32_t bins = tc::smem_u32(hist);
     each_group([&](uint4 v) {
         top2 = sm_max2(sm_max2(top2, sm_max2(v.x, v.y)), sm_max2(v.z, v.w));
-        const bool same = v.x == v.y && v.z == v.w && v.x == v.z && v.x >> 16 == (v.x & 0xffffu);
-        const uint32_t add = same ? 8 : 1;  // (a row of one value would add to one counter 32 times a warp)
+        const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+        bool outside = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (k > 0 && same) break;
-            const uint32_t b = sm_half(v, k);
-            const int bin = sm_bin(b, SM_WINDOWS);
-            if (bin >= 0) {
-                atomicAdd(&hist[bin], add);
-            } else {
-                const uint32_t d = sm_order(b);
-                if (sm_counts(d)) {
-                    if (d > 0x8000u + SM_LOW) below = min(below, d); else odd = true;
-                }
+            const uint32_t w = w4[k >> 1], mag4 = (k & 1 ? w >> 14 : w << 2) & 0x1fffcu;  // 4 times the magnitude's bits
+            uint32_t negative;  // all ones, or 0
+            asm("prmt.b32 %0, %1, 0, %2;" : "=r"(negative) : "r"(w), "r"(k & 1 ? 0xbbbbu : 0x9999u));
+            // the address of sm_bin's counter: bins + 4 (SM_SIDE - 1 - t), or + 4 (SM_SIDE + 1 + t), t the bits above SM_LOW
+            constexpr uint32_t POS = 4 * (SM_SIDE - 1 + SM_LOW) + 1, NEG = 4 * (SM_SIDE + 1) - 4 * SM_LOW;
+            const uint32_t to = (mag4 ^ ~negative) + (negative & (NEG - POS)) + (bins + POS);
+            if (mag4 - 4 * SM_LOW < 4 * SM_SIDE)
+                asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(to) : "memory");
+            else
+                outside = true;
+        }
+        if (outside) {
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t b = sm_half(v, k), d = sm_order(b);
+                const int bin = sm_bin(b, SM_WINDOWS);
+                if (bin == (int)SM_SIDE) atomicAdd(&hist[bin], 1);
+                if (bin >= 0 || !sm_counts(d)) continue;
+                if (d > 0x8000u + SM_LOW) below = min(below, d); else odd = true;
             }
         }
     });
@@ -257,46 +276,54 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     // the least weight that min_p leaves (NaN: none)
     const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;
 
-    // ---- a window's counts and weights; cb and sb: candidates and weights before this warp's values, cnt and sum of them,
+    // ---- a window's counts and weights; cb and sb: candidates and weights before this thread's step, cnt and sum of it,
     // cw, sw and hw of the window (hw: of at least `floor`)
     uint32_t window = SM_WINDOWS, cb = 0, cnt = 0, cw = 0;
     unsigned long long sb = 0, sum = 0, sw = 0, hw = 0;
     auto scan = [&](uint32_t c_before, unsigned long long s_before) {
-        cnt = 0, sum = 0;
-        unsigned long long high = 0;
-        uint32_t n[K::STEPS];
+        constexpr int MINE = K::STEPS / SM_WARPS;  // steps of a warp, in turn: the values that occur are neighbours
+        uint32_t n[MINE];
 #pragma unroll
-        for (int i = 0; i < K::STEPS; ++i) {
-            const uint32_t at = warp * K::WS + 32 * i + lane;
+        for (int i = 0; i < MINE; ++i) {
+            const uint32_t at = 32 * (SM_WARPS * i + warp) + lane;
             n[i] = 0;
 #pragma unroll
             for (int c = 0; c < C; ++c) n[i] += C > 1 ? sm_get32(&hist[rank * K::SEG + at], c) : hist[at];
             if (C > 1) counts[at] = n[i];
         }
-#pragma unroll
-        for (int i = 0; i < K::STEPS; ++i) {
-            const uint32_t at = warp * K::WS + 32 * i + lane;
-            if (!__any_sync(0xffffffffu, n[i])) continue;
-            const unsigned long long w = n[i] ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
-            weights[at] = w;
-            cnt += n[i];
-            sum += n[i] * w;
-            high += w >= floor ? n[i] * w : 0;
+#pragma unroll 4
+        for (int i = 0; i < MINE; ++i) {
+            const uint32_t step = SM_WARPS * i + warp, c = __reduce_add_sync(0xffffffffu, n[i]);
+            unsigned long long s = 0, h = 0;
+            if (c) {
+                const unsigned long long w = n[i] ? weight(sm_bin_value(rank * K::SEG + 32 * step + lane, window)) : 0;
+                s = sm_warp_sum(n[i] * w);
+                h = floor == 0 ? s : sm_warp_sum(w >= floor ? n[i] * w : 0ull);
+            }
+            if (lane == 0) step_count[step] = c, step_sum[step] = s, step_high[step] = h;
         }
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        sum = sm_warp_sum(sum);
+        __syncthreads();
+        unsigned long long high = 0;
+        cnt = 0, sum = 0;
+        if (tid < K::STEPS) cnt = step_count[tid], sum = step_sum[tid], high = step_high[tid];
+        const uint32_t ic = sm_warp_scan(cnt);
+        const unsigned long long is = sm_warp_scan(sum);
         high = sm_warp_sum(high);
-        if (lane == 0) sh.wcount[warp] = cnt, sh.wsum[warp] = sum, sh.whigh[warp] = high;
+        if (lane == 31) sh.wcount[warp] = ic, sh.wsum[warp] = is, sh.whigh[warp] = high;
         __syncthreads();
         uint32_t call = 0;
         unsigned long long sall = 0, hall = 0;
-        cb = c_before, sb = s_before;
+        cb = c_before + ic - cnt, sb = s_before + is - sum;
 #pragma unroll
         for (int i = 0; i < SM_WARPS; ++i) {
             const uint32_t y = sh.wcount[i];
             const unsigned long long z = sh.wsum[i];
             if (i < warp) cb += y, sb += z;
             call += y, sall += z, hall += sh.whigh[i];
+        }
+        if (C == 1) {
+            cw = call, sw = sall, hw = hall;
+            return;
         }
         if (tid < C) {
             sm_put32(&sh.count[rank], tid, call);
@@ -313,25 +340,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
             hw += sh.high[c];
         }
     };
-    // The first value of this warp at which `there`(candidates, weights up to its end) holds: tell(its place in the CTA's
-    // values, its count and weight, weights and candidates before it) by one lane. All lanes of one warp call it.
-    auto find = [&](auto &&there, auto &&tell) {
-        uint32_t c = cb;
-        unsigned long long s = sb;
-        for (int i = 0; i < K::STEPS; ++i) {
-            const uint32_t at = warp * K::WS + 32 * i + lane, n = counts[at];
-            if (!__any_sync(0xffffffffu, n)) continue;
-            const unsigned long long w = n ? weights[at] : 0;
-            const uint32_t ic = sm_warp_scan(n);
-            const unsigned long long is = sm_warp_scan(n * w);
-            const uint32_t hit = __ballot_sync(0xffffffffu, n && there(c + ic, s + is));
-            if (hit) {
-                if (lane == __ffs(hit) - 1) tell(at, n, w, s + is - n * w, c + ic - n);
-                return;
-            }
-            c += __shfl_sync(0xffffffffu, ic, 31);
-            s += __shfl_sync(0xffffffffu, is, 31);
-        }
+    // Where `here` holds for one thread of the cluster (a border lies in its step): the first value at which
+    // `there`(candidates, weights up to its end) holds; tell(its bin, its count and weight, weights and candidates before
+    // it) by one lane. Whole warps call it.
+    auto find = [&](bool here, auto &&there, auto &&tell) {
+        const uint32_t owner = __ballot_sync(0xffffffffu, here);
+        if (!owner) return;
+        const int l = __ffs(owner) - 1;
+        const uint32_t at = 32 * (32 * warp + l) + lane, c = __shfl_sync(0xffffffffu, cb, l), n = counts[at];
+        const unsigned long long s = __shfl_sync(0xffffffffu, sb, l), w = n ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
+        const uint32_t ic = sm_warp_scan(n);
+        const unsigned long long is = sm_warp_scan(n * w);
+        const uint32_t hit = __ballot_sync(0xffffffffu, n && there(c + ic, s + is));
+        if (lane == __ffs(hit) - 1) tell(rank * K::SEG + at, n, w, s + is - n * w, c + ic - n);
     };
     // Moves on to a window (the usual one is there already).
     auto count_window = [&](uint32_t to) {
@@ -368,8 +389,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     uint32_t total = 0;
     unsigned long long mass = 0, high = 0;
     sweep([&] {
-        if (k_of && cb < k_of && k_of <= cb + cnt)
-            find([&](uint32_t c, unsigned long long) { return c >= k_of; },
+        if (k_of)
+            find(cb < k_of && k_of <= cb + cnt, [&](uint32_t c, unsigned long long) { return c >= k_of; },
                  [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t c) {
                      for (int i = 0; i < C; ++i) sm_put64(&sh.top_k, i, s + (k_of - c) * w);
                  });
@@ -387,11 +408,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         const unsigned long long share = __double2ull_ru(fmax((double)p, 0.0) * (double)mass);  // (at most mass)
         if (share) {
             sweep([&] {
-                if (sb < share && share <= sb + sum)
-                    find([&](uint32_t, unsigned long long s) { return s >= share; },
-                         [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t) {
-                             for (int i = 0; i < C; ++i) sm_put64(&sh.top_p, i, s + (share - s + w - 1) / w * w);
-                         });
+                find(sb < share && share <= sb + sum, [&](uint32_t, unsigned long long s) { return s >= share; },
+                     [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t) {
+                         for (int i = 0; i < C; ++i) sm_put64(&sh.top_p, i, s + (share - s + w - 1) / w * w);
+                     });
                 return false;
             });
             sm_sync<C>();
@@ -405,17 +425,16 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     // ---- the token's value, and which of its occurrences
     const unsigned long long target = greedy ? 0 : (unsigned long long)((double)fminf(fmaxf(u, 0.f), 0x1.fffffep-1f) * (double)kept);  // (NaN: 0)
     sweep([&] {
-        if (sb <= target && target < sb + sum)
-            find([&](uint32_t, unsigned long long s) { return s > target; },
-                 [&](uint32_t at, uint32_t n, unsigned long long w, unsigned long long s, uint32_t) {
-                     const uint32_t nth = greedy ? n - 1 : (uint32_t)((target - s) / w);
-                     for (int i = 0; i < C; ++i) {
-                         sm_put32(&sh.bin, i, rank * K::SEG + at);
-                         sm_put32(&sh.nth, i, nth);
-                         sm_put32(&sh.found, i, 1);
-                     }
-                     if (a.probs) a.probs[row] = greedy ? 1.f : (float)((double)w / (double)kept);
-                 });
+        find(sb <= target && target < sb + sum, [&](uint32_t, unsigned long long s) { return s > target; },
+             [&](uint32_t bin, uint32_t n, unsigned long long w, unsigned long long s, uint32_t) {
+                 const uint32_t nth = greedy ? n - 1 : (uint32_t)((target - s) / w);
+                 for (int i = 0; i < C; ++i) {
+                     sm_put32(&sh.bin, i, bin);
+                     sm_put32(&sh.nth, i, nth);
+                     sm_put32(&sh.found, i, 1);
+                 }
+                 if (a.probs) a.probs[row] = greedy ? 1.f : (float)((double)w / (double)kept);
+             });
         sm_sync<C>();
         return sh.found != 0;
     });
@@ -434,53 +453,49 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     }
     if constexpr (C > 1) tc::cluster_sync();  // no CTA ends while its counters are read
     if (!mine) return;
-    const uint32_t per_warp = (g1 - g0 + SM_WARPS - 1) / SM_WARPS, w0 = min(g0 + warp * per_warp, g1), w1 = min(w0 + per_warp, g1);
-    // bit k of byte i: whether element k of group g + 32 i + lane is one, SM_BATCH groups at a time
-    auto matches = [&](uint32_t g) {
-        uint4 v[SM_BATCH];
-#pragma unroll
-        for (int i = 0; i < SM_BATCH; ++i)
-            v[i] = g + 32 * i + lane < w1 ? x.group(g + 32 * i + lane) : make_uint4(SM_NONE, SM_NONE, SM_NONE, SM_NONE);
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < SM_BATCH; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) bits |= (uint32_t)(sm_bin(sm_half(v[i], k), window) == (int)bin) << (8 * i + k);
-        return bits;
+    // A half of w that equals the value's bits (those of 0 with either sign) is 0 in y, and the sum's top bit stays clear for it.
+    const uint32_t code = __float_as_uint(sm_bin_value(bin, window)) >> 16, twice = code * 0x10001u, care = code ? 0xffffffffu : 0x7fff7fffu;
+    auto equal2 = [&](uint32_t w) {  // bits 15 and 31
+        const uint32_t y = (w & care) ^ twice;
+        return ~(((y & 0x7fff7fffu) + 0x7fff7fffu) | y) & 0x80008000u;
     };
-    uint32_t m = 0;
-    for (uint32_t g = w0; g < w1; g += 32 * SM_BATCH) m += __popc(matches(g));
-    m = __reduce_add_sync(0xffffffffu, m);
-    if (lane == 0) sh.wcount[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < warp; ++i) {
-        const uint32_t y = sh.wcount[i];
-        if (nth < y) return;  // an earlier warp has it
-        nth -= y;
+    auto equal8 = [&](const uint4 &v) {  // element 2 k in bit 15 - k, 2 k + 1 in bit 31 - k
+        return equal2(v.x) | equal2(v.y) >> 1 | equal2(v.z) >> 2 | equal2(v.w) >> 3;
+    };
+    const uint4 nothing = make_uint4(~twice, ~twice, ~twice, ~twice);  // (0: 0xffff, not 0 with a sign either)
+    // the part that holds it in 16 runs, one a warp, until a run is one batch of a warp
+    uint32_t lo = g0, hi = g1;
+    while (hi - lo > 32 * SM_BATCH) {
+        const uint32_t run = (hi - lo + SM_WARPS - 1) / SM_WARPS, w0 = min(lo + warp * run, hi), w1 = min(w0 + run, hi);
+        uint32_t m = 0;
+        for (uint32_t g = w0 + lane; g < w1; g += 32 * SM_BATCH) {
+            uint4 v[SM_BATCH];
+#pragma unroll
+            for (int i = 0; i < SM_BATCH; ++i) v[i] = g + 32 * i < w1 ? x.group(g + 32 * i) : nothing;
+#pragma unroll
+            for (int i = 0; i < SM_BATCH; ++i) m += __popc(equal8(v[i]));
+        }
+        m = __reduce_add_sync(0xffffffffu, m);
+        __syncthreads();
+        if (lane == 0) sh.wcount[warp] = m;
+        __syncthreads();
+        int i = 0;
+        for (; i < SM_WARPS - 1 && nth >= sh.wcount[i]; ++i) nth -= sh.wcount[i];
+        lo = min(lo + i * run, hi);
+        hi = min(lo + run, hi);
     }
-    if (nth >= m) return;
-    for (uint32_t g = w0;; g += 32 * SM_BATCH) {  // (it is there)
-        const uint32_t bits = matches(g);
-        const uint32_t all = __reduce_add_sync(0xffffffffu, __popc(bits));
-        if (nth >= all) {
-            nth -= all;
-            continue;
+    if (warp != 0) return;
+    for (uint32_t g = lo; g < hi; g += 32) {
+        const uint32_t bits = g + lane < hi ? equal8(x.group(g + lane)) : 0, y = __popc(bits), incl = sm_warp_scan(y);
+        if (nth >= incl - y && nth < incl) {
+            uint32_t left = nth - (incl - y), e = 0;
+            for (;; ++e)  // elements in order
+                if (bits >> (e & 1 ? 31 - e / 2 : 15 - e / 2) & 1 && left-- == 0) break;
+            a.tokens[row] = 8 * (g + lane) + e - x.skew;
         }
-#pragma unroll
-        for (int i = 0; i < SM_BATCH; ++i) {
-            const uint32_t mine8 = bits >> (8 * i) & 0xffu, y = __popc(mine8);
-            uint32_t incl = y;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t z = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += z;
-            }
-            if (nth >= incl - y && nth < incl)
-                a.tokens[row] = 8 * (g + 32 * i + lane) + __fns(mine8, 0, nth - (incl - y) + 1) - x.skew;
-            const uint32_t some = __shfl_sync(0xffffffffu, incl, 31);
-            if (nth < some) return;
-            nth -= some;
-        }
+        const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
+        if (nth < all) return;
+        nth -= all;
     }
 }
 
