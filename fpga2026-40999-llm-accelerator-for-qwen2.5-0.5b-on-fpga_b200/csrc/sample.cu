@@ -36,7 +36,7 @@ constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_MAX_CTAS = 8;
 constexpr uint32_t SM_BINS = 12288, SM_WINDOWS = (65536 + SM_BINS - 1) / SM_BINS;
 // The usual window: magnitudes from SM_LOW on (as bf16 bits), SM_SIDE of them on each side of 0.
 constexpr uint32_t SM_LOW = 0x2c00, SM_SIDE = 47 * 128;
-constexpr int SM_BATCH = 4;                // 16-byte loads of a thread in flight
+constexpr int SM_BATCH = 2, SM_LOOK = 8;   // 16-byte loads of a thread in flight: counting, and at the last look
 constexpr uint32_t SM_NONE = 0xff80ff80u;  // two logits of -infinity
 
 // What a cluster's CTAs tell one another; written by their peers.
@@ -102,6 +102,11 @@ __device__ __forceinline__ int sm_bin(uint32_t b, uint32_t window) {
     const uint32_t d = sm_order(b);
     return sm_counts(d) && d / SM_BINS == window ? (int)(d % SM_BINS) : -1;
 }
+// The counter of a bin: in the usual window magnitudes rise on both sides, so that counting needs a sign and a sum.
+__device__ __forceinline__ uint32_t sm_place(uint32_t bin, uint32_t window) {
+    if (window != SM_WINDOWS || bin > 2 * SM_SIDE) return bin;
+    return bin < SM_SIDE ? SM_SIDE - 1 - bin : bin == SM_SIDE ? 2 * SM_SIDE : bin - 1;
+}
 __device__ __forceinline__ float sm_bin_value(uint32_t bin, uint32_t window) {
     if (window == SM_WINDOWS)
         return bf2f(bin < SM_SIDE ? SM_LOW + SM_SIDE - 1 - bin : bin == SM_SIDE ? 0u : 0x8000u | (SM_LOW + bin - SM_SIDE - 1));
@@ -109,20 +114,22 @@ __device__ __forceinline__ float sm_bin_value(uint32_t bin, uint32_t window) {
 }
 
 // The logits of a row in 16-byte groups by their addresses: group i has the elements 8 i - skew ..
+static __device__ __noinline__ uint4 sm_edge(const uint16_t *base, uint32_t at, uint32_t begin, uint32_t end) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t b = at + k >= begin && at + k < end ? base[at + k] : 0xff80u;  // -infinity
+        w[k >> 1] = k & 1 ? w[k >> 1] | b << 16 : b;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 struct SmRow {
     const uint16_t *base;  // the group that holds element 0
     uint32_t skew, vocab;
+    uint32_t whole0, whole;  // groups whole0 .. whole0 + whole - 1 lie inside the row
     __device__ __forceinline__ uint4 group(uint32_t i) const {
-        const uint32_t lo = 8 * i;
-        if (lo >= skew && lo + 8 <= skew + vocab) return *reinterpret_cast<const uint4 *>(base + lo);
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t e = lo + k;
-            const uint32_t b = e >= skew && e < skew + vocab ? base[e] : 0xff80u;  // -infinity
-            w[k >> 1] = k & 1 ? w[k >> 1] | b << 16 : b;
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        if (i - whole0 < whole) return *reinterpret_cast<const uint4 *>(base + 8 * i);
+        return sm_edge(base, 8 * i, skew, skew + vocab);
     }
 };
 __device__ __forceinline__ uint32_t sm_half(const uint4 &v, int k) {
@@ -154,6 +161,16 @@ __device__ __forceinline__ T sm_warp_scan(T v) {  // inclusive
     }
     return v;
 }
+// Of two bf16 pairs, all ones in the halves for which it holds.
+__device__ __forceinline__ uint32_t sm_ge2(uint32_t a, uint32_t b) {
+    return __hge2_mask(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+}
+__device__ __forceinline__ uint32_t sm_lt2(uint32_t a, uint32_t b) {
+    return __hlt2_mask(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+}
+__device__ __forceinline__ uint32_t sm_eq2(uint32_t a, uint32_t b) {
+    return __heq2_mask(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+}
 __device__ __forceinline__ uint32_t sm_max2(uint32_t a, uint32_t b) {  // of two bf16 pairs; NaN counts as nothing
     uint32_t d;
     asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -176,6 +193,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     x.base = reinterpret_cast<const uint16_t *>(at & ~(uintptr_t)15);
     x.skew = (uint32_t)(at & 15) / 2;
     x.vocab = a.vocab;
+    x.whole0 = x.skew ? 1 : 0;
+    x.whole = max((x.skew + a.vocab) / 8, x.whole0) - x.whole0;
     const uint32_t groups = (x.skew + a.vocab + 7) / 8, g0 = min(rank * a.part, groups), g1 = min(g0 + a.part, groups);
     const float temperature = a.temperature ? a.temperature[row] : 1.f;
     const bool greedy = !(temperature > 0.f);
@@ -189,20 +208,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     };
     // visit(16 bytes) for this CTA's part, SM_BATCH loads of a thread in flight
     auto each_group = [&](auto &&visit) {
-        uint4 v[SM_BATCH], next[SM_BATCH];
-        auto load = [&](uint32_t g) {
+        uint4 next[SM_BATCH];
 #pragma unroll
-            for (int i = 0; i < SM_BATCH; ++i)
-                if (g + i * SM_THREADS < g1) next[i] = x.group(g + i * SM_THREADS);
-        };
-        load(g0 + tid);
+        for (int i = 0; i < SM_BATCH; ++i)
+            if (g0 + tid + i * SM_THREADS < g1) next[i] = x.group(g0 + tid + i * SM_THREADS);
         for (uint32_t g = g0 + tid; g < g1; g += SM_BATCH * SM_THREADS) {
 #pragma unroll
-            for (int i = 0; i < SM_BATCH; ++i) v[i] = next[i];
-            load(g + SM_BATCH * SM_THREADS);
-#pragma unroll
-            for (int i = 0; i < SM_BATCH; ++i)
-                if (g + i * SM_THREADS < g1) visit(v[i]);
+            for (int i = 0; i < SM_BATCH; ++i) {
+                const uint4 v = next[i];
+                const uint32_t ahead = g + (SM_BATCH + i) * SM_THREADS;
+                if (ahead < g1) next[i] = x.group(ahead);
+                if (g + i * SM_THREADS < g1) visit(v);
+            }
         }
     };
     if (tid == 0) sh.wodd = 0, sh.found = 0;
@@ -211,29 +228,34 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     bool odd = false;
     const uint32_t bins = tc::smem_u32(hist);
     each_group([&](uint4 v) {
-        top2 = sm_max2(sm_max2(top2, sm_max2(v.x, v.y)), sm_max2(v.z, v.w));
         const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-        bool outside = false;
+        uint32_t inside = 0xffffffffu;  // halves whose value has a counter
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t w = w4[k >> 1], mag4 = (k & 1 ? w >> 14 : w << 2) & 0x1fffcu;  // 4 times the magnitude's bits
-            uint32_t negative;  // all ones, or 0
-            asm("prmt.b32 %0, %1, 0, %2;" : "=r"(negative) : "r"(w), "r"(k & 1 ? 0xbbbbu : 0x9999u));
-            // the address of sm_bin's counter: bins + 4 (SM_SIDE - 1 - t), or + 4 (SM_SIDE + 1 + t), t the bits above SM_LOW
-            constexpr uint32_t POS = 4 * (SM_SIDE - 1 + SM_LOW) + 1, NEG = 4 * (SM_SIDE + 1) - 4 * SM_LOW;
-            const uint32_t to = (mag4 ^ ~negative) + (negative & (NEG - POS)) + (bins + POS);
-            if (mag4 - 4 * SM_LOW < 4 * SM_SIDE)
-                asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(to) : "memory");
-            else
-                outside = true;
+        for (int k = 0; k < 4; ++k) {
+            top2 = sm_max2(top2, w4[k]);
+            const uint32_t mag = w4[k] & 0x7fff7fffu;
+            inside &= sm_ge2(mag, SM_LOW * 0x10001u) & sm_lt2(mag, (SM_LOW + SM_SIDE) * 0x10001u);
         }
-        if (outside) {
+        if (inside == 0xffffffffu) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                // bins + 4 t, or + 4 (SM_SIDE + t), t the magnitude's bits above SM_LOW
+                const uint32_t w = w4[k >> 1], mag4 = (k & 1 ? w >> 14 : w << 2) & 0x1fffcu;
+                uint32_t negative;  // all ones, or 0
+                asm("prmt.b32 %0, %1, 0, %2;" : "=r"(negative) : "r"(w), "r"(k & 1 ? 0xbbbbu : 0x9999u));
+                const uint32_t to = mag4 + (negative & (4 * SM_SIDE)) + (bins - 4 * SM_LOW);
+                asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(to) : "memory");
+            }
+        } else {
+#pragma unroll 1
             for (int k = 0; k < 8; ++k) {
                 const uint32_t b = sm_half(v, k), d = sm_order(b);
                 const int bin = sm_bin(b, SM_WINDOWS);
-                if (bin == (int)SM_SIDE) atomicAdd(&hist[bin], 1);
-                if (bin >= 0 || !sm_counts(d)) continue;
-                if (d > 0x8000u + SM_LOW) below = min(below, d); else odd = true;
+                if (bin >= 0)
+                    atomicAdd(&hist[sm_place(bin, SM_WINDOWS)], 1);
+                else if (sm_counts(d)) {
+                    if (d > 0x8000u + SM_LOW) below = min(below, d); else odd = true;
+                }
             }
         }
     });
@@ -268,9 +290,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         }
         return;  // (no CTA reads another's memory any more)
     }
-    const double top = sm_value(first), T = temperature, unit = ldexp(1.0, a.unit);  // weights are whole numbers of 1 / unit
+    // Weights are whole numbers of 1 / unit. 1 / T is rounded once: a weight is off by some 2^-52 of its exponent (at most
+    // 45 where it counts), less than half a unit, and each value is spared a division.
+    const double top = sm_value(first), slope = 1.0 / temperature, unit = ldexp(1.0, a.unit);
+    const bool sharp = greedy || isinf(top);  // only the largest counts
     auto weight = [&](double l) {
-        return __double2ull_rn((l == top ? 1.0 : greedy ? 0.0 : exp((l - top) / T)) * unit);
+        return __double2ull_rn((l == top ? 1.0 : sharp ? 0.0 : exp((l - top) * slope)) * unit);
     };
     const bool usual = !odd && (below == 0xffffu || weight(sm_value(below)) == 0);
     // the least weight that min_p leaves (NaN: none)
@@ -282,23 +307,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     unsigned long long sb = 0, sum = 0, sw = 0, hw = 0;
     auto scan = [&](uint32_t c_before, unsigned long long s_before) {
         constexpr int MINE = K::STEPS / SM_WARPS;  // steps of a warp, in turn: the values that occur are neighbours
-        uint32_t n[MINE];
-#pragma unroll
+#pragma unroll(MINE < 6 ? MINE : 6)
         for (int i = 0; i < MINE; ++i) {
-            const uint32_t at = 32 * (SM_WARPS * i + warp) + lane;
-            n[i] = 0;
+            const uint32_t step = SM_WARPS * i + warp, at = 32 * step + lane, place = sm_place(rank * K::SEG + at, window);
+            uint32_t n = 0;
 #pragma unroll
-            for (int c = 0; c < C; ++c) n[i] += C > 1 ? sm_get32(&hist[rank * K::SEG + at], c) : hist[at];
-            if (C > 1) counts[at] = n[i];
-        }
-#pragma unroll 4
-        for (int i = 0; i < MINE; ++i) {
-            const uint32_t step = SM_WARPS * i + warp, c = __reduce_add_sync(0xffffffffu, n[i]);
+            for (int c = 0; c < C; ++c) n += C > 1 ? sm_get32(&hist[place], c) : hist[place];
+            if (C > 1) counts[at] = n;
+            const uint32_t c = __reduce_add_sync(0xffffffffu, n);
             unsigned long long s = 0, h = 0;
             if (c) {
-                const unsigned long long w = n[i] ? weight(sm_bin_value(rank * K::SEG + 32 * step + lane, window)) : 0;
-                s = sm_warp_sum(n[i] * w);
-                h = floor == 0 ? s : sm_warp_sum(w >= floor ? n[i] * w : 0ull);
+                const unsigned long long w = n ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
+                s = sm_warp_sum(n * w);
+                h = floor == 0 ? s : sm_warp_sum(w >= floor ? n * w : 0ull);
             }
             if (lane == 0) step_count[step] = c, step_sum[step] = s, step_high[step] = h;
         }
@@ -347,7 +368,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         const uint32_t owner = __ballot_sync(0xffffffffu, here);
         if (!owner) return;
         const int l = __ffs(owner) - 1;
-        const uint32_t at = 32 * (32 * warp + l) + lane, c = __shfl_sync(0xffffffffu, cb, l), n = counts[at];
+        const uint32_t at = 32 * (32 * warp + l) + lane, c = __shfl_sync(0xffffffffu, cb, l);
+        const uint32_t n = C > 1 ? counts[at] : hist[sm_place(at, window)];
         const unsigned long long s = __shfl_sync(0xffffffffu, sb, l), w = n ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
         const uint32_t ic = sm_warp_scan(n);
         const unsigned long long is = sm_warp_scan(n * w);
@@ -363,7 +385,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
 #pragma unroll 1
             for (int k = 0; k < 8; ++k) {
                 const int bin = sm_bin(sm_half(v, k), to);
-                if (bin >= 0) atomicAdd(&hist[bin], 1);
+                if (bin >= 0) atomicAdd(&hist[bin], 1);  // (sm_place is itself there)
             }
         });
         sm_sync<C>();
@@ -444,7 +466,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     uint32_t nth = sh.nth;
     bool mine = false;
     for (int c = 0; c < C; ++c) {
-        const uint32_t here = sm_get32(&hist[bin], c);
+        const uint32_t here = sm_get32(&hist[sm_place(bin, window)], c);
         if (nth < here) {
             mine = c == (int)rank;
             break;
@@ -453,27 +475,23 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     }
     if constexpr (C > 1) tc::cluster_sync();  // no CTA ends while its counters are read
     if (!mine) return;
-    // A half of w that equals the value's bits (those of 0 with either sign) is 0 in y, and the sum's top bit stays clear for it.
-    const uint32_t code = __float_as_uint(sm_bin_value(bin, window)) >> 16, twice = code * 0x10001u, care = code ? 0xffffffffu : 0x7fff7fffu;
-    auto equal2 = [&](uint32_t w) {  // bits 15 and 31
-        const uint32_t y = (w & care) ^ twice;
-        return ~(((y & 0x7fff7fffu) + 0x7fff7fffu) | y) & 0x80008000u;
+    const uint32_t twice = (__float_as_uint(sm_bin_value(bin, window)) >> 16) * 0x10001u;
+    auto equal8 = [&](const uint4 &v) {  // element 2 k in bit k, 2 k + 1 in bit 16 + k
+        return (sm_eq2(v.x, twice) & 0x10001u) | (sm_eq2(v.y, twice) & 0x20002u) | (sm_eq2(v.z, twice) & 0x40004u) |
+               (sm_eq2(v.w, twice) & 0x80008u);
     };
-    auto equal8 = [&](const uint4 &v) {  // element 2 k in bit 15 - k, 2 k + 1 in bit 31 - k
-        return equal2(v.x) | equal2(v.y) >> 1 | equal2(v.z) >> 2 | equal2(v.w) >> 3;
-    };
-    const uint4 nothing = make_uint4(~twice, ~twice, ~twice, ~twice);  // (0: 0xffff, not 0 with a sign either)
-    // the part that holds it in 16 runs, one a warp, until a run is one batch of a warp
+    const uint4 nothing = make_uint4(SM_NONE, SM_NONE, SM_NONE, SM_NONE);
+    // the part that holds it in 16 runs, one a warp, until a run is short
     uint32_t lo = g0, hi = g1;
-    while (hi - lo > 32 * SM_BATCH) {
+    while (hi - lo > 128) {
         const uint32_t run = (hi - lo + SM_WARPS - 1) / SM_WARPS, w0 = min(lo + warp * run, hi), w1 = min(w0 + run, hi);
         uint32_t m = 0;
-        for (uint32_t g = w0 + lane; g < w1; g += 32 * SM_BATCH) {
-            uint4 v[SM_BATCH];
+        for (uint32_t g = w0 + lane; g < w1; g += 32 * SM_LOOK) {
+            uint4 v[SM_LOOK];
 #pragma unroll
-            for (int i = 0; i < SM_BATCH; ++i) v[i] = g + 32 * i < w1 ? x.group(g + 32 * i) : nothing;
+            for (int i = 0; i < SM_LOOK; ++i) v[i] = g + 32 * i < w1 ? x.group(g + 32 * i) : nothing;
 #pragma unroll
-            for (int i = 0; i < SM_BATCH; ++i) m += __popc(equal8(v[i]));
+            for (int i = 0; i < SM_LOOK; ++i) m += __popc(equal8(v[i]));
         }
         m = __reduce_add_sync(0xffffffffu, m);
         __syncthreads();
@@ -490,7 +508,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         if (nth >= incl - y && nth < incl) {
             uint32_t left = nth - (incl - y), e = 0;
             for (;; ++e)  // elements in order
-                if (bits >> (e & 1 ? 31 - e / 2 : 15 - e / 2) & 1 && left-- == 0) break;
+                if (bits >> (e & 1 ? 16 + e / 2 : e / 2) & 1 && left-- == 0) break;
             a.tokens[row] = 8 * (g + lane) + e - x.skew;
         }
         const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
