@@ -38,6 +38,7 @@ constexpr uint32_t SM_BINS = 12288, SM_WINDOWS = (65536 + SM_BINS - 1) / SM_BINS
 constexpr uint32_t SM_LOW = 0x2c00, SM_SIDE = 47 * 128;
 constexpr int SM_BATCH = 2, SM_LOOK = 8;   // 16-byte loads of a thread in flight: counting, and at the last look
 constexpr uint32_t SM_NONE = 0xff80ff80u;  // two logits of -infinity
+constexpr uint32_t SM_BELOW = (0x8000u | (SM_LOW + SM_SIDE - 1)) * 0x10001u;  // two of the lowest of the window
 
 // What a cluster's CTAs tell one another; written by their peers.
 struct SmShared {
@@ -224,42 +225,56 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     };
     if (tid == 0) sh.wodd = 0, sh.found = 0;
     clear();
-    uint32_t top2 = SM_NONE, below = 0xffffu;
+    uint32_t top2 = SM_NONE, below2 = SM_NONE;
     bool odd = false;
     const uint32_t bins = tc::smem_u32(hist);
     each_group([&](uint4 v) {
         const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-        uint32_t inside = 0xffffffffu;  // halves whose value has a counter
+        uint32_t in[4];  // halves whose value has a counter of its sign and magnitude
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             top2 = sm_max2(top2, w4[k]);
             const uint32_t mag = w4[k] & 0x7fff7fffu;
-            inside &= sm_ge2(mag, SM_LOW * 0x10001u) & sm_lt2(mag, (SM_LOW + SM_SIDE) * 0x10001u);
+            in[k] = sm_ge2(mag, SM_LOW * 0x10001u) & sm_lt2(mag, (SM_LOW + SM_SIDE) * 0x10001u);
         }
-        if (inside == 0xffffffffu) {
+        // element k's counter: bins + 4 t, or + 4 (SM_SIDE + t), t the magnitude's bits above SM_LOW
+        auto counter = [&](int k) {
+            const uint32_t w = w4[k >> 1], mag4 = (k & 1 ? w >> 14 : w << 2) & 0x1fffcu;
+            uint32_t negative;  // all ones, or 0
+            asm("prmt.b32 %0, %1, 0, %2;" : "=r"(negative) : "r"(w), "r"(k & 1 ? 0xbbbbu : 0x9999u));
+            return mag4 + (negative & (4 * SM_SIDE)) + (bins - 4 * SM_LOW);
+        };
+        if ((in[0] & in[1] & in[2] & in[3]) == 0xffffffffu) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                // bins + 4 t, or + 4 (SM_SIDE + t), t the magnitude's bits above SM_LOW
-                const uint32_t w = w4[k >> 1], mag4 = (k & 1 ? w >> 14 : w << 2) & 0x1fffcu;
-                uint32_t negative;  // all ones, or 0
-                asm("prmt.b32 %0, %1, 0, %2;" : "=r"(negative) : "r"(w), "r"(k & 1 ? 0xbbbbu : 0x9999u));
-                const uint32_t to = mag4 + (negative & (4 * SM_SIDE)) + (bins - 4 * SM_LOW);
-                asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(to) : "memory");
-            }
-        } else {
-#pragma unroll 1
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t b = sm_half(v, k), d = sm_order(b);
-                const int bin = sm_bin(b, SM_WINDOWS);
-                if (bin >= 0)
-                    atomicAdd(&hist[sm_place(bin, SM_WINDOWS)], 1);
-                else if (sm_counts(d)) {
-                    if (d > 0x8000u + SM_LOW) below = min(below, d); else odd = true;
-                }
-            }
+            for (int k = 0; k < 8; ++k) asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(counter(k)) : "memory");
+            return;
+        }
+        // some that have none: below the window, as masked ones, or 0, NaN and the rest
+        uint32_t rest = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t low = sm_lt2(w4[k], SM_BELOW);
+            below2 = sm_max2(below2, (w4[k] & low) | (SM_NONE & ~low));
+            rest |= ~(in[k] | low) & (0x00010001u << k);  // element 2 k in bit k, 2 k + 1 in bit 16 + k
+        }
+        if (in[0] | in[1] | in[2] | in[3]) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(counter(k)),
+                             "r"(in[k >> 1] & (k & 1 ? 0xffff0000u : 0xffffu))
+                             : "memory");
+        }
+        for (; rest; rest &= rest - 1) {
+            const int i = __ffs(rest) - 1;
+            const uint32_t w = (i & 3) < 2 ? (i & 1 ? v.y : v.x) : (i & 1 ? v.w : v.z), b = i < 16 ? w & 0xffffu : w >> 16;
+            if ((b & 0x7fffu) == 0)
+                atomicAdd(&hist[sm_place(SM_SIDE, SM_WINDOWS)], 1);
+            else if (sm_counts(sm_order(b)))
+                odd = true;
         }
     });
     uint32_t first = min(sm_order(top2 & 0xffffu), sm_order(top2 >> 16));  // (-infinity: no candidate)
+    uint32_t below = min(sm_order(below2 & 0xffffu), sm_order(below2 >> 16));
     first = __reduce_min_sync(0xffffffffu, first);
     below = __reduce_min_sync(0xffffffffu, below);
     if (lane == 0) sh.wcount[warp] = first, sh.wbelow[warp] = below;
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     auto weight = [&](double l) {
         return __double2ull_rn((l == top ? 1.0 : sharp ? 0.0 : exp((l - top) * slope)) * unit);
     };
-    const bool usual = !odd && (below == 0xffffu || weight(sm_value(below)) == 0);
+    const bool usual = !odd && (!sm_counts(below) || weight(sm_value(below)) == 0);
     // the least weight that min_p leaves (NaN: none)
     const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;
 
