@@ -74,7 +74,11 @@ __device__ __forceinline__ void rot_turn(uint4 &v0, uint4 &v1, const RotAngles &
 }
 
 // ---------------------------------------------------------------- rotation of heads
-constexpr int RT_THREADS = 256, RT_HEADS = 4;
+// A thread has one item of RT_HEADS heads of a row: their loads are in flight together
+// and the angles are read once for them. Bound by HBM: 32768 rows of 40 heads x 128,
+// half of each turned in pairs, 103 us on the device (672 MB, the copy rate); two
+// heads a thread 105 us. 64 rows of 16 heads x 64 3.9 us.
+constexpr int RT_THREADS = 128, RT_HEADS = 4;
 template <bool PAIRS>
 __global__ void __launch_bounds__(RT_THREADS)
     rotary_kernel(RotaryView t, const uint16_t *x, uint64_t x_stride, uint32_t heads, uint32_t dim, uint32_t rows,
@@ -116,45 +120,56 @@ int launch_rotary(const RotaryView &t, const uint16_t *x, uint64_t x_stride, uin
 }
 
 // ---------------------------------------------------------------- rotated append
-// blockIdx.y: up to AR_HEADS query heads, one key head, or one value head. A
-// thread has one item of a (row, head); the DIM / 16 threads of a head are
-// neighbours and agree on its row.
-constexpr int AR_THREADS = 256, AR_HEADS = 4;
+// blockIdx.y: up to AR_HEADS query heads, or some key or value heads. A thread has
+// one item of them; the DIM / 16 threads of a head are neighbours and agree on its
+// row. Bound by HBM for prompts and by the chain of sequence, length and page for
+// single tokens: 12.8k rows of 32 + 8 + 8 heads x 128 bf16 52 us on the device (318 MB,
+// 94 % of the copy rate), 7.4k rows of 14 + 2 + 2 x 64 KV8 10.7 us (33 MB), 64 rows 5.1 us.
+// With two query heads a thread 54, 10.8 and 5.0 us, with seven 60, 13.1 and 6.3; KV8 keys
+// two at a time 12.7 us (their divisions), bf16 ones one at a time 57 us.
+constexpr int AR_THREADS = 128, AR_HEADS = 4;
+template <bool KV8>
+struct ArKv {
+    static constexpr int HEADS = KV8 ? 1 : 4;
+};
 template <bool KV8, int DIM, bool PAIRS>
 __global__ void __launch_bounds__(AR_THREADS) paged_append_rotary_kernel(PagedView c, RotaryView t, AppendRotary a) {
     constexpr uint32_t ITEMS = DIM / 16;
     const uint64_t n = (uint64_t)blockIdx.x * AR_THREADS + threadIdx.x;
     const uint32_t row = (uint32_t)(n / ITEMS), item = (uint32_t)(n % ITEMS);
     if (row >= a.rows) return;  // (a head's threads leave together)
-    const uint32_t nq = (a.q_heads + AR_HEADS - 1) / AR_HEADS, y = blockIdx.y;
-    const bool is_q = y < nq, is_v = y >= nq + c.hkv;
-    const uint32_t head = is_q ? y * AR_HEADS : y - nq - (is_v ? c.hkv : 0);
-    const uint32_t count = is_q ? min(a.q_heads - head, (uint32_t)AR_HEADS) : 1;
+    constexpr int KVH = ArKv<KV8>::HEADS;
+    static_assert(KVH <= AR_HEADS, "v");
+    const uint32_t nq = (a.q_heads + AR_HEADS - 1) / AR_HEADS, nk = (c.hkv + KVH - 1) / KVH, y = blockIdx.y;
+    const bool is_q = y < nq, is_v = y >= nq + nk;
+    const uint32_t head = is_q ? AR_HEADS * y : KVH * (y - nq - (is_v ? nk : 0));
+    const int count = (int)(is_q ? min(a.q_heads - head, (uint32_t)AR_HEADS) : min(c.hkv - head, (uint32_t)KVH));
     const RotItem r = is_v ? RotItem{16 * item, 16 * item + 8, 0, false} : rot_item<PAIRS>(item, t.rotated);
     const uint32_t seq = a.seqs[row], pos = a.positions[row];
-    const uint16_t *src = is_q ? a.q + row * a.q_stride : (is_v ? a.v : a.k) + row * a.kv_stride;
+    const uint16_t *src = (is_q ? a.q + row * a.q_stride : (is_v ? a.v : a.k) + row * a.kv_stride) + head * DIM;
     uint4 v[AR_HEADS][2];
 #pragma unroll
     for (int i = 0; i < AR_HEADS; ++i) {
-        if (i >= (int)count) break;
-        v[i][0] = *reinterpret_cast<const uint4 *>(src + (head + i) * DIM + r.d0);
-        v[i][1] = *reinterpret_cast<const uint4 *>(src + (head + i) * DIM + r.d1);
+        if (i >= count) break;
+        v[i][0] = *reinterpret_cast<const uint4 *>(src + i * DIM + r.d0);
+        v[i][1] = *reinterpret_cast<const uint4 *>(src + i * DIM + r.d1);
     }
+    // (the angles do not wait for the page)
+    RotAngles g;
+    if (r.turn && pos < t.positions) rot_angles(g, t.table + (uint64_t)pos * t.rotated, r.at, t.rotated);
     uint32_t page = PG_NO_PAGE;
     if (pos < t.positions && pos < (uint32_t)paged_length(c, seq))
         page = c.table[(uint64_t)seq * c.max_pages + (pos >> c.tshift)];
-    RotAngles g;
-    if (r.turn && page < c.pages) rot_angles(g, t.table + (uint64_t)pos * t.rotated, r.at, t.rotated);
     if (page >= c.pages) return;
     if (r.turn) {
 #pragma unroll
         for (int i = 0; i < AR_HEADS; ++i)
-            if (i < (int)count) rot_turn<PAIRS>(v[i][0], v[i][1], g);
+            if (i < count) rot_turn<PAIRS>(v[i][0], v[i][1], g);
     }
     if (is_q) {
 #pragma unroll
         for (int i = 0; i < AR_HEADS; ++i) {
-            if (i >= (int)count) break;
+            if (i >= count) break;
             uint16_t *p = a.q_out + row * a.q_out_stride + (head + i) * DIM;
             *reinterpret_cast<uint4 *>(p + r.d0) = v[i][0];
             *reinterpret_cast<uint4 *>(p + r.d1) = v[i][1];
@@ -162,43 +177,47 @@ __global__ void __launch_bounds__(AR_THREADS) paged_append_rotary_kernel(PagedVi
         return;
     }
     uint8_t *pool = const_cast<uint8_t *>(is_v ? c.v : c.k);
-    const uint64_t dst = paged_row(c, page, head) + (pos & ((1u << c.tshift) - 1));
-    if constexpr (!KV8) {
-        *reinterpret_cast<uint4 *>(pool + (dst * DIM + r.d0) * 2) = v[0][0];
-        *reinterpret_cast<uint4 *>(pool + (dst * DIM + r.d1) * 2) = v[0][1];
-    } else {
-        // the rule of paged_append_kernel, on the bf16 values
-        const uint32_t w[8] = {v[0][0].x, v[0][0].y, v[0][0].z, v[0][0].w, v[0][1].x, v[0][1].y, v[0][1].z, v[0][1].w};
-        float x[16], amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[2 * j] = bflo(w[j]);
-            x[2 * j + 1] = bfhi(w[j]);
-        }
+    for (int i = 0; i < KVH; ++i) {
+        if (i >= count) break;
+        const uint64_t dst = paged_row(c, page, head + i) + (pos & ((1u << c.tshift) - 1));
+        if constexpr (!KV8) {
+            *reinterpret_cast<uint4 *>(pool + (dst * DIM + r.d0) * 2) = v[i][0];
+            *reinterpret_cast<uint4 *>(pool + (dst * DIM + r.d1) * 2) = v[i][1];
+        } else {
+            // the rule of paged_append_kernel, on the bf16 values
+            const uint32_t w[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+            float x[16], amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(x[j]));
-        const uint32_t mates = ((1u << ITEMS) - 1) << (threadIdx.x & 31 & ~(ITEMS - 1));  // this head's threads
-#pragma unroll
-        for (int o = ITEMS / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mates, amax, o));
-        const float s = __fdiv_rn(amax, 127.0f);
-        uint32_t b[4] = {0u, 0u, 0u, 0u};
-        if (s > 0.f) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int code = (int)fminf(fmaxf(rintf(__fdiv_rn(x[j], s)), -127.f), 127.f);
-                b[j >> 2] |= ((uint32_t)code & 0xffu) << (8 * (j & 3));
+            for (int j = 0; j < 8; ++j) {
+                x[2 * j] = bflo(w[j]);
+                x[2 * j + 1] = bfhi(w[j]);
             }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(x[j]));
+            const uint32_t mates = ((1u << ITEMS) - 1) << (threadIdx.x & 31 & ~(ITEMS - 1));  // this head's threads
+#pragma unroll
+            for (int o = ITEMS / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mates, amax, o));
+            const float s = __fdiv_rn(amax, 127.0f);
+            uint32_t b[4] = {0u, 0u, 0u, 0u};
+            if (s > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int code = (int)fminf(fmaxf(rintf(__fdiv_rn(x[j], s)), -127.f), 127.f);
+                    b[j >> 2] |= ((uint32_t)code & 0xffu) << (8 * (j & 3));
+                }
+            }
+            *reinterpret_cast<uint2 *>(pool + dst * DIM + r.d0) = make_uint2(b[0], b[1]);
+            *reinterpret_cast<uint2 *>(pool + dst * DIM + r.d1) = make_uint2(b[2], b[3]);
+            if (item == 0) const_cast<float *>(is_v ? c.vs : c.ks)[dst] = s;
         }
-        *reinterpret_cast<uint2 *>(pool + dst * DIM + r.d0) = make_uint2(b[0], b[1]);
-        *reinterpret_cast<uint2 *>(pool + dst * DIM + r.d1) = make_uint2(b[2], b[3]);
-        if (item == 0) const_cast<float *>(is_v ? c.vs : c.ks)[dst] = s;
     }
 }
 
 template <bool KV8, int DIM>
 static int launch_append_rotary(const PagedView &c, const RotaryView &t, const AppendRotary &a, cudaStream_t st) {
     const uint64_t threads = (uint64_t)a.rows * (DIM / 16);
-    const dim3 grid((unsigned)((threads + AR_THREADS - 1) / AR_THREADS), (a.q_heads + AR_HEADS - 1) / AR_HEADS + 2 * c.hkv);
+    const dim3 grid((unsigned)((threads + AR_THREADS - 1) / AR_THREADS), (a.q_heads + AR_HEADS - 1) / AR_HEADS + 2 * ((c.hkv + ArKv<KV8>::HEADS - 1) / ArKv<KV8>::HEADS));
     auto *kernel = t.pairs ? paged_append_rotary_kernel<KV8, DIM, true> : paged_append_rotary_kernel<KV8, DIM, false>;
     kernel<<<grid, AR_THREADS, 0, st>>>(c, t, a);
     return QB_LAUNCH_CHECK();
