@@ -217,3 +217,55 @@ def test_captured_replayed_and_on_another_stream():
         sync()
         assert np.array_equal(host(tokens).view(np.uint32), sample(x, nu, np.full(6, 0.8))[0])
     del keep
+
+
+SPECIAL = [2.0 ** 8, -2.0 ** 8, 255.0, -255.0, 254.0, 2.0 ** -39, -2.0 ** -39, 2.0 ** -40, -2.0 ** -40, 0.0, -0.0, 1e-38, -1e-39, 9.2e-41,
+           300.0, -300.0, 1.0, -1.0, 1.0078125, LOWEST, -INF, NAN, -1e4]
+
+
+@pytest.mark.parametrize('temperature', [0.05, 1.0, 60.0, 1e5])
+@pytest.mark.parametrize('upto', [1e9, 255.5, 1.5])
+@pytest.mark.parametrize('vocab', [37, 1000, 40000])
+def test_values_at_the_edges_of_what_is_counted(temperature, upto, vocab):
+    """Zeros, the smallest and largest values, masks and ordinary logits side by side, in every order."""
+    r = np.random.default_rng(vocab)
+    some = np.array([v for v in SPECIAL if not v > upto])
+    x = r.standard_normal((24, vocab)) * 0.7
+    for i in range(24):
+        special = r.random(vocab) < (0.02, 0.3, 0.95)[i % 3]
+        x[i, special] = r.choice(some, special.sum())
+    check_all(x, r.random(24, np.float32), np.full(24, temperature), np.where(np.arange(24) % 4 == 0, 20, 0),
+              np.where(np.arange(24) % 4 == 1, 0.9, 1.0), np.where(np.arange(24) % 4 == 2, 0.05, 0.0))
+
+
+@pytest.mark.parametrize('k', range(12))
+def test_a_mask_with_a_value_at_each_place_of_a_load(k):
+    """One allowed token among masked ones: 16-byte loads with one counted element each."""
+    for hidden in (-INF, LOWEST, NAN, -1000.0):
+        x = np.full((3, 4096), hidden)
+        x[0, k::16] = np.linspace(-3, 3, len(range(k, 4096, 16)))
+        x[1, 100 + k] = 0.0
+        x[2, 4095 - k] = -20.0
+        tokens, _ = check_all(x, np.array([0.37, 0.5, 0.9], np.float32), np.full(3, 0.7))
+        assert tokens[1] == 100 + k and tokens[2] == 4095 - k
+
+
+def test_more_rows_than_the_gpu_holds_at_once():
+    x, u = rows_of(77, 700, 300)
+    check_all(x, u, np.linspace(0.2, 2, 700), np.arange(700) % 5 * 9, np.linspace(0.3, 1.1, 700))
+
+
+def test_two_streams_at_once():
+    torch = torch_cuda()
+    jobs = []
+    for seed, (rows, vocab) in enumerate(((3, 151936), (40, 20000), (200, 5000))):
+        x, u = rows_of(seed, rows, vocab)
+        jobs.append((x, u, dev(to_bits(x).view(np.int16)), dev(u), dev(np.zeros(rows, np.int32)), torch.cuda.Stream()))
+    sync()
+    for _ in range(10):
+        for x, u, logits, ud, tokens, st in jobs:
+            assert L().qwen_b200_op_sample(vp(logits), x.shape[1], x.shape[0], x.shape[1], None, None, None, None, vp(ud), vp(tokens),
+                                           None, ctypes.c_void_p(st.cuda_stream)) == 0
+    sync()
+    for x, u, logits, ud, tokens, st in jobs:
+        assert np.array_equal(host(tokens).view(np.uint32), sample(x, u)[0])
