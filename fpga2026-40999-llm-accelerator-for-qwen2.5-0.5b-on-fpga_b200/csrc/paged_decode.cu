@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
     if constexpr (DIRECT) {
         const uint32_t unit = blockIdx.x / w.parts, part = blockIdx.x % w.parts;
         if (w.parts > 1) pd_cluster_arrive();
-        // Blocks of two warps and fewer come several to an SM, neighbours together: neighbours are different rows there, or one
+        // Blocks of few warps come several to an SM, neighbours together: neighbours are different rows there, or one
         // SM would get all KV heads of a long one (1024 blocks with 1 to 512 keys: 47 us for the loop, not 27).
         constexpr bool SPREAD = SHARED && NW < 8;
         row = SPREAD ? unit % a.rows : unit / w.items;
@@ -987,10 +987,11 @@ template <bool KV8, int DIM, int NW>
 static int launch_rows(const PagedAttnArgs &a, const PdWork &w, uint32_t units, uint32_t sms, cudaStream_t st) {
     using C = PdCfg<KV8, DIM, NW>;
     auto *kernel = paged_decode_kernel<KV8, DIM, true, true, NW>;
-    // Blocks start as SMs come free of the tile kernel: without a limit the first ones would take as many as they hold
-    // and the others none. Shared memory that nothing uses keeps it at an even share.
-    const uint32_t share = (units + sms - 1) / sms, fair = (PD_SM_BYTES / (share ? share : 1) - PD_STATIC_BYTES) & ~15u;
-    const uint32_t smem = fair > C::SMEM ? fair : C::SMEM;
+    // Behind the tile kernel blocks start as SMs come free: without a limit the first ones would take as many as they hold
+    // and the others none. Shared memory that nothing uses keeps it at an even share (256 rows on 4096 keys 47 -> 43 us).
+    const uint32_t share = (units + sms - 1) / sms, even = PD_SM_BYTES / share;
+    uint32_t smem = C::SMEM;
+    if (w.tiles && even > smem + PD_STATIC_BYTES) smem = (even - PD_STATIC_BYTES) & ~15u;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
     return launch_pdl(kernel, dim3(units), dim3(C::THREADS), smem, st, 1, a, w);
 }
@@ -1010,11 +1011,15 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
         most = most < seen ? most : seen;
     }
     if constexpr (SHARED) {
-        // Many rows with little of their own: two warps an item, so that an SM has many items' chains of length,
-        // page and key in flight.
-        if (units >= 2 * (uint32_t)sms) {
+        // Many items: fewer warps for each, so that an SM has more chains of length, page and key in flight, and some 16
+        // warps in all as the decode kernel has. With 8, 4 and 2 warps, us a call: 300 items of 14 heads on 2 of 64 dims KV8
+        // with up to 256 own keys 10.9, 8.2, 8.8, with 4096 37.6, 48.8, 70.6; 512 items, 512 keys 16.4, 13.2, 13.9, 2048 keys
+        // 36.4, 35.4, 41.4; 1200 items, 500 keys 37.8, 27.6, 25.6; of 32 heads on 8 of 128 dims bf16 512 items, 512 keys
+        // 33.7, 26.4, 24.5, 2048 keys 57.3, 60.0, 61.9; 1024 items behind tiles, 300 keys 78.8, 54.7, 47.5.
+        if (units >= 3 * (uint32_t)sms) {
             w.parts = 1;
-            return launch_rows<KV8, DIM, 2>(a, w, units, sms, st);
+            return units >= 6 * (uint32_t)sms ? launch_rows<KV8, DIM, 2>(a, w, units, sms, st)
+                                                    : launch_rows<KV8, DIM, 4>(a, w, units, sms, st);
         }
     }
     const uint64_t want = (most + PD_PART_KEYS - 1) / PD_PART_KEYS, room = units < slots ? slots / units : 1;

@@ -156,6 +156,14 @@ def test_many_groups(fmt):
 
 
 @FORMATS
+def test_more_rows_and_heads_than_fit_the_gpu(fmt):
+    """Some 70 blocks of the row kernel for each SM."""
+    r = np.random.default_rng(2)
+    groups = [(20, [20 + int(x) for x in r.integers(0, 9, 1300)])]
+    run(1300, fmt, 64, 16, groups, kv_heads=8, group=1)
+
+
+@FORMATS
 @DIMS
 def test_sequences_shorter_than_the_prefix(fmt, dim):
     """The prefix is a claim about the tokens that two sequences both have."""
