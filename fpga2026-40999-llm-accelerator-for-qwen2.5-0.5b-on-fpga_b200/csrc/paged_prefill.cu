@@ -421,7 +421,12 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     const uint32_t per = (a.n + C::WARPS - 1) / C::WARPS, i0 = min(warp * per, a.n), i1 = min(i0 + per, a.n);
     unsigned long long mine = 0;
     bool dead = false;
-    for (uint32_t b = i0; b < i1; b += 32) mine += __reduce_add_sync(0xffffffffu, pp_units_lane<SHARED>(a, w, b, i1, dead));
+    uint32_t kept_units = 0;  // SHARED: those of the warp's first 32 groups, whose loads depend on one another (1 us)
+    for (uint32_t b = i0; b < i1; b += 32) {
+        const uint32_t u = pp_units_lane<SHARED>(a, w, b, i1, dead);
+        if (SHARED && b == i0) kept_units = u;
+        mine += __reduce_add_sync(0xffffffffu, u);
+    }
     dead = __any_sync(0xffffffffu, dead);
     if (lane == 0) {
         wsum[warp] = mine;
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
     if (books || (active && before * a.c.hkv <= u0 && u0 < (before + mine) * a.c.hkv)) {
         unsigned long long p = before;
         for (uint32_t b = i0; b < i1; b += 32) {
-            uint32_t u = pp_units_lane<SHARED>(a, w, b, i1, dead), x = u;
+            uint32_t u = SHARED && b == i0 ? kept_units : pp_units_lane<SHARED>(a, w, b, i1, dead), x = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
