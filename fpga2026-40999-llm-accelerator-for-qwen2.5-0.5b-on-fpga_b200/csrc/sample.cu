@@ -22,16 +22,16 @@
 //
 // A cluster of C CTAs has a row: each counts a part of it, then takes 12288 / C
 // values, 32 a step: a warp adds the CTAs' counts of a step over distributed
-// shared memory, forms the weights and sums them; a thread has the sums of a step,
-// and the one in whose step a border lies finds it with its warp and tells the
-// others.
+// shared memory, forms the weights, sums them and gives the sums to every CTA.
+// From there each CTA finds every border by itself: a thread has the sums of a
+// step, and the one in whose step a border lies looks closer with its warp.
 //
 // Bound by counting where every logit matters: adds to shared memory take 3.4
 // clocks a warp at random banks (1.0 without conflicts; copies of the counters
 // do not help), 17 us of 256 rows of 151936 on 148 SMs, and about 12 instructions a
 // logit. 256 rows, top_p alone, 49 us (DRAM floor 12): counting 28, sums 8, the
 // last look 11. 64 rows with all filters and 8 masked rows 21 us on the device, one
-// row 12: there latency, of the loads, three exchanges and the sums. Cluster
+// row 11.5: there latency, of the loads, two exchanges and the sums. Cluster
 // sizes: one wave of two CTAs an SM (256 rows by 4 CTAs each 129 us where one each
 // took 104, both before the packed comparisons).
 #include "kernels.h"
@@ -54,13 +54,11 @@ struct SmShared {
     uint32_t first[SM_MAX_CTAS];           // lowest order (largest logit) of each CTA's part
     uint32_t below[SM_MAX_CTAS];           // the same of its values below the usual window
     uint32_t odd[SM_MAX_CTAS];             // whether it has values that the window's two sides do not hold
-    uint32_t count[SM_MAX_CTAS];           // candidates of its values
-    unsigned long long sum[SM_MAX_CTAS];   // their weights
-    unsigned long long high[SM_MAX_CTAS];  // and those of at least min_p
+    // this CTA's own
     unsigned long long top_k, top_p;       // weights of the k first, and of those that top_p leaves
     uint32_t bin, nth;                     // the token: nth occurrence of a value
     uint32_t found;                        // in this window
-    uint32_t wcount[SM_WARPS], wbelow[SM_WARPS], wodd;  // this CTA's own
+    uint32_t wcount[SM_WARPS], wbelow[SM_WARPS], wodd;
     unsigned long long wsum[SM_WARPS], whigh[SM_WARPS];
 };
 
@@ -147,13 +145,14 @@ __device__ __forceinline__ uint32_t sm_half(const uint4 &v, int k) {
     return k & 1 ? w >> 16 : w & 0xffffu;
 }
 
-// Shared memory beside SmShared: the histogram, of this CTA's values the counts of all CTAs, and of its steps the weights,
+// Shared memory beside SmShared: the histogram, of this CTA's values the counts of all CTAs, and of all steps the weights,
 // those of at least min_p, and the counts.
+constexpr int SM_STEPS = SM_BINS / 32;
 template <int C>
 struct SmCfg {
     static constexpr int SEG = SM_BINS / C, STEPS = SEG / 32;  // values and steps of a CTA
-    static constexpr int COUNTS = SM_BINS * 4, SUMS = COUNTS + (C > 1 ? SEG * 4 : 0), BYTES = SUMS + STEPS * 20;
-    static_assert(STEPS % SM_WARPS == 0 && STEPS <= SM_THREADS, "steps");
+    static constexpr int COUNTS = SM_BINS * 4, SUMS = COUNTS + (C > 1 ? SEG * 4 : 0), BYTES = SUMS + SM_STEPS * 20;
+    static_assert(STEPS % SM_WARPS == 0 && SM_STEPS <= SM_THREADS, "steps");
 };
 
 template <typename T>
@@ -194,8 +193,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     __shared__ SmShared sh;
     uint32_t *const hist = reinterpret_cast<uint32_t *>(smem);
     uint32_t *const counts = reinterpret_cast<uint32_t *>(smem + (C > 1 ? K::COUNTS : 0));
-    unsigned long long *const step_sum = reinterpret_cast<unsigned long long *>(smem + K::SUMS), *const step_high = step_sum + K::STEPS;
-    uint32_t *const step_count = reinterpret_cast<uint32_t *>(step_high + K::STEPS);
+    unsigned long long *const step_sum = reinterpret_cast<unsigned long long *>(smem + K::SUMS), *const step_high = step_sum + SM_STEPS;
+    uint32_t *const step_count = reinterpret_cast<uint32_t *>(step_high + SM_STEPS);
     const uint32_t rank = C > 1 ? sm_rank() : 0, row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + row * a.stride);
@@ -345,60 +344,48 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
                 s = sm_warp_sum(n * w);
                 h = floor == 0 ? s : sm_warp_sum(w >= floor ? n * w : 0ull);
             }
-            if (lane == 0) step_count[step] = c, step_sum[step] = s, step_high[step] = h;
+            const uint32_t to = rank * K::STEPS + step;
+            if (C == 1) {
+                if (lane == 0) step_count[to] = c, step_sum[to] = s, step_high[to] = h;
+            } else if (lane < C) {
+                sm_put32(&step_count[to], lane, c);
+                sm_put64(&step_sum[to], lane, s);
+                sm_put64(&step_high[to], lane, h);
+            }
         }
-        __syncthreads();
+        sm_sync<C>();
         unsigned long long high = 0;
         cnt = 0, sum = 0;
-        if (tid < K::STEPS) cnt = step_count[tid], sum = step_sum[tid], high = step_high[tid];
+        if (tid < SM_STEPS) cnt = step_count[tid], sum = step_sum[tid], high = step_high[tid];
         const uint32_t ic = sm_warp_scan(cnt);
         const unsigned long long is = sm_warp_scan(sum);
         high = sm_warp_sum(high);
         if (lane == 31) sh.wcount[warp] = ic, sh.wsum[warp] = is, sh.whigh[warp] = high;
         __syncthreads();
-        uint32_t call = 0;
-        unsigned long long sall = 0, hall = 0;
         cb = c_before + ic - cnt, sb = s_before + is - sum;
+        cw = 0, sw = 0, hw = 0;
 #pragma unroll
         for (int i = 0; i < SM_WARPS; ++i) {
             const uint32_t y = sh.wcount[i];
             const unsigned long long z = sh.wsum[i];
             if (i < warp) cb += y, sb += z;
-            call += y, sall += z, hall += sh.whigh[i];
-        }
-        if (C == 1) {
-            cw = call, sw = sall, hw = hall;
-            return;
-        }
-        if (tid < C) {
-            sm_put32(&sh.count[rank], tid, call);
-            sm_put64(&sh.sum[rank], tid, sall);
-            sm_put64(&sh.high[rank], tid, hall);
-        }
-        sm_sync<C>();
-        cw = 0, sw = 0, hw = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (c < (int)rank) cb += sh.count[c], sb += sh.sum[c];
-            cw += sh.count[c];
-            sw += sh.sum[c];
-            hw += sh.high[c];
+            cw += y, sw += z, hw += sh.whigh[i];
         }
     };
-    // Where `here` holds for one thread of the cluster (a border lies in its step): the first value at which
-    // `there`(candidates, weights up to its end) holds; tell(its bin, its count and weight, weights and candidates before
-    // it) by one lane. Whole warps call it.
+    // Where `here` holds for one thread (a border lies in its step): the first value at which `there`(candidates, weights up
+    // to its end) holds; tell(its bin, its count and weight, weights and candidates before it) by one lane. Whole warps call
+    // it, every CTA with the same result.
     auto find = [&](bool here, auto &&there, auto &&tell) {
         const uint32_t owner = __ballot_sync(0xffffffffu, here);
         if (!owner) return;
         const int l = __ffs(owner) - 1;
-        const uint32_t at = 32 * (32 * warp + l) + lane, c = __shfl_sync(0xffffffffu, cb, l);
-        const uint32_t n = C > 1 ? counts[at] : hist[sm_place(at, window)];
-        const unsigned long long s = __shfl_sync(0xffffffffu, sb, l), w = n ? weight(sm_bin_value(rank * K::SEG + at, window)) : 0;
+        const uint32_t step = 32 * warp + l, at = 32 * step + lane, c = __shfl_sync(0xffffffffu, cb, l);
+        const uint32_t n = C > 1 ? sm_get32(&counts[at % K::SEG], step / K::STEPS) : hist[sm_place(at, window)];
+        const unsigned long long s = __shfl_sync(0xffffffffu, sb, l), w = n ? weight(sm_bin_value(at, window)) : 0;
         const uint32_t ic = sm_warp_scan(n);
         const unsigned long long is = sm_warp_scan(n * w);
         const uint32_t hit = __ballot_sync(0xffffffffu, n && there(c + ic, s + is));
-        if (lane == __ffs(hit) - 1) tell(rank * K::SEG + at, n, w, s + is - n * w, c + ic - n);
+        if (lane == __ffs(hit) - 1) tell(at, n, w, s + is - n * w, c + ic - n);
     };
     // Moves on to a window (the usual one is there already).
     auto count_window = [&](uint32_t to) {
@@ -438,13 +425,13 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         if (k_of)
             find(cb < k_of && k_of <= cb + cnt, [&](uint32_t c, unsigned long long) { return c >= k_of; },
                  [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t c) {
-                     for (int i = 0; i < C; ++i) sm_put64(&sh.top_k, i, s + (k_of - c) * w);
+                     sh.top_k = s + (k_of - c) * w;
                  });
         total += cw, mass += sw, high += hw;
         return false;
     });
     if (k_of && k_of < total) {
-        sm_sync<C>();
+        __syncthreads();
         mass = sh.top_k;
     }
     // ---- the kept candidates: of the k first, those with less than top_p of their weights before them, and min_p themselves.
@@ -456,11 +443,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
             sweep([&] {
                 find(sb < share && share <= sb + sum, [&](uint32_t, unsigned long long s) { return s >= share; },
                      [&](uint32_t, uint32_t, unsigned long long w, unsigned long long s, uint32_t) {
-                         for (int i = 0; i < C; ++i) sm_put64(&sh.top_p, i, s + (share - s + w - 1) / w * w);
+                         sh.top_p = s + (share - s + w - 1) / w * w;
                      });
                 return false;
             });
-            sm_sync<C>();
+            __syncthreads();
             kept = min(kept, sh.top_p);
         } else {
             kept = 0;
@@ -473,15 +460,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     sweep([&] {
         find(sb <= target && target < sb + sum, [&](uint32_t, unsigned long long s) { return s > target; },
              [&](uint32_t bin, uint32_t n, unsigned long long w, unsigned long long s, uint32_t) {
-                 const uint32_t nth = greedy ? n - 1 : (uint32_t)((target - s) / w);
-                 for (int i = 0; i < C; ++i) {
-                     sm_put32(&sh.bin, i, bin);
-                     sm_put32(&sh.nth, i, nth);
-                     sm_put32(&sh.found, i, 1);
-                 }
-                 if (a.probs) a.probs[row] = greedy ? 1.f : (float)((double)w / (double)kept);
+                 sh.bin = bin;
+                 sh.nth = greedy ? n - 1 : (uint32_t)((target - s) / w);
+                 sh.found = 1;
+                 if (a.probs && rank == 0) a.probs[row] = greedy ? 1.f : (float)((double)w / (double)kept);
              });
-        sm_sync<C>();
+        __syncthreads();
         return sh.found != 0;
     });
 
