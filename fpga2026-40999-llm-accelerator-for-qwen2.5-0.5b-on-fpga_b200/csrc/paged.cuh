@@ -110,12 +110,13 @@ struct SharedGroup {
     uint32_t row0, rows, seq;
     int keys;
 };
-// Whether a group is worth the tile kernel: rows * keys * KV heads * dims from 2^25 on. Its launch and the join of its
-// pieces take some 12 us whatever the size, and the row kernel finds shared pages in L2. Without and with the tiles: 14 heads
-// on 2 of 64 dims KV8, 64 rows on 2048 keys (2^24) 14.4 and 23.2 us, 256 rows on 4096 (2^27) 119 and 43; 32 heads on 8 of
-// 128 dims bf16, 32 rows on 512 keys (2^24) 16.1 and 20.8 us, 1024 (2^25) 21.6 and 23.0, 64 rows on 1024 (2^26) 28.9 and 22.4;
-// 4 groups of 8 rows on 2048 (2^24 each) 33.9 and 31.8.
-constexpr uint64_t SHARED_WORK = 1ull << 25;
+// Whether a group is worth the tile kernel: rows * keys * KV heads * dims from 3 * 2^24 on. Its launch and the join of its
+// pieces take some 12 us whatever the size, and the row kernel finds shared pages in L2. Row by row and with tiles, us a
+// call, 64 own keys a row: 14 heads on 2 of 64 dims KV8, 64 rows on 2048 keys (2^24) 14.3 and 23.3, 4096 (2^25) 21.3 and 25.0,
+// 8192 (2^26) 35.2 and 27.8, 256 rows on 4096 (2^27) 64.0 and 34.1; 32 heads on 8 of 128 dims bf16, 32 rows on 512 keys
+// (2^24) 16.0 and 21.3, 1024 (2^25) 21.5 and 23.6, 2048 (2^26) 32.4 and 25.1, 64 rows on 4096 (2^28) 96.3 and 36.7; of 64 dims
+// bf16 (2^25) 18.9 and 18.5, of 128 KV8 20.1 and 21.0; 2 rows on 32768 keys (2^26) 59.3 and 52.4.
+constexpr uint64_t SHARED_WORK = 3ull << 24;
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
     SharedGroup s;
     s.row0 = min(a.starts[g], a.rows);

@@ -420,12 +420,12 @@ def test_samples_of_one_prompt(fmt):
 
 
 # ---------------------------------------------------------------- groups large enough for tiles of query rows
-# (rows * shared keys * KV heads * dims of 2^25 and more)
-BIG = pytest.mark.parametrize('dim,rows,prefix', [(64, 130, 520), (128, 100, 333)])
+# (rows * shared keys * KV heads * dims of 3 * 2^24 and more)
+BIG = pytest.mark.parametrize('dim,rows,prefix', [(64, 195, 520), (128, 150, 333)])
 
 
 def big(seed, fmt, dim, rows, prefix, page=64, kv_heads=8, group=2, own=40, **more):
-    assert rows * prefix * kv_heads * dim >= 1 << 25
+    assert rows * prefix * kv_heads * dim >= 3 << 24
     r = np.random.default_rng(seed)
     return [(prefix, [prefix + int(x) for x in r.integers(0, own, rows)])], dict(kv_heads=kv_heads, group=group, **more)
 
@@ -443,14 +443,14 @@ def test_tiles_pages(fmt, dim, rows, prefix, page, copies):
 @DIMS
 @pytest.mark.parametrize('prefix', [513, 575, 576, 577, 639, 640, 641, 767, 768, 1024])
 def test_tiles_prefix_edges(fmt, dim, prefix):
-    groups, more = big(prefix, fmt, dim, 128, prefix)
+    groups, more = big(prefix, fmt, dim, 200, prefix)
     run(prefix, fmt, dim, 32, groups, **more)
 
 
 @FORMATS
 @pytest.mark.parametrize('dim,kv_heads,group,rows,prefix', [
-    (64, 1, 1, 520, 1024), (64, 2, 7, 256, 1030), (64, 8, 1, 300, 260), (128, 4, 3, 171, 400), (128, 2, 8, 129, 1100),
-    (128, 1, 17, 260, 1025), (64, 3, 9, 400, 450), (128, 1, 70, 257, 1100), (64, 32, 5, 60, 300)])
+    (64, 1, 1, 780, 1024), (64, 2, 7, 384, 1030), (64, 8, 1, 380, 260), (128, 4, 3, 247, 400), (128, 2, 8, 180, 1100),
+    (128, 1, 17, 385, 1025), (64, 3, 9, 585, 450), (128, 1, 70, 358, 1100), (64, 32, 5, 82, 300)])
 def test_tiles_head_layouts(fmt, dim, kv_heads, group, rows, prefix):
     """Tiles that end inside a row's heads, at them, and rows over several tiles."""
     groups, more = big(rows, fmt, dim, rows, prefix, kv_heads=kv_heads, group=group)
@@ -545,7 +545,7 @@ def test_tiles_one_key_outweighs_the_rest(fmt, dim, rows, prefix, where):
 @DIMS
 def test_tiles_of_values_that_nobody_sees(fmt, dim):
     """What the pages hold behind the prefix of the first sequence and behind each length does not matter (NaN there)."""
-    groups = [(577, [577] + [577 + i % 7 for i in range(127)])]
+    groups = [(577, [577] + [577 + i % 7 for i in range(179)])]
     run(17, fmt, dim, 256, groups, kv_heads=8, group=1)
 
 
@@ -575,24 +575,24 @@ def test_tiles_give_the_same_bits_again_and_with_two_streams():
 def test_tiles_captured_and_replayed_as_the_prefix_changes():
     """A graph of the call answers for groups that are worth tiles and for those that are not."""
     torch = torch_cuda()
-    groups, _ = big(22, KV8, 128, 100, 400)
+    groups, _ = big(22, KV8, 128, 130, 400)
     c = shared_cache(22, KV8, 128, 64, groups, kv_heads=8)
     keep = Keep()
     kv = c.upload(keep)
-    q = bf16(c.rand(100, 16, 128) * 2)
-    qd, out = dev(bits(q).view(np.int16)), dev(np.zeros((100, 2048), np.int16))
-    starts, prefix = dev(u32([0, 100])), dev(u32([400]))
-    ws = dev(np.zeros(L().qwen_b200_paged_decode_shared_workspace(ref(kv), 16, 1, 100), np.uint8))
+    q = bf16(c.rand(130, 16, 128) * 2)
+    qd, out = dev(bits(q).view(np.int16)), dev(np.zeros((130, 2048), np.int16))
+    starts, prefix = dev(u32([0, 130])), dev(u32([400]))
+    ws = dev(np.zeros(L().qwen_b200_paged_decode_shared_workspace(ref(kv), 16, 1, 130), np.uint8))
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
 
     def call():
-        assert L().qwen_b200_op_paged_decode_shared(ref(kv), 0, vp(qd), 2048, 16, 1, vp(starts), vp(prefix), 100, None, 0.088,
+        assert L().qwen_b200_op_paged_decode_shared(ref(kv), 0, vp(qd), 2048, 16, 1, vp(starts), vp(prefix), 130, None, 0.088,
                                                     vp(out), 2048, vp(ws), ws.numel(), ctypes.c_void_p(side.cuda_stream)) == 0
     call()
     side.synchronize()
     with torch.cuda.graph(graph, stream=side):
         call()
-    exact, tol = attention(c, 0, q, np.arange(100), 0.088)
+    exact, tol = attention(c, 0, q, np.arange(130), 0.088)
     for p in (400, 20, 399, 0, 350):
         prefix.copy_(torch.from_numpy(u32([p])))
         out.zero_()
