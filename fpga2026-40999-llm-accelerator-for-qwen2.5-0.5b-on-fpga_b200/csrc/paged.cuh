@@ -156,6 +156,7 @@ int launch_paged_append(const qwen_b200_paged_kv &kv, uint32_t layer, const uint
                         uint64_t row_stride, uint32_t rows, const uint32_t *seqs, const uint32_t *positions,
                         cudaStream_t st);
 size_t paged_shared_ws(uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows);
+bool paged_shared_fits(const PagedAttnArgs &a);
 int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st);
 // Its two halves: the shared tokens by tiles of query rows, then each row's own tokens joined with those.
 size_t paged_shared_pieces_bytes(uint32_t dim);

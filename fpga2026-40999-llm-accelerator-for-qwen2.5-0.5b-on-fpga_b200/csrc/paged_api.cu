@@ -229,13 +229,14 @@ int qwen_b200_op_paged_decode_shared(const qwen_b200_paged_kv *kv, uint32_t laye
     if (int rc = attn_check(kv, layer, q, q_stride, q_heads, rows, scale, ctx, ctx_stride, workspace)) return rc;
     if (!starts || !prefix || !n || n > 65536 || rows > 65536 || !words_aligned({seqs, starts, prefix}))
         return QWEN_B200_EINVAL;
-    if (int rc = paged_check_device(*kv, {q, seqs, starts, prefix, ctx, workspace})) return rc;
-    if (workspace_bytes < paged_shared_ws(q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     PagedAttnArgs a = attn_args(*kv, layer, q, q_stride, q_heads, seqs, 0, 0, scale, ctx, ctx_stride);
     a.rows = rows;
     a.n = n;
     a.starts = starts;
     a.prefix = prefix;
+    if (!paged_shared_fits(a)) return QWEN_B200_EINVAL;
+    if (int rc = paged_check_device(*kv, {q, seqs, starts, prefix, ctx, workspace})) return rc;
+    if (workspace_bytes < paged_shared_ws(q_heads, kv->head_dim, n, rows)) return QWEN_B200_EINVAL;
     return launch_paged_shared(a, workspace, (cudaStream_t)stream);
 }
 

@@ -1070,8 +1070,6 @@ int launch_shared_rows(const PagedAttnArgs &a, const SharedParts &parts, bool ti
     w.items = a.c.hkv * w.hb;
     w.sh = parts;
     w.tiles = tiles;
-    if ((uint64_t)a.rows * w.items * PD_HEADS >= 1ull << 31) return -1;
-    if ((uint64_t)a.rows * w.items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 3) >= 1ull << 32) return -1;
     const int n = sms < PD_MAX_SMS ? sms : PD_MAX_SMS;
     if (a.format == QWEN_B200_KV8)
         return a.dim == 64 ? launch_decode<true, 64, true>(a, w, n, st) : launch_decode<true, 128, true>(a, w, n, st);

@@ -197,19 +197,21 @@ __device__ __forceinline__ uint32_t pp_units_lane(const PagedAttnArgs &a, const 
     const uint32_t i = base + (threadIdx.x & 31);
     PpSeqInfo s = {};
     uint32_t u = 0;
-    if (i < end) {
-        s = pp_seq<SHARED>(a, w, i);
-        if constexpr (SHARED) return (uint32_t)s.nt * pp_blocks<true>(a, w, s.pos0, s.mrows, 0).n;
-        if (pp_dead(s) > pp_dead_alone(a)) dead = true;
-        if (s.nt <= 4)
-            for (int k = 0; k < s.nt; ++k) u += pp_blocks<false>(a, w, s.pos0, s.mrows, k).n;
-    }
-    if constexpr (SHARED) return 0;
-    for (uint32_t todo = __ballot_sync(0xffffffffu, s.nt > 4); todo; todo &= todo - 1) {
-        const int l = __ffs(todo) - 1;
-        const uint32_t x = pp_units_warp<false>(a, w, __shfl_sync(0xffffffffu, s.pos0, l), __shfl_sync(0xffffffffu, s.mrows, l),
-                                         __shfl_sync(0xffffffffu, s.nt, l));
-        if ((int)(threadIdx.x & 31) == l) u = x;
+    if (i < end) s = pp_seq<SHARED>(a, w, i);
+    if constexpr (SHARED) {
+        if (i < end) u = (uint32_t)s.nt * pp_blocks<true>(a, w, s.pos0, s.mrows, 0).n;
+    } else {
+        if (i < end) {
+            if (pp_dead(s) > pp_dead_alone(a)) dead = true;
+            if (s.nt <= 4)
+                for (int k = 0; k < s.nt; ++k) u += pp_blocks<false>(a, w, s.pos0, s.mrows, k).n;
+        }
+        for (uint32_t todo = __ballot_sync(0xffffffffu, s.nt > 4); todo; todo &= todo - 1) {
+            const int l = __ffs(todo) - 1;
+            const uint32_t x = pp_units_warp<false>(a, w, __shfl_sync(0xffffffffu, s.pos0, l), __shfl_sync(0xffffffffu, s.mrows, l),
+                                                    __shfl_sync(0xffffffffu, s.nt, l));
+            if ((int)(threadIdx.x & 31) == l) u = x;
+        }
     }
     return u;
 }

@@ -20,9 +20,15 @@ size_t paged_shared_ws(uint32_t q_heads, uint32_t dim, uint32_t n, uint32_t rows
     return 256 + up256(((size_t)n + 1) * 8) + paged_shared_pieces_bytes(dim) + up256(heads * 8) + heads * dim * 4;
 }
 
+// The tile kernel's blocks and the row kernel's keys are counted in 32 bits.
+bool paged_shared_fits(const PagedAttnArgs &a) {
+    const uint64_t group = a.qh / a.c.hkv, items = a.c.hkv * ((group + 7) / 8);
+    if (a.rows * group >= 1ull << 31 || a.rows * items * 8 >= 1ull << 31) return false;
+    return paged_prefill_fits(a) && a.rows * items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 3) < 1ull << 32;
+}
+
 int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     const size_t heads = (size_t)a.rows * a.qh;
-    if ((uint64_t)a.rows * (a.qh / a.c.hkv) >= 1ull << 31 || !paged_prefill_fits(a)) return -1;
     char *p = (char *)ws + 256;
     SharedParts parts = {};
     parts.base = reinterpret_cast<unsigned long long *>(p);

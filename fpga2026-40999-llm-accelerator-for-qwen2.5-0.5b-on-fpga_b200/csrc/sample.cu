@@ -210,6 +210,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     const uint32_t k_of = a.top_k && !greedy ? a.top_k[row] : 0;
     const float p = a.top_p && !greedy ? a.top_p[row] : 1.f, least = a.min_p && !greedy ? a.min_p[row] : 0.f, u = a.u[row];
 
+    // Weights are whole numbers of 1 / unit. 1 / T is rounded to 64 bits first, which takes a weight e^-x off by up to
+    // x e^-x 2^-53 (less than half a unit from vocabularies of 256 on) and spares each value a division.
+    const double slope = 1.0 / temperature, unit = __longlong_as_double((long long)(1023 + a.unit) << 52);
+    // the least weight that min_p leaves (NaN: none)
+    const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;
+
     // ---- this CTA's part of the row, counted in the usual window
     auto clear = [&] {
         for (uint32_t i = tid; i < SM_BINS / 4; i += SM_THREADS) reinterpret_cast<uint4 *>(hist)[i] = make_uint4(0, 0, 0, 0);
@@ -313,16 +319,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
         }
         return;  // (no CTA reads another's memory any more)
     }
-    // Weights are whole numbers of 1 / unit. 1 / T is rounded to 64 bits first, which takes a weight e^-x off by up to
-    // x e^-x 2^-53 (less than half a unit from vocabularies of 256 on) and spares each value a division.
-    const double top = sm_value(first), slope = 1.0 / temperature, unit = ldexp(1.0, a.unit);
+    const double top = sm_value(first);
     const bool sharp = greedy || isinf(top);  // only the largest counts
     auto weight = [&](double l) {
         return __double2ull_rn((l == top ? 1.0 : sharp ? 0.0 : exp((l - top) * slope)) * unit);
     };
     const bool usual = !odd && (!sm_counts(below) || weight(sm_value(below)) == 0);
-    // the least weight that min_p leaves (NaN: none)
-    const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;
 
     // ---- a window's counts and weights; cb and sb: candidates and weights before this thread's step, cnt and sum of it,
     // cw, sw and hw of the window (hw: of at least `floor`)

@@ -97,6 +97,15 @@ def test_workspace_sizes():
     assert calls(ws_bytes=n - 1, rows=4)['shared']() in (_lib.EINVAL, _lib.EDEVICE)
 
 
+@pytest.mark.parametrize('change,rows,heads,n', [
+    (dict(kv_heads=1, page_stride=64, layer_stride=32 * 64), 65536, 65536, 1),  # rows * (q_heads / kv_heads) of 2^32
+    (dict(max_pages=1 << 24), 65536, 14, 65536),                                # blocks of tiles
+    (dict(max_pages=1 << 24), 4096, 14, 1),                                     # keys of rows
+], ids=['rows', 'blocks', 'keys'])
+def test_shared_calls_of_more_than_32_bits_count_are_refused(change, rows, heads, n):
+    assert calls(kv(**change), rows=rows, heads=heads, n=n, stride=1 << 22, out_stride=1 << 22)['shared']() == _lib.EINVAL
+
+
 def test_memory_that_is_not_the_current_devices_is_refused():
     """Host memory: EINVAL where there is a GPU, EDEVICE where there is none; nothing is launched either way."""
     buf = (ctypes.c_uint8 * 4096)()
