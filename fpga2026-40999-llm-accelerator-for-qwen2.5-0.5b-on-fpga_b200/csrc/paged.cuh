@@ -102,7 +102,8 @@ struct PagedAttnArgs {
     uint32_t window, sinks;
     float scale;
     uint32_t format, dim;
-    const uint32_t *prefix = nullptr;  // shared decode: tokens that a group's sequences share
+    const uint32_t *prefix = nullptr;  // shared decode: tokens that a group's sequences share,
+    uint32_t long_keys = 0;            // and how many of them are shared whatever the work
 };
 // A group of sequences that share their first tokens: its rows of q, and how many tokens of its first row's sequence
 // the tile kernel takes for all of them (0: none, each row takes its whole context).
@@ -117,13 +118,22 @@ struct SharedGroup {
 // (2^24) 16.0 and 21.3, 1024 (2^25) 21.5 and 23.6, 2048 (2^26) 32.4 and 25.1, 64 rows on 4096 (2^28) 96.3 and 36.7; of 64 dims
 // bf16 (2^25) 18.9 and 18.5, of 128 KV8 20.1 and 21.0; 2 rows on 32768 keys (2^26) 59.3 and 52.4.
 constexpr uint64_t SHARED_WORK = 3ull << 24;
+// From three items (row, KV head, block of 8 heads) an SM on the row kernel takes fewer warps for each, which a long context
+// keeps busy after all others are done: there every prefix of SHARED_LONG keys goes to the tiles. Without and with that: 4 groups
+// of 128 rows, one of them of few rows on some 6000 keys, 136 and 69 us; 32 groups of 4 rows on 2048 keys (32 heads on 8 of 128
+// dims bf16) 106 and 79, on 4096 193 and 124; 16 groups of 16 rows on 2048 (14 on 2 of 64 KV8) 39 and 27; but 64 groups of 4
+// rows there 40 and 55, 32 groups of 2 rows of 128 dims 61 and 76. From 1024 keys on 32 groups of 4 rows 63 and 56, 16 of 4 38
+// and 40.
+constexpr uint32_t SHARED_LONG = 2048;
+inline bool shared_few_warps(uint64_t items, int sms) { return items >= 3 * (uint64_t)sms; }
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
     SharedGroup s;
     s.row0 = min(a.starts[g], a.rows);
     s.rows = min(max(a.starts[g + 1], s.row0), a.rows) - s.row0;
     s.seq = s.rows == 0 ? QWEN_B200_NO_SEQ : a.seqs ? a.seqs[s.row0] : s.row0;
     s.keys = min((int)min(a.prefix[g], 0x7fffffffu), paged_length(a.c, s.seq));
-    if (s.rows < 2 || (uint64_t)s.rows * s.keys < (SHARED_WORK / a.dim + a.c.hkv - 1) / a.c.hkv) s.keys = 0;
+    if (s.rows < 2 || ((uint32_t)s.keys < a.long_keys && (uint64_t)s.rows * s.keys < (SHARED_WORK / a.dim + a.c.hkv - 1) / a.c.hkv))
+        s.keys = 0;
     return s;
 }
 // The group that a row belongs to; false for none. starts is not decreasing.

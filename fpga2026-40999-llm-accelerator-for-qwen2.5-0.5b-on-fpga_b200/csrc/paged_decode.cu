@@ -1016,7 +1016,7 @@ static int launch_decode(const PagedAttnArgs &a, PdWork w, int sms, cudaStream_t
         // with up to 256 own keys 10.9, 8.2, 8.8, with 4096 37.6, 48.8, 70.6; 512 items, 512 keys 16.4, 13.2, 13.9, 2048 keys
         // 36.4, 35.4, 41.4; 1200 items, 500 keys 37.8, 27.6, 25.6; of 32 heads on 8 of 128 dims bf16 512 items, 512 keys
         // 33.7, 26.4, 24.5, 2048 keys 57.3, 60.0, 61.9; 1024 items behind tiles, 300 keys 78.8, 54.7, 47.5.
-        if (units >= 3 * (uint32_t)sms) {
+        if (shared_few_warps(units, sms)) {
             w.parts = 1;
             return units >= 6 * (uint32_t)sms ? launch_rows<KV8, DIM, 2>(a, w, units, sms, st)
                                                     : launch_rows<KV8, DIM, 4>(a, w, units, sms, st);

@@ -27,7 +27,11 @@ bool paged_shared_fits(const PagedAttnArgs &a) {
     return paged_prefill_fits(a) && a.rows * items * ((((uint64_t)a.c.max_pages << a.c.tshift) >> 4) + 3) < 1ull << 32;
 }
 
-int launch_paged_shared(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
+int launch_paged_shared(const PagedAttnArgs &args, void *ws, cudaStream_t st) {
+    const int sms = paged_sms();
+    if (sms <= 0) return -3;
+    PagedAttnArgs a = args;
+    a.long_keys = shared_few_warps((uint64_t)a.rows * a.c.hkv * ((a.qh / a.c.hkv + 7) / 8), sms) ? SHARED_LONG : 0xffffffffu;
     const size_t heads = (size_t)a.rows * a.qh;
     char *p = (char *)ws + 256;
     SharedParts parts = {};

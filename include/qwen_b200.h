@@ -608,6 +608,8 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * it, so a group whose first row is no sequence shares nothing. Tokens from
  * prefix[g] on are each sequence's own. A sequence may be shorter than the prefix. There is no window: under one, a shared prefix soon
  * lies behind it, and qwen_b200_op_paged_decode reads no more than the window.
+ * Sequences whose own tokens are many belong there too: a batch of many rows is
+ * laid out for a long shared part and a short one of each row's own.
  * n groups (1 .. 65536, empty ones allowed), rows <= 65536. starts is [n + 1]
  * on the device, not decreasing; rows in front of starts[0] and at or behind
  * starts[n] are left as they were, rows with no key are zero. rows * (q_heads /

@@ -600,3 +600,13 @@ def test_tiles_captured_and_replayed_as_the_prefix_changes():
         graph.replay()
         sync()
         assert_within(unbits(host(out)).reshape(q.shape), exact, tol, str(p))
+
+
+@FORMATS
+@DIMS
+def test_tiles_for_few_rows_with_a_long_prefix_among_many(fmt, dim):
+    """From three items an SM on, prefixes of 2048 keys go to the tiles whatever their rows; others of the call do not."""
+    r = np.random.default_rng(dim)
+    groups = [(70, [70 + int(x) for x in r.integers(0, 50, 40)]), (2048, [2100, 2048]), (2047, [2050, 2060]), (2300, [2301, 2500, 100]),
+              (64, [64 + int(x) for x in r.integers(0, 50, 30)])]
+    run(dim, fmt, dim, 64, groups, kv_heads=8, group=3)
