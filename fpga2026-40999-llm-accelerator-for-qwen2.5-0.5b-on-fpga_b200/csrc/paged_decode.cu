@@ -992,7 +992,9 @@ static int launch_rows(const PagedAttnArgs &a, const PdWork &w, uint32_t units, 
     const uint32_t share = (units + sms - 1) / sms, even = PD_SM_BYTES / share;
     uint32_t smem = C::SMEM;
     if (w.tiles && even > smem + PD_STATIC_BYTES) smem = (even - PD_STATIC_BYTES) & ~15u;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
+    // (the limit is the kernel's, not the call's: another thread's call may set it between this and the launch)
+    constexpr int MOST = PD_SM_BYTES - PD_STATIC_BYTES;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess) return -3;
     return launch_pdl(kernel, dim3(units), dim3(C::THREADS), smem, st, 1, a, w);
 }
 

@@ -269,3 +269,9 @@ def test_two_streams_at_once():
     sync()
     for x, u, logits, ud, tokens, st in jobs:
         assert np.array_equal(host(tokens).view(np.uint32), sample(x, u)[0])
+
+
+def test_as_many_rows_as_a_call_takes():
+    u = np.random.default_rng(3).random(65536, np.float32)
+    tokens, probs = sample(np.zeros((65536, 4)), u)
+    assert np.array_equal(tokens, np.floor(u * 4).astype(np.uint32)) and (probs == 0.25).all()

@@ -610,3 +610,36 @@ def test_tiles_for_few_rows_with_a_long_prefix_among_many(fmt, dim):
     groups = [(70, [70 + int(x) for x in r.integers(0, 50, 40)]), (2048, [2100, 2048]), (2047, [2050, 2060]), (2300, [2301, 2500, 100]),
               (64, [64 + int(x) for x in r.integers(0, 50, 30)])]
     run(dim, fmt, dim, 64, groups, kv_heads=8, group=3)
+
+
+def test_two_host_threads_with_calls_of_other_sizes():
+    """Each call's blocks ask for shared memory by the call's size: one thread's call does not get in another's way."""
+    import threading
+    torch = torch_cuda()
+    keep, jobs = Keep(), []
+    for seed, (rows, prefix) in enumerate(((120, 900), (450, 300))):
+        groups, _ = big(seed, KV8, 64, rows, prefix)
+        c = shared_cache(seed, KV8, 64, 64, groups, kv_heads=8)
+        kv = c.upload(keep)
+        q = bf16(c.rand(rows, 16, 64) * 2)
+        n = L().qwen_b200_paged_decode_shared_workspace(ref(kv), 16, 1, rows)
+        jobs.append((c, kv, q, dev(bits(q).view(np.int16)), dev(np.zeros((rows, 1024), np.int16)), dev(np.zeros(n, np.uint8)),
+                     dev(u32([0, rows])), dev(u32([prefix])), torch.cuda.Stream(), []))
+    sync()
+
+    def work(job):
+        c, kv, q, qd, out, ws, starts, prefix, st, codes = job
+        for _ in range(300):
+            codes.append(L().qwen_b200_op_paged_decode_shared(ref(kv), 0, vp(qd), 1024, 16, 1, vp(starts), vp(prefix), len(q), None,
+                                                              0.125, vp(out), 1024, vp(ws), ws.numel(),
+                                                              ctypes.c_void_p(st.cuda_stream)))
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    sync()
+    for c, kv, q, qd, out, ws, starts, prefix, st, codes in jobs:
+        assert not any(codes)
+        exact, tol = attention(c, 0, q, np.arange(len(q)), 0.125)
+        assert_within(unbits(host(out)).reshape(q.shape), exact, tol)
