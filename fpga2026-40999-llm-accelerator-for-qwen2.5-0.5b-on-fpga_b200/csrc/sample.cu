@@ -83,6 +83,16 @@ __device__ __forceinline__ uint32_t sm_get32(const void *p, uint32_t rank) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sm_remote(p, rank)) : "memory");
     return v;
 }
+// All CTAs of the row have started: a store to another's shared memory is defined from then on. Arrived at first thing, waited
+// for behind the counting.
+template <int C>
+__device__ __forceinline__ void sm_arrive() {
+    if constexpr (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+template <int C>
+__device__ __forceinline__ void sm_started() {
+    if constexpr (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // All CTAs of the row.
 template <int C>
 __device__ __forceinline__ void sm_sync() {
@@ -195,6 +205,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     uint32_t *const counts = reinterpret_cast<uint32_t *>(smem + (C > 1 ? K::COUNTS : 0));
     unsigned long long *const step_sum = reinterpret_cast<unsigned long long *>(smem + K::SUMS), *const step_high = step_sum + SM_STEPS;
     uint32_t *const step_count = reinterpret_cast<uint32_t *>(step_high + SM_STEPS);
+    sm_arrive<C>();
     const uint32_t rank = C > 1 ? sm_rank() : 0, row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + row * a.stride);
@@ -294,6 +305,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     if (lane == 0) sh.wcount[warp] = first, sh.wbelow[warp] = below;
     if (odd) sh.wodd = 1;
     __syncthreads();
+    sm_started<C>();
     if (warp == 0) {
         first = __reduce_min_sync(0xffffffffu, sh.wcount[lane % SM_WARPS]);
         below = __reduce_min_sync(0xffffffffu, sh.wbelow[lane % SM_WARPS]);
