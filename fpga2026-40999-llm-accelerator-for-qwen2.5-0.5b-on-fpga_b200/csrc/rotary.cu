@@ -8,6 +8,7 @@
 // bf16, so the fused append gives the bits of the two calls that it replaces.
 // cos and sin come from a table: an angle of a far position needs 64 bits
 // (65536 rad in fp32 is off by 2^-9), too many for the kernel.
+#include <float.h>
 #include <math.h>
 
 #include "paged.cuh"
@@ -259,6 +260,9 @@ extern "C" int qwen_b200_rotary_table(const qwen_b200_rotary_angles *a, uint32_t
         size = factor > 1.0 ? 0.1 * log(factor) + 1 : 1.0;
     }
     if (a->size > 0.0) size = a->size;
+    if (!(size <= FLT_MAX)) return QWEN_B200_EINVAL;  // (the last position's angles and the size bound every entry)
+    for (uint32_t i = 0; i < half; ++i)
+        if (!isfinite((positions - 1.0) * freq[i])) return QWEN_B200_EINVAL;
 #pragma omp parallel for
     for (int64_t p = 0; p < (int64_t)positions; ++p)
         for (uint32_t i = 0; i < half; ++i) {

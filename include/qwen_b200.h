@@ -461,7 +461,8 @@ typedef struct qwen_b200_rotary {
  *           positions, f_i / factor for those that turn less than `slow` times, a
  *           ramp over the pairs between (Peng et al. 2023; usually 32 and 1)
  * cos and sin are multiplied by `size`; 0 stands for 1, with YARN for 0.1
- * ln(factor) + 1. EINVAL for values that give no table. */
+ * ln(factor) + 1. EINVAL for values that give no table, and for those whose
+ * angles or entries would not be finite. */
 #define QWEN_B200_ROTARY_PLAIN 0u
 #define QWEN_B200_ROTARY_LINEAR 1u
 #define QWEN_B200_ROTARY_NTK 2u
