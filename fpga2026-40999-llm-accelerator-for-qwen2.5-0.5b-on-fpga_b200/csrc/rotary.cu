@@ -254,7 +254,8 @@ extern "C" int qwen_b200_rotary_table(const qwen_b200_rotary_angles *a, uint32_t
         auto pair_of = [&](double turns) { return rot * log(a->trained / (turns * 2 * M_PI)) / (2 * log(theta)); };
         const double low = fmax(floor(pair_of(a->fast)), 0.0), high = fmin(ceil(pair_of(a->slow)), rot - 1.0);
         for (uint32_t i = 0; i < half; ++i) {
-            const double ramp = fmin(fmax((i - low) / fmax(high - low, 0.001), 0.0), 1.0);
+            // (no pair turns as often as `slow` if the border lies at or in front of pair 0)
+            const double ramp = high <= 0 ? 1.0 : fmin(fmax((i - low) / fmax(high - low, 0.001), 0.0), 1.0);
             freq[i] = freq[i] * (1 - ramp) + freq[i] / factor * ramp;
         }
         size = factor > 1.0 ? 0.1 * log(factor) + 1 : 1.0;

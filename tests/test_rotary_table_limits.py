@@ -32,3 +32,12 @@ def test_settings_whose_table_would_have_infinities_or_nan_are_refused(change):
 def test_settings_at_the_ends_of_their_ranges_give_a_table(change):
     rc, out = table(**change)
     assert rc == _lib.OK and np.isfinite(out).all() and (out != 7).all()
+
+
+@pytest.mark.parametrize('trained,slow', [(64, 16.0), (4, 1.0), (1, 0.5)])
+def test_yarn_where_every_pair_turns_less_than_slow_times(trained, slow):
+    """Pair 0 turns trained / (2 pi) times: below `slow` it is divided by the factor like all behind it."""
+    assert trained / (2 * np.pi) < slow
+    rc, out = table(scaling=_lib.ROTARY_YARN, trained=trained, slow=slow, factor=4.0, size=1.0)
+    plain, exact = table(scaling=_lib.ROTARY_LINEAR, factor=4.0)
+    assert rc == plain == _lib.OK and np.array_equal(out, exact)
