@@ -427,6 +427,9 @@ __global__ void __launch_bounds__(32 * NW, PdCfg<KV8, DIM, NW>::MINB) paged_deco
                 const SharedGroup sg = shared_group(a, share.group);
                 share.keys = (uint32_t)sg.keys;
                 share.at = row - sg.row0;
+                // A row that ends inside the shared keys takes its own instead: a tile's product gives the others' values the
+                // weight 0 there, and 0 times an infinity or NaN is not 0 (codes are finite, and their scales are masked).
+                if (!KV8 && paged_length(a.c, a.seqs ? a.seqs[row] : row) < sg.keys) share.keys = 0;
             }
         }
         const PdRow R = SHARED ? pd_own<C::LOG>(a, row, share.keys) : pd_row<C::LOG>(a, row);

@@ -607,7 +607,8 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * are read from the pages of the group's first row (in groups too small for that to
  * pay, from each sequence's own); a prefix longer than that sequence is cut to
  * it, so a group whose first row is no sequence shares nothing. Tokens from
- * prefix[g] on are each sequence's own. A sequence may be shorter than the prefix. There is no window: under one, a shared prefix soon
+ * prefix[g] on are each sequence's own. A sequence may be shorter than the prefix
+ * (in bf16 pools it then reads its own tokens). There is no window: under one, a shared prefix soon
  * lies behind it, and qwen_b200_op_paged_decode reads no more than the window.
  * Sequences whose own tokens are many belong there too: a batch of many rows is
  * laid out for a long shared part and a short one of each row's own.
@@ -616,10 +617,9 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * starts[n] are left as they were, rows with no key are zero. rows * (q_heads /
  * kv_heads) and blocks are limited as in qwen_b200_op_paged_prefill, rows and keys as
  * in qwen_b200_op_paged_decode. Softmax weights of shared tokens are rounded as in the
- * former, those of a sequence's own as in the latter; NaN and infinities in
- * values of a prefix that some row sees may reach the rows of its group. The
- * workspace (qwen_b200_paged_decode_shared_workspace; calls that overlap need one
- * each) may hold anything, but its first 4 bytes become non-zero if a bounded
+ * former, those of a sequence's own as in the latter. What a row does not see does
+ * not reach it, NaN and infinities included. The workspace (qwen_b200_paged_decode_shared_workspace;
+ * calls that overlap need one each) may hold anything, but its first 4 bytes become non-zero if a bounded
  * device wait expired (ctx is then not valid): a caller that wants to know
  * zeroes them before. */
 size_t qwen_b200_paged_decode_shared_workspace(const qwen_b200_paged_kv *kv, uint32_t q_heads, uint32_t n, uint32_t rows);

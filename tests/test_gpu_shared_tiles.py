@@ -167,3 +167,46 @@ def test_own_keys_behind_tiles_hold_weights_in_16_bits(fmt, dim, n, few_rows):
     assert ran and (got == got[:1]).all()
     for h in range(14):
         assert (np.abs(got[0, h] - out[h // 7]) <= bound[h // 7]).all()
+
+
+# ---------------------------------------------------------------- rows that see less than their group shares
+@FORMATS
+@pytest.mark.parametrize('dim,kv_heads,group,rows,prefix', [(64, 8, 2, 195, 520), (128, 8, 2, 150, 333), (64, 2, 7, 64, 8192)])
+def test_values_that_a_row_does_not_see_do_not_reach_it(fmt, dim, kv_heads, group, rows, prefix):
+    """NaN and infinities in shared keys and values behind a row's last token, and behind none at all, as in a group that
+    has no tiles. Rows that do see them are not looked at."""
+    lens = [prefix + 40] + [prefix + i % 30 for i in range(rows - 1)]
+    short = np.arange(1, 12)
+    lens[1:12] = [1, 0, 5, 63, 64, 65, 100, 127, 128, 129, 200]
+    c = shared_cache(rows, fmt, dim, 64, [(prefix, lens)], kv_heads)
+    q = bf16(c.rand(rows, kv_heads * group, dim) * 2)
+    seqs = np.arange(rows)
+    seqs[[20, rows - 1]] = NO_SEQ
+    clean = np.concatenate([short, [20, rows - 1]])
+    exact, tol = attention(c, 0, q[clean], seqs[clean], dim ** -0.5)
+    bad = np.arange(200, prefix)  # (every short row ends in front of it)
+    p, t = c.at(0, bad)
+    for name, value in (('vs', np.nan), ('ks', np.inf)) if fmt == KV8 else (('v', np.nan), ('k', np.inf)):
+        getattr(c, name)[0, p, :, t] = value
+    keep = Keep()
+    got, ran = call(c, c.upload(keep), q, [0, rows], [prefix], seqs, dim ** -0.5)
+    assert ran
+    assert_within(got[clean], exact, tol)
+    assert not got[[2, 20, rows - 1]].any()
+
+
+@FORMATS
+@pytest.mark.parametrize('dim,kv_heads,group,rows,prefix', [(64, 8, 2, 195, 520), (128, 8, 2, 150, 333), (64, 2, 7, 64, 8200)])
+def test_the_first_rows_own_values_do_not_reach_the_others(fmt, dim, kv_heads, group, rows, prefix):
+    """The shared keys are read from the first row's pages, the last of which holds tokens of its own."""
+    lens = [prefix + 40] + [prefix + i % 30 for i in range(rows - 1)]
+    c = shared_cache(rows, fmt, dim, 64, [(prefix, lens)], kv_heads)
+    q = bf16(c.rand(rows, kv_heads * group, dim) * 2)
+    exact, tol = attention(c, 0, q, np.arange(rows), dim ** -0.5)
+    p, t = c.at(0, np.arange(prefix, prefix + 40))
+    for name, value in (('vs', np.nan), ('ks', np.inf)) if fmt == KV8 else (('v', np.nan), ('k', np.inf)):
+        getattr(c, name)[0, p, :, t] = value
+    keep = Keep()
+    got, ran = call(c, c.upload(keep), q, [0, rows], [prefix], None, dim ** -0.5)
+    assert ran and np.isnan(got[0]).all()
+    assert_within(got[1:], exact[1:], tol[1:])
