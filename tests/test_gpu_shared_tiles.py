@@ -210,3 +210,28 @@ def test_the_first_rows_own_values_do_not_reach_the_others(fmt, dim, kv_heads, g
     got, ran = call(c, c.upload(keep), q, [0, rows], [prefix], None, dim ** -0.5)
     assert ran and np.isnan(got[0]).all()
     assert_within(got[1:], exact[1:], tol[1:])
+
+
+# ---------------------------------------------------------------- which calls go to the tiles
+@FORMATS
+@pytest.mark.parametrize('dim,group,groups', [(64, 64, [(4096, 64)]), (128, 32, [(2048, 120)]), (64, 16, [(40, 220), (2300, 4)])])
+def test_many_heads_on_one_kv_head(fmt, dim, group, groups):
+    """Three (row, block of 8 heads) items an SM, though rows x keys x KV heads x dims would be too few with the widest
+    table: prefixes of 2048 keys go to the tiles."""
+    r = np.random.default_rng(group)
+    members = [(p, [p + int(x) for x in r.integers(0, 40, n)]) for p, n in groups]
+    c = shared_cache(group, fmt, dim, 64, members, 1)
+    rows = c.seqs
+    assert rows * (group // 8) >= 3 * sms() and rows * c.max_pages * c.T * dim < WORK
+    keep = Keep()
+    check(c, c.upload(keep), bf16(c.rand(rows, group, dim) * 2), np.concatenate([[0], np.cumsum([n for _, n in groups])]),
+          [p for p, _ in groups])
+
+
+def test_one_row_has_no_tiles():
+    c = shared_cache(1, KV8, 64, 256, [(30000, [30000])], 2)
+    c.table = np.concatenate([c.table, np.full((1, 2000), 1 << 30, np.uint32)], 1)
+    c.max_pages += 2000
+    assert c.max_pages * c.T * 2 * 64 >= WORK
+    keep = Keep()
+    check(c, c.upload(keep), bf16(c.rand(1, 14, 64) * 2), [0, 1], [30000], tiles=False)
