@@ -123,7 +123,7 @@ constexpr uint64_t SHARED_WORK = 3ull << 24;
 // Without and with that: 128 rows in 4 groups, one of them of few rows on some 6000 keys, 136 and 69 us; 32 groups of 4 rows
 // on 2048 keys (32 heads on 8 of 128 dims bf16) 106 and 79, on 4096 193 and 124; 16 groups of 16 rows on 2048 (14 on 2 of 64
 // KV8) 39 and 27; but 64 groups of 4 rows there 40 and 55, 32 groups of 2 rows of 128 dims 61 and 76. Many heads on one KV
-// head of 64 dims KV8: 64 rows of 64 heads on 2048 keys 41 and 31, on 4096 70 and 37, 32 groups of 4 rows of 32 heads on
+// head of 64 dims KV8: 64 rows of 64 heads on 2048 keys 41 and 31, on 4096 70 and 39, 32 groups of 4 rows of 32 heads on
 // 2048 43 and 35. From 1024 keys on 32 groups of 4 rows 63 and 56, 16 of 4 38 and 40.
 constexpr uint32_t SHARED_LONG = 2048;
 inline bool shared_few_warps(uint64_t items, int sms) { return items >= 3 * (uint64_t)sms; }
@@ -152,6 +152,7 @@ __device__ __forceinline__ bool shared_find(const PagedAttnArgs &a, uint32_t row
 // (two a CTA at most: [m tile][l tile][o dim / 4][tile][4]), or whole, then by flattened row of a KV head:
 // [hkv][rows * group] (m, l), [hkv][dim / 4][rows * group][4] o. (A thread of the tile kernel has a row: with four dims of
 // all rows side by side its stores are whole lines; [row][dim] took 3 us more.)
+constexpr uint32_t SHARED_BLOCK = 128, SHARED_LEAST = 1, SHARED_MAX_CTAS = 192;  // keys of a block, blocks of a CTA at least, CTAs
 struct SharedParts {
     unsigned long long *base;  // [n + 1] units of one KV head in the groups before
     float *pieces, *ml, *o;

@@ -62,6 +62,7 @@ struct PdCfg {
     static constexpr int RING = NW * STAGES * STEP_BYTES;
     // over the drained ring: the warps' contexts, and the maxima (then factors) and sums of a shared prefix's pieces
     static constexpr int OS = NW * PD_HEADS * (DIM + 1), PF = PD_HEADS * PD_MAX_SMS;
+    static_assert(PD_MAX_SMS >= SHARED_MAX_CTAS, "pieces of a tile");
     static constexpr int OUT = (OS + 2 * PF) * 4;
     static constexpr int SMEM = RING > OUT ? RING : OUT;
     static constexpr int PIECE = 2 * PD_HEADS + PD_HEADS * DIM;  // floats of a partial result: m, l, o
@@ -207,9 +208,9 @@ struct PdPieces {
 template <int DIM>
 __device__ __forceinline__ PdPieces pd_pieces(const PagedAttnArgs &a, const PdWork &w, uint32_t row, const PdShare &share, uint32_t kvh,
                                               uint32_t h) {
-    const uint32_t blocks = (share.keys + 127) >> 7, m = share.at * w.group + h, size = w.sh.tile * (DIM + 2);
+    const uint32_t blocks = (share.keys + SHARED_BLOCK - 1) / SHARED_BLOCK, m = share.at * w.group + h, size = w.sh.tile * (DIM + 2);
     const unsigned long long all = w.sh.base[a.n], b0 = w.sh.base[share.group], units = w.sh.base[share.group + 1] - b0;  // of a KV head
-    const UnitSplit split(all * a.c.hkv, w.sh.ctas, 1);
+    const UnitSplit split(all * a.c.hkv, w.sh.ctas, SHARED_LEAST);
     const unsigned long long u0 = b0 * a.c.hkv + kvh * units + (unsigned long long)(m / w.sh.tile) * blocks;
     const uint32_t c0 = split.cta_of(u0);
     PdPieces p;

@@ -1399,6 +1399,8 @@ int launch_paged_prefill(const PagedAttnArgs &a, void *ws, cudaStream_t st) {
     return a.dim == 64 ? launch_prefill<false, 64>(a, w, st) : launch_prefill<false, 128>(a, w, st);
 }
 
+// The row kernel finds a tile's pieces by the same numbering.
+static_assert(PP_BLK == SHARED_BLOCK && PP_MIN_UNITS == SHARED_LEAST && PP_MAX_SMS <= SHARED_MAX_CTAS, "shared prefixes");
 size_t paged_shared_pieces_bytes(uint32_t dim) {
     const size_t tile = dim == 64 ? PpCfg<false, 64>::TILE : PpCfg<false, 128>::TILE;
     return (size_t)PP_MAX_SMS * 2 * (2 * tile + tile * dim) * 4;
