@@ -288,9 +288,7 @@ int qwen_b200_op_sample(const uint16_t *logits, uint64_t stride, uint32_t rows, 
     if (stride < vocab || stride > 1ull << 32 || ((uintptr_t)logits & 1)) return QWEN_B200_EINVAL;
     if (!words_aligned({temperature, top_k, top_p, min_p, u, tokens, probs})) return QWEN_B200_EINVAL;
     if (int rc = check_pointers({logits, temperature, top_k, top_p, min_p, u, tokens, probs})) return rc;
-    const int sms = paged_sms();
-    if (sms <= 0) return QWEN_B200_EDEVICE;
-    return launch_sample({logits, stride, rows, vocab, temperature, top_p, min_p, u, top_k, tokens, probs, 0, 0}, sms,
+    return launch_sample({logits, stride, rows, vocab, temperature, top_p, min_p, u, top_k, tokens, probs, 0, 0},
                          (cudaStream_t)stream);
 }
 

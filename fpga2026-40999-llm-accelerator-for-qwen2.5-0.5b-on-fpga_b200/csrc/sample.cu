@@ -31,9 +31,11 @@
 // do not help), 17 us of 256 rows of 151936 on 148 SMs, and about 12 instructions a
 // logit. 256 rows, top_p alone, 49 us (DRAM floor 12): counting 28, sums 8, the
 // last look 11. 64 rows with all filters and 8 masked rows 21 us on the device, one
-// row 11.5: there latency, of the loads, two exchanges and the sums. Cluster
-// sizes: one wave of two CTAs an SM (256 rows by 4 CTAs each 129 us where one each
-// took 104, both before the packed comparisons).
+// row 11.5: there latency, of the loads, two exchanges and the sums.
+// CTAs of a row: as many of 8, 4, 2 and 1 as leave room for all rows at once (33, 71 and
+// 148 rows on 148 SMs). Rows of 151936, top_p, by 8, 4, 2 and 1 CTAs each, us of a captured
+// call with L2 flushed: 33 rows 27, 29, 33, 41; 37 rows 39, 27, 33, 39; 64 rows 47, 29, 33, 41;
+// 74 rows 57, 43, 33, 39; 148 rows 92, 61, 39, 41; 149 rows 92, 61, 53, 51; 256 rows 143, 90, 68, 53.
 #include "kernels.h"
 #include "qwen_b200.h"
 #include "sample.cuh"
@@ -546,13 +548,44 @@ static int launch_sample_ctas(SampleArgs a, uint32_t groups, cudaStream_t st) {
     return launch_pdl(sample_kernel<C>, dim3(a.rows * C), dim3(SM_THREADS), SmCfg<C>::BYTES, st, C, a);
 }
 
-int launch_sample(SampleArgs a, int sms, cudaStream_t st) {
+// Whether the current device holds `rows` clusters of C CTAs at once (a cluster lies within a group of SMs, so they are fewer
+// than the SMs' room by itself); asked once per device and size.
+template <int C>
+static bool sample_fits(uint32_t rows) {
+    static int known[64];  // 1 + the clusters, written with the same value by every thread that finds 0
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int n = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(C);
+        cfg.blockDim = dim3(SM_THREADS);
+        cfg.dynamicSmemBytes = SmCfg<C>::BYTES;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = C;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmCfg<C>::BYTES) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, sample_kernel<C>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            clusters = 0;
+        }
+        n = 1 + clusters;
+        __atomic_store_n(&known[dev], n, __ATOMIC_RELAXED);
+    }
+    return rows <= (uint32_t)(n - 1);
+}
+
+int launch_sample(SampleArgs a, cudaStream_t st) {
     const uint32_t groups = (a.vocab + 7 + 7) / 8;
     a.unit = __builtin_clz(a.vocab) + 31;  // 63 - bits of the vocabulary: the sums stay below 2^63
-    const uint32_t slots = 2 * (uint32_t)sms, most = (groups + 511) / 512;  // (a CTA has work for its threads)
-    if (a.rows * 8 <= slots && most >= 8) return launch_sample_ctas<8>(a, groups, st);
-    if (a.rows * 4 <= slots && most >= 4) return launch_sample_ctas<4>(a, groups, st);
-    if (a.rows * 2 <= slots && most >= 2) return launch_sample_ctas<2>(a, groups, st);
+    const uint32_t most = (groups + 511) / 512;  // (a CTA has work for its threads)
+    if (most >= 8 && sample_fits<8>(a.rows)) return launch_sample_ctas<8>(a, groups, st);
+    if (most >= 4 && sample_fits<4>(a.rows)) return launch_sample_ctas<4>(a, groups, st);
+    if (most >= 2 && sample_fits<2>(a.rows)) return launch_sample_ctas<2>(a, groups, st);
     return launch_sample_ctas<1>(a, groups, st);
 }
 

@@ -17,6 +17,6 @@ struct SampleArgs {
     uint32_t part;  // 16-byte groups that each CTA of a row counts
     int unit;       // weights are whole multiples of 2^-unit
 };
-int launch_sample(SampleArgs a, int sms, cudaStream_t st);
+int launch_sample(SampleArgs a, cudaStream_t st);
 
 }  // namespace qb
