@@ -223,8 +223,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     const uint32_t k_of = a.top_k && !greedy ? a.top_k[row] : 0;
     const float p = a.top_p && !greedy ? a.top_p[row] : 1.f, least = a.min_p && !greedy ? a.min_p[row] : 0.f, u = a.u[row];
 
-    // Weights are whole numbers of 1 / unit. 1 / T is rounded to 64 bits first, which takes a weight e^-x off by up to
-    // x e^-x 2^-53 (less than half a unit from vocabularies of 256 on) and spares each value a division.
+    // Weights are whole numbers of 1 / unit, from an exponential in 64 bits. 1 / T is rounded first, which spares each value a
+    // division: it, l - top and their product take a weight e^-x off by up to x e^-x 2^-53 each (x e^-x is at most 0.37), exp
+    // by its last place, 2^-53 below 1: 2.2 * 2^-53 in all, less than half a unit from vocabularies of 4096 on.
     const double slope = 1.0 / temperature, unit = __longlong_as_double((long long)(1023 + a.unit) << 52);
     // the least weight that min_p leaves (NaN: none)
     const unsigned long long floor = least <= 0.f ? 0 : least <= 1.f ? __double2ull_ru(least * unit) : ~0ull;

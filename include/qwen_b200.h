@@ -426,9 +426,10 @@ int qwen_b200_op_lm_head_argmax(const uint16_t *x, uint32_t rows, const uint16_t
  * NaN and -infinity are no candidates; a row without any gives
  * QWEN_B200_NO_TOKEN with probability 0. Next to a logit of +infinity the
  * others weigh nothing. u outside of [0, 1) counts as its nearer end (NaN as 0), a NaN in
- * top_p or min_p keeps the first candidate only. Weights are rounded to whole
- * multiples of 2^-(63 - bits of vocab) and summed exactly, so the result depends on the
- * row alone. vocab <= 524216, rows <= 65536. */
+ * top_p or min_p keeps the first candidate only. Weights are formed in 64 bits
+ * (within 2^-51 of their definition), rounded to whole multiples of 2^-(63 - bits of
+ * vocab) and summed exactly, so the result depends on the row alone. vocab <= 524216,
+ * rows <= 65536. */
 #define QWEN_B200_NO_TOKEN 0xffffffffu
 int qwen_b200_op_sample(const uint16_t *logits, uint64_t stride, uint32_t rows, uint32_t vocab, const float *temperature,
                         const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *tokens,
@@ -616,8 +617,13 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * on the device, not decreasing; rows in front of starts[0] and at or behind
  * starts[n] are left as they were, rows with no key are zero. rows * (q_heads /
  * kv_heads) and blocks are limited as in qwen_b200_op_paged_prefill, rows and keys as
- * in qwen_b200_op_paged_decode. Softmax weights of shared tokens are rounded as in the
- * former, those of a sequence's own as in the latter. What a row does not see does
+ * in qwen_b200_op_paged_decode. Softmax weights of a sequence's own tokens are held as
+ * in the latter. Those of shared tokens are held so too where each row reads them by
+ * itself, and are rounded to bf16 as in the former where the group is worth tiles of
+ * query rows: that depends on its rows, shared tokens, KV heads and head_dim (from a
+ * product of 3 * 2^24 on) and, in calls of many rows and heads, on its shared tokens
+ * alone (2048 and more), so a row's last bits may change with the batch that it is
+ * in. What a row does not see does
  * not reach it, NaN and infinities included. The workspace (qwen_b200_paged_decode_shared_workspace;
  * calls that overlap need one each) may hold anything, but its first 4 bytes become non-zero if a bounded
  * device wait expired (ctx is then not valid): a caller that wants to know
