@@ -119,12 +119,16 @@ struct SharedGroup {
 // bf16 (2^25) 18.9 and 18.5, of 128 KV8 20.1 and 21.0; 2 rows on 32768 keys (2^26) 59.3 and 52.4.
 constexpr uint64_t SHARED_WORK = 3ull << 24;
 // From three items (row, KV head, block of 8 heads) an SM on the row kernel takes fewer warps for each, which a long context
-// keeps busy after all others are done: there every prefix of SHARED_LONG keys and two or more rows goes to the tiles.
-// Without and with that: 128 rows in 4 groups, one of them of few rows on some 6000 keys, 136 and 69 us; 32 groups of 4 rows
-// on 2048 keys (32 heads on 8 of 128 dims bf16) 106 and 79, on 4096 193 and 124; 16 groups of 16 rows on 2048 (14 on 2 of 64
-// KV8) 39 and 27; but 64 groups of 4 rows there 40 and 55, 32 groups of 2 rows of 128 dims 61 and 76. Many heads on one KV
-// head of 64 dims KV8: 64 rows of 64 heads on 2048 keys 41 and 31, on 4096 70 and 39, 32 groups of 4 rows of 32 heads on
-// 2048 43 and 35. From 1024 keys on 32 groups of 4 rows 63 and 56, 16 of 4 38 and 40.
+// keeps busy after all others are done: there every prefix of SHARED_LONG keys and two or more rows goes to the tiles. That
+// is for groups that are long beside the others. Without and with it, us a call, 14 heads on 2 of 64 dims KV8: 228 rows on
+// 512 keys and 2 on 2048 33 and 23, on 4096 47 and 31, on 32000 250 and 41; 32 heads on 8 of 128 dims bf16, 128 rows in 4
+// groups on some 6000 keys, two of them of 4 rows 227 and 74, one of 12 rows 150 and 74. Where all groups are long it gains
+// if they have rows enough for their tiles (rows * blocks of heads * dims of 512): 16 groups of 16 rows on 2048 KV8 47 and
+// 35, 32 of 8 47 and 43, 32 of 4 rows of 128 dims bf16 113 and 88, 32 of 4 rows of 32 heads on 1 of 64 dims 41 and 33, of 32
+// heads on 2 41 and 41, and loses if not: 64 groups of 4 rows on 2048 47 and 61, on 4096 76 and 98, 32 of 2 rows of 128 dims
+// bf16 76 and 86, KV8 on 4096 119 and 188. A group cannot tell the two apart by itself. From 1024 keys on 32 groups of 4
+// rows of 128 dims 63 and 56, 16 of 4 38 and 40. 64 rows of 64 heads on 1 of 64 dims KV8 on 2048 41 and 31, on 4096 70 and
+// 39.
 constexpr uint32_t SHARED_LONG = 2048;
 inline bool shared_few_warps(uint64_t items, int sms) { return items >= 3 * (uint64_t)sms; }
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
