@@ -112,23 +112,23 @@ struct SharedGroup {
     int keys;
 };
 // Whether a group is worth the tile kernel: rows * keys * KV heads * dims from 3 * 2^24 on. Its launch and the join of its
-// pieces take some 12 us whatever the size, and the row kernel finds shared pages in L2. Row by row and with tiles, us a
-// call, 64 own keys a row: 14 heads on 2 of 64 dims KV8, 64 rows on 2048 keys (2^24) 14.3 and 23.3, 4096 (2^25) 21.3 and 25.0,
-// 8192 (2^26) 35.2 and 27.8, 256 rows on 4096 (2^27) 64.0 and 34.1; 32 heads on 8 of 128 dims bf16, 32 rows on 512 keys
-// (2^24) 16.0 and 21.3, 1024 (2^25) 21.5 and 23.6, 2048 (2^26) 32.4 and 25.1, 64 rows on 4096 (2^28) 96.3 and 36.7; of 64 dims
-// bf16 (2^25) 18.9 and 18.5, of 128 KV8 20.1 and 21.0; 2 rows on 32768 keys (2^26) 59.3 and 52.4.
+// pieces take some 12 us whatever the size, and the row kernel finds shared pages in L2. Row by row and with tiles, us of a
+// captured call with L2 flushed, 64 own keys a row: 14 heads on 2 of 64 dims KV8, 64 rows on 2048 keys (2^24) 18 and 31,
+// 4096 (2^25) 27 and 33, 6144 (3 * 2^24) 33 and 35, 8192 (2^26) 41 and 35, 256 rows on 4096 (2^27) 70 and 43; 32 heads on 8
+// of 128 dims bf16, 32 rows on 512 keys (2^24) 21 and 29, 1024 (2^25) 27 and 31, 1536 (3 * 2^24) 33 and 33, 2048 (2^26) 39
+// and 33, 64 rows on 4096 (2^28) 104 and 45, 2 rows on 32768 (2^26) 68 and 64; of 64 dims bf16 64 rows on 1024 (2^25) 25 and
+// 27, of 128 KV8 32 rows on 1024 (2^25) 25 and 29.
 constexpr uint64_t SHARED_WORK = 3ull << 24;
 // From three items (row, KV head, block of 8 heads) an SM on the row kernel takes fewer warps for each, which a long context
 // keeps busy after all others are done: there every prefix of SHARED_LONG keys and two or more rows goes to the tiles. That
-// is for groups that are long beside the others. Without and with it, us a call, 14 heads on 2 of 64 dims KV8: 228 rows on
-// 512 keys and 2 on 2048 33 and 23, on 4096 47 and 31, on 32000 250 and 41; 32 heads on 8 of 128 dims bf16, 128 rows in 4
-// groups on some 6000 keys, two of them of 4 rows 227 and 74, one of 12 rows 150 and 74. Where all groups are long it gains
-// if they have rows enough for their tiles (rows * blocks of heads * dims of 512): 16 groups of 16 rows on 2048 KV8 47 and
-// 35, 32 of 8 47 and 43, 32 of 4 rows of 128 dims bf16 113 and 88, 32 of 4 rows of 32 heads on 1 of 64 dims 41 and 33, of 32
-// heads on 2 41 and 41, and loses if not: 64 groups of 4 rows on 2048 47 and 61, on 4096 76 and 98, 32 of 2 rows of 128 dims
-// bf16 76 and 86, KV8 on 4096 119 and 188. A group cannot tell the two apart by itself. From 1024 keys on 32 groups of 4
-// rows of 128 dims 63 and 56, 16 of 4 38 and 40. 64 rows of 64 heads on 1 of 64 dims KV8 on 2048 41 and 31, on 4096 70 and
-// 39.
+// is for groups that are long beside the others. Without and with it, us as above, 14 heads on 2 of 64 dims KV8: 228 rows on
+// 512 keys and 2 on 2048 25 and 25, on 4096 37 and 31, on 32000 190 and 43; 32 heads on 8 of 128 dims bf16, 128 rows in 4
+// groups on some 6000 keys, two of them of 4 rows 227 and 80, one of 12 rows 150 and 78. Where all groups are long it gains
+// if they have rows enough for their tiles: 16 groups of 16 rows on 2048 KV8 41 and 37, 32 of 4 rows of 128 dims bf16 107
+// and 94, 32 of 4 rows of 32 heads on 1 of 64 dims 41 and 35, of 32 heads on 2 41 and 43, 64 rows of 64 heads on 1 on 2048
+// 41 and 33, on 4096 70 and 41, and loses if not: 32 groups of 8 rows on 2048 41 and 47, 64 of 4 41 and 68, on 4096 72 and
+// 110, 32 of 2 rows of 128 dims bf16 72 and 92, KV8 on 4096 115 and 195. A group cannot tell the two apart by itself. From
+// 1024 keys on 32 groups of 4 rows of 128 dims 66 and 68, 16 of 4 41 and 49.
 constexpr uint32_t SHARED_LONG = 2048;
 inline bool shared_few_warps(uint64_t items, int sms) { return items >= 3 * (uint64_t)sms; }
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {

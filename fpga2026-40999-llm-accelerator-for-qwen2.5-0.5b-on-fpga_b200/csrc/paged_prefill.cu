@@ -33,6 +33,12 @@
 // of 32 keys for each tile: 390 us for the first case below, against 336 with the
 // softmax code of that time.)
 //
+// Shared prefixes (SHARED) take their weights as two bf16 parts, 16 bits together as in
+// decode attention, so that a row's precision does not depend on the rows beside it:
+// 32 keys' weights fill the 32 columns of their scores (16 of high parts, 16 of low ones)
+// and the second product runs over both. 256 rows on 4096 keys 41.0 -> 43.5 us a call, 128 rows
+// in 4 groups 71 -> 74 us, the error against 64 bits 0.0023 -> 0.0017, that of rounding the result.
+//
 // Warps (one CTA per SM, registers moved to the softmax warps):
 //   0 ..      four softmax warps per MMA tile, one thread per row
 //   then 4    tile warps: queries (cp.async), key masks and scales, KV8 codes to
@@ -285,6 +291,15 @@ __device__ __forceinline__ uint32_t pp_pack(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
+}
+// Four weights as bf16 pairs p[0], p[1]; FINE: and what is left of them, as bf16 too, in p[16], p[17].
+template <bool FINE>
+__device__ __forceinline__ void pp_weights(uint32_t *p, const float (&e)[4]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        p[k] = pp_pack(e[2 * k], e[2 * k + 1]);
+        if constexpr (FINE) p[16 + k] = pp_pack(e[2 * k] - bflo(p[k]), e[2 * k + 1] - bfhi(p[k]));
+    }
 }
 __device__ __forceinline__ void pp_cp16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -568,14 +583,14 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                 // 64 at once at 64 dims: 336 us against 303 for the first case above; 32 at 128 dims: 535 us against
                 // 517 for the second. A second copy of this code behind the test, for the rows that fail it,
                 // in place of the path below: 338 and 543 us.
-                constexpr int COLS = DIM == 64 ? 32 : 64;
+                constexpr int COLS = DIM == 64 ? 32 : 64, PARTS = SHARED ? 2 : 1;  // columns at a time; bf16 parts of a weight
                 int c = 0;  // keys done
                 if (full && !far) {
                     // every key counts: the weights as they are with the row's reference, unless they sum to more
                     // than 2^15 or a row's first ones to less than 2^-20
 #pragma unroll 1
                     for (; c < 64; c += COLS) {
-                        uint32_t p[COLS / 2];
+                        uint32_t p[COLS / 2 * PARTS];
                         const float4 *kc = kf + c / 4, *vc = vf + c / 4;
                         unsigned long long part[2] = {0ull, 0ull};
                         const unsigned long long mu = dup2(-m);
@@ -603,11 +618,14 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                     unpk2(mul2(pk2(e[0], e[1]), pk2(v4.x, v4.y)), e[0], e[1]);
                                     unpk2(mul2(pk2(e[2], e[3]), pk2(v4.z, v4.w)), e[2], e[3]);
                                 }
-                                p[j / 2] = pp_pack(e[0], e[1]);
-                                p[j / 2 + 1] = pp_pack(e[2], e[3]);
-                                if constexpr (!KV8) {  // the rounded weights: what dominates a row cancels exactly
-                                    part[0] = add2(part[0], pk2(bflo(p[j / 2]), bfhi(p[j / 2])));
-                                    part[1] = add2(part[1], pk2(bflo(p[j / 2 + 1]), bfhi(p[j / 2 + 1])));
+                                uint32_t *const pj = p + (SHARED ? j / 32 * 32 + j % 32 / 2 : j / 2);
+                                pp_weights<SHARED>(pj, e);
+                                if constexpr (SHARED && !KV8) {
+                                    part[0] = add2(part[0], pk2(e[0], e[1]));
+                                    part[1] = add2(part[1], pk2(e[2], e[3]));
+                                } else if constexpr (!KV8) {  // the rounded weights: what dominates a row cancels exactly
+                                    part[0] = add2(part[0], pk2(bflo(pj[0]), bfhi(pj[0])));
+                                    part[1] = add2(part[1], pk2(bflo(pj[1]), bfhi(pj[1])));
                                 }
                             }
                         }
@@ -618,7 +636,9 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         fresh = false;
                         l += sum;
                         // over columns whose scores have been read
-                        if constexpr (COLS == 64)
+                        if constexpr (SHARED) {
+                            for (int k = 0; k < COLS; k += 32) pp_st32(sh + c + k, p + k);
+                        } else if constexpr (COLS == 64)
                             pp_st32(sh, p);
                         else
                             pp_st16(sh + c / 2, p);
@@ -633,11 +653,17 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                     for (; c < 64; c += 32) {
                         const uint32_t sc = sh + c, bt = c == 0 ? bits[0] : bits[1];
                         const float4 *kc = kf + c / 4, *vc = vf + c / 4;
-                        uint32_t p[16];
+                        uint32_t p[16 * PARTS];
+                        auto store = [&] {
+                            if constexpr (SHARED)
+                                pp_st32(sh + c, p);
+                            else
+                                pp_st16(sh + c / 2, p);
+                        };
                         if (!__any_sync(0xffffffffu, bt != 0)) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) p[j] = 0;
-                            pp_st16(sh + c / 2, p);
+                            for (int j = 0; j < 16 * PARTS; ++j) p[j] = 0;
+                            store();
                             continue;
                         }
                         float sum;
@@ -672,9 +698,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                         for (int k = 0; k < 4; ++k)  // 0 whatever the scale of a value that the row does not see
                                             e[k] = bt & (1u << (j + k)) ? e[k] : 0.f;
                                     }
-                                    p[j / 2] = pp_pack(e[0], e[1]);
-                                    p[j / 2 + 1] = pp_pack(e[2], e[3]);
-                                    if constexpr (!KV8) {
+                                    pp_weights<SHARED>(p + j / 2, e);
+                                    if constexpr (SHARED && !KV8) {
+                                        part[0] = add2(part[0], pk2(e[0], e[1]));
+                                        part[1] = add2(part[1], pk2(e[2], e[3]));
+                                    } else if constexpr (!KV8) {
                                         part[0] = add2(part[0], pk2(bflo(p[j / 2]), bfhi(p[j / 2])));
                                         part[1] = add2(part[1], pk2(bflo(p[j / 2 + 1]), bfhi(p[j / 2 + 1])));
                                     }
@@ -733,7 +761,7 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                                 }
                             }
 #pragma unroll 1
-                            for (int j = 0; j < c / 2; j += 8) {  // this step's weights so far
+                            for (int j = 0; j < c / 2 * PARTS; j += 8) {  // this step's weights so far
                                 uint32_t o[8];
                                 pp_st_wait();
                                 pp_ld8(sh + j, o);
@@ -746,11 +774,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                         }
                         fresh = fresh && bt == 0;
                         l += sum;
-                        pp_st16(sh + c / 2, p);
+                        store();
                     }
                 } else {
                     const uint32_t zero[32] = {};
-                    pp_st32(sh, zero);
+                    for (int k = 0; k < PARTS; ++k) pp_st32(sh + 32 * k, zero);
                 }
                 if (!ok) break;
                 pp_st_wait();
@@ -1006,8 +1034,11 @@ __global__ void __launch_bounds__(PpCfg<KV8, DIM>::THREADS, 1) paged_prefill_ker
                             if (product) {
                                 const uint64_t vd = v_desc + (((vt % C::SLOTS) * C::TILE_BYTES + ph * 8192) >> 4);
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    pp_mma_ts(tmem + 256 + x * DIM, sc + 8 * j, vd + j * (2048 >> 4), id_pv, pn > 0 || j > 0);
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint32_t pj = SHARED ? sc + 32 * (j >> 1) + 8 * (j & 1) : sc + 8 * j;
+                                    pp_mma_ts(tmem + 256 + x * DIM, pj, vd + j * (2048 >> 4), id_pv, pn > 0 || j > 0);
+                                    if constexpr (SHARED) pp_mma_ts(tmem + 256 + x * DIM, pj + 16, vd + j * (2048 >> 4), id_pv, true);
+                                }
                             }
                             if (scores) {
                                 const uint64_t qd = q_desc + (((qb * C::TILES + x) * C::TILE_BYTES) >> 4),

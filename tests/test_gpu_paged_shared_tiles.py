@@ -118,7 +118,7 @@ def test_whole_and_ragged_tiles_of_query_rows(fmt, dim, group, rows):
     check(c, c.upload(keep), bf16(c.rand(rows, 8 * group, dim) * 2), [0, rows], [prefix])
 
 
-# ---------------------------------------------------------------- the row kernel's softmax weights
+# ---------------------------------------------------------------- softmax weights
 @FORMATS
 @DIMS
 @pytest.mark.parametrize('n', [64, 200])
@@ -164,6 +164,23 @@ def test_own_keys_behind_tiles_hold_weights_in_16_bits(fmt, dim, n, few_rows):
     out, size, bound = expected(w, v, n, most)
     keep = Keep()
     got, ran = call(b, b.upload(keep), np.repeat(q, rows, 0), [0, rows], [prefix], np.zeros(rows), 0.5)
+    assert ran and (got == got[:1]).all()
+    for h in range(14):
+        assert (np.abs(got[0, h] - out[h // 7]) <= bound[h // 7]).all()
+
+
+@FORMATS
+@DIMS
+@pytest.mark.parametrize('n', [64, 200])
+@pytest.mark.parametrize('part', [1, 2])
+def test_tiles_hold_weights_in_16_bits(fmt, dim, n, part):
+    """All of a row's keys, or the first half of them, as its group's shared ones: a row's result has the precision of
+    qwen_b200_op_paged_decode whatever the batch that it is in."""
+    c, q, w, v, most = cancelling(fmt, dim, n, 0.5)
+    rows = -(-WORK // (n // part * 2 * dim))
+    out, size, bound = expected(w, v, n, most)
+    keep = Keep()
+    got, ran = call(c, c.upload(keep), np.repeat(q, rows, 0), [0, rows], [n // part], np.zeros(rows), 0.5)
     assert ran and (got == got[:1]).all()
     for h in range(14):
         assert (np.abs(got[0, h] - out[h // 7]) <= bound[h // 7]).all()
