@@ -103,7 +103,8 @@ struct PagedAttnArgs {
     float scale;
     uint32_t format, dim;
     const uint32_t *prefix = nullptr;  // shared decode: tokens that a group's sequences share,
-    uint32_t long_keys = 0;            // and how many of them are shared whatever the work
+    uint32_t long_keys = 0;            // how many of them go to the tiles whatever the work,
+    uint64_t tile_work = 0;            // and from how many rows * tokens on all do
 };
 // A group of sequences that share their first tokens: its rows of q, and how many tokens of its first row's sequence
 // the tile kernel takes for all of them (0: none, each row takes its whole context).
@@ -131,14 +132,16 @@ constexpr uint64_t SHARED_WORK = 3ull << 24;
 // 1024 keys on 32 groups of 4 rows of 128 dims 66 and 68, 16 of 4 41 and 49.
 constexpr uint32_t SHARED_LONG = 2048;
 inline bool shared_few_warps(uint64_t items, int sms) { return items >= 3 * (uint64_t)sms; }
+__host__ __device__ __forceinline__ bool shared_worth(const PagedAttnArgs &a, uint32_t rows, uint64_t keys) {
+    return rows >= 2 && (keys >= a.long_keys || rows * keys >= a.tile_work);
+}
 __device__ __forceinline__ SharedGroup shared_group(const PagedAttnArgs &a, uint32_t g) {
     SharedGroup s;
     s.row0 = min(a.starts[g], a.rows);
     s.rows = min(max(a.starts[g + 1], s.row0), a.rows) - s.row0;
     s.seq = s.rows == 0 ? QWEN_B200_NO_SEQ : a.seqs ? a.seqs[s.row0] : s.row0;
     s.keys = min((int)min(a.prefix[g], 0x7fffffffu), paged_length(a.c, s.seq));
-    if (s.rows < 2 || ((uint32_t)s.keys < a.long_keys && (uint64_t)s.rows * s.keys < (SHARED_WORK / a.dim + a.c.hkv - 1) / a.c.hkv))
-        s.keys = 0;
+    if (!shared_worth(a, s.rows, (uint32_t)s.keys)) s.keys = 0;
     return s;
 }
 // The group that a row belongs to; false for none. starts is not decreasing.

@@ -41,9 +41,9 @@ int launch_paged_shared(const PagedAttnArgs &args, void *ws, cudaStream_t st) {
     p += paged_shared_pieces_bytes(a.dim);
     parts.ml = reinterpret_cast<float *>(p);
     parts.o = reinterpret_cast<float *>(p + up256(heads * 8));
-    // The host knows no prefix, but no group can be worth the tile kernel (shared_group) that is not with all rows and the widest table.
-    const uint64_t most = (uint64_t)a.c.max_pages << a.c.tshift;
-    const bool tiles = a.rows >= 2 && (most >= a.long_keys || (unsigned __int128)a.rows * most * a.c.hkv * a.dim >= SHARED_WORK);
+    a.tile_work = (SHARED_WORK / a.dim + a.c.hkv - 1) / a.c.hkv;
+    // The host knows no prefix, but no group is worth the tile kernel where all rows with the widest table are not.
+    const bool tiles = shared_worth(a, a.rows, (uint64_t)a.c.max_pages << a.c.tshift);
     PdlChain chain;
     if (tiles)
         if (int rc = launch_shared_tiles(a, parts, (unsigned *)ws, st)) return rc;
