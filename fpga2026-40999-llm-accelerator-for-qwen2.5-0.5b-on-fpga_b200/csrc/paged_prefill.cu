@@ -36,8 +36,8 @@
 // Shared prefixes (SHARED) take their weights as two bf16 parts, 16 bits together as in
 // decode attention, so that a row's precision does not depend on the rows beside it:
 // 32 keys' weights fill the 32 columns of their scores (16 of high parts, 16 of low ones)
-// and the second product runs over both. 256 rows on 4096 keys 41.0 -> 43.5 us a call, 128 rows
-// in 4 groups 71 -> 74 us, the error against 64 bits 0.0023 -> 0.0017, that of rounding the result.
+// and the second product runs over both. 256 rows on 4096 keys 41.0 -> 43.2 us a call, 128 rows
+// in 4 groups 71 -> 73 us, the error against 64 bits 0.0023 -> 0.0017, that of rounding the result.
 //
 // Warps (one CTA per SM, registers moved to the softmax warps):
 //   0 ..      four softmax warps per MMA tile, one thread per row
