@@ -617,10 +617,10 @@ int qwen_b200_op_paged_prefill(const qwen_b200_paged_kv *kv, uint32_t layer, con
  * on the device, not decreasing; rows in front of starts[0] and at or behind
  * starts[n] are left as they were, rows with no key are zero. rows * (q_heads /
  * kv_heads) and blocks are limited as in qwen_b200_op_paged_prefill, rows and keys as
- * in qwen_b200_op_paged_decode, and so are the softmax weights held and the sums; which
- * tokens are read once for a group, and so the order of the sums and the last bits, also depends on
- * the batch. What a row does not see does not reach it, NaN and infinities
- * included. The workspace (qwen_b200_paged_decode_shared_workspace;
+ * in qwen_b200_op_paged_decode, whose weights of 16 bits and fp32 sums these are. Which
+ * tokens are read once for a group, and with it the order of the sums and the last
+ * bits, depends on the whole call's sizes. What a row does not see does not reach it,
+ * NaN and infinities included. The workspace (qwen_b200_paged_decode_shared_workspace;
  * calls that overlap need one each) may hold anything, but its first 4 bytes become non-zero if a bounded
  * device wait expired (ctx is then not valid): a caller that wants to know
  * zeroes them before. */
